@@ -329,6 +329,39 @@ int g2v_covariance_from_scale_rotation_backward(int n, const float* scales, cons
                                                 const float* grad_covariances, float* grad_scales,
                                                 float* grad_rotations, void* stream);
 
+/* ---- query/key norms with rotary positions ---------------------------------------------------
+ * For Gaussians (or other tokens at positions) that attend to one another before the splat: the root-mean-square
+ * norm of every head of the queries and keys and its rotation by the token's position, in one pass.  No counterpart
+ * in the reference.  For a row x of head_dim values, weight w and position p (num_axes coordinates):
+ *     r = (mean x^2 + eps)^-1/2,  y = w x r,  theta_i = sum_a p_a freqs[a][i]  (i < num_pairs),
+ *     (out_2i, out_2i+1) = (y_2i cos - y_2i+1 sin, y_2i sin + y_2i+1 cos),  out_d = y_d for d >= 2 num_pairs.
+ * q (batch, n_q, heads_q, head_dim) and k (batch, n_k, heads_k, head_dim) of dtype (G2V_DTYPE_F32 or
+ * G2V_DTYPE_BF16), unit stride along head_dim, *_strides in elements along batch, tokens and heads; q_out and k_out
+ * are contiguous and of the same type (rounded once).  q_weight, k_weight (head_dim) float32, NULL for ones;
+ * q_positions (batch, n_q, num_axes), k_positions (batch, n_k, num_axes) and freqs (num_axes, num_pairs) float32,
+ * contiguous.  k_positions NULL: the keys are the queries' tokens (n_k == n_q).  heads_k == 0: queries alone.
+ * head_dim <= 256, num_axes <= 8, 2 num_pairs <= head_dim.  Sums are float32.  Asynchronous.
+ *
+ * The backward maps the upstream gradients (strided like q and k) to grad_q, grad_k (contiguous, dtype) and, where
+ * not NULL, float32 grad_q_weight, grad_k_weight (head_dim) and grad_q_positions, grad_k_positions (with shared
+ * positions grad_q_positions holds the sum and grad_k_positions is unused).  Deterministic: fixed summation order. */
+int g2v_qk_norm_rotary_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int num_axes,
+                               int num_pairs, const void* q, const long long q_strides[3], const void* k,
+                               const long long k_strides[3], int dtype, const float* q_weight,
+                               const float* k_weight, const float* q_positions, const float* k_positions,
+                               const float* freqs, float eps, void* q_out, void* k_out, void* stream);
+size_t g2v_qk_norm_rotary_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim,
+                                             int num_axes, int dtype, int shared_positions);
+int g2v_qk_norm_rotary_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int num_axes,
+                                int num_pairs, const void* q, const long long q_strides[3], const void* k,
+                                const long long k_strides[3], int dtype, const float* q_weight,
+                                const float* k_weight, const float* q_positions, const float* k_positions,
+                                const float* freqs, float eps, const void* grad_q_out,
+                                const long long grad_q_out_strides[3], const void* grad_k_out,
+                                const long long grad_k_out_strides[3], void* grad_q, void* grad_k,
+                                float* grad_q_weight, float* grad_k_weight, float* grad_q_positions,
+                                float* grad_k_positions, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- per-kernel timing (benchmarks) --------------------------------------------------------
  * No counterpart in the reference (which times the whole forward/backward with one CUDA event
  * pair, src/cuda_gaussian_voxelizer.cu:1549-1555, :1905-1913).  While enabled, every kernel launch

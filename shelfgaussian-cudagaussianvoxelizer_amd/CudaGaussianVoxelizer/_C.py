@@ -14,7 +14,8 @@ from . import _lib
 
 __all__ = ["gaussian_voxelizer_forward", "gaussian_voxelizer_backward", "gaussian_voxelizer_forward_batched",
            "CudaFeatsCosinelossForward", "CudaFeatsCosinelossBackward", "build_t2g", "grid_dims",
-           "covariance_from_scale_rotation", "covariance_from_scale_rotation_backward"]
+           "covariance_from_scale_rotation", "covariance_from_scale_rotation_backward",
+           "qk_norm_rotary_forward", "qk_norm_rotary_backward"]
 
 
 def _ptr(t):
@@ -789,3 +790,107 @@ def covariance_from_scale_rotation_backward(scales, rotations, grad_cov):
                                                                    _ptr(gq), _stream(dev)),
                    "covariance_from_scale_rotation_backward")
     return gs, gq
+
+
+def _heads_input(t, name, like=None):
+    """(B, N, H, D) rows of float32 or bfloat16 on the GPU, in any layout with unit stride along D (others are
+    copied); like: the tensor whose type and device it has to share."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} must be a GPU tensor, got {t.device}")
+    if t.dtype not in _FEAT_DTYPES:
+        raise RuntimeError(f"expected scalar type Float or BFloat16 for {name} but found {t.dtype}")
+    if t.dim() != 4:
+        raise RuntimeError(f"{name} must be (B, N, H, D), got {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise RuntimeError(f"{name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    t = t.detach()
+    return t if t.stride(3) == 1 else t.contiguous()
+
+
+def _strides(t):
+    return None if t is None else (ctypes.c_longlong * 3)(*t.stride()[:3])
+
+
+def _plain_f32(t, name, shape, device):
+    """A contiguous float32 tensor of this shape on this device (None passes)."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or tuple(t.shape) != shape:
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise RuntimeError(f"{name} must be float32 {shape} on {device}, got {got}")
+    return t.detach().contiguous()
+
+
+def _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions):
+    q = _heads_input(q, "q")
+    B, nq, hq, D = q.shape
+    dev = q.device
+    if k is not None:
+        k = _heads_input(k, "k", q)
+        if k.shape[0] != B or k.shape[3] != D or (k_positions is None and k.shape[1] != nq):
+            raise RuntimeError(f"k {tuple(k.shape)} does not go with q {tuple(q.shape)}"
+                               + ("" if k_positions is not None else " (without k_positions the tokens are the same)"))
+    nk, hk = (0, 0) if k is None else (k.shape[1], k.shape[2])
+    if not isinstance(freqs, torch.Tensor) or freqs.dim() != 2:
+        raise RuntimeError("freqs must be (axes, pairs)")
+    axes, pairs = freqs.shape
+    freqs = _plain_f32(freqs, "freqs", (axes, pairs), dev)
+    positions = _plain_f32(positions, "positions", (B, nq, axes), dev)
+    if positions is None:
+        raise RuntimeError("positions must be a tensor")
+    k_positions = _plain_f32(k_positions, "k_positions", (B, nk, axes), dev) if k is not None else None
+    q_weight = _plain_f32(q_weight, "q_weight", (D,), dev)
+    k_weight = _plain_f32(k_weight, "k_weight", (D,), dev)
+    sizes = (B, nq, nk if k_positions is not None or k is None else nq, hq, hk, D, axes)
+    return q, k, positions, freqs, q_weight, k_weight, k_positions, sizes, pairs
+
+
+def qk_norm_rotary_forward(q, k, positions, freqs, q_weight=None, k_weight=None, k_positions=None, eps=1e-6):
+    """(q', k'): the root-mean-square norm of every head of q (B, Nq, Hq, D) and k (B, Nk, Hk, D; or None), times
+    q_weight / k_weight (D,), and its rotation by the token's position: pair i of a head turns by the angle
+    sum_a positions[..., a] freqs[a, i].  k_positions None: the keys are the queries' tokens."""
+    lib = _lib.load()
+    q, k, pos, freqs, qw, kw, kpos, sizes, pairs = _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions)
+    dev = q.device
+    with _OnDevice(dev):
+        oq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        ok = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+        _lib.check(lib.g2v_qk_norm_rotary_forward(*sizes, pairs, _ptr(q), _strides(q), _ptr(k), _strides(k),
+                                                  _FEAT_DTYPES[q.dtype], _ptr(qw), _ptr(kw), _ptr(pos), _ptr(kpos),
+                                                  _ptr(freqs), float(eps), _ptr(oq), _ptr(ok), _stream(dev)),
+                   "qk_norm_rotary_forward")
+    return oq, ok
+
+
+def qk_norm_rotary_backward(grad_q_out, grad_k_out, q, k, positions, freqs, q_weight=None, k_weight=None,
+                            k_positions=None, eps=1e-6, want_weights=(True, True), want_positions=(True, True)):
+    """(grad_q, grad_k, grad_q_weight, grad_k_weight, grad_positions, grad_k_positions) of qk_norm_rotary_forward; the
+    float32 weight and position gradients are None where not wanted (grad_k_positions also with shared positions,
+    whose gradient is grad_positions)."""
+    lib = _lib.load()
+    q, k, pos, freqs, qw, kw, kpos, sizes, pairs = _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions)
+    dev = q.device
+    gq = _heads_input(grad_q_out, "grad_q_out", q)
+    gk = None if k is None else _heads_input(grad_k_out, "grad_k_out", q)
+    if gq.shape != q.shape or (k is not None and gk.shape != k.shape):
+        raise RuntimeError(f"gradients must be {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
+    D = q.shape[3]
+    with _OnDevice(dev):
+        f32 = dict(dtype=torch.float32, device=dev)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+        dqw = torch.empty(D, **f32) if want_weights[0] else None
+        dkw = torch.empty(D, **f32) if want_weights[1] and k is not None else None
+        dpos = torch.empty(pos.shape, **f32) if want_positions[0] else None
+        dkpos = torch.empty(kpos.shape, **f32) if want_positions[1] and kpos is not None else None
+        ws = torch.empty(lib.g2v_qk_norm_rotary_backward_workspace(*sizes, _FEAT_DTYPES[q.dtype], 1 if kpos is None else 0),
+                         dtype=torch.uint8, device=dev)
+        _lib.check(lib.g2v_qk_norm_rotary_backward(*sizes, pairs, _ptr(q), _strides(q), _ptr(k), _strides(k),
+                                                   _FEAT_DTYPES[q.dtype], _ptr(qw), _ptr(kw), _ptr(pos), _ptr(kpos),
+                                                   _ptr(freqs), float(eps), _ptr(gq), _strides(gq), _ptr(gk),
+                                                   _strides(gk), _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(dpos),
+                                                   _ptr(dkpos), _ptr(ws), ws.numel(), _stream(dev)),
+                   "qk_norm_rotary_backward")
+    return dq, dk, dqw, dkw, dpos, dkpos

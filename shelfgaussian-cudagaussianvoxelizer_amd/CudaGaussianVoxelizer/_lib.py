@@ -67,6 +67,12 @@ SIGNATURES = {
     "g2v_cosine_loss_backward": (_i, [_ll, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "g2v_covariance_from_scale_rotation": (_i, [_i, _vp, _vp, _vp, _vp]),
     "g2v_covariance_from_scale_rotation_backward": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "g2v_qk_norm_rotary_forward": (_i, [_i] * 8 + [_vp, _llp, _vp, _llp, _i, _vp, _vp, _vp, _vp, _vp,
+                                                   ctypes.c_float, _vp, _vp, _vp]),
+    "g2v_qk_norm_rotary_backward_workspace": (_sz, [_i] * 9),
+    "g2v_qk_norm_rotary_backward": (_i, [_i] * 8 + [_vp, _llp, _vp, _llp, _i, _vp, _vp, _vp, _vp, _vp,
+                                                    ctypes.c_float, _vp, _llp, _vp, _llp, _vp, _vp, _vp, _vp, _vp,
+                                                    _vp, _vp, _sz, _vp]),
     "g2v_profile_enable": (_i, [_i]),
     "g2v_profile_reset": (_i, []),
     "g2v_profile_collect": (_i, []),
@@ -95,7 +101,10 @@ def load():
         raise ImportError(f"{LIB_PATH} has ABI {got}, this package expects {ABI_VERSION}: rebuild it "
                           "(python shelfgaussian-cudagaussianvoxelizer_amd/build.py)")
     for name, (res, args) in SIGNATURES.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:   # entry points are added without a new ABI: an earlier build lacks the latest
+            raise ImportError(f"{LIB_PATH} has no {name}: rebuild it "
+                              "(python shelfgaussian-cudagaussianvoxelizer_amd/build.py)")
         fn.restype = res
         fn.argtypes = args
     _lib = lib

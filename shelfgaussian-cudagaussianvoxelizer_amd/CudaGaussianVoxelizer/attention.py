@@ -1,0 +1,77 @@
+"""Gaussians that attend to one another before the splat: norms of queries and keys with the rotation by their
+positions.  No counterpart in the reference, whose features arrive finished; the kernels live in libg2v_hip.so and are
+reached through ``_C`` on the caller's current stream.
+"""
+import math
+
+import torch
+
+from . import _C
+
+__all__ = ["qk_norm_rotary", "rotary_frequencies"]
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _QkNormRotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, q_weight, k_weight, k_positions, eps):
+        ctx.save_for_backward(q, k, positions, freqs, q_weight, k_weight, k_positions)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return _C.qk_norm_rotary_forward(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
+
+    @staticmethod
+    def backward(ctx, grad_q_out, grad_k_out):
+        q, k, positions, freqs, q_weight, k_weight, k_positions = ctx.saved_tensors
+        if grad_q_out is None and grad_k_out is None:
+            return (None,) * 8
+        if grad_q_out is None:
+            grad_q_out = torch.zeros_like(q)
+        if grad_k_out is None and k is not None:
+            grad_k_out = torch.zeros_like(k)
+        need = ctx.needs_input_grad
+        dq, dk, dqw, dkw, dpos, dkpos = _C.qk_norm_rotary_backward(
+            grad_q_out, grad_k_out, q, k, positions, freqs, q_weight, k_weight, k_positions, ctx.eps,
+            want_weights=(need[4], need[5]), want_positions=(need[2], need[6]))
+        return dq, dk, dpos, None, dqw, dkw, dkpos, None
+
+
+def qk_norm_rotary(q, k, positions, freqs, q_weight=None, k_weight=None, *, k_positions=None, eps=1e-6):
+    """Norms of queries and keys for each head and their rotation by the tokens' positions, in one pass.
+
+    q (B, Nq, Hq, D) and k (B, Nk, Hk, D; None: queries alone) are float32 or bfloat16 in any layout with unit stride
+    along D (views of a fused projection are read in place).  positions (B, Nq, A) float32 are coordinates of any kind
+    (the Gaussians' means in metres, pixels, time); k_positions (B, Nk, A) those of the keys, None when queries and
+    keys are the same tokens.  freqs (A, P) float32, 2 P <= D: pair (2 i, 2 i + 1) of a head turns by the angle
+    sum_a positions[..., a] freqs[a, i], what is left of D stays (rotary_frequencies makes the usual table).
+    q_weight and k_weight (D,) scale the normed rows.  Returns (q', k') of q's type, contiguous.
+
+    Gradients flow to q, k, the weights and the positions; freqs is a constant."""
+    if isinstance(freqs, torch.Tensor) and freqs.requires_grad:
+        raise RuntimeError("freqs is a constant of qk_norm_rotary: it gets no gradient")
+    if q_weight is not None and q_weight.dtype == torch.bfloat16:
+        q_weight = q_weight.float()
+    if k_weight is not None and k_weight.dtype == torch.bfloat16:
+        k_weight = k_weight.float()
+    if _needs_grad(q, k, positions, q_weight, k_weight, k_positions):
+        return _QkNormRotaryFunction.apply(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
+    return _C.qk_norm_rotary_forward(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
+
+
+def rotary_frequencies(head_dim, axes=3, wavelengths=(0.8, 160.0), device="cuda"):
+    """(axes, P) float32 table of qk_norm_rotary: each axis turns an equal share of the head's pairs, with wavelengths
+    (in the positions' unit) spread geometrically over the given range; pairs that do not divide stay unrotated.  The
+    default range is two voxels of 0.4 m to twice a scene of 80 m."""
+    each = head_dim // 2 // axes
+    lo, hi = float(wavelengths[0]), float(wavelengths[1])
+    if each < 1 or not 0.0 < lo <= hi:
+        raise RuntimeError(f"rotary_frequencies: {head_dim} values hold no pair for each of {axes} axes, or bad "
+                           f"wavelengths {wavelengths}")
+    table = torch.zeros(axes, axes * each, dtype=torch.float32)
+    step = torch.arange(each, dtype=torch.float64) / max(1, each - 1)
+    for a in range(axes):
+        table[a, a * each:(a + 1) * each] = (2.0 * math.pi / (lo * (hi / lo) ** step)).float()
+    return table.to(device)

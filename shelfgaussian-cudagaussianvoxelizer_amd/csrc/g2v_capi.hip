@@ -24,6 +24,21 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+}  // namespace
+
+namespace g2v {
+void api_begin() { g_err[0] = 0; }
+int api_fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+}  // namespace g2v
+
+namespace {
+
 int hip_fail(hipError_t e, const char* where) {
     return fail(G2V_ERR_HIP, "%s: %s", where, hipGetErrorString(e));
 }

@@ -26,6 +26,10 @@ struct Carver {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// g2v_last_error's message, for entry points outside g2v_capi.hip: cleared on entry; code is returned.
+void api_begin();
+int api_fail(int code, const char* fmt, ...);
+
 // ---- CSR build (g2v_csr.hip) ------------------------------------------------------------
 // Regions: 2 x 2 tiles in x, y and up to 4 tiles in z (the feature-gradient phase's work units, and the
 // coarse boxes by which the tile lists are built).
@@ -234,6 +238,35 @@ hipError_t launch_cosine_backward(int64_t V, int C, const float* label, const ui
 hipError_t launch_cov_from_scale_rot(int n, const float* scales, const float* rotations, float* cov, hipStream_t s);
 hipError_t launch_cov_from_scale_rot_bwd(int n, const float* scales, const float* rotations, const float* grad_cov,
                                          float* grad_scales, float* grad_rotations, hipStream_t s);
+
+// ---- norms of queries and keys with rotary positions (g2v_qknorm.hip) -----------------------
+// Index 0: queries, 1: keys.  Rows x[k] at element strides (sb, sn, sh) of scene, token and head; out and dx are
+// contiguous (batch, n, heads, dim).
+struct QkNormArgs {
+    int batch, n[2], heads[2], dim, axes, pairs;
+    int shared;                    // keys are the queries' tokens: pos[0] serves both
+    float eps;
+    const void* x[2];
+    int64_t sb[2], sn[2], sh[2];
+    const float* w[2];             // (dim), null: ones
+    const float* pos[2];           // (batch, n, axes)
+    const float* freqs;            // (axes, pairs)
+    void* out[2];
+    // backward
+    const void* g[2];
+    int64_t gsb[2], gsn[2], gsh[2];
+    void* dx[2];
+    float* dw[2];                  // (dim), null: not wanted
+    float* dpos[2];                // (batch, n, axes), null: not wanted
+    // set by the launches
+    int shift, chunk, blocks0;
+    int64_t dpos_tokens;
+    float *dw_part, *dpos_part;
+};
+constexpr int kQnBwdBlocks = 1024;   // workgroups of a side in the backward (4 per CU): the rows of dL/dw's partial sums
+hipError_t launch_qk_norm_rotary(const QkNormArgs& a, int dtype, hipStream_t s);
+size_t qk_norm_bwd_workspace(const QkNormArgs& a, int dtype);
+hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& a, int dtype, void* ws, hipStream_t s);
 
 // Brackets one kernel launch with HIP events when profiling is enabled (g2v_profile.hip).
 class ProfMark {
