@@ -362,6 +362,38 @@ int g2v_qk_norm_rotary_backward(int batch, int n_q, int n_k, int heads_q, int he
                                 float* grad_q_weight, float* grad_k_weight, float* grad_q_positions,
                                 float* grad_k_positions, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention ------------------------------------------------------------------------------
+ * Attention of a set of queries (Gaussians, or a query that pools a scene) over a set of keys (Gaussians or image
+ * tokens), without an order among them.  No counterpart in the reference.
+ *     out = softmax(scale q k^T over the valid keys) v
+ * q, out (batch, n_q, heads_q, head_dim); k, v (batch, n_k, heads_k, head_dim); heads_q a multiple of heads_k (query
+ * heads h heads_q / heads_k ... share key head h); dtype G2V_DTYPE_F32 or G2V_DTYPE_BF16 for all; strides in elements
+ * along batch, tokens and heads, unit stride along head_dim; out contiguous.  head_dim <= 128, scale > 0.
+ * key_mask (batch, n_k) bytes: 0 where a key is not attended to (NULL: none); what such a key's rows hold is never read.
+ * A query without any key gives 0.  lse (batch, heads_q, n_q) float32, NULL where no backward follows: the base-2
+ * logarithm of the sum of 2^(scale log2(e) q.k), +inf for a query without keys.  key_list (batch n_k + batch ints,
+ * needed with key_mask) receives the valid keys of every scene and their number, for the backward.
+ * Sums and softmax statistics are float32; bfloat16 probabilities are rounded to nearest even for their product.
+ * in_place: whether every tensor is bfloat16 with head_dim and strides multiples of 8 and 16-byte aligned data (others
+ * are packed into the workspace first; pass 0 when unsure).  Asynchronous. */
+size_t g2v_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                       int in_place);
+int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                          const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                          const long long v_strides[3], int dtype, const unsigned char* key_mask, float scale, void* out,
+                          float* lse, int* key_list, void* workspace, size_t workspace_bytes, void* stream);
+
+/* g2v_attention_backward: gradients of g2v_attention_forward's inputs from its out, lse and key_list (NULL without a
+ * mask) and the upstream gradient (strided like q); contiguous, of dtype.  Probabilities are recomputed.  grad_q, or
+ * grad_k with grad_v, may be NULL; masked keys get 0.  Deterministic: no atomics, fixed summation order.  Asynchronous. */
+size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                        int in_place);
+int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                           const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                           const long long v_strides[3], int dtype, const int* key_list, float scale, const void* out,
+                           const float* lse, const void* grad_out, const long long grad_out_strides[3], void* grad_q,
+                           void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- per-kernel timing (benchmarks) --------------------------------------------------------
  * No counterpart in the reference (which times the whole forward/backward with one CUDA event
  * pair, src/cuda_gaussian_voxelizer.cu:1549-1555, :1905-1913).  While enabled, every kernel launch

@@ -15,7 +15,7 @@ from . import _lib
 __all__ = ["gaussian_voxelizer_forward", "gaussian_voxelizer_backward", "gaussian_voxelizer_forward_batched",
            "CudaFeatsCosinelossForward", "CudaFeatsCosinelossBackward", "build_t2g", "grid_dims",
            "covariance_from_scale_rotation", "covariance_from_scale_rotation_backward",
-           "qk_norm_rotary_forward", "qk_norm_rotary_backward"]
+           "qk_norm_rotary_forward", "qk_norm_rotary_backward", "attention_forward", "attention_backward"]
 
 
 def _ptr(t):
@@ -894,3 +894,76 @@ def qk_norm_rotary_backward(grad_q_out, grad_k_out, q, k, positions, freqs, q_we
                                                    _ptr(dkpos), _ptr(ws), ws.numel(), _stream(dev)),
                    "qk_norm_rotary_backward")
     return dq, dk, dqw, dkw, dpos, dkpos
+
+
+def _attention_inputs(q, k, v, scale):
+    q = _heads_input(q, "q")
+    k, v = _heads_input(k, "k", q), _heads_input(v, "v", q)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
+    B, nq, hq, D = q.shape
+    sizes = (B, nq, k.shape[1], hq, k.shape[2], D)
+    return q, k, v, sizes, float(D ** -0.5 if scale is None else scale)
+
+
+def _in_place(*tensors):
+    """Whether the kernels read these rows where they are (include/g2v.h: in_place)."""
+    for t in tensors:
+        a, b, c, _ = t.stride()
+        if t.dtype != torch.bfloat16 or (a | b | c | t.shape[3]) % 8 or t.data_ptr() % 16 or not 0 <= b < 1 << 24:
+            return 0
+    return 1
+
+
+def attention_forward(q, k, v, key_mask=None, scale=None, want_lse=False):
+    """(out, lse, key_list): softmax(scale q k^T over the valid keys) v for q (B, Nq, Hq, D) and k, v (B, Nk, Hkv, D), Hq a
+    multiple of Hkv; scale None: D^-1/2.  key_mask (B, Nk) bool, False where a key is not attended to.  lse (None unless
+    wanted) and key_list (None without a mask) are what attention_backward takes."""
+    lib = _lib.load()
+    q, k, v, sizes, scale = _attention_inputs(q, k, v, scale)
+    B, nq, nk, hq = sizes[:4]
+    dev, fdt = q.device, _FEAT_DTYPES[q.dtype]
+    if key_mask is not None:
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype != torch.bool or key_mask.device != dev \
+                or tuple(key_mask.shape) != (B, nk):
+            raise RuntimeError(f"key_mask must be a bool tensor {(B, nk)} on {dev}")
+        key_mask = key_mask.contiguous()
+    with _OnDevice(dev):
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        lse = torch.empty(B, hq, nq, dtype=torch.float32, device=dev) if want_lse else None
+        lst = None if key_mask is None else torch.empty(B * (nk + 1), dtype=torch.int32, device=dev)
+        ws = torch.empty(lib.g2v_attention_forward_workspace(*sizes, fdt, _in_place(q, k, v)), dtype=torch.uint8, device=dev)
+        _lib.check(lib.g2v_attention_forward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
+                                             _ptr(key_mask), scale, _ptr(out), _ptr(lse), _ptr(lst), _ptr(ws), ws.numel(),
+                                             _stream(dev)), "attention_forward")
+    return out, lse, lst
+
+
+def attention_backward(grad_out, q, k, v, out, lse, key_list=None, scale=None, want_q=True, want_kv=True):
+    """(grad_q, grad_k, grad_v) of attention_forward from its results; None where not wanted."""
+    lib = _lib.load()
+    q, k, v, sizes, scale = _attention_inputs(q, k, v, scale)
+    B, nq, nk, hq = sizes[:4]
+    dev, fdt = q.device, _FEAT_DTYPES[q.dtype]
+    g = _heads_input(grad_out, "grad_out", q)
+    if g.shape != q.shape:
+        raise RuntimeError(f"grad_out must be {tuple(q.shape)}, got {tuple(g.shape)}")
+    _check_saved(out, "out", q.dtype, dev)
+    _check_saved(lse, "lse", torch.float32, dev)
+    if out.shape != q.shape or tuple(lse.shape) != (B, hq, nq):
+        raise RuntimeError(f"out {tuple(out.shape)} and lse {tuple(lse.shape)} do not go with q {tuple(q.shape)}")
+    if key_list is not None:
+        _check_saved(key_list, "key_list", torch.int32, dev)
+        if key_list.numel() != B * (nk + 1):
+            raise RuntimeError(f"key_list must hold {B * (nk + 1)} values, got {key_list.numel()}")
+    with _OnDevice(dev):
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
+        dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
+        dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
+        ws = torch.empty(lib.g2v_attention_backward_workspace(*sizes, fdt, _in_place(q, k, v, g)), dtype=torch.uint8,
+                         device=dev)
+        _lib.check(lib.g2v_attention_backward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
+                                              _ptr(key_list), scale, _ptr(out), _ptr(lse), _ptr(g), _strides(g), _ptr(dq),
+                                              _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)),
+                   "attention_backward")
+    return dq, dk, dv

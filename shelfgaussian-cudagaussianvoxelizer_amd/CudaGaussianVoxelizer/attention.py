@@ -8,7 +8,7 @@ import torch
 
 from . import _C
 
-__all__ = ["qk_norm_rotary", "rotary_frequencies"]
+__all__ = ["qk_norm_rotary", "rotary_frequencies", "gaussian_attention"]
 
 
 def _needs_grad(*tensors):
@@ -75,3 +75,35 @@ def rotary_frequencies(head_dim, axes=3, wavelengths=(0.8, 160.0), device="cuda"
     for a in range(axes):
         table[a, a * each:(a + 1) * each] = (2.0 * math.pi / (lo * (hi / lo) ** step)).float()
     return table.to(device)
+
+
+class _GaussianAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, scale):
+        out, lse, key_list = _C.attention_forward(q, k, v, key_mask, scale, want_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, key_list)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, key_list = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return _C.attention_backward(grad_out, q, k, v, out, lse, key_list, ctx.scale, want_q=need[0],
+                                     want_kv=need[1] or need[2]) + (None, None)
+
+
+def gaussian_attention(q, k, v, key_mask=None, scale=None):
+    """softmax(scale q k^T over the valid keys) v, without an order among queries or keys.
+
+    q (B, Nq, Hq, D) and k, v (B, Nk, Hkv, D) are float32 or bfloat16 in any layout with unit stride along D; Hq is a
+    multiple of Hkv (consecutive query heads share a key head), D at most 128.  key_mask (B, Nk) bool is False at keys
+    that are not attended to (padding of a batch, pruned Gaussians): what their rows hold, NaN included, reaches no result
+    and they get zero gradients; a query without any key gives zeros.  scale None: D^-1/2.  Returns (B, Nq, Hq, D) of
+    q's type, contiguous.  Any number of queries and keys, zero and one included: a single query that pools a scene has its
+    keys split over the GPU.
+
+    Gradients flow to q, k and v; the backward recomputes the probabilities and gives the same bits on every run."""
+    if _needs_grad(q, k, v):
+        return _GaussianAttentionFunction.apply(q, k, v, key_mask, scale)
+    return _C.attention_forward(q, k, v, key_mask, scale)[0]

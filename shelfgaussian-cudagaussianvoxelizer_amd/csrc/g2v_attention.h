@@ -1,0 +1,263 @@
+// Device side shared by the attention kernels (g2v_attention_fwd.hip, g2v_attention_bwd.hip).
+//
+// Matrix products run on v_mfma_f32_32x32x16_bf16.  Lane l of a wave holds, with n = l % 32 and g = l / 32,
+//   A (32 x 16): row n, contraction slots 8g .. 8g+7;   B (16 x 32): column n, the same slots;
+//   C (32 x 32): column n, rows 8 (i / 4) + 4 g + i % 4 in registers i = 0 .. 15.
+// The contraction's order is free as long as A and B agree on it.  So a product's result C goes straight into the next
+// product as B, without leaving its lane: registers 8 s .. 8 s + 7 are the slots of step s, which stand for rows
+// 16 s + 4 g + {0..3} and 16 s + 8 + 4 g + {0..3}; the other operand reads its rows in that order (tr_frag).
+// Scores are computed with the long axis in the registers and the workgroup's own rows in the lanes (S^T = K Q^T for the
+// forward and dQ, S = Q K^T for dK and dV): softmax statistics are one number a lane.
+//
+// float32 inputs are held as three bfloat16 planes, x = x0 + x1 + x2 exactly to 24 bits, and a product takes the six terms
+// x_i y_j with i + j <= 2; what is dropped is below 2^-24 of each product.  At six bfloat16 products a float32 product
+// runs 2.7 times as fast as on the float32 matrix instructions (1/16 of the bfloat16 rate).
+#pragma once
+#include "g2v_internal.h"
+
+namespace g2v {
+namespace attn {
+
+typedef __attribute__((address_space(3))) char* lds_t;
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Rows of one tensor as the kernels read them: bfloat16, 16-byte chunks, byte strides of scene, token and head; a plane's
+// chunks past `chunks` do not exist in memory and count as zero.  Packed tensors have their planes one after another.
+struct RowSrc {
+    const char* p;
+    int64_t sb, sn, sh;
+    int chunks;
+};
+
+// The chunk c of row r of a tile sits at slot swz(r, c): the 16 rows of an LDS cycle's A reads (one chunk each), and the
+// four rows of a transposed read (four neighbouring chunks each), then fall on different banks.
+template <int DP>
+__device__ __forceinline__ int swz(int r, int c) {
+    if constexpr (DP == 64) return c ^ ((((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1));
+    else if constexpr (DP == 128) return c ^ (((r & 3) << 2) | ((r >> 2) & 3));
+    else return c ^ ((r >> 2) & 3);
+}
+
+__device__ __forceinline__ uint32_t lds_off(const void* p) { return (uint32_t)(uintptr_t)(lds_t)p; }
+
+// Direct-to-LDS loads: lane l's 16 (4) bytes land at lds + 16 l (4 l), whatever lanes are off.  Inline assembly, so that
+// the compiler ties no wait to them: tile_barrier waits.
+__device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma16(const void* addr, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds) : "memory");
+}
+
+// Every load and LDS operation of this wave done, then the other waves met.
+__device__ __forceinline__ void tile_barrier() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// A tile of ROWS rows of one tensor in LDS: [plane][row][DP], swizzled, filled by NT threads.
+template <int NP, int DP, int ROWS, int NT>
+struct Tile {
+    static constexpr int C = DP / 8;                    // chunks of a row
+    static constexpr int kChunks = NP * ROWS * C;
+    static constexpr int kBytes = kChunks * 16;
+    static constexpr int kIter = (kChunks + NT - 1) / NT;
+
+    int row[kIter];         // this thread's row of each load
+    uint32_t off[kIter];    // byte offset of its chunk in the row
+    bool on[kIter];         // the chunk exists
+
+    __device__ __forceinline__ void init(const RowSrc& s) {
+#pragma unroll
+        for (int it = 0; it < kIter; ++it) {
+            const int L = it * NT + threadIdx.x;
+            const int pl = L / (ROWS * C), rem = L % (ROWS * C);
+            row[it] = rem / C;
+            const int c = swz<DP>(row[it], rem % C);
+            off[it] = (uint32_t)(pl * C + c) * 16;
+            on[it] = c < s.chunks && L < kChunks;
+        }
+    }
+    __device__ __forceinline__ uint32_t dst(uint32_t lds, int it) const {
+        return lds + it * NT * 16 + (uint32_t)uniform(threadIdx.x >> 6) * 1024;
+    }
+    // Rows [j0, j0 + ROWS) of base, all of them there.
+    __device__ __forceinline__ void load(const char* base, int64_t sn, int64_t j0, uint32_t lds) const {
+        const char* p = base + j0 * sn;
+#pragma unroll
+        for (int it = 0; it < kIter; ++it)
+            if (on[it]) dma16(p, (uint32_t)row[it] * (uint32_t)sn + off[it], dst(lds, it));
+    }
+    // The rows that idx names (an index below 0: zeros).
+    __device__ __forceinline__ void load_indexed(const char* base, int64_t sn, const int (&idx)[kIter], char* lds) const {
+#pragma unroll
+        for (int it = 0; it < kIter; ++it) {
+            if (on[it]) {
+                if (idx[it] >= 0) dma16(base + idx[it] * sn + off[it], dst(lds_off(lds), it));
+                else *reinterpret_cast<f32x4*>(lds + (it * NT + threadIdx.x) * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+    }
+};
+
+// Chunks that do not exist are zero for the whole kernel: cleared once, before the first load.
+template <int NT>
+__device__ __forceinline__ void clear_lds(char* lds, int bytes) {
+    for (int i = threadIdx.x * 16; i < bytes; i += NT * 16) *reinterpret_cast<f32x4*>(lds + i) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    __syncthreads();
+}
+
+// A operand from a tile: rows 32 rb .. 32 rb + 31, contraction over d in 16 ks .. 16 ks + 15.
+template <int DP>
+__device__ __forceinline__ bf16x8 row_frag(const char* tile, int rb, int ks) {
+    const int l = threadIdx.x & 63, n = l & 31, g = l >> 5;
+    return *reinterpret_cast<const bf16x8*>(tile + (rb * 32 + n) * (DP * 2) + swz<DP>(n, 2 * ks + g) * 16);
+}
+
+// A operand of the transposed tile: rows d = 32 t .. 32 t + 31, contraction over the tile's rows 32 rb + 16 s .. + 15 in
+// the order of a result's registers.  Each read transposes 4 x 16 values within 16 lanes.
+template <int DP>
+__device__ __forceinline__ bf16x8 tr_frag(const char* tile, int rb, int s, int t) {
+    const int l = threadIdx.x & 63, g = l >> 5, dh = (l >> 4) & 1, i = l & 15;
+    const int c = 4 * t + 2 * dh + ((i & 3) >> 1);
+    typedef __attribute__((address_space(3))) s16x4* p_t;
+    s16x4 x[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int r = 8 * j + 4 * g + (i >> 2);     // of 16: the swizzle looks at no higher bit
+        x[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (p_t)(tile + (rb * 32 + 16 * s + r) * (DP * 2) + swz<DP>(r, c) * 16 + (i & 1) * 8));
+    }
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// B operand from memory: this lane's row, contraction over d in 16 ks .. + 15 of plane pl; zero where there is none.
+template <int DP>
+__device__ __forceinline__ bf16x8 mem_frag(const char* row, bool have, int chunks, int pl, int ks) {
+    const int c = 2 * ks + ((threadIdx.x >> 5) & 1);
+    if (have && c < chunks) return *reinterpret_cast<const bf16x8*>(row + (pl * (DP / 8) + c) * 16);
+    return __builtin_bit_cast(bf16x8, s16x8{0, 0, 0, 0, 0, 0, 0, 0});
+}
+
+// acc += A B, with NP planes of each.
+template <int NP>
+__device__ __forceinline__ f32x16 mma(const bf16x8 (&a)[NP], const bf16x8 (&b)[NP], f32x16 acc) {
+#pragma unroll
+    for (int o = NP - 1; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i <= o; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[o - i], acc, 0, 0, 0);
+    return acc;
+}
+
+// Registers 8 s .. 8 s + 7 of a result as the B operand of step s.  One plane rounds to nearest even (2^-9 of each
+// probability or score gradient, independent errors that average out over the sum); three keep 24 bits.
+template <int NP>
+__device__ __forceinline__ void to_operand(const f32x16& x, int s, bf16x8 (&o)[NP]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float r = x[8 * s + j];
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) {
+            const __bf16 h = (__bf16)r;
+            o[pl][j] = h;
+            r -= (float)h;
+        }
+    }
+}
+
+// Max / sum of a lane and the lane 32 away, in both.  (The swap's results are read as numbers first: __builtin_bit_cast of
+// a vector's element takes element 0 with this compiler.)
+__device__ __forceinline__ void half_swap(float v, float& x, float& y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const unsigned lo = r[0], hi = r[1];
+    x = __uint_as_float(lo);
+    y = __uint_as_float(hi);
+}
+__device__ __forceinline__ float half_max(float v) {
+    float x, y;
+    half_swap(v, x, y);
+    return fmaxf(x, y);
+}
+__device__ __forceinline__ float half_sum(float v) {
+    float x, y;
+    half_swap(v, x, y);
+    return x + y;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Tile row of register i of a result.
+__device__ __forceinline__ int reg_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (i & 3); }
+
+// Four neighbouring values of a row, d of D, stored in the row's type.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int d, int D, float x0, float x1, float x2, float x3) {
+    const float x[4] = {x0, x1, x2, x3};
+    if ((D & 3) == 0) {
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        if (d < D) *reinterpret_cast<v4*>(row + d) = v4{(T)x0, (T)x1, (T)x2, (T)x3};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (d + j < D) row[d + j] = (T)x[j];
+    }
+}
+
+// A workgroup's item: head (scene b, key head h), tile and split, heads fastest, so that with 8 heads or a multiple the
+// workgroups of a head share an XCD's L2 (workgroups go to the 8 XCDs in turn).
+struct Item {
+    int b, h, bh, tile, split;
+};
+__device__ __forceinline__ Item item_of(int id, int bhs, int hk, int tiles) {
+    Item w;
+    w.bh = id % bhs;
+    const int rest = id / bhs;
+    w.tile = rest % tiles;
+    w.split = rest / tiles;
+    w.b = w.bh / hk;
+    w.h = w.bh % hk;
+    return w;
+}
+
+// Units [lo, hi) of `all` that fall to a split.
+__device__ __forceinline__ void split_range(int all, int split, int splits, int& lo, int& hi) {
+    const int per = (all + splits - 1) / splits;
+    lo = split * per;
+    lo = lo < all ? lo : all;
+    hi = lo + per < all ? lo + per : all;
+}
+
+}  // namespace attn
+
+struct AttnFwd {
+    attn::RowSrc q, k, v;
+    const int* list;    // (batch, nk) valid keys first, or null
+    const int* count;   // (batch) valid keys
+    int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
+    float c;            // scale log2(e)
+    void* out;          // (batch, nq, hq, dim)
+    float* lse;         // (batch, hq, nq) log2 of the sum of 2^(c s); +inf for a row without keys
+    float* part_o;      // (splits, bhs, group nq, DP)
+    float* part_ml;     // (splits, bhs, group nq, 2)
+};
+
+struct AttnBwd {
+    attn::RowSrc q, k, v, g;
+    const int* list;
+    const int* count;
+    int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
+    int nqp;             // nq rounded up to 64: rows of lse and delta, padded with +inf and 0
+    float c, scale;
+    const float *lse, *delta;   // (batch, hq, nqp)
+    void *dq, *dk, *dv;
+    float* part;         // dq: (splits, bhs, group nq, DP); dk and dv: (splits, bhs, 2, nk, DP)
+};
+
+}  // namespace g2v

@@ -1,0 +1,483 @@
+// Attention over sets of Gaussians, backward, from the inputs, the row sums of the forward (lse) and dO:
+//
+//   P = 2^(c S - lse),  dP = dO V^T,  dS = P (dP - delta),  delta = sum_d dO O,
+//   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K.
+//
+// The probabilities are recomputed, twice: once by workgroups that own keys (dK, dV; the queries pass by) and once by
+// workgroups that own queries (dQ; the keys pass by).  That is seven products of the scores' size instead of five, and
+// nothing is added to memory that another workgroup adds to: gradients are the same on every run, and shared key heads are
+// summed over their query heads in registers.
+#include "g2v_attention.h"
+
+namespace g2v {
+namespace {
+using namespace attn;
+
+// dQ: rows in the lanes as in the forward, S^T = K Q^T and dP^T = V dO^T, dQ^T += K^T dS^T.
+template <int NP, int DP, int NQB, int NW, int KT, typename T>
+__global__ void __launch_bounds__(NW * 64) k_attn_dq(AttnBwd a) {
+    constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
+    typedef Tile<NP, DP, KT, NT> TileT;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
+    const int rows = a.group * a.nq;
+    const int r0 = (w.tile * NW + uniform(threadIdx.x >> 6)) * (NQB * 32) + (threadIdx.x & 31);
+    const int n = a.list ? a.count[w.b] : a.nk;
+    const int* list = a.list ? a.list + (int64_t)w.b * a.nk : nullptr;
+    const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
+    const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
+    int t0, t1;
+    split_range((n + KT - 1) / KT, w.split, a.splits, t0, t1);
+    if (n < 2) t1 = t0;    // one key: its probability is 1 whatever q is
+
+    bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
+    float lse[NQB], delta[NQB];
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
+        const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
+        const char* qrow = a.q.p + w.b * a.q.sb + tok * a.q.sn + head * a.q.sh;
+        const char* grow = a.g.p + w.b * a.g.sb + tok * a.g.sn + head * a.g.sh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl) {
+                q[b][ks][pl] = mem_frag<DP>(qrow, r < rows, a.q.chunks, pl, ks);
+                g[b][ks][pl] = mem_frag<DP>(grow, r < rows, a.g.chunks, pl, ks);
+            }
+        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
+        lse[b] = a.lse[at];
+        delta[b] = a.delta[at];
+    }
+
+    TileT tile;
+    tile.init(a.k);
+    if (a.k.chunks < TileT::C) clear_lds<NT>(&lds[0][0][0], sizeof(lds));
+    int idx[TileT::kIter];
+    auto fetch_index = [&](int t) {
+#pragma unroll
+        for (int it = 0; it < TileT::kIter; ++it) {
+            const int j = t * KT + tile.row[it];
+            idx[it] = j < n ? (list ? list[j] : j) : -1;
+        }
+    };
+    auto load = [&](int t, int buf) {
+        if (!list && (t + 1) * KT <= n) {
+            tile.load(kbase, a.k.sn, (int64_t)t * KT, lds_off(lds[buf][0]));
+            tile.load(vbase, a.v.sn, (int64_t)t * KT, lds_off(lds[buf][1]));
+        } else {
+            tile.load_indexed(kbase, a.k.sn, idx, lds[buf][0]);
+            tile.load_indexed(vbase, a.v.sn, idx, lds[buf][1]);
+        }
+    };
+
+    f32x16 dq[DB][NQB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < NQB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
+    if (t0 < t1) {
+        fetch_index(t0);
+        load(t0, 0);
+        fetch_index(t0 + 1);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        tile_barrier();
+        if (t + 1 < t1) {
+            load(t + 1, buf ^ 1);
+            fetch_index(t + 2);
+        }
+        const char* kt = lds[buf][0];
+        const char* vt = lds[buf][1];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            f32x16 s[NQB], dp[NQB];
+#pragma unroll
+            for (int b = 0; b < NQB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = dp[b][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 fk[NP], fv[NP];
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) {
+                    fk[pl] = row_frag<DP>(kt + pl * KT * DP * 2, kb, ks);
+                    fv[pl] = row_frag<DP>(vt + pl * KT * DP * 2, kb, ks);
+                }
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) {
+                    s[b] = mma<NP>(fk, q[b][ks], s[b]);
+                    dp[b] = mma<NP>(fv, g[b][ks], dp[b]);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NQB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[b][i] = exp2_fast(fmaf(s[b][i], a.c, -lse[b])) * (dp[b][i] - delta[b]);
+            if ((t + 1) * KT > n) {   // the last tile's rows past the end
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t * KT + kb * 32 + reg_row(i) >= n)
+#pragma unroll
+                        for (int b = 0; b < NQB; ++b) s[b][i] = 0.0f;
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                bf16x8 p[NQB][NP];
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) to_operand<NP>(s[b], st, p[b]);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    bf16x8 f[NP];
+#pragma unroll
+                    for (int pl = 0; pl < NP; ++pl) f[pl] = tr_frag<DP>(kt + pl * KT * DP * 2, kb, st, d);
+#pragma unroll
+                    for (int b = 0; b < NQB; ++b) dq[d][b] = mma<NP>(f, p[b], dq[d][b]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        const int r = r0 + 32 * b;
+        if (r >= rows) continue;
+        if (a.splits > 1) {
+            float* out = a.part + (((int64_t)w.split * a.bhs + w.bh) * rows + r) * DP;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4*>(out + 32 * d + reg_row(i)) =
+                        f32x4{dq[d][b][i], dq[d][b][i + 1], dq[d][b][i + 2], dq[d][b][i + 3]};
+            continue;
+        }
+        const int tok = r / a.group, head = w.h * a.group + r - tok * a.group;
+        T* row = static_cast<T*>(a.dq) + (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                store4<T>(row, 32 * d + reg_row(i), a.dim, dq[d][b][i] * a.scale, dq[d][b][i + 1] * a.scale,
+                          dq[d][b][i + 2] * a.scale, dq[d][b][i + 3] * a.scale);
+    }
+}
+
+// dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
+// dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
+template <int NP, int DP, int NKB, int NW, int QT, typename T>
+__global__ void __launch_bounds__(NW * 64) k_attn_dkv(AttnBwd a) {
+    constexpr int NT = NW * 64, QB = QT / 32, KS = DP / 16, DB = DP / 32;
+    typedef Tile<NP, DP, QT, NT> TileT;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][64];   // lse and delta of the tile's rows
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
+    const int wave = uniform(threadIdx.x >> 6);
+    const int j0 = (w.tile * NW + wave) * (NKB * 32) + (threadIdx.x & 31);
+    const int n = a.list ? a.count[w.b] : a.nk;
+    const int* list = a.list ? a.list + (int64_t)w.b * a.nk : nullptr;
+    const int per = (a.nq + QT - 1) / QT;     // tiles of a query head
+    int u0, u1;
+    split_range(per * a.group, w.split, a.splits, u0, u1);
+    if (w.tile * (NW * NKB * 32) >= n) u1 = u0;    // no valid key: nothing to add up
+
+    bf16x8 k[NKB][KS][NP], v[NKB][KS][NP];
+    int64_t key[NKB];
+#pragma unroll
+    for (int b = 0; b < NKB; ++b) {
+        const int j = j0 + 32 * b, jc = j < a.nk ? j : a.nk - 1;
+        key[b] = list ? list[jc] : jc;
+        const char* krow = a.k.p + w.b * a.k.sb + w.h * a.k.sh + key[b] * a.k.sn;
+        const char* vrow = a.v.p + w.b * a.v.sb + w.h * a.v.sh + key[b] * a.v.sn;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl) {
+                k[b][ks][pl] = mem_frag<DP>(krow, j < n, a.k.chunks, pl, ks);
+                v[b][ks][pl] = mem_frag<DP>(vrow, j < n, a.v.chunks, pl, ks);
+            }
+    }
+
+    TileT tile;
+    tile.init(a.q);
+    if (a.q.chunks < TileT::C) clear_lds<NT>(&lds[0][0][0], sizeof(lds));
+    auto load = [&](int u, int buf) {
+        const int hd = u / per, t = u - hd * per, head = w.h * a.group + hd;
+        const char* qbase = a.q.p + w.b * a.q.sb + head * a.q.sh;
+        const char* gbase = a.g.p + w.b * a.g.sb + head * a.g.sh;
+        if ((t + 1) * QT <= a.nq) {
+            tile.load(qbase, a.q.sn, (int64_t)t * QT, lds_off(lds[buf][0]));
+            tile.load(gbase, a.g.sn, (int64_t)t * QT, lds_off(lds[buf][1]));
+        } else {
+            int idx[TileT::kIter];
+#pragma unroll
+            for (int it = 0; it < TileT::kIter; ++it) {
+                const int r = t * QT + tile.row[it];
+                idx[it] = r < a.nq ? r : -1;
+            }
+            tile.load_indexed(qbase, a.q.sn, idx, lds[buf][0]);
+            tile.load_indexed(gbase, a.g.sn, idx, lds[buf][1]);
+        }
+        // rows past the end are there in the padded statistics: lse +inf makes their probabilities 0
+        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + t * QT;
+        const uint32_t lane = threadIdx.x & 63;
+        if (wave == 0 && lane < QT) dma4(a.lse + at, lane * 4, lds_off(stat[buf][0]));
+        if (wave == NW - 1 && lane < QT) dma4(a.delta + at, lane * 4, lds_off(stat[buf][1]));
+    };
+
+    f32x16 dk[DB][NKB], dv[DB][NKB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[d][b][i] = dv[d][b][i] = 0.0f;
+    if (u0 < u1) load(u0, 0);
+    for (int u = u0; u < u1; ++u) {
+        const int buf = (u - u0) & 1;
+        tile_barrier();
+        if (u + 1 < u1) load(u + 1, buf ^ 1);
+        const char* qt = lds[buf][0];
+        const char* gt = lds[buf][1];
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            f32x16 s[NKB], dp[NKB];
+#pragma unroll
+            for (int b = 0; b < NKB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = dp[b][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 fq[NP], fg[NP];
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) {
+                    fq[pl] = row_frag<DP>(qt + pl * QT * DP * 2, qb, ks);
+                    fg[pl] = row_frag<DP>(gt + pl * QT * DP * 2, qb, ks);
+                }
+#pragma unroll
+                for (int b = 0; b < NKB; ++b) {
+                    s[b] = mma<NP>(fq, k[b][ks], s[b]);
+                    dp[b] = mma<NP>(fg, v[b][ks], dp[b]);
+                }
+            }
+            const int g4 = 4 * ((threadIdx.x >> 5) & 1);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[buf][0][qb * 32 + 2 * i + g4]);
+                const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[buf][1][qb * 32 + 2 * i + g4]);
+#pragma unroll
+                for (int b = 0; b < NKB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[b][i + j] = exp2_fast(fmaf(s[b][i + j], a.c, -ls[j]));
+                        dp[b][i + j] = s[b][i + j] * (dp[b][i + j] - de[j]);
+                    }
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                bf16x8 p[NKB][NP], ds[NKB][NP];
+#pragma unroll
+                for (int b = 0; b < NKB; ++b) {
+                    to_operand<NP>(s[b], st, p[b]);
+                    to_operand<NP>(dp[b], st, ds[b]);
+                }
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    bf16x8 fg[NP], fq[NP];
+#pragma unroll
+                    for (int pl = 0; pl < NP; ++pl) {
+                        fg[pl] = tr_frag<DP>(gt + pl * QT * DP * 2, qb, st, d);
+                        fq[pl] = tr_frag<DP>(qt + pl * QT * DP * 2, qb, st, d);
+                    }
+#pragma unroll
+                    for (int b = 0; b < NKB; ++b) {
+                        dv[d][b] = mma<NP>(fg, p[b], dv[d][b]);
+                        dk[d][b] = mma<NP>(fq, ds[b], dk[d][b]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NKB; ++b) {
+        const int j = j0 + 32 * b;
+        if (j >= a.nk) continue;
+        if (a.splits > 1) {
+            if (j >= n) continue;   // k_attn_dkv_join writes zeros without looking
+            float* out = a.part + (((int64_t)w.split * a.bhs + w.bh) * a.nk + j) * (2 * DP);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    *reinterpret_cast<f32x4*>(out + 32 * d + reg_row(i)) =
+                        f32x4{dk[d][b][i], dk[d][b][i + 1], dk[d][b][i + 2], dk[d][b][i + 3]};
+                    *reinterpret_cast<f32x4*>(out + DP + 32 * d + reg_row(i)) =
+                        f32x4{dv[d][b][i], dv[d][b][i + 1], dv[d][b][i + 2], dv[d][b][i + 3]};
+                }
+            continue;
+        }
+        const bool valid = j < n;   // a masked key's gradients are zero, whatever its row holds
+        const int64_t at = (((int64_t)w.b * a.nk + key[b]) * a.hk + w.h) * a.dim;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                float x[4], y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = valid && n > 1 ? dk[d][b][i + e] * a.scale : 0.0f;   // one key: its probability is 1
+                    y[e] = valid ? dv[d][b][i + e] : 0.0f;
+                }
+                store4<T>(static_cast<T*>(a.dk) + at, 32 * d + reg_row(i), a.dim, x[0], x[1], x[2], x[3]);
+                store4<T>(static_cast<T*>(a.dv) + at, 32 * d + reg_row(i), a.dim, y[0], y[1], y[2], y[3]);
+            }
+    }
+}
+
+// Sums of the splits, in their order.
+template <int DP, typename T>
+__global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a) {
+    const int rows = a.group * a.nq;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.bhs * rows;
+    const int64_t at = e / (DP / 4);
+    const int d = (int)(e % (DP / 4)) * 4;
+    if (at >= all) return;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; ++s) o += *reinterpret_cast<const f32x4*>(a.part + (s * all + at) * DP + d);
+    const int bh = (int)(at / rows), r = (int)(at % rows);
+    const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
+    T* row = static_cast<T*>(a.dq) + (((int64_t)b * a.nq + tok) * a.hq + head) * a.dim;
+    store4<T>(row, d, a.dim, o[0] * a.scale, o[1] * a.scale, o[2] * a.scale, o[3] * a.scale);
+}
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.bhs * a.nk;
+    const int64_t at = e / (DP / 2);
+    const int d = (int)(e % (DP / 2)) * 4;    // dK, then dV
+    if (at >= all) return;
+    const int bh = (int)(at / a.nk), j = (int)(at % a.nk), b = bh / a.hk;
+    const int n = a.list ? a.count[b] : a.nk;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (j < n && (n > 1 || d >= DP))    // one key: its probability is 1 whatever k is
+        for (int s = 0; s < a.splits; ++s) o += *reinterpret_cast<const f32x4*>(a.part + (s * all + at) * (2 * DP) + d);
+    const int64_t key = a.list ? a.list[(int64_t)b * a.nk + j] : j;
+    const float f = d < DP ? a.scale : 1.0f;
+    T* row = static_cast<T*>(d < DP ? a.dk : a.dv) + (((int64_t)b * a.nk + key) * a.hk + bh % a.hk) * a.dim;
+    store4<T>(row, d < DP ? d : d - DP, a.dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+}
+
+// delta = sum_d dO O of a row and its lse, both padded to nqp rows of a head.  16 lanes a row.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nqp, int heads, int dim, const T* out, const T* g,
+                                                    int64_t gsb, int64_t gsn, int64_t gsh, const float* lse, float* lse_p,
+                                                    float* delta) {
+    const int64_t e = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (e >= rows) return;
+    const int sub = threadIdx.x & 15;
+    const int64_t bh = e / nqp;
+    const int i = (int)(e % nqp);
+    const int64_t b = bh / heads, h = bh % heads;
+    float v = 0.0f;
+    if (i < nq) {
+        const T* o = out + ((b * nq + i) * heads + h) * dim;
+        const T* r = g + b * gsb + i * gsn + h * gsh;
+        for (int d = sub; d < dim; d += 16) v = fmaf((float)o[d], (float)r[d], v);
+    }
+    for (int m = 8; m > 0; m >>= 1) v += __shfl_xor(v, m);
+    if (sub == 0) {
+        delta[e] = v;
+        lse_p[e] = i < nq ? lse[bh * nq + i] : INFINITY;
+    }
+}
+
+template <int NP, int DP, int NQB, int NW, int KT, typename T>
+hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
+    G2V_LAUNCH((k_attn_dq<NP, DP, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
+    if (a.splits > 1) {
+        const int64_t threads = (int64_t)a.bhs * a.group * a.nq * (DP / 4);
+        G2V_LAUNCH((k_attn_dq_join<DP, T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, a);
+    }
+    return hipGetLastError();
+}
+template <int NP, int DP, int NKB, int NW, int QT, typename T>
+hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
+    G2V_LAUNCH((k_attn_dkv<NP, DP, NKB, NW, QT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
+    if (a.splits > 1) {
+        const int64_t threads = (int64_t)a.bhs * a.nk * (DP / 2);
+        G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+AttnShape attn_dq_shape(bool f32, int dp) {
+    AttnShape g;
+    g.waves = 4;
+    g.blocks = !f32 && dp <= 64 ? 2 : 1;
+    g.tile = f32 && dp > 32 ? 32 : 64;
+    g.per_cu = f32 && dp > 32 ? 1 : 2;
+    return g;
+}
+AttnShape attn_dkv_shape(bool f32, int dp) {
+    AttnShape g;
+    g.waves = 4;
+    g.blocks = 1;
+    g.tile = f32 && dp > 32 ? 32 : 64;
+    g.per_cu = (f32 && dp > 32) || dp > 96 ? 1 : 2;
+    return g;
+}
+
+hipError_t launch_attn_dq(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
+    if (f32) {
+        switch (dp) {
+            case 32: return dq_launch<3, 32, 1, 4, 64, float>(a, s);
+            case 64: return dq_launch<3, 64, 1, 4, 32, float>(a, s);
+            case 96: return dq_launch<3, 96, 1, 4, 32, float>(a, s);
+            default: return dq_launch<3, 128, 1, 4, 32, float>(a, s);
+        }
+    }
+    switch (dp) {
+        case 32: return dq_launch<1, 32, 2, 4, 64, __bf16>(a, s);
+        case 64: return dq_launch<1, 64, 2, 4, 64, __bf16>(a, s);
+        case 96: return dq_launch<1, 96, 1, 4, 64, __bf16>(a, s);
+        default: return dq_launch<1, 128, 1, 4, 64, __bf16>(a, s);
+    }
+}
+
+hipError_t launch_attn_dkv(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
+    if (f32) {
+        switch (dp) {
+            case 32: return dkv_launch<3, 32, 1, 4, 64, float>(a, s);
+            case 64: return dkv_launch<3, 64, 1, 4, 32, float>(a, s);
+            case 96: return dkv_launch<3, 96, 1, 4, 32, float>(a, s);
+            default: return dkv_launch<3, 128, 1, 4, 32, float>(a, s);
+        }
+    }
+    switch (dp) {
+        case 32: return dkv_launch<1, 32, 1, 4, 64, __bf16>(a, s);
+        case 64: return dkv_launch<1, 64, 1, 4, 64, __bf16>(a, s);
+        case 96: return dkv_launch<1, 96, 1, 4, 64, __bf16>(a, s);
+        default: return dkv_launch<1, 128, 1, 4, 64, __bf16>(a, s);
+    }
+}
+
+hipError_t launch_attn_delta(int batch, int nq, int nqp, int heads, int dim, const void* out, const void* g, int64_t gsb,
+                             int64_t gsn, int64_t gsh, bool f32, const float* lse, float* lse_p, float* delta, hipStream_t s) {
+    const int64_t rows = (int64_t)batch * heads * nqp;
+    if (rows == 0) return hipSuccess;
+    const dim3 grid((unsigned)ceil_div(rows, 16));
+    if (f32)
+        G2V_LAUNCH((k_attn_delta<float>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, static_cast<const float*>(out),
+                   static_cast<const float*>(g), gsb, gsn, gsh, lse, lse_p, delta);
+    else
+        G2V_LAUNCH((k_attn_delta<__bf16>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, static_cast<const __bf16*>(out),
+                   static_cast<const __bf16*>(g), gsb, gsn, gsh, lse, lse_p, delta);
+    return hipGetLastError();
+}
+
+}  // namespace g2v

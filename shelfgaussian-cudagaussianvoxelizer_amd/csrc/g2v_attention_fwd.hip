@@ -1,0 +1,342 @@
+// Attention over sets of Gaussians, forward: O = softmax(scale Q K^T) V over the valid keys of each scene.
+//
+// One pass over the keys with the running maximum and sum of the softmax.  The query heads that share a key head are rows
+// of one problem (row r = query r / group, head r % group), so K and V are read once for all of them.  A wave owns NQB
+// blocks of 32 rows: their Q stays in registers as B operands, K and V tiles come through LDS (direct loads, two tiles
+// deep), S^T = K Q^T lands with a lane per row and goes through exp2 straight into O^T += V^T P^T (no exchange of P).
+// Few rows: the keys are dealt to `splits` workgroups and k_attn_join joins them.
+#include "g2v_attention.h"
+
+namespace g2v {
+namespace {
+using namespace attn;
+
+constexpr float kLazy = 8.0f;   // the maximum in use may trail the true one by a factor of 2^8
+
+template <int NP, int DP, int NQB, int NW, int KT, typename T>
+__global__ void __launch_bounds__(NW * 64) k_attn_fwd(AttnFwd a) {
+    constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
+    typedef Tile<NP, DP, KT, NT> TileT;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
+    const int lane = threadIdx.x & 63, rows = a.group * a.nq;
+    const int r0 = (w.tile * NW + uniform(threadIdx.x >> 6)) * (NQB * 32) + (lane & 31);
+    const int n = a.list ? a.count[w.b] : a.nk;
+    const int* list = a.list ? a.list + (int64_t)w.b * a.nk : nullptr;
+    const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
+    const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
+    int t0, t1;
+    split_range((n + KT - 1) / KT, w.split, a.splits, t0, t1);
+
+    bf16x8 q[NQB][KS][NP];
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
+        const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
+        const char* row = a.q.p + w.b * a.q.sb + tok * a.q.sn + head * a.q.sh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl) q[b][ks][pl] = mem_frag<DP>(row, r < rows, a.q.chunks, pl, ks);
+    }
+
+    TileT tile;
+    tile.init(a.k);
+    if (a.k.chunks < TileT::C) clear_lds<NT>(&lds[0][0][0], sizeof(lds));
+    int idx[TileT::kIter];
+    auto fetch_index = [&](int t) {
+#pragma unroll
+        for (int it = 0; it < TileT::kIter; ++it) {
+            const int j = t * KT + tile.row[it];
+            idx[it] = j < n ? (list ? list[j] : j) : -1;
+        }
+    };
+    auto load = [&](int t, int buf) {
+        if (!list && (t + 1) * KT <= n) {
+            tile.load(kbase, a.k.sn, (int64_t)t * KT, lds_off(lds[buf][0]));
+            tile.load(vbase, a.v.sn, (int64_t)t * KT, lds_off(lds[buf][1]));
+        } else {
+            tile.load_indexed(kbase, a.k.sn, idx, lds[buf][0]);
+            tile.load_indexed(vbase, a.v.sn, idx, lds[buf][1]);
+        }
+    };
+
+    f32x16 o[DB][NQB];
+    float m[NQB], limit[NQB], l[NQB];
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        m[b] = limit[b] = -INFINITY;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][b][i] = 0.0f;
+    }
+    if (t0 < t1) {
+        fetch_index(t0);
+        load(t0, 0);
+        fetch_index(t0 + 1);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        tile_barrier();
+        if (t + 1 < t1) {
+            load(t + 1, buf ^ 1);
+            fetch_index(t + 2);
+        }
+        const char* kt = lds[buf][0];
+        const char* vt = lds[buf][1];
+        f32x16 s[KB][NQB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int b = 0; b < NQB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][b][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 f[NP];
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) f[pl] = row_frag<DP>(kt + pl * KT * DP * 2, kb, ks);
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) s[kb][b] = mma<NP>(f, q[b][ks], s[kb][b]);
+            }
+        }
+        if ((t + 1) * KT > n) {   // the last tile's rows past the end
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t * KT + kb * 32 + reg_row(i) >= n)
+#pragma unroll
+                        for (int b = 0; b < NQB; ++b) s[kb][b][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int b = 0; b < NQB; ++b) {
+            float top = s[0][b][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][b][i]);
+            top = half_max(top);
+            if (__any(top > limit[b])) {   // rarely, after the first tiles
+                const float up = fmaxf(m[b], top);
+                const float f = m[b] == up ? 1.0f : exp2_fast((m[b] - up) * a.c);
+                m[b] = up;
+                limit[b] = up + kLazy / a.c;
+                l[b] *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][b][i] *= f;
+            }
+            const float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;
+            float sum = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[kb][b][i] = exp2_fast(fmaf(s[kb][b][i], a.c, -mc));
+                    sum += s[kb][b][i];
+                }
+            l[b] += sum;
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                bf16x8 p[NQB][NP];
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) to_operand<NP>(s[kb][b], st, p[b]);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    bf16x8 f[NP];
+#pragma unroll
+                    for (int pl = 0; pl < NP; ++pl) f[pl] = tr_frag<DP>(vt + pl * KT * DP * 2, kb, st, d);
+#pragma unroll
+                    for (int b = 0; b < NQB; ++b) o[d][b] = mma<NP>(f, p[b], o[d][b]);
+                }
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        const int r = r0 + 32 * b;
+        const float total = half_sum(l[b]);
+        if (r >= rows) continue;
+        if (a.splits > 1) {
+            const int64_t at = ((int64_t)w.split * a.bhs + w.bh) * rows + r;
+            if (lane < 32) {
+                a.part_ml[2 * at] = m[b] * a.c;
+                a.part_ml[2 * at + 1] = total;
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4*>(a.part_o + at * DP + 32 * d + reg_row(i)) =
+                        f32x4{o[d][b][i], o[d][b][i + 1], o[d][b][i + 2], o[d][b][i + 3]};
+            continue;
+        }
+        const int tok = r / a.group, head = w.h * a.group + r - tok * a.group;
+        const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+        if (a.lse && lane < 32)
+            a.lse[((int64_t)w.b * a.hq + head) * a.nq + tok] = total > 0.0f ? fmaf(m[b], a.c, log2f(total)) : INFINITY;
+        T* row = static_cast<T*>(a.out) + (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                store4<T>(row, 32 * d + reg_row(i), a.dim, o[d][b][i] * inv, o[d][b][i + 1] * inv, o[d][b][i + 2] * inv,
+                          o[d][b][i + 3] * inv);
+    }
+}
+
+// Joins the splits of a row: O = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M).  DP / 4 lanes a row.
+template <int DP, typename T>
+__global__ void __launch_bounds__(256) k_attn_join(AttnFwd a) {
+    const int rows = a.group * a.nq;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.bhs * rows;
+    const int64_t at = e / (DP / 4);
+    const int d = (int)(e % (DP / 4)) * 4;
+    if (at >= all) return;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * all + at)]);
+    float total = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t p = s * all + at;
+        const float l = a.part_ml[2 * p + 1];
+        if (l == 0.0f) continue;   // a split without keys (its maximum is the lowest value)
+        const float f = exp2_fast(a.part_ml[2 * p] - top);
+        total = fmaf(l, f, total);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + p * DP + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], f, o[j]);
+    }
+    const int bh = (int)(at / rows), r = (int)(at % rows);
+    const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
+    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+    if (a.lse && d == 0) a.lse[((int64_t)b * a.hq + head) * a.nq + tok] = total > 0.0f ? top + log2f(total) : INFINITY;
+    T* row = static_cast<T*>(a.out) + (((int64_t)b * a.nq + tok) * a.hq + head) * a.dim;
+    store4<T>(row, d, a.dim, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+}
+
+// ---- what both directions prepare -----------------------------------------------------------------------------------
+
+constexpr int kListThreads = 1024;
+
+// Valid keys of a scene in ascending order, then the others; their number in count.  One workgroup a scene.
+__global__ void __launch_bounds__(kListThreads) k_attn_list(int nk, const unsigned char* mask, int* list, int* count) {
+    __shared__ int sums[kListThreads / 64];
+    const unsigned char* mk = mask + (int64_t)blockIdx.x * nk;
+    int* out = list + (int64_t)blockIdx.x * nk;
+    const int per = (nk + kListThreads - 1) / kListThreads;
+    const int lo = min((int)threadIdx.x * per, nk), hi = min(lo + per, nk);
+    int mine = 0;
+    for (int j = lo; j < hi; ++j) mine += mk[j] != 0;
+    int scan = mine;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int v = __shfl_up(scan, d);
+        if (lane >= d) scan += v;
+    }
+    if (lane == 63) sums[wave] = scan;
+    __syncthreads();
+    int before = 0, total = 0;
+    for (int i = 0; i < kListThreads / 64; ++i) {
+        if (i < wave) before += sums[i];
+        total += sums[i];
+    }
+    int at = before + scan - mine;              // valid keys before lo
+    int other = total + lo - at;                // the others before lo come after all valid ones
+    for (int j = lo; j < hi; ++j) {
+        if (mk[j]) out[at++] = j;
+        else out[other++] = j;
+    }
+    if (threadIdx.x == 0) count[blockIdx.x] = total;
+}
+
+// Rows of one tensor as NP bfloat16 planes of DP values each, contiguous (batch, heads, n): what the kernels cannot read
+// in place (float32, and rows that are not whole 16-byte chunks).  A thread writes one chunk of every plane.
+template <int NP, typename T>
+__global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
+    const int C = a.dp / 8;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int64_t row = e / C;
+    const int c = (int)(e % C);
+    int k = 0;
+    while (k < a.tensors && row >= a.rows[k]) row -= a.rows[k++];
+    if (k >= a.tensors) return;
+    const int64_t bh = row / a.n[k], i = row % a.n[k];
+    const T* src = static_cast<const T*>(a.src[k]) + bh / a.heads[k] * a.sb[k] + i * a.sn[k] + bh % a.heads[k] * a.sh[k];
+    bf16x8 o[NP];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float r = c * 8 + j < a.dim ? (float)src[c * 8 + j] : 0.0f;
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) {
+            const __bf16 h = (__bf16)r;
+            o[pl][j] = h;
+            r = __builtin_isfinite((float)h) ? r - (float)h : 0.0f;   // an infinity is its first plane alone
+        }
+    }
+#pragma unroll
+    for (int pl = 0; pl < NP; ++pl)
+        *reinterpret_cast<bf16x8*>(static_cast<char*>(a.dst[k]) + ((row * NP + pl) * C + c) * 16) = o[pl];
+}
+
+template <int NP, int DP, int NQB, int NW, int KT, typename T>
+hipError_t fwd_launch(const AttnFwd& a, hipStream_t s) {
+    G2V_LAUNCH((k_attn_fwd<NP, DP, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
+    if (a.splits > 1) {
+        const int64_t threads = (int64_t)a.bhs * a.group * a.nq * (DP / 4);
+        G2V_LAUNCH((k_attn_join<DP, T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows) {
+    (void)rows;
+    AttnShape g;
+    g.waves = 4;
+    g.blocks = !f32 && dp <= 64 ? 2 : 1;
+    g.tile = f32 && dp > 32 ? 32 : 64;
+    g.per_cu = f32 && dp > 64 ? 1 : 2;
+    return g;
+}
+
+hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s) {
+    if (f32) {
+        switch (dp) {
+            case 32: return fwd_launch<3, 32, 1, 4, 64, float>(a, s);
+            case 64: return fwd_launch<3, 64, 1, 4, 32, float>(a, s);
+            case 96: return fwd_launch<3, 96, 1, 4, 32, float>(a, s);
+            default: return fwd_launch<3, 128, 1, 4, 32, float>(a, s);
+        }
+    }
+    switch (dp) {
+        case 32: return fwd_launch<1, 32, 2, 4, 64, __bf16>(a, s);
+        case 64: return fwd_launch<1, 64, 2, 4, 64, __bf16>(a, s);
+        case 96: return fwd_launch<1, 96, 1, 4, 64, __bf16>(a, s);
+        default: return fwd_launch<1, 128, 1, 4, 64, __bf16>(a, s);
+    }
+}
+
+hipError_t launch_attn_list(int batch, int nk, const unsigned char* mask, int* list, int* count, hipStream_t s) {
+    if (batch > 0) G2V_LAUNCH(k_attn_list, dim3(batch), dim3(kListThreads), 0, s, nk, mask, list, count);
+    return hipGetLastError();
+}
+
+hipError_t launch_attn_pack(const AttnPack& a, bool f32, hipStream_t s) {
+    int64_t rows = 0;
+    for (int k = 0; k < a.tensors; ++k) rows += a.rows[k];
+    if (rows == 0) return hipSuccess;
+    const dim3 grid((unsigned)ceil_div(rows * (a.dp / 8), 256));
+    if (f32) G2V_LAUNCH((k_attn_pack<3, float>), grid, dim3(256), 0, s, a);
+    else G2V_LAUNCH((k_attn_pack<1, __bf16>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace g2v

@@ -2,9 +2,10 @@
 // the query/key norms with rotary positions and of the attention.
 #include <limits.h>
 #include <math.h>
+#include <algorithm>
 
 #include "../../include/g2v.h"
-#include "g2v_internal.h"
+#include "g2v_attention.h"
 
 using namespace g2v;
 
@@ -75,7 +76,334 @@ int qn_fill(QkNormArgs& a, const void* q, const long long* qs, const void* k, co
     return G2V_OK;
 }
 
+// ---- attention --------------------------------------------------------------------------------
+
+constexpr int kCus = 256;
+
+// Into how many workgroups the long axis (`units` tiles) of each of `wgs` workgroups goes.  unit_us: time of a tile in a
+// workgroup that shares its CU with another; join_us: writing and adding one split's partial results.  A CU runs
+// its workgroups two at a time; one without a partner takes about 0.65 of the time of two.
+int attn_splits(int64_t wgs, int units, double unit_us, double join_us) {
+    auto cost = [&](int s) {
+        const int64_t n = ceil_div(wgs * s, kCus);
+        const double us = (0.5 * n + 0.15 * (n & 1)) * (ceil_div(units, s) + 2) * unit_us;
+        return s == 1 ? us : us + 5.0 + s * join_us;
+    };
+    int best = 1;
+    for (int s = 2; s <= 64 && s <= units; ++s)
+        if (cost(s) < cost(best)) best = s;
+    return best;
+}
+
+struct AttnSizes {
+    int batch, nq, nk, hq, hk, dim, dp, group, bhs;
+    bool f32;
+    int64_t rows() const { return (int64_t)group * nq; }
+};
+
+int attn_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype, AttnSizes& z) {
+    if (batch < 0 || n_q < 0 || n_k < 0) return api_fail(G2V_ERR_INVALID, "negative size: batch %d, n %d / %d", batch, n_q, n_k);
+    if (heads_q < 1 || heads_k < 1 || heads_q % heads_k)
+        return api_fail(G2V_ERR_INVALID, "heads_q = %d is not a multiple of heads_k = %d", heads_q, heads_k);
+    if (head_dim < 1 || head_dim > 128) return api_fail(G2V_ERR_INVALID, "head_dim = %d (1 to 128)", head_dim);
+    if (dtype != G2V_DTYPE_F32 && dtype != G2V_DTYPE_BF16)
+        return api_fail(G2V_ERR_INVALID, "dtype = %d (G2V_DTYPE_F32 or G2V_DTYPE_BF16)", dtype);
+    z.batch = batch;
+    z.nq = n_q;
+    z.nk = n_k;
+    z.hq = heads_q;
+    z.hk = heads_k;
+    z.dim = head_dim;
+    z.dp = attn_dp(head_dim);
+    z.group = heads_q / heads_k;
+    z.f32 = dtype == G2V_DTYPE_F32;
+    // rows of a key head and workgroups are counted in 32 bits
+    if ((double)heads_q / heads_k * n_q > 1e9 || n_k > 1000000000 || (double)batch * heads_q > 65535.0 ||
+        (double)batch * n_k > 2e9)
+        return api_fail(G2V_ERR_LIMIT, "batch %d x heads %d (limit 65535), rows %d x %d and keys %d (limit 1e9)", batch, heads_q,
+                        n_q, z.group, n_k);
+    z.bhs = batch * heads_k;
+    return G2V_OK;
+}
+
+struct AttnRun {
+    AttnShape shape;
+    int tiles, splits;
+};
+// Tiles of `mine` rows and splits of the `passing` rows (in `streams` runs that end inside a tile each); products: of
+// the scores' size that the kernel takes; width: values of a row's partial result.
+AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing, int streams, int products, int width) {
+    AttnRun r;
+    r.shape = g;
+    const int own = g.waves * g.blocks * 32;
+    r.tiles = (int)ceil_div(mine, own);
+    const int64_t units = ceil_div(passing, g.tile) * streams;
+    const double flops = 2.0 * products * own * g.tile * z.dp;
+    const double unit_us = std::max(1.0, flops * 2.0 / ((z.f32 ? 0.12e9 : 0.7e9) / kCus));
+    const double join_us = 8.0 * mine * z.bhs * width / 3e6;
+    r.splits = attn_splits((int64_t)z.bhs * r.tiles, (int)std::min<int64_t>(units, 1 << 30), unit_us, join_us);
+    return r;
+}
+
+struct Strided {
+    const void* p;
+    const long long* s;
+    int n, heads;
+};
+
+// bfloat16 rows of whole 16-byte chunks at 16-byte boundaries are read where they are.
+bool attn_in_place(const AttnSizes& z, const Strided* t, int count) {
+    if (z.f32 || z.dim % 8) return false;
+    for (int i = 0; i < count; ++i) {
+        if (reinterpret_cast<uintptr_t>(t[i].p) % 16) return false;
+        for (int k = 0; k < 3; ++k)
+            if (t[i].s[k] % 8) return false;
+        if (t[i].s[1] < 0 || t[i].s[1] >= (1 << 24)) return false;   // a tile's rows within 32-bit offsets
+    }
+    return true;
+}
+
+size_t attn_packed_bytes(const AttnSizes& z, int64_t n, int heads) {
+    return (size_t)z.batch * heads * n * (z.f32 ? 3 : 1) * z.dp * 2;
+}
+
+// The tensors as the kernels read them; what cannot be read in place is packed into c's space.
+hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool packed, Carver& c, attn::RowSrc* out,
+                        hipStream_t s) {
+    AttnPack a = {};
+    a.tensors = count;
+    a.dim = z.dim;
+    a.dp = z.dp;
+    for (int i = 0; i < count; ++i) {
+        if (!packed) {
+            out[i] = {static_cast<const char*>(t[i].p), t[i].s[0] * 2, t[i].s[1] * 2, t[i].s[2] * 2, z.dim / 8};
+            continue;
+        }
+        const int64_t row = (int64_t)(z.f32 ? 3 : 1) * z.dp * 2;
+        char* dst = c.take<char>(attn_packed_bytes(z, t[i].n, t[i].heads));
+        a.src[i] = t[i].p;
+        a.sb[i] = t[i].s[0];
+        a.sn[i] = t[i].s[1];
+        a.sh[i] = t[i].s[2];
+        a.n[i] = t[i].n;
+        a.heads[i] = t[i].heads;
+        a.rows[i] = (int64_t)z.batch * t[i].heads * t[i].n;
+        a.dst[i] = dst;
+        out[i] = {dst, row * t[i].n * t[i].heads, row, row * t[i].n, z.dp / 8};
+    }
+    return packed ? launch_attn_pack(a, z.f32, s) : hipSuccess;
+}
+
+AttnRun attn_fwd_run(const AttnSizes& z) {
+    return attn_run(z, attn_fwd_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 2, z.dp);
+}
+AttnRun attn_dq_run(const AttnSizes& z) { return attn_run(z, attn_dq_shape(z.f32, z.dp), z.rows(), z.nk, 1, 3, z.dp); }
+AttnRun attn_dkv_run(const AttnSizes& z) {
+    return attn_run(z, attn_dkv_shape(z.f32, z.dp), z.nk, z.nq, z.group, 4, 2 * z.dp);
+}
+
+struct AttnFwdWs {
+    float *part_o, *part_ml;
+};
+AttnFwdWs carve_attn_fwd(Carver& c, const AttnSizes& z, const AttnRun& r) {
+    AttnFwdWs w = {nullptr, nullptr};
+    if (r.splits > 1) {
+        const size_t rows = (size_t)r.splits * z.bhs * z.rows();
+        w.part_o = c.take<float>(rows * z.dp);
+        w.part_ml = c.take<float>(rows * 2);
+    }
+    return w;
+}
+void carve_packed(Carver& c, const AttnSizes& z, bool backward) {
+    c.take<char>(attn_packed_bytes(z, z.nq, z.hq));
+    c.take<char>(attn_packed_bytes(z, z.nk, z.hk));
+    c.take<char>(attn_packed_bytes(z, z.nk, z.hk));
+    if (backward) c.take<char>(attn_packed_bytes(z, z.nq, z.hq));
+}
+struct AttnBwdWs {
+    int nqp;
+    float *lse, *delta, *part;
+};
+AttnBwdWs carve_attn_bwd(Carver& c, const AttnSizes& z, const AttnRun& dq, const AttnRun& dkv) {
+    AttnBwdWs w;
+    w.nqp = (int)((z.nq + 63) / 64 * 64);
+    w.lse = c.take<float>((size_t)z.batch * z.hq * w.nqp);
+    w.delta = c.take<float>((size_t)z.batch * z.hq * w.nqp);
+    // one area: the two kernels run one after the other
+    size_t part = 0;
+    if (dq.splits > 1) part = (size_t)dq.splits * z.bhs * z.rows() * z.dp;
+    if (dkv.splits > 1) part = std::max(part, (size_t)dkv.splits * z.bhs * z.nk * 2 * z.dp);
+    w.part = part ? c.take<float>(part) : nullptr;
+    return w;
+}
+
+size_t attn_fwd_bytes(const AttnSizes& z, bool packed) {
+    Carver c(nullptr, (size_t)-1);
+    carve_attn_fwd(c, z, attn_fwd_run(z));
+    if (packed) carve_packed(c, z, false);
+    return c.off + 256;
+}
+size_t attn_bwd_bytes(const AttnSizes& z, bool packed) {
+    Carver c(nullptr, (size_t)-1);
+    carve_attn_bwd(c, z, attn_dq_run(z), attn_dkv_run(z));
+    if (packed) carve_packed(c, z, true);
+    return c.off + 256;
+}
+
+int attn_scale(float scale) {
+    if (!(scale > 0.0f) || !isfinite(scale * attn::kLog2e))
+        return api_fail(G2V_ERR_INVALID, "scale = %g (positive and finite)", (double)scale);
+    return G2V_OK;
+}
+
 }  // namespace
+
+extern "C" {
+
+size_t g2v_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                       int in_place) {
+    AttnSizes z;
+    if (attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z) != G2V_OK) return 0;
+    return attn_fwd_bytes(z, z.f32 || !in_place);
+}
+
+int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                          const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                          const long long v_strides[3], int dtype, const unsigned char* key_mask, float scale, void* out,
+                          float* lse, int* key_list, void* workspace, size_t workspace_bytes, void* stream) {
+    api_begin();
+    AttnSizes z;
+    int rc = attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z);
+    if (rc != G2V_OK) return rc;
+    rc = attn_scale(scale);
+    if (rc != G2V_OK) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool keys = (int64_t)batch * n_k > 0;
+    if (keys && key_mask) {   // also without queries: the backward writes the keys' gradients by this list
+        if (!key_list) return api_fail(G2V_ERR_INVALID, "key_mask without key_list");
+        G2V_HIP(launch_attn_list(batch, n_k, key_mask, key_list, key_list + (int64_t)batch * n_k, s));
+    }
+    if ((int64_t)batch * n_q == 0) return G2V_OK;
+    if (!out || !q || !q_strides || (keys && (!k || !v || !k_strides || !v_strides)))
+        return api_fail(G2V_ERR_INVALID, "null q, k, v, strides or out");
+    static const long long none[3] = {0, 0, 0};
+    const Strided t[3] = {{q, q_strides, n_q, heads_q}, {k, keys ? k_strides : none, n_k, heads_k}, {v, keys ? v_strides : none, n_k, heads_k}};
+    const bool packed = !attn_in_place(z, t, 3);
+    const size_t need = attn_fwd_bytes(z, packed);
+    if (!workspace || workspace_bytes < need)
+        return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
+    const AttnRun r = attn_fwd_run(z);
+    Carver c(workspace, workspace_bytes);
+    const AttnFwdWs w = carve_attn_fwd(c, z, r);
+    attn::RowSrc src[3];
+    G2V_HIP(attn_sources(z, t, 3, packed, c, src, s));
+    AttnFwd a = {};
+    a.q = src[0];
+    a.k = src[1];
+    a.v = src[2];
+    if (keys && key_mask) {
+        a.list = key_list;
+        a.count = key_list + (int64_t)batch * n_k;
+    }
+    a.nq = n_q;
+    a.nk = n_k;
+    a.hq = heads_q;
+    a.hk = heads_k;
+    a.group = z.group;
+    a.dim = head_dim;
+    a.bhs = z.bhs;
+    a.tiles = r.tiles;
+    a.splits = r.splits;
+    a.c = scale * attn::kLog2e;
+    a.out = out;
+    a.lse = lse;
+    a.part_o = w.part_o;
+    a.part_ml = w.part_ml;
+    G2V_HIP(launch_attn_fwd(a, z.f32, z.dp, s));
+    return G2V_OK;
+}
+
+size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                        int in_place) {
+    AttnSizes z;
+    if (attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z) != G2V_OK) return 0;
+    return attn_bwd_bytes(z, z.f32 || !in_place);
+}
+
+int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                           const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                           const long long v_strides[3], int dtype, const int* key_list, float scale, const void* out,
+                           const float* lse, const void* grad_out, const long long grad_out_strides[3], void* grad_q,
+                           void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
+    api_begin();
+    AttnSizes z;
+    int rc = attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z);
+    if (rc != G2V_OK) return rc;
+    rc = attn_scale(scale);
+    if (rc != G2V_OK) return rc;
+    const bool queries = (int64_t)batch * n_q > 0, keys = (int64_t)batch * n_k > 0;
+    if (!queries && !keys) return G2V_OK;
+    if ((grad_k == nullptr) != (grad_v == nullptr)) return api_fail(G2V_ERR_INVALID, "grad_k and grad_v go together");
+    if ((queries && (!q || !q_strides || !out || !lse || !grad_out || !grad_out_strides)) ||
+        (keys && (!k || !v || !k_strides || !v_strides)))
+        return api_fail(G2V_ERR_INVALID, "null q, k, v, out, lse, grad_out or strides");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    static const long long none[3] = {0, 0, 0};
+    const long long* sq = queries ? q_strides : none;
+    const long long* sg = queries ? grad_out_strides : none;
+    const long long* sk = keys ? k_strides : none;
+    const long long* sv = keys ? v_strides : none;
+    const Strided t[4] = {{q, sq, n_q, heads_q}, {k, sk, n_k, heads_k}, {v, sv, n_k, heads_k}, {grad_out, sg, n_q, heads_q}};
+    const bool packed = !attn_in_place(z, t, 4);
+    const size_t need = attn_bwd_bytes(z, packed);
+    if (!workspace || workspace_bytes < need)
+        return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
+    const AttnRun rq = attn_dq_run(z), rk = attn_dkv_run(z);
+    Carver c(workspace, workspace_bytes);
+    const AttnBwdWs w = carve_attn_bwd(c, z, rq, rk);
+    attn::RowSrc src[4];
+    G2V_HIP(attn_sources(z, t, 4, packed, c, src, s));
+    G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
+                              w.delta, s));
+    AttnBwd a = {};
+    a.q = src[0];
+    a.k = src[1];
+    a.v = src[2];
+    a.g = src[3];
+    if (keys && key_list) {
+        a.list = key_list;
+        a.count = key_list + (int64_t)batch * n_k;
+    }
+    a.nq = n_q;
+    a.nk = n_k;
+    a.hq = heads_q;
+    a.hk = heads_k;
+    a.group = z.group;
+    a.dim = head_dim;
+    a.bhs = z.bhs;
+    a.nqp = w.nqp;
+    a.c = scale * attn::kLog2e;
+    a.scale = scale;
+    a.lse = w.lse;
+    a.delta = w.delta;
+    a.dq = grad_q;
+    a.dk = grad_k;
+    a.dv = grad_v;
+    a.part = w.part;
+    if (grad_k && keys) {
+        a.tiles = rk.tiles;
+        a.splits = rk.splits;
+        G2V_HIP(launch_attn_dkv(a, z.f32, z.dp, s));
+    }
+    if (grad_q && queries) {
+        a.tiles = rq.tiles;
+        a.splits = rq.splits;
+        G2V_HIP(launch_attn_dq(a, z.f32, z.dp, s));
+    }
+    return G2V_OK;
+}
+
+}  // extern "C"
 
 extern "C" {
 

@@ -268,6 +268,35 @@ hipError_t launch_qk_norm_rotary(const QkNormArgs& a, int dtype, hipStream_t s);
 size_t qk_norm_bwd_workspace(const QkNormArgs& a, int dtype);
 hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& a, int dtype, void* ws, hipStream_t s);
 
+// ---- attention (g2v_attention_fwd.hip, g2v_attention_bwd.hip) -------------------------------
+struct AttnFwd;
+struct AttnBwd;
+// Up to four tensors (batch, n, heads, dim) at element strides sb, sn, sh, packed as bfloat16 planes of dp values.
+struct AttnPack {
+    int tensors, dim, dp;
+    const void* src[4];
+    int64_t sb[4], sn[4], sh[4];
+    int n[4], heads[4];
+    int64_t rows[4];   // batch heads n
+    void* dst[4];
+};
+// A kernel's workgroup: waves, blocks of 32 rows of a wave, rows of a tile of the long axis, workgroups that fit a CU.
+struct AttnShape {
+    int waves, blocks, tile, per_cu;
+};
+inline int attn_dp(int dim) { return (dim + 31) / 32 * 32; }
+AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows);
+AttnShape attn_dq_shape(bool f32, int dp);
+AttnShape attn_dkv_shape(bool f32, int dp);
+hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s);
+hipError_t launch_attn_list(int batch, int nk, const unsigned char* mask, int* list, int* count, hipStream_t s);
+hipError_t launch_attn_pack(const AttnPack& a, bool f32, hipStream_t s);
+// lse and delta = sum_d g out of every row, padded to nqp rows of a head (+inf and 0).
+hipError_t launch_attn_delta(int batch, int nq, int nqp, int heads, int dim, const void* out, const void* g, int64_t gsb,
+                             int64_t gsn, int64_t gsh, bool f32, const float* lse, float* lse_p, float* delta, hipStream_t s);
+hipError_t launch_attn_dq(const AttnBwd& a, bool f32, int dp, hipStream_t s);
+hipError_t launch_attn_dkv(const AttnBwd& a, bool f32, int dp, hipStream_t s);
+
 // Brackets one kernel launch with HIP events when profiling is enabled (g2v_profile.hip).
 class ProfMark {
   public:

@@ -1,0 +1,277 @@
+"""GPU parity of gaussian_attention (g2v_attention_*) against a plain float64 statement of the formula, whose gradients are
+the formula's, and against differences of that statement.
+
+Tolerances (L2-relative).  float32: products keep 24 bits and sum in float32, scores of up to about 20 carry 20 x 2^-24 into
+the exponent and so into each probability: a few 1e-6, below 1e-5.  bfloat16: an output is rounded once (2^-9 at most, 2^-10.8
+in the mean square), its probabilities too, independently; together below 4e-3.  A gradient is a product with rounded
+score gradients, whose delta takes the rounded output: below 8e-3.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TOL = {torch.float32: (1e-5, 1e-5), torch.bfloat16: (4e-3, 8e-3)}
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+def rel(x, y):
+    x, y = x.detach().double().cpu(), y.detach().double().cpu()
+    n = float(y.norm())
+    return float((x - y).norm()) / n if n > 0 else float(x.norm())
+
+
+def plain(q, k, v, mask, g=None, scale=None):
+    """float64 (on the CPU): output and, with g, the gradients of q, k, v.  Masked keys are left out, not weighted with 0."""
+    B, nq, hq, D = q.shape
+    group = hq // k.shape[2]
+    scale = D ** -0.5 if scale is None else scale
+    q, k, v = (t.detach().double().cpu() for t in (q, k, v))
+    out, dq, dk, dv = (torch.zeros_like(t) for t in (q, q, k, v))
+    for b in range(B):
+        keys = torch.arange(k.shape[1]) if mask is None else mask[b].cpu().nonzero()[:, 0]
+        if not len(keys):
+            continue
+        for h in range(hq):
+            K, V = k[b, keys, h // group], v[b, keys, h // group]
+            p = torch.softmax(scale * q[b, :, h] @ K.T, -1)
+            out[b, :, h] = p @ V
+            if g is not None:
+                G = g[b, :, h].detach().double().cpu()
+                dp = G @ V.T
+                ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * scale
+                dq[b, :, h] = ds @ K
+                dk[b, keys, h // group] += ds.T @ q[b, :, h]
+                dv[b, keys, h // group] += p.T @ G
+    return out, dq, dk, dv
+
+
+def make(B, nq, nk, hq, hk, D, dtype, seed, size=1.0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)   # noqa: E731
+    q, k, v, go = r(B, nq, hq, D) * size, r(B, nk, hk, D) * size, r(B, nk, hk, D), r(B, nq, hq, D)
+    return [t.to(dtype) for t in (q, k, v, go)]
+
+
+def random_mask(B, nk, keep, seed):
+    return torch.rand(B, nk, generator=torch.Generator().manual_seed(seed)) < keep
+
+
+def check(q, k, v, g, mask, dtype, scale=None):
+    from CudaGaussianVoxelizer import gaussian_attention
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    cm = None if mask is None else mask.cuda()
+    out = gaussian_attention(*leaves, key_mask=cm, scale=scale)
+    with torch.no_grad():
+        assert torch.equal(gaussian_attention(*leaves, key_mask=cm, scale=scale), out)
+    out.backward(g.cuda())
+    want = plain(q, k, v, mask, g, scale)
+    errs = [rel(a, b) for a, b in zip([out] + [t.grad for t in leaves], want)]
+    say(" ".join(f"{e:.1e}" for e in errs))
+    assert out.dtype == dtype and out.is_contiguous()
+    assert errs[0] < TOL[dtype][0] and max(errs[1:]) < TOL[dtype][1], errs
+    if mask is not None:
+        off = ~mask
+        for t in leaves[1:]:
+            assert torch.count_nonzero(t.grad.cpu()[off]) == 0
+
+
+BOTH = [torch.float32, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("D", [1, 7, 8, 24, 32, 33, 64, 72, 75, 96, 100, 128])
+def test_widths(D, dtype):
+    check(*make(2, 70, 150, 4, 2, D, dtype, D), None, dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk", [(1, 1), (1, 2), (2, 1), (31, 33), (32, 32), (33, 31), (64, 64), (63, 65), (65, 127),
+                                   (128, 129), (257, 300), (300, 257), (1, 5000), (3, 4999), (5000, 1), (700, 1500)])
+def test_lengths(nq, nk, dtype):
+    check(*make(1, nq, nk, 2, 2, 64, dtype, nq * 7 + nk), None, dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("hq,hk,nq", [(8, 1, 1), (6, 2, 40), (12, 4, 65), (5, 5, 33), (7, 1, 100)])
+def test_shared_key_heads(hq, hk, nq, dtype):
+    check(*make(2, nq, 90, hq, hk, 32, dtype, hq), None, dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("D", [32, 64, 75, 128])
+@pytest.mark.parametrize("keep", [0.03, 0.5, 0.97])
+def test_masks(keep, D, dtype):
+    """One scene keeps no key, one a single key, the rest a share; a mask that keeps all equals none."""
+    B, nk = 4, 300
+    q, k, v, g = make(B, 70, nk, 4, 2, D, dtype, D)
+    mask = random_mask(B, nk, keep, D)
+    mask[0] = False
+    mask[1] = False
+    mask[1, 177] = True
+    check(q, k, v, g, mask, dtype)
+    from CudaGaussianVoxelizer import gaussian_attention
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    assert torch.count_nonzero(gaussian_attention(q, k, v, mask.cuda())[0]) == 0
+    assert torch.equal(gaussian_attention(q, k, v, torch.ones_like(mask).cuda()), gaussian_attention(q, k, v))
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("nq", [1, 70])
+def test_masked_rows_are_not_read(nq, dtype):
+    """NaN, infinities and the type's extremes in masked rows change no bit of any result."""
+    from CudaGaussianVoxelizer import gaussian_attention
+    B, nk = 2, 400
+    q, k, v, g = (t.cuda() for t in make(B, nq, nk, 4, 4, 40, dtype, 3))
+    mask = random_mask(B, nk, 0.6, 4).cuda()
+    results = []
+    for bad in (0.0, float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).min, torch.finfo(dtype).max):
+        kb, vb = (torch.where(mask[:, :, None, None], t, torch.full_like(t, bad)) for t in (k, v))
+        leaves = [t.detach().clone().requires_grad_() for t in (q, kb, vb)]
+        out = gaussian_attention(*leaves, key_mask=mask)
+        out.backward(g)
+        results.append([out.detach()] + [t.grad for t in leaves])
+    for r in results[1:]:
+        for a, b in zip(r, results[0]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+def test_large_scores(dtype):
+    """Scores of hundreds: the running maximum moves often and most probabilities vanish."""
+    q, k, v, g = make(1, 100, 500, 2, 2, 64, dtype, 8, size=1.0)
+    q = q * torch.linspace(0.1, 8.0, 100)[None, :, None, None].to(dtype)
+    k = k * torch.linspace(0.2, 6.0, 500)[None, :, None, None].to(dtype)
+    from CudaGaussianVoxelizer import gaussian_attention
+    out = gaussian_attention(q.cuda(), k.cuda(), v.cuda())
+    # a score of 200 carries 200 x 2^-24 (float32) into the exponent: 2e-5 of a probability
+    assert rel(out, plain(q, k, v, None)[0]) < (5e-5 if dtype == torch.float32 else 4e-3)
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("scale", [0.01, 1.0])
+def test_scale(scale, dtype):
+    check(*make(1, 50, 200, 2, 2, 64, dtype, 9, size=0.7), None, dtype, scale)
+
+
+@pytest.mark.parametrize("D", [16, 64])
+def test_gradient_against_differences(D):
+    """Central differences of the float64 statement along random directions (step 1e-5: error about 1e-9)."""
+    from CudaGaussianVoxelizer import gaussian_attention
+    q, k, v, g = make(2, 20, 45, 4, 2, D, torch.float32, 11)
+    mask = random_mask(2, 45, 0.7, 5)
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    gaussian_attention(*leaves, key_mask=mask.cuda()).backward(g.cuda())
+    base = [t.double() for t in (q, k, v)]
+    gen = torch.Generator().manual_seed(1)
+    for i in range(3):
+        u = torch.randn(base[i].shape, generator=gen).double()
+        vals = []
+        for s in (1, -1):
+            m = list(base)
+            m[i] = base[i] + s * 1e-5 * u
+            vals.append(float((plain(*m, mask)[0] * g.double()).sum()))
+        got = leaves[i].grad.double().cpu()
+        want = (vals[0] - vals[1]) / 2e-5
+        assert abs(float((got * u).sum()) - want) <= 1e-5 * float((got.abs() * u.abs()).sum()), i
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 36])
+def test_layouts(D, dtype):
+    """Views of a fused projection, heads-first storage, data off 16-byte boundaries and transposed rows give the
+    contiguous tensors' results bit for bit; expanded heads and scenes too."""
+    from CudaGaussianVoxelizer import _C
+    B, n, h = 2, 130, 2
+    q, k, v, g = (t.cuda() for t in make(B, n, n, h, h, D, dtype, 6))
+    want = _C.attention_forward(q, k, v, want_lse=True)
+    gwant = _C.attention_backward(g, q, k, v, want[0], want[1])
+
+    def views(t):
+        fused = torch.randn(B, n, 3 * h, D, device="cuda").to(dtype)
+        fused[:, :, h:2 * h] = t
+        yield fused[:, :, h:2 * h]
+        yield t.transpose(1, 2).contiguous().transpose(1, 2)
+        flat = torch.zeros(t.numel() + 1, dtype=dtype, device="cuda")
+        flat[1:] = t.flatten()
+        yield flat[1:].view(t.shape)
+        yield t.transpose(2, 3).contiguous().transpose(2, 3)
+
+    for qv, kv, vv, gv in zip(views(q), views(k), views(v), views(g)):
+        got = _C.attention_forward(qv, kv, vv, want_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for a, b in zip(_C.attention_backward(gv, qv, kv, vv, got[0], got[1]), gwant):
+            assert torch.equal(a, b)
+    one = k[:1, :, :1].expand(B, n, h, D)
+    assert torch.equal(_C.attention_forward(q, one, one)[0], _C.attention_forward(q, one.contiguous(), one.contiguous())[0])
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+def test_empty(dtype):
+    from CudaGaussianVoxelizer import gaussian_attention
+    for B, nq, nk in ((0, 3, 4), (2, 0, 5), (2, 5, 0), (2, 0, 0)):
+        q, k, v, g = make(B, nq, nk, 4, 2, 32, dtype, 1)
+        leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+        for mask in (None, torch.ones(B, nk, dtype=torch.bool, device="cuda")):
+            out = gaussian_attention(*leaves, key_mask=mask)
+            assert out.shape == q.shape and torch.count_nonzero(out) == 0
+            for t, grad in zip(leaves, torch.autograd.grad(out, leaves, g.cuda())):
+                assert grad.shape == t.shape and torch.count_nonzero(grad) == 0
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk", [(1, 9000), (2100, 2100)])
+def test_runs_are_equal_and_streams_are_the_callers(nq, nk, dtype):
+    """Three passes without a wait between them, the second on other inputs, on a stream of the caller's."""
+    from CudaGaussianVoxelizer import _C
+    sets = [[t.cuda() for t in make(1, nq, nk, 4, 4, 64, dtype, s)] for s in (1, 2)]
+
+    def both(q, k, v, g):
+        out, lse, _ = _C.attention_forward(q, k, v, want_lse=True)
+        return (out,) + _C.attention_backward(g, q, k, v, out, lse)
+
+    want = both(*sets[0])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        first = both(*sets[0])
+        both(*sets[1])
+        last = both(*sets[0])
+    s.synchronize()
+    for a, b, c in zip(want, first, last):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_partial_gradients():
+    """Only the wanted gradients are computed, and they are the same."""
+    from CudaGaussianVoxelizer import gaussian_attention
+    q, k, v, g = (t.cuda() for t in make(1, 60, 80, 2, 2, 32, torch.bfloat16, 2))
+    full = [t.clone().requires_grad_() for t in (q, k, v)]
+    gaussian_attention(*full).backward(g)
+    for i in range(3):
+        some = [t.clone().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        gaussian_attention(*some).backward(g)
+        assert torch.equal(some[i].grad, full[i].grad)
+        assert all(t.grad is None for j, t in enumerate(some) if j != i)
+
+
+def test_refusals():
+    from CudaGaussianVoxelizer import gaussian_attention
+    q = torch.ones(1, 4, 4, 16, device="cuda")
+    k = torch.ones(1, 6, 2, 16, device="cuda")
+    good = dict(q=q, k=k, v=k)
+    gaussian_attention(**good)
+    wide = torch.ones(1, 4, 4, 129, device="cuda")
+    bad = [
+        dict(q=q.half()), dict(q=q.double()), dict(q=q.cpu()), dict(q=q[0]), dict(k=k.bfloat16()), dict(v=k[:, :5]),
+        dict(v=k[..., :8]), dict(q=q[:, :, :3]), dict(k=k.expand(2, 6, 2, 16), v=k.expand(2, 6, 2, 16)), dict(q=q[:, :, :0]),
+        dict(q=wide, k=wide, v=wide), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")),
+        dict(key_mask=torch.ones(1, 6, device="cuda")), dict(key_mask=torch.ones(1, 5, dtype=torch.bool, device="cuda")),
+        dict(key_mask=torch.ones(1, 6, dtype=torch.bool)), dict(q=None),
+    ]
+    for b in bad:
+        with pytest.raises(RuntimeError):
+            gaussian_attention(**dict(good, **b))
