@@ -15,7 +15,7 @@ using namespace attn;
 
 // dQ: rows in the lanes as in the forward, S^T = K Q^T and dP^T = V dO^T, dQ^T += K^T dS^T.
 template <int NP, int DP, int NQB, int NW, int KT, typename T>
-__global__ void __launch_bounds__(NW * 64) k_attn_dq(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a) {
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(NW * 64) k_attn_dq(AttnBwd a) {
 // dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
-__global__ void __launch_bounds__(NW * 64) k_attn_dkv(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_dkv(AttnBwd a) {
     constexpr int NT = NW * 64, QB = QT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, QT, NT> TileT;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];

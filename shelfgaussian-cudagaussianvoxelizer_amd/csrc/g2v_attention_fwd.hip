@@ -14,7 +14,7 @@ using namespace attn;
 constexpr float kLazy = 8.0f;   // the maximum in use may trail the true one by a factor of 2^8
 
 template <int NP, int DP, int NQB, int NW, int KT, typename T>
-__global__ void __launch_bounds__(NW * 64) k_attn_fwd(AttnFwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a) {
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
