@@ -370,7 +370,8 @@ int g2v_qk_norm_rotary_backward(int batch, int n_q, int n_k, int heads_q, int he
  * heads h heads_q / heads_k ... share key head h); dtype G2V_DTYPE_F32 or G2V_DTYPE_BF16 for all; strides in elements
  * along batch, tokens and heads, unit stride along head_dim; out contiguous.  head_dim <= 128, scale > 0.
  * key_mask (batch, n_k) bytes: 0 where a key is not attended to (NULL: none); what such a key's rows hold is never read.
- * A query without any key gives 0.  lse (batch, heads_q, n_q) float32, NULL where no backward follows: the base-2
+ * A query without any key gives 0.  out_rest (like out, NULL where not wanted, unused for float32) receives what
+ * rounding to bfloat16 took from out, for a backward whose row sums of grad_out out are not off by it.  lse (batch, heads_q, n_q) float32, NULL where no backward follows: the base-2
  * logarithm of the sum of 2^(scale log2(e) q.k), +inf for a query without keys.  key_list (batch n_k + batch ints,
  * needed with key_mask) receives the valid keys of every scene and their number, for the backward.
  * Sums and softmax statistics are float32; bfloat16 probabilities are rounded to nearest even for their product.
@@ -381,17 +382,17 @@ size_t g2v_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q,
 int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
                           const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
                           const long long v_strides[3], int dtype, const unsigned char* key_mask, float scale, void* out,
-                          float* lse, int* key_list, void* workspace, size_t workspace_bytes, void* stream);
+                          void* out_rest, float* lse, int* key_list, void* workspace, size_t workspace_bytes, void* stream);
 
-/* g2v_attention_backward: gradients of g2v_attention_forward's inputs from its out, lse and key_list (NULL without a
- * mask) and the upstream gradient (strided like q); contiguous, of dtype.  Probabilities are recomputed.  grad_q, or
+/* g2v_attention_backward: gradients of g2v_attention_forward's inputs from its out, out_rest (or NULL), lse and key_list
+ * (NULL without a mask) and the upstream gradient (strided like q); contiguous, of dtype.  Probabilities are recomputed.  grad_q, or
  * grad_k with grad_v, may be NULL; masked keys get 0.  Deterministic: no atomics, fixed summation order.  Asynchronous. */
 size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
                                         int in_place);
 int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
                            const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
                            const long long v_strides[3], int dtype, const int* key_list, float scale, const void* out,
-                           const float* lse, const void* grad_out, const long long grad_out_strides[3], void* grad_q,
+                           const void* out_rest, const float* lse, const void* grad_out, const long long grad_out_strides[3], void* grad_q,
                            void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- per-kernel timing (benchmarks) --------------------------------------------------------

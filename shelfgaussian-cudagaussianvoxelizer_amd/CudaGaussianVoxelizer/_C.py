@@ -915,10 +915,11 @@ def _in_place(*tensors):
     return 1
 
 
-def attention_forward(q, k, v, key_mask=None, scale=None, want_lse=False):
-    """(out, lse, key_list): softmax(scale q k^T over the valid keys) v for q (B, Nq, Hq, D) and k, v (B, Nk, Hkv, D), Hq a
-    multiple of Hkv; scale None: D^-1/2.  key_mask (B, Nk) bool, False where a key is not attended to.  lse (None unless
-    wanted) and key_list (None without a mask) are what attention_backward takes."""
+def attention_forward(q, k, v, key_mask=None, scale=None, for_backward=False):
+    """(out, rest, lse, key_list): softmax(scale q k^T over the valid keys) v for q (B, Nq, Hq, D) and k, v (B, Nk, Hkv, D), Hq a
+    multiple of Hkv; scale None: D^-1/2.  key_mask (B, Nk) bool, False where a key is not attended to.  rest (what
+    rounding took from a bfloat16 out) and lse, None unless for_backward, and key_list, None without a mask, are what
+    attention_backward takes."""
     lib = _lib.load()
     q, k, v, sizes, scale = _attention_inputs(q, k, v, scale)
     B, nq, nk, hq = sizes[:4]
@@ -930,16 +931,17 @@ def attention_forward(q, k, v, key_mask=None, scale=None, want_lse=False):
         key_mask = key_mask.contiguous()
     with _OnDevice(dev):
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        lse = torch.empty(B, hq, nq, dtype=torch.float32, device=dev) if want_lse else None
+        rest = torch.empty_like(out) if for_backward and q.dtype == torch.bfloat16 else None
+        lse = torch.empty(B, hq, nq, dtype=torch.float32, device=dev) if for_backward else None
         lst = None if key_mask is None else torch.empty(B * (nk + 1), dtype=torch.int32, device=dev)
         ws = torch.empty(lib.g2v_attention_forward_workspace(*sizes, fdt, _in_place(q, k, v)), dtype=torch.uint8, device=dev)
         _lib.check(lib.g2v_attention_forward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
-                                             _ptr(key_mask), scale, _ptr(out), _ptr(lse), _ptr(lst), _ptr(ws), ws.numel(),
-                                             _stream(dev)), "attention_forward")
-    return out, lse, lst
+                                             _ptr(key_mask), scale, _ptr(out), _ptr(rest), _ptr(lse), _ptr(lst), _ptr(ws),
+                                             ws.numel(), _stream(dev)), "attention_forward")
+    return out, rest, lse, lst
 
 
-def attention_backward(grad_out, q, k, v, out, lse, key_list=None, scale=None, want_q=True, want_kv=True):
+def attention_backward(grad_out, q, k, v, out, rest, lse, key_list=None, scale=None, want_q=True, want_kv=True):
     """(grad_q, grad_k, grad_v) of attention_forward from its results; None where not wanted."""
     lib = _lib.load()
     q, k, v, sizes, scale = _attention_inputs(q, k, v, scale)
@@ -950,6 +952,10 @@ def attention_backward(grad_out, q, k, v, out, lse, key_list=None, scale=None, w
         raise RuntimeError(f"grad_out must be {tuple(q.shape)}, got {tuple(g.shape)}")
     _check_saved(out, "out", q.dtype, dev)
     _check_saved(lse, "lse", torch.float32, dev)
+    if rest is not None:
+        _check_saved(rest, "rest", torch.bfloat16, dev)
+        if rest.shape != out.shape:
+            raise RuntimeError(f"rest must be {tuple(out.shape)}, got {tuple(rest.shape)}")
     if out.shape != q.shape or tuple(lse.shape) != (B, hq, nq):
         raise RuntimeError(f"out {tuple(out.shape)} and lse {tuple(lse.shape)} do not go with q {tuple(q.shape)}")
     if key_list is not None:
@@ -963,7 +969,7 @@ def attention_backward(grad_out, q, k, v, out, lse, key_list=None, scale=None, w
         ws = torch.empty(lib.g2v_attention_backward_workspace(*sizes, fdt, _in_place(q, k, v, g)), dtype=torch.uint8,
                          device=dev)
         _lib.check(lib.g2v_attention_backward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
-                                              _ptr(key_list), scale, _ptr(out), _ptr(lse), _ptr(g), _strides(g), _ptr(dq),
-                                              _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)),
+                                              _ptr(key_list), scale, _ptr(out), _ptr(rest), _ptr(lse), _ptr(g), _strides(g),
+                                              _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)),
                    "attention_backward")
     return dq, dk, dv

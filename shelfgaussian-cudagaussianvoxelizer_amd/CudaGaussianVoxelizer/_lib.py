@@ -75,10 +75,10 @@ SIGNATURES = {
                                                     _vp, _vp, _sz, _vp]),
     "g2v_attention_forward_workspace": (_sz, [_i] * 8),
     "g2v_attention_forward": (_i, [_i] * 6 + [_vp, _llp, _vp, _llp, _vp, _llp, _i, _vp, ctypes.c_float, _vp, _vp, _vp,
-                                              _vp, _sz, _vp]),
+                                              _vp, _vp, _sz, _vp]),
     "g2v_attention_backward_workspace": (_sz, [_i] * 8),
     "g2v_attention_backward": (_i, [_i] * 6 + [_vp, _llp, _vp, _llp, _vp, _llp, _i, _vp, ctypes.c_float, _vp, _vp, _vp,
-                                               _llp, _vp, _vp, _vp, _vp, _sz, _vp]),
+                                               _vp, _llp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "g2v_profile_enable": (_i, [_i]),
     "g2v_profile_reset": (_i, []),
     "g2v_profile_collect": (_i, []),

@@ -80,16 +80,16 @@ def rotary_frequencies(head_dim, axes=3, wavelengths=(0.8, 160.0), device="cuda"
 class _GaussianAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_mask, scale):
-        out, lse, key_list = _C.attention_forward(q, k, v, key_mask, scale, want_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, key_list)
+        out, rest, lse, key_list = _C.attention_forward(q, k, v, key_mask, scale, for_backward=True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, key_list)
         ctx.scale = scale
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        q, k, v, out, lse, key_list = ctx.saved_tensors
+        q, k, v, out, rest, lse, key_list = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return _C.attention_backward(grad_out, q, k, v, out, lse, key_list, ctx.scale, want_q=need[0],
+        return _C.attention_backward(grad_out, q, k, v, out, rest, lse, key_list, ctx.scale, want_q=need[0],
                                      want_kv=need[1] or need[2]) + (None, None)
 
 

@@ -146,13 +146,15 @@ __device__ __forceinline__ bf16x8 mem_frag(const char* row, bool have, int chunk
     return __builtin_bit_cast(bf16x8, s16x8{0, 0, 0, 0, 0, 0, 0, 0});
 }
 
-// acc += A B, with NP planes of each.
-template <int NP>
-__device__ __forceinline__ f32x16 mma(const bf16x8 (&a)[NP], const bf16x8 (&b)[NP], f32x16 acc) {
+// acc += A B, with NA and NB planes: the terms of the first max(NA, NB) orders.
+template <int NA, int NB>
+__device__ __forceinline__ f32x16 mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x16 acc) {
+    constexpr int N = NA > NB ? NA : NB;
 #pragma unroll
-    for (int o = NP - 1; o >= 0; --o)
+    for (int o = N - 1; o >= 0; --o)
 #pragma unroll
-        for (int i = 0; i <= o; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[o - i], acc, 0, 0, 0);
+        for (int i = 0; i <= o; ++i)
+            if (i < NA && o - i < NB) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[o - i], acc, 0, 0, 0);
     return acc;
 }
 
@@ -210,6 +212,9 @@ __device__ __forceinline__ void store4(T* row, int d, int D, float x0, float x1,
     }
 }
 
+// The same for what bfloat16 rounding leaves of the values.
+__device__ __forceinline__ float lost_by_rounding(float x) { return x - (float)(__bf16)x; }
+
 // A workgroup's item: head (scene b, key head h), tile and split, heads fastest, so that with 8 heads or a multiple the
 // workgroups of a head share an XCD's L2 (workgroups go to the 8 XCDs in turn).
 struct Item {
@@ -243,6 +248,7 @@ struct AttnFwd {
     int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
     float c;            // scale log2(e)
     void* out;          // (batch, nq, hq, dim)
+    void* rest;         // like out: what rounding to bfloat16 left of it, or null
     float* lse;         // (batch, hq, nq) log2 of the sum of 2^(c s); +inf for a row without keys
     float* part_o;      // (splits, bhs, group nq, DP)
     float* part_ml;     // (splits, bhs, group nq, 2)

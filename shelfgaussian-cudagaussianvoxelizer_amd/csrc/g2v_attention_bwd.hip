@@ -16,6 +16,10 @@ using namespace attn;
 // dQ: rows in the lanes as in the forward, S^T = K Q^T and dP^T = V dO^T, dQ^T += K^T dS^T.
 template <int NP, int DP, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a) {
+    // planes of dS in its product with K: two of bfloat16 for bfloat16 inputs.  The keys that a query attends to share
+    // a direction, their dS sum to zero, and what is left of dQ is small beside the terms: rounding dS to 2^-9
+    // alone puts dQ 3.0e-3 off (its own rounding: 1.7e-3), a second plane leaves 2.0e-3 for a third more products here
+    constexpr int NS = NP == 1 ? 2 : NP;
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
@@ -109,8 +113,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
                 }
 #pragma unroll
                 for (int b = 0; b < NQB; ++b) {
-                    s[b] = mma<NP>(fk, q[b][ks], s[b]);
-                    dp[b] = mma<NP>(fv, g[b][ks], dp[b]);
+                    s[b] = mma(fk, q[b][ks], s[b]);
+                    dp[b] = mma(fv, g[b][ks], dp[b]);
                 }
             }
 #pragma unroll
@@ -127,16 +131,16 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                bf16x8 p[NQB][NP];
+                bf16x8 p[NQB][NS];
 #pragma unroll
-                for (int b = 0; b < NQB; ++b) to_operand<NP>(s[b], st, p[b]);
+                for (int b = 0; b < NQB; ++b) to_operand<NS>(s[b], st, p[b]);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     bf16x8 f[NP];
 #pragma unroll
                     for (int pl = 0; pl < NP; ++pl) f[pl] = tr_frag<DP>(kt + pl * KT * DP * 2, kb, st, d);
 #pragma unroll
-                    for (int b = 0; b < NQB; ++b) dq[d][b] = mma<NP>(f, p[b], dq[d][b]);
+                    for (int b = 0; b < NQB; ++b) dq[d][b] = mma(f, p[b], dq[d][b]);
                 }
             }
         }
@@ -259,8 +263,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
                 }
 #pragma unroll
                 for (int b = 0; b < NKB; ++b) {
-                    s[b] = mma<NP>(fq, k[b][ks], s[b]);
-                    dp[b] = mma<NP>(fg, v[b][ks], dp[b]);
+                    s[b] = mma(fq, k[b][ks], s[b]);
+                    dp[b] = mma(fg, v[b][ks], dp[b]);
                 }
             }
             const int g4 = 4 * ((threadIdx.x >> 5) & 1);
@@ -294,8 +298,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
                     }
 #pragma unroll
                     for (int b = 0; b < NKB; ++b) {
-                        dv[d][b] = mma<NP>(fg, p[b], dv[d][b]);
-                        dk[d][b] = mma<NP>(fq, ds[b], dk[d][b]);
+                        dv[d][b] = mma(fg, p[b], dv[d][b]);
+                        dk[d][b] = mma(fq, ds[b], dk[d][b]);
                     }
                 }
             }
@@ -372,8 +376,8 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a) {
 
 // delta = sum_d dO O of a row and its lse, both padded to nqp rows of a head.  16 lanes a row.
 template <typename T>
-__global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nqp, int heads, int dim, const T* out, const T* g,
-                                                    int64_t gsb, int64_t gsn, int64_t gsh, const float* lse, float* lse_p,
+__global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nqp, int heads, int dim, const T* out, const T* rest,
+                                                    const T* g, int64_t gsb, int64_t gsn, int64_t gsh, const float* lse, float* lse_p,
                                                     float* delta) {
     const int64_t e = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     if (e >= rows) return;
@@ -385,7 +389,8 @@ __global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nq
     if (i < nq) {
         const T* o = out + ((b * nq + i) * heads + h) * dim;
         const T* r = g + b * gsb + i * gsn + h * gsh;
-        for (int d = sub; d < dim; d += 16) v = fmaf((float)o[d], (float)r[d], v);
+        const T* l = rest ? rest + (o - out) : nullptr;
+        for (int d = sub; d < dim; d += 16) v = fmaf(l ? (float)o[d] + (float)l[d] : (float)o[d], (float)r[d], v);
     }
     for (int m = 8; m > 0; m >>= 1) v += __shfl_xor(v, m);
     if (sub == 0) {
@@ -466,17 +471,17 @@ hipError_t launch_attn_dkv(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
     }
 }
 
-hipError_t launch_attn_delta(int batch, int nq, int nqp, int heads, int dim, const void* out, const void* g, int64_t gsb,
-                             int64_t gsn, int64_t gsh, bool f32, const float* lse, float* lse_p, float* delta, hipStream_t s) {
+hipError_t launch_attn_delta(int batch, int nq, int nqp, int heads, int dim, const void* out, const void* rest, const void* g,
+                             int64_t gsb, int64_t gsn, int64_t gsh, bool f32, const float* lse, float* lse_p, float* delta, hipStream_t s) {
     const int64_t rows = (int64_t)batch * heads * nqp;
     if (rows == 0) return hipSuccess;
     const dim3 grid((unsigned)ceil_div(rows, 16));
     if (f32)
         G2V_LAUNCH((k_attn_delta<float>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, static_cast<const float*>(out),
-                   static_cast<const float*>(g), gsb, gsn, gsh, lse, lse_p, delta);
+                   static_cast<const float*>(nullptr), static_cast<const float*>(g), gsb, gsn, gsh, lse, lse_p, delta);
     else
         G2V_LAUNCH((k_attn_delta<__bf16>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, static_cast<const __bf16*>(out),
-                   static_cast<const __bf16*>(g), gsb, gsn, gsh, lse, lse_p, delta);
+                   static_cast<const __bf16*>(rest), static_cast<const __bf16*>(g), gsb, gsn, gsh, lse, lse_p, delta);
     return hipGetLastError();
 }
 

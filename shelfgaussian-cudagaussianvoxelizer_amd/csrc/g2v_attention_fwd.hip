@@ -13,6 +13,18 @@ using namespace attn;
 
 constexpr float kLazy = 8.0f;   // the maximum in use may trail the true one by a factor of 2^8
 
+// Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
+// to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
+// the same error on all of them, which their sum dS K does not average out (dQ then 3.2e-3 off instead of 2.2e-3).
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, float x0, float x1, float x2, float x3) {
+    store4<T>(static_cast<T*>(a.out) + at, d, a.dim, x0, x1, x2, x3);
+    if constexpr (sizeof(T) == 2)
+        if (a.rest)
+            store4<T>(static_cast<T*>(a.rest) + at, d, a.dim, lost_by_rounding(x0), lost_by_rounding(x1),
+                      lost_by_rounding(x2), lost_by_rounding(x3));
+}
+
 template <int NP, int DP, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a) {
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
@@ -99,7 +111,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
 #pragma unroll
                 for (int pl = 0; pl < NP; ++pl) f[pl] = row_frag<DP>(kt + pl * KT * DP * 2, kb, ks);
 #pragma unroll
-                for (int b = 0; b < NQB; ++b) s[kb][b] = mma<NP>(f, q[b][ks], s[kb][b]);
+                for (int b = 0; b < NQB; ++b) s[kb][b] = mma(f, q[b][ks], s[kb][b]);
             }
         }
         if ((t + 1) * KT > n) {   // the last tile's rows past the end
@@ -154,7 +166,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
 #pragma unroll
                     for (int pl = 0; pl < NP; ++pl) f[pl] = tr_frag<DP>(vt + pl * KT * DP * 2, kb, st, d);
 #pragma unroll
-                    for (int b = 0; b < NQB; ++b) o[d][b] = mma<NP>(f, p[b], o[d][b]);
+                    for (int b = 0; b < NQB; ++b) o[d][b] = mma(f, p[b], o[d][b]);
                 }
             }
     }
@@ -181,13 +193,13 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
         const float inv = total > 0.0f ? 1.0f / total : 0.0f;
         if (a.lse && lane < 32)
             a.lse[((int64_t)w.b * a.hq + head) * a.nq + tok] = total > 0.0f ? fmaf(m[b], a.c, log2f(total)) : INFINITY;
-        T* row = static_cast<T*>(a.out) + (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+        const int64_t at = (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                store4<T>(row, 32 * d + reg_row(i), a.dim, o[d][b][i] * inv, o[d][b][i + 1] * inv, o[d][b][i + 2] * inv,
-                          o[d][b][i + 3] * inv);
+                store_out<T>(a, at, 32 * d + reg_row(i), o[d][b][i] * inv, o[d][b][i + 1] * inv, o[d][b][i + 2] * inv,
+                             o[d][b][i + 3] * inv);
     }
 }
 
@@ -217,8 +229,7 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnFwd a) {
     const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
     const float inv = total > 0.0f ? 1.0f / total : 0.0f;
     if (a.lse && d == 0) a.lse[((int64_t)b * a.hq + head) * a.nq + tok] = total > 0.0f ? top + log2f(total) : INFINITY;
-    T* row = static_cast<T*>(a.out) + (((int64_t)b * a.nq + tok) * a.hq + head) * a.dim;
-    store4<T>(row, d, a.dim, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    store_out<T>(a, (((int64_t)b * a.nq + tok) * a.hq + head) * a.dim, d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 // ---- what both directions prepare -----------------------------------------------------------------------------------

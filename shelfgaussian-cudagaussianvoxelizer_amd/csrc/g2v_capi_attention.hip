@@ -270,7 +270,7 @@ size_t g2v_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q,
 int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
                           const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
                           const long long v_strides[3], int dtype, const unsigned char* key_mask, float scale, void* out,
-                          float* lse, int* key_list, void* workspace, size_t workspace_bytes, void* stream) {
+                          void* out_rest, float* lse, int* key_list, void* workspace, size_t workspace_bytes, void* stream) {
     api_begin();
     AttnSizes z;
     int rc = attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z);
@@ -316,6 +316,7 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
     a.splits = r.splits;
     a.c = scale * attn::kLog2e;
     a.out = out;
+    a.rest = out_rest;
     a.lse = lse;
     a.part_o = w.part_o;
     a.part_ml = w.part_ml;
@@ -333,7 +334,7 @@ size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q
 int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
                            const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
                            const long long v_strides[3], int dtype, const int* key_list, float scale, const void* out,
-                           const float* lse, const void* grad_out, const long long grad_out_strides[3], void* grad_q,
+                           const void* out_rest, const float* lse, const void* grad_out, const long long grad_out_strides[3], void* grad_q,
                            void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
     api_begin();
     AttnSizes z;
@@ -363,7 +364,7 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     const AttnBwdWs w = carve_attn_bwd(c, z, rq, rk);
     attn::RowSrc src[4];
     G2V_HIP(attn_sources(z, t, 4, packed, c, src, s));
-    G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
+    G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, out_rest, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
                               w.delta, s));
     AttnBwd a = {};
     a.q = src[0];

@@ -187,8 +187,8 @@ def test_layouts(D, dtype):
     from CudaGaussianVoxelizer import _C
     B, n, h = 2, 130, 2
     q, k, v, g = (t.cuda() for t in make(B, n, n, h, h, D, dtype, 6))
-    want = _C.attention_forward(q, k, v, want_lse=True)
-    gwant = _C.attention_backward(g, q, k, v, want[0], want[1])
+    want = _C.attention_forward(q, k, v, for_backward=True)
+    gwant = _C.attention_backward(g, q, k, v, *want[:3])
 
     def views(t):
         fused = torch.randn(B, n, 3 * h, D, device="cuda").to(dtype)
@@ -201,9 +201,9 @@ def test_layouts(D, dtype):
         yield t.transpose(2, 3).contiguous().transpose(2, 3)
 
     for qv, kv, vv, gv in zip(views(q), views(k), views(v), views(g)):
-        got = _C.attention_forward(qv, kv, vv, want_lse=True)
-        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
-        for a, b in zip(_C.attention_backward(gv, qv, kv, vv, got[0], got[1]), gwant):
+        got = _C.attention_forward(qv, kv, vv, for_backward=True)
+        assert all(a is b is None or torch.equal(a, b) for a, b in zip(got, want))
+        for a, b in zip(_C.attention_backward(gv, qv, kv, vv, *got[:3]), gwant):
             assert torch.equal(a, b)
     one = k[:1, :, :1].expand(B, n, h, D)
     assert torch.equal(_C.attention_forward(q, one, one)[0], _C.attention_forward(q, one.contiguous(), one.contiguous())[0])
@@ -230,8 +230,8 @@ def test_runs_are_equal_and_streams_are_the_callers(nq, nk, dtype):
     sets = [[t.cuda() for t in make(1, nq, nk, 4, 4, 64, dtype, s)] for s in (1, 2)]
 
     def both(q, k, v, g):
-        out, lse, _ = _C.attention_forward(q, k, v, want_lse=True)
-        return (out,) + _C.attention_backward(g, q, k, v, out, lse)
+        out, rest, lse, _ = _C.attention_forward(q, k, v, for_backward=True)
+        return (out,) + _C.attention_backward(g, q, k, v, out, rest, lse)
 
     want = both(*sets[0])
     s = torch.cuda.Stream()
