@@ -376,9 +376,10 @@ int g2v_qk_norm_rotary_backward(int batch, int n_q, int n_k, int heads_q, int he
  * needed with key_mask) receives the valid keys of every scene and their number, for the backward.
  * Sums and softmax statistics are float32; bfloat16 probabilities are rounded to nearest even for their product.
  * in_place: whether every tensor is bfloat16 with head_dim and strides multiples of 8 and 16-byte aligned data (others
- * are packed into the workspace first; pass 0 when unsure).  Asynchronous. */
+ * are packed into the workspace first; pass 0 when unsure).  masked: whether key_mask / key_list will be given (valid
+ * keys are packed too).  Asynchronous. */
 size_t g2v_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
-                                       int in_place);
+                                       int in_place, int masked);
 int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
                           const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
                           const long long v_strides[3], int dtype, const unsigned char* key_mask, float scale, void* out,
@@ -388,7 +389,7 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
  * (NULL without a mask) and the upstream gradient (strided like q); contiguous, of dtype.  Probabilities are recomputed.  grad_q, or
  * grad_k with grad_v, may be NULL; masked keys get 0.  Deterministic: no atomics, fixed summation order.  Asynchronous. */
 size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
-                                        int in_place);
+                                        int in_place, int masked);
 int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
                            const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
                            const long long v_strides[3], int dtype, const int* key_list, float scale, const void* out,

@@ -934,7 +934,8 @@ def attention_forward(q, k, v, key_mask=None, scale=None, for_backward=False):
         rest = torch.empty_like(out) if for_backward and q.dtype == torch.bfloat16 else None
         lse = torch.empty(B, hq, nq, dtype=torch.float32, device=dev) if for_backward else None
         lst = None if key_mask is None else torch.empty(B * (nk + 1), dtype=torch.int32, device=dev)
-        ws = torch.empty(lib.g2v_attention_forward_workspace(*sizes, fdt, _in_place(q, k, v)), dtype=torch.uint8, device=dev)
+        ws = torch.empty(lib.g2v_attention_forward_workspace(*sizes, fdt, _in_place(q, k, v), 0 if lst is None else 1),
+                         dtype=torch.uint8, device=dev)
         _lib.check(lib.g2v_attention_forward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
                                              _ptr(key_mask), scale, _ptr(out), _ptr(rest), _ptr(lse), _ptr(lst), _ptr(ws),
                                              ws.numel(), _stream(dev)), "attention_forward")
@@ -966,8 +967,9 @@ def attention_backward(grad_out, q, k, v, out, rest, lse, key_list=None, scale=N
         dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
         dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
         dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
-        ws = torch.empty(lib.g2v_attention_backward_workspace(*sizes, fdt, _in_place(q, k, v, g)), dtype=torch.uint8,
-                         device=dev)
+        ws = torch.empty(lib.g2v_attention_backward_workspace(*sizes, fdt, _in_place(q, k, v, g),
+                                                              0 if key_list is None else 1),
+                         dtype=torch.uint8, device=dev)
         _lib.check(lib.g2v_attention_backward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
                                               _ptr(key_list), scale, _ptr(out), _ptr(rest), _ptr(lse), _ptr(g), _strides(g),
                                               _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)),

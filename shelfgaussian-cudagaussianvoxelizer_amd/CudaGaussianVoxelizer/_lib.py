@@ -73,10 +73,10 @@ SIGNATURES = {
     "g2v_qk_norm_rotary_backward": (_i, [_i] * 8 + [_vp, _llp, _vp, _llp, _i, _vp, _vp, _vp, _vp, _vp,
                                                     ctypes.c_float, _vp, _llp, _vp, _llp, _vp, _vp, _vp, _vp, _vp,
                                                     _vp, _vp, _sz, _vp]),
-    "g2v_attention_forward_workspace": (_sz, [_i] * 8),
+    "g2v_attention_forward_workspace": (_sz, [_i] * 9),
     "g2v_attention_forward": (_i, [_i] * 6 + [_vp, _llp, _vp, _llp, _vp, _llp, _i, _vp, ctypes.c_float, _vp, _vp, _vp,
                                               _vp, _vp, _sz, _vp]),
-    "g2v_attention_backward_workspace": (_sz, [_i] * 8),
+    "g2v_attention_backward_workspace": (_sz, [_i] * 9),
     "g2v_attention_backward": (_i, [_i] * 6 + [_vp, _llp, _vp, _llp, _vp, _llp, _i, _vp, ctypes.c_float, _vp, _vp, _vp,
                                                _vp, _llp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "g2v_profile_enable": (_i, [_i]),

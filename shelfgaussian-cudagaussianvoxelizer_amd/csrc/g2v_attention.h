@@ -95,14 +95,13 @@ struct Tile {
         for (int it = 0; it < kIter; ++it)
             if (on[it]) dma16(p, (uint32_t)row[it] * (uint32_t)sn + off[it], dst(lds, it));
     }
-    // The rows that idx names (an index below 0: zeros).
-    __device__ __forceinline__ void load_indexed(const char* base, int64_t sn, const int (&idx)[kIter], char* lds) const {
+    // Rows [j0, n) of base, zeros up to ROWS.
+    __device__ __forceinline__ void load_tail(const char* base, int64_t sn, int64_t j0, int64_t n, char* lds) const {
 #pragma unroll
         for (int it = 0; it < kIter; ++it) {
-            if (on[it]) {
-                if (idx[it] >= 0) dma16(base + idx[it] * sn + off[it], dst(lds_off(lds), it));
-                else *reinterpret_cast<f32x4*>(lds + (it * NT + threadIdx.x) * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+            if (!on[it]) continue;
+            if (j0 + row[it] < n) dma16(base + (j0 + row[it]) * sn + off[it], dst(lds_off(lds), it));
+            else *reinterpret_cast<f32x4*>(lds + (it * NT + threadIdx.x) * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
 };
@@ -243,8 +242,7 @@ __device__ __forceinline__ void split_range(int all, int split, int splits, int&
 
 struct AttnFwd {
     attn::RowSrc q, k, v;
-    const int* list;    // (batch, nk) valid keys first, or null
-    const int* count;   // (batch) valid keys
+    const int* count;   // (batch) valid keys, the first rows of k and v; null: nk
     int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
     float c;            // scale log2(e)
     void* out;          // (batch, nq, hq, dim)
@@ -256,8 +254,8 @@ struct AttnFwd {
 
 struct AttnBwd {
     attn::RowSrc q, k, v, g;
-    const int* list;
-    const int* count;
+    const int* count;    // as in AttnFwd
+    const int* list;     // (batch, nk) the keys that the rows of k and v are, valid ones first; null: in order
     int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
     int nqp;             // nq rounded up to 64: rows of lse and delta, padded with +inf and 0
     float c, scale;

@@ -26,8 +26,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int rows = a.group * a.nq;
     const int r0 = (w.tile * NW + uniform(threadIdx.x >> 6)) * (NQB * 32) + (threadIdx.x & 31);
-    const int n = a.list ? a.count[w.b] : a.nk;
-    const int* list = a.list ? a.list + (int64_t)w.b * a.nk : nullptr;
+    const int n = a.count ? a.count[w.b] : a.nk;
     const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
     const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
     int t0, t1;
@@ -57,21 +56,13 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
     TileT tile;
     tile.init(a.k);
     if (a.k.chunks < TileT::C) clear_lds<NT>(&lds[0][0][0], sizeof(lds));
-    int idx[TileT::kIter];
-    auto fetch_index = [&](int t) {
-#pragma unroll
-        for (int it = 0; it < TileT::kIter; ++it) {
-            const int j = t * KT + tile.row[it];
-            idx[it] = j < n ? (list ? list[j] : j) : -1;
-        }
-    };
     auto load = [&](int t, int buf) {
-        if (!list && (t + 1) * KT <= n) {
+        if ((t + 1) * KT <= n) {
             tile.load(kbase, a.k.sn, (int64_t)t * KT, lds_off(lds[buf][0]));
             tile.load(vbase, a.v.sn, (int64_t)t * KT, lds_off(lds[buf][1]));
         } else {
-            tile.load_indexed(kbase, a.k.sn, idx, lds[buf][0]);
-            tile.load_indexed(vbase, a.v.sn, idx, lds[buf][1]);
+            tile.load_tail(kbase, a.k.sn, (int64_t)t * KT, n, lds[buf][0]);
+            tile.load_tail(vbase, a.v.sn, (int64_t)t * KT, n, lds[buf][1]);
         }
     };
 
@@ -82,18 +73,11 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
         for (int b = 0; b < NQB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
-    if (t0 < t1) {
-        fetch_index(t0);
-        load(t0, 0);
-        fetch_index(t0 + 1);
-    }
+    if (t0 < t1) load(t0, 0);
     for (int t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1;
         tile_barrier();
-        if (t + 1 < t1) {
-            load(t + 1, buf ^ 1);
-            fetch_index(t + 2);
-        }
+        if (t + 1 < t1) load(t + 1, buf ^ 1);
         const char* kt = lds[buf][0];
         const char* vt = lds[buf][1];
 #pragma unroll
@@ -181,21 +165,18 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int wave = uniform(threadIdx.x >> 6);
     const int j0 = (w.tile * NW + wave) * (NKB * 32) + (threadIdx.x & 31);
-    const int n = a.list ? a.count[w.b] : a.nk;
-    const int* list = a.list ? a.list + (int64_t)w.b * a.nk : nullptr;
+    const int n = a.count ? a.count[w.b] : a.nk;
     const int per = (a.nq + QT - 1) / QT;     // tiles of a query head
     int u0, u1;
     split_range(per * a.group, w.split, a.splits, u0, u1);
     if (w.tile * (NW * NKB * 32) >= n) u1 = u0;    // no valid key: nothing to add up
 
     bf16x8 k[NKB][KS][NP], v[NKB][KS][NP];
-    int64_t key[NKB];
 #pragma unroll
     for (int b = 0; b < NKB; ++b) {
-        const int j = j0 + 32 * b, jc = j < a.nk ? j : a.nk - 1;
-        key[b] = list ? list[jc] : jc;
-        const char* krow = a.k.p + w.b * a.k.sb + w.h * a.k.sh + key[b] * a.k.sn;
-        const char* vrow = a.v.p + w.b * a.v.sb + w.h * a.v.sh + key[b] * a.v.sn;
+        const int j = j0 + 32 * b;
+        const char* krow = a.k.p + w.b * a.k.sb + w.h * a.k.sh + j * a.k.sn;
+        const char* vrow = a.v.p + w.b * a.v.sb + w.h * a.v.sh + j * a.v.sn;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -216,14 +197,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
             tile.load(qbase, a.q.sn, (int64_t)t * QT, lds_off(lds[buf][0]));
             tile.load(gbase, a.g.sn, (int64_t)t * QT, lds_off(lds[buf][1]));
         } else {
-            int idx[TileT::kIter];
-#pragma unroll
-            for (int it = 0; it < TileT::kIter; ++it) {
-                const int r = t * QT + tile.row[it];
-                idx[it] = r < a.nq ? r : -1;
-            }
-            tile.load_indexed(qbase, a.q.sn, idx, lds[buf][0]);
-            tile.load_indexed(gbase, a.g.sn, idx, lds[buf][1]);
+            tile.load_tail(qbase, a.q.sn, (int64_t)t * QT, a.nq, lds[buf][0]);
+            tile.load_tail(gbase, a.g.sn, (int64_t)t * QT, a.nq, lds[buf][1]);
         }
         // rows past the end are there in the padded statistics: lse +inf makes their probabilities 0
         const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + t * QT;
@@ -324,7 +299,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
             continue;
         }
         const bool valid = j < n;   // a masked key's gradients are zero, whatever its row holds
-        const int64_t at = (((int64_t)w.b * a.nk + key[b]) * a.hk + w.h) * a.dim;
+        const int64_t key = a.list ? a.list[(int64_t)w.b * a.nk + j] : j;
+        const int64_t at = (((int64_t)w.b * a.nk + key) * a.hk + w.h) * a.dim;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -364,7 +340,7 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a) {
     const int d = (int)(e % (DP / 2)) * 4;    // dK, then dV
     if (at >= all) return;
     const int bh = (int)(at / a.nk), j = (int)(at % a.nk), b = bh / a.hk;
-    const int n = a.list ? a.count[b] : a.nk;
+    const int n = a.count ? a.count[b] : a.nk;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     if (j < n && (n > 1 || d >= DP))    // one key: its probability is 1 whatever k is
         for (int s = 0; s < a.splits; ++s) o += *reinterpret_cast<const f32x4*>(a.part + (s * all + at) * (2 * DP) + d);

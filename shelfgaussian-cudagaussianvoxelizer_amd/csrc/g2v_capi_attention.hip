@@ -149,6 +149,7 @@ struct Strided {
     const void* p;
     const long long* s;
     int n, heads;
+    bool keys;
 };
 
 // bfloat16 rows of whole 16-byte chunks at 16-byte boundaries are read where they are.
@@ -167,31 +168,37 @@ size_t attn_packed_bytes(const AttnSizes& z, int64_t n, int heads) {
     return (size_t)z.batch * heads * n * (z.f32 ? 3 : 1) * z.dp * 2;
 }
 
-// The tensors as the kernels read them; what cannot be read in place is packed into c's space.
-hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool packed, Carver& c, attn::RowSrc* out,
-                        hipStream_t s) {
+// The tensors as the kernels read them.  What cannot be read in place is packed into c's space (all of a call, or none),
+// and the keys of a masked call are: the valid ones one after another.
+hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool packed, const int* key_list, Carver& c,
+                        attn::RowSrc* out, hipStream_t s) {
     AttnPack a = {};
-    a.tensors = count;
     a.dim = z.dim;
     a.dp = z.dp;
+    if (key_list) {
+        a.list = key_list;
+        a.count = key_list + (int64_t)z.batch * z.nk;
+    }
     for (int i = 0; i < count; ++i) {
-        if (!packed) {
+        if (!packed && !(key_list && t[i].keys)) {
             out[i] = {static_cast<const char*>(t[i].p), t[i].s[0] * 2, t[i].s[1] * 2, t[i].s[2] * 2, z.dim / 8};
             continue;
         }
         const int64_t row = (int64_t)(z.f32 ? 3 : 1) * z.dp * 2;
         char* dst = c.take<char>(attn_packed_bytes(z, t[i].n, t[i].heads));
-        a.src[i] = t[i].p;
-        a.sb[i] = t[i].s[0];
-        a.sn[i] = t[i].s[1];
-        a.sh[i] = t[i].s[2];
-        a.n[i] = t[i].n;
-        a.heads[i] = t[i].heads;
-        a.rows[i] = (int64_t)z.batch * t[i].heads * t[i].n;
-        a.dst[i] = dst;
+        const int k = a.tensors++;
+        a.src[k] = t[i].p;
+        a.sb[k] = t[i].s[0];
+        a.sn[k] = t[i].s[1];
+        a.sh[k] = t[i].s[2];
+        a.n[k] = t[i].n;
+        a.heads[k] = t[i].heads;
+        a.rows[k] = (int64_t)z.batch * t[i].heads * t[i].n;
+        a.keys[k] = t[i].keys;
+        a.dst[k] = dst;
         out[i] = {dst, row * t[i].n * t[i].heads, row, row * t[i].n, z.dp / 8};
     }
-    return packed ? launch_attn_pack(a, z.f32, s) : hipSuccess;
+    return a.tensors ? launch_attn_pack(a, z.f32, s) : hipSuccess;
 }
 
 AttnRun attn_fwd_run(const AttnSizes& z) {
@@ -214,11 +221,14 @@ AttnFwdWs carve_attn_fwd(Carver& c, const AttnSizes& z, const AttnRun& r) {
     }
     return w;
 }
-void carve_packed(Carver& c, const AttnSizes& z, bool backward) {
-    c.take<char>(attn_packed_bytes(z, z.nq, z.hq));
-    c.take<char>(attn_packed_bytes(z, z.nk, z.hk));
-    c.take<char>(attn_packed_bytes(z, z.nk, z.hk));
-    if (backward) c.take<char>(attn_packed_bytes(z, z.nq, z.hq));
+// packed: all tensors; masked: k and v.
+void carve_packed(Carver& c, const AttnSizes& z, bool packed, bool masked, bool backward) {
+    if (packed) c.take<char>(attn_packed_bytes(z, z.nq, z.hq));
+    if (packed || masked) {
+        c.take<char>(attn_packed_bytes(z, z.nk, z.hk));
+        c.take<char>(attn_packed_bytes(z, z.nk, z.hk));
+    }
+    if (packed && backward) c.take<char>(attn_packed_bytes(z, z.nq, z.hq));
 }
 struct AttnBwdWs {
     int nqp;
@@ -237,16 +247,16 @@ AttnBwdWs carve_attn_bwd(Carver& c, const AttnSizes& z, const AttnRun& dq, const
     return w;
 }
 
-size_t attn_fwd_bytes(const AttnSizes& z, bool packed) {
+size_t attn_fwd_bytes(const AttnSizes& z, bool packed, bool masked) {
     Carver c(nullptr, (size_t)-1);
     carve_attn_fwd(c, z, attn_fwd_run(z));
-    if (packed) carve_packed(c, z, false);
+    carve_packed(c, z, packed, masked, false);
     return c.off + 256;
 }
-size_t attn_bwd_bytes(const AttnSizes& z, bool packed) {
+size_t attn_bwd_bytes(const AttnSizes& z, bool packed, bool masked) {
     Carver c(nullptr, (size_t)-1);
     carve_attn_bwd(c, z, attn_dq_run(z), attn_dkv_run(z));
-    if (packed) carve_packed(c, z, true);
+    carve_packed(c, z, packed, masked, true);
     return c.off + 256;
 }
 
@@ -261,10 +271,10 @@ int attn_scale(float scale) {
 extern "C" {
 
 size_t g2v_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
-                                       int in_place) {
+                                       int in_place, int masked) {
     AttnSizes z;
     if (attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z) != G2V_OK) return 0;
-    return attn_fwd_bytes(z, z.f32 || !in_place);
+    return attn_fwd_bytes(z, z.f32 || !in_place, masked != 0);
 }
 
 int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -287,24 +297,24 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
     if (!out || !q || !q_strides || (keys && (!k || !v || !k_strides || !v_strides)))
         return api_fail(G2V_ERR_INVALID, "null q, k, v, strides or out");
     static const long long none[3] = {0, 0, 0};
-    const Strided t[3] = {{q, q_strides, n_q, heads_q}, {k, keys ? k_strides : none, n_k, heads_k}, {v, keys ? v_strides : none, n_k, heads_k}};
+    const int* list = keys && key_mask ? key_list : nullptr;
+    const Strided t[3] = {{q, q_strides, n_q, heads_q, false},
+                          {k, keys ? k_strides : none, n_k, heads_k, true},
+                          {v, keys ? v_strides : none, n_k, heads_k, true}};
     const bool packed = !attn_in_place(z, t, 3);
-    const size_t need = attn_fwd_bytes(z, packed);
+    const size_t need = attn_fwd_bytes(z, packed, list != nullptr);
     if (!workspace || workspace_bytes < need)
         return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
     const AttnRun r = attn_fwd_run(z);
     Carver c(workspace, workspace_bytes);
     const AttnFwdWs w = carve_attn_fwd(c, z, r);
     attn::RowSrc src[3];
-    G2V_HIP(attn_sources(z, t, 3, packed, c, src, s));
+    G2V_HIP(attn_sources(z, t, 3, packed, list, c, src, s));
     AttnFwd a = {};
     a.q = src[0];
     a.k = src[1];
     a.v = src[2];
-    if (keys && key_mask) {
-        a.list = key_list;
-        a.count = key_list + (int64_t)batch * n_k;
-    }
+    if (list) a.count = list + (int64_t)batch * n_k;
     a.nq = n_q;
     a.nk = n_k;
     a.hq = heads_q;
@@ -325,10 +335,10 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
 }
 
 size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
-                                        int in_place) {
+                                        int in_place, int masked) {
     AttnSizes z;
     if (attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z) != G2V_OK) return 0;
-    return attn_bwd_bytes(z, z.f32 || !in_place);
+    return attn_bwd_bytes(z, z.f32 || !in_place, masked != 0);
 }
 
 int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -354,16 +364,18 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     const long long* sg = queries ? grad_out_strides : none;
     const long long* sk = keys ? k_strides : none;
     const long long* sv = keys ? v_strides : none;
-    const Strided t[4] = {{q, sq, n_q, heads_q}, {k, sk, n_k, heads_k}, {v, sv, n_k, heads_k}, {grad_out, sg, n_q, heads_q}};
+    const int* list = keys ? key_list : nullptr;
+    const Strided t[4] = {{q, sq, n_q, heads_q, false}, {k, sk, n_k, heads_k, true}, {v, sv, n_k, heads_k, true},
+                          {grad_out, sg, n_q, heads_q, false}};
     const bool packed = !attn_in_place(z, t, 4);
-    const size_t need = attn_bwd_bytes(z, packed);
+    const size_t need = attn_bwd_bytes(z, packed, list != nullptr);
     if (!workspace || workspace_bytes < need)
         return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
     const AttnRun rq = attn_dq_run(z), rk = attn_dkv_run(z);
     Carver c(workspace, workspace_bytes);
     const AttnBwdWs w = carve_attn_bwd(c, z, rq, rk);
     attn::RowSrc src[4];
-    G2V_HIP(attn_sources(z, t, 4, packed, c, src, s));
+    G2V_HIP(attn_sources(z, t, 4, packed, list, c, src, s));
     G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, out_rest, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
                               w.delta, s));
     AttnBwd a = {};
@@ -371,10 +383,8 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     a.k = src[1];
     a.v = src[2];
     a.g = src[3];
-    if (keys && key_list) {
-        a.list = key_list;
-        a.count = key_list + (int64_t)batch * n_k;
-    }
+    if (list) a.count = list + (int64_t)batch * n_k;
+    a.list = list;
     a.nq = n_q;
     a.nk = n_k;
     a.hq = heads_q;

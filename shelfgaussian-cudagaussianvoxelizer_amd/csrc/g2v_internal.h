@@ -278,6 +278,8 @@ struct AttnPack {
     int64_t sb[4], sn[4], sh[4];
     int n[4], heads[4];
     int64_t rows[4];   // batch heads n
+    bool keys[4];      // of the keys: with count, the valid ones in list's order
+    const int *count, *list;
     void* dst[4];
 };
 // A kernel's workgroup: waves, blocks of 32 rows of a wave, rows of a tile of the long axis, workgroups that fit a CU.
