@@ -173,6 +173,14 @@ __device__ __forceinline__ void to_operand(const f32x16& x, int s, bf16x8 (&o)[N
     }
 }
 
+// acc + the sum of an operand's eight values.
+__device__ __forceinline__ float add_operand(const bf16x8& x, float acc) {
+    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[j], x[j + 1]}, one, acc, false);
+    return acc;
+}
+
 // Max / sum of a lane and the lane 32 away, in both.  (The swap's results are read as numbers first: __builtin_bit_cast of
 // a vector's element takes element 0 with this compiler.)
 __device__ __forceinline__ void half_swap(float v, float& x, float& y) {

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
             for (int st = 0; st < 2; ++st) {
                 bf16x8 p[NQB][NS];
 #pragma unroll
-                for (int b = 0; b < NQB; ++b) to_operand<NS>(s[b], st, p[b]);
+                for (int b = 0; b < NQB; ++b) to_operand(s[b], st, p[b]);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     bf16x8 f[NP];
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
                 bf16x8 p[NKB][NP], ds[NKB][NP];
 #pragma unroll
                 for (int b = 0; b < NKB; ++b) {
-                    to_operand<NP>(s[b], st, p[b]);
-                    to_operand<NP>(dp[b], st, ds[b]);
+                    to_operand(s[b], st, p[b]);
+                    to_operand(dp[b], st, ds[b]);
                 }
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {

@@ -11,7 +11,10 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-constexpr float kLazy = 8.0f;   // the maximum in use may trail the true one by a factor of 2^8
+// The maximum in use is that of a wave's first tile, and is taken anew from a tile in which a row's sum of probabilities
+// passes this: any finite reference does in float32 as long as nothing overflows, so that most tiles skip the maximum
+// (a tenth of the vector instructions; matrix and vector work of a SIMD take their time one after the other).
+constexpr float kFar = 1048576.0f;
 
 // Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
 // to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
@@ -65,10 +68,10 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
     };
 
     f32x16 o[DB][NQB];
-    float m[NQB], limit[NQB], l[NQB];
+    float m[NQB], l[NQB];
 #pragma unroll
     for (int b = 0; b < NQB; ++b) {
-        m[b] = limit[b] = -INFINITY;
+        m[b] = -INFINITY;
         l[b] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -82,77 +85,88 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
         if (t + 1 < t1) load(t + 1, buf ^ 1);
         const char* kt = lds[buf][0];
         const char* vt = lds[buf][1];
-        f32x16 s[KB][NQB];
+        bf16x8 p[KB][2][NQB][NP];
+        float sum[NQB];
+        for (bool fresh = t == t0;; fresh = true) {
+            f32x16 s[KB][NQB];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
+            for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-            for (int b = 0; b < NQB; ++b)
+                for (int b = 0; b < NQB; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[kb][b][i] = 0.0f;
+                    for (int i = 0; i < 16; ++i) s[kb][b][i] = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                bf16x8 f[NP];
+                for (int ks = 0; ks < KS; ++ks) {
+                    bf16x8 f[NP];
 #pragma unroll
-                for (int pl = 0; pl < NP; ++pl) f[pl] = row_frag<DP>(kt + pl * KT * DP * 2, kb, ks);
+                    for (int pl = 0; pl < NP; ++pl) f[pl] = row_frag<DP>(kt + pl * KT * DP * 2, kb, ks);
 #pragma unroll
-                for (int b = 0; b < NQB; ++b) s[kb][b] = mma(f, q[b][ks], s[kb][b]);
-            }
-        }
-        if ((t + 1) * KT > n) {   // the last tile's rows past the end
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (t * KT + kb * 32 + reg_row(i) >= n)
-#pragma unroll
-                        for (int b = 0; b < NQB; ++b) s[kb][b][i] = -INFINITY;
-        }
-#pragma unroll
-        for (int b = 0; b < NQB; ++b) {
-            float top = s[0][b][0];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][b][i]);
-            top = half_max(top);
-            if (__any(top > limit[b])) {   // rarely, after the first tiles
-                const float up = fmaxf(m[b], top);
-                const float f = m[b] == up ? 1.0f : exp2_fast((m[b] - up) * a.c);
-                m[b] = up;
-                limit[b] = up + kLazy / a.c;
-                l[b] *= f;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][b][i] *= f;
-            }
-            const float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;
-            float sum = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[kb][b][i] = exp2_fast(fmaf(s[kb][b][i], a.c, -mc));
-                    sum += s[kb][b][i];
+                    for (int b = 0; b < NQB; ++b) s[kb][b] = mma(f, q[b][ks], s[kb][b]);
                 }
-            l[b] += sum;
+            }
+            if ((t + 1) * KT > n) {   // the last tile's rows past the end
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (t * KT + kb * 32 + reg_row(i) >= n)
+#pragma unroll
+                            for (int b = 0; b < NQB; ++b) s[kb][b][i] = -INFINITY;
+            }
+            if (fresh) {
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) {
+                    float top = m[b];
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][b][i]);
+                    top = half_max(top);
+                    const float f = m[b] == top ? 1.0f : exp2_fast((m[b] - top) * a.c);
+                    m[b] = top;
+                    l[b] *= f;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][b][i] *= f;
+                }
+            }
+            bool over = false;
+#pragma unroll
+            for (int b = 0; b < NQB; ++b) {
+                const float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;
+                sum[b] = 0.0f;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[kb][b][i] = exp2_fast(fmaf(s[kb][b][i], a.c, -mc));
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        to_operand(s[kb][b], st, p[kb][st][b]);
+                        if constexpr (NP == 1) sum[b] = add_operand(p[kb][st][b][0], sum[b]);
+                    }
+                    if constexpr (NP > 1)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum[b] += s[kb][b][i];
+                }
+                over = over || sum[b] > kFar;
+            }
+            if (fresh || !__any(over)) break;
         }
+#pragma unroll
+        for (int b = 0; b < NQB; ++b) l[b] += sum[b];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                bf16x8 p[NQB][NP];
-#pragma unroll
-                for (int b = 0; b < NQB; ++b) to_operand<NP>(s[kb][b], st, p[b]);
+            for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     bf16x8 f[NP];
 #pragma unroll
                     for (int pl = 0; pl < NP; ++pl) f[pl] = tr_frag<DP>(vt + pl * KT * DP * 2, kb, st, d);
 #pragma unroll
-                    for (int b = 0; b < NQB; ++b) o[d][b] = mma(f, p[b], o[d][b]);
+                    for (int b = 0; b < NQB; ++b) o[d][b] = mma(f, p[kb][st][b], o[d][b]);
                 }
-            }
     }
 #pragma unroll
     for (int b = 0; b < NQB; ++b) {
