@@ -22,7 +22,7 @@ int qn_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim
     if (batch < 0 || n_q < 0 || n_k < 0 || heads_q < 0 || heads_k < 0)
         return api_fail(G2V_ERR_INVALID, "negative size: batch %d, n %d / %d, heads %d / %d", batch, n_q, n_k, heads_q, heads_k);
     if (head_dim < 1 || head_dim > 256) return api_fail(G2V_ERR_INVALID, "head_dim = %d (1 to 256)", head_dim);
-    if (num_axes < 1 || num_axes > 8) return api_fail(G2V_ERR_INVALID, "num_axes = %d (1 to 8)", num_axes);
+    if (num_axes < 1 || num_axes > kQnAxes) return api_fail(G2V_ERR_INVALID, "num_axes = %d (1 to %d)", num_axes, kQnAxes);
     if (num_pairs < 0 || 2 * num_pairs > head_dim)
         return api_fail(G2V_ERR_INVALID, "num_pairs = %d (0 to head_dim / 2 = %d)", num_pairs, head_dim / 2);
     if (dtype != G2V_DTYPE_F32 && dtype != G2V_DTYPE_BF16)
@@ -30,8 +30,8 @@ int qn_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim
     if (shared && heads_k > 0 && n_k != n_q)
         return api_fail(G2V_ERR_INVALID, "shared positions need n_k == n_q, got %d and %d", n_k, n_q);
     // workgroups along the tokens are counted in 32 bits
-    if ((double)batch * n_q > 1e9 || (double)batch * n_k > 1e9 || heads_q > 65536 || heads_k > 65536)
-        return api_fail(G2V_ERR_LIMIT, "batch %d x n %d / %d tokens (limit 1e9), heads %d / %d (limit 65536)", batch, n_q, n_k,
+    if ((double)batch * n_q > 1e9 || (double)batch * n_k > 1e9 || heads_q > 8192 || heads_k > 8192)
+        return api_fail(G2V_ERR_LIMIT, "batch %d x n %d / %d tokens (limit 1e9), heads %d / %d (limit 8192)", batch, n_q, n_k,
                         heads_q, heads_k);
     return G2V_OK;
 }

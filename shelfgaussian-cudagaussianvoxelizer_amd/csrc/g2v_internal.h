@@ -259,11 +259,11 @@ struct QkNormArgs {
     float* dw[2];                  // (dim), null: not wanted
     float* dpos[2];                // (batch, n, axes), null: not wanted
     // set by the launches
-    int shift, chunk, blocks0;
-    int64_t dpos_tokens;
-    float *dw_part, *dpos_part;
+    int shift, heads_shift, blocks0;
+    float* dw_part;
 };
-constexpr int kQnBwdBlocks = 1024;   // workgroups of a side in the backward (4 per CU): the rows of dL/dw's partial sums
+constexpr int kQnAxes = 8;           // most coordinates of a position
+constexpr int kQnBwdBlocks = 2048;   // most workgroups of a side in the backward: the rows of dL/dw's partial sums
 hipError_t launch_qk_norm_rotary(const QkNormArgs& a, int dtype, hipStream_t s);
 size_t qk_norm_bwd_workspace(const QkNormArgs& a, int dtype);
 hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& a, int dtype, void* ws, hipStream_t s);

@@ -10,9 +10,12 @@
 //   dL/dtheta_i = sum over the token's heads of dy_2i+1 y_2i - dy_2i y_2i+1  (a cross product: the same before and
 //   after the rotation),   dL/dp_a = sum_i F[a][i] dL/dtheta_i.
 //
-// Bound by bytes: each row is read and written once (forward) or two rows read and one written (backward).  A token
-// takes 2^shift neighbouring lanes of a wave, 16 bytes of its row each, and walks its heads: the sines, cosines and the
-// sums over heads (dtheta, dw) stay in the lanes that need them.
+// Bound by bytes: each row is read and written once (forward), or two rows are read and one is written (backward).  A
+// workgroup takes a few neighbouring tokens: their sines and cosines are computed once for all heads (a sincosf or a few a
+// thread) and go through LDS.  A row is read by a group of 2^shift lanes, 16 bytes a lane; 2^heads_shift neighbouring
+// groups take a token's heads in turn, so that a wave reads pieces of a few rows' length each (with all of a token's heads
+// walked by one group a wave's loads fell on eight tokens' single rows and moved 2.8 TB/s instead of 4.5), and what belongs
+// to the token (its angles, the sum of their gradients over its heads) stays in registers.
 #include "../../include/g2v.h"
 #include "g2v_internal.h"
 
@@ -20,7 +23,8 @@ namespace g2v {
 namespace {
 
 constexpr int kQnThreads = 256;
-constexpr int kQnUnroll = 4;       // heads whose loads are in flight together
+constexpr int kQnUnroll = 4;       // rows whose loads a thread has in flight, forward
+constexpr int kQnAhead = 2;        // the same, backward (two tensors)
 
 template <typename T>
 struct QnVec;
@@ -35,107 +39,159 @@ struct QnVec<__bf16> {
     typedef bf16x8 raw;
 };
 
-// Elements [d, d + n) of a row, zero past the end.
+// Elements [d, d + n) of a row, zero past the end.  AL: rows and D are whole 16-byte vectors; else a vector within the row
+// is still one access (global memory takes any alignment), and only the row's last elements go one by one.
 template <typename T, bool AL>
 __device__ __forceinline__ typename QnVec<T>::raw qn_load(const T* row, int d, int D) {
-    typename QnVec<T>::raw v;
-    if constexpr (AL) {
-        if (d < D) v = *reinterpret_cast<const typename QnVec<T>::raw*>(row + d);
-        else
+    typedef typename QnVec<T>::raw raw;
+    typedef raw raw_any __attribute__((aligned(sizeof(T))));
+    raw v;
 #pragma unroll
-            for (int j = 0; j < QnVec<T>::n; ++j) v[j] = (T)0.0f;
+    for (int j = 0; j < QnVec<T>::n; ++j) v[j] = (T)0.0f;
+    if constexpr (AL) {
+        if (d < D) v = *reinterpret_cast<const raw*>(row + d);
+    } else if (d + QnVec<T>::n <= D) {
+        v = *reinterpret_cast<const raw_any*>(row + d);
     } else {
 #pragma unroll
-        for (int j = 0; j < QnVec<T>::n; ++j) v[j] = d + j < D ? row[d + j] : (T)0.0f;
+        for (int j = 0; j < QnVec<T>::n; ++j)
+            if (d + j < D) v[j] = row[d + j];
     }
     return v;
 }
-// AL: the vector is stored whole (row and D are multiples of its 16 bytes).
 template <typename T, bool AL>
 __device__ __forceinline__ void qn_store(T* row, int d, int D, const float (&o)[QnVec<T>::n]) {
     constexpr int n = QnVec<T>::n;
-    if constexpr (AL) {
-        typename QnVec<T>::raw v;
+    typedef typename QnVec<T>::raw raw;
+    typedef raw raw_any __attribute__((aligned(sizeof(T))));
+    raw v;
 #pragma unroll
-        for (int j = 0; j < n; ++j) v[j] = (T)o[j];
-        if (d < D) *reinterpret_cast<typename QnVec<T>::raw*>(row + d) = v;
+    for (int j = 0; j < n; ++j) v[j] = (T)o[j];
+    if constexpr (AL) {
+        if (d < D) *reinterpret_cast<raw*>(row + d) = v;
+    } else if (d + n <= D) {
+        *reinterpret_cast<raw_any*>(row + d) = v;
     } else {
 #pragma unroll
         for (int j = 0; j < n; ++j)
-            if (d + j < D) row[d + j] = (T)o[j];
+            if (d + j < D) row[d + j] = v[j];
     }
 }
 
-// Sum over the 2^shift lanes of a token.
+// Sum over the 2^shift lanes of a token.  Within 16 lanes by data-parallel moves: after the steps before it every
+// lane of a mirrored half holds the same sum, so a mirror serves as the exchange of the next size.
+template <int kCtrl>
+__device__ __forceinline__ float dpp_add(float v) {
+    const int o = __builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xF, 0xF, true);
+    return v + __int_as_float(o);
+}
 __device__ __forceinline__ float token_sum(float v, int shift) {
-    for (int m = (1 << shift) >> 1; m > 0; m >>= 1) v += __shfl_xor(v, m);
+    if (shift > 0) v = dpp_add<0xB1>(v);     // quad_perm 1 0 3 2
+    if (shift > 1) v = dpp_add<0x4E>(v);     // quad_perm 2 3 0 1
+    if (shift > 2) v = dpp_add<0x141>(v);    // row_half_mirror
+    if (shift > 3) v = dpp_add<0x140>(v);    // row_mirror
+    if (shift > 4) v += __shfl_xor(v, 16);
+    if (shift > 5) v += __shfl_xor(v, 32);
     return v;
 }
 
-// A workgroup's part of the problem: which tokens' side (queries, keys, or both when they share positions).
-struct QnPart {
+// A workgroup's side of the problem: queries, keys, or both when they share positions.
+struct QnSide {
     int64_t tokens;    // B n
     int n;             // tokens of a scene
-    int h0, h1;        // heads, of the heads_q query heads followed by the heads_k key heads
+    int h0, h1;        // heads, of the query heads followed by the key heads
     const float* pos;
 };
 
-__device__ __forceinline__ QnPart qn_part(const QkNormArgs& a, int side) {
-    QnPart p;
-    const int all = a.heads[0] + a.heads[1];
+__device__ __forceinline__ QnSide qn_side(const QkNormArgs& a, int side) {
+    QnSide p;
     p.n = a.n[side];
     p.tokens = (int64_t)a.batch * p.n;
     p.h0 = side ? a.heads[0] : 0;
-    p.h1 = a.shared || side ? all : a.heads[0];
+    p.h1 = a.shared || side ? a.heads[0] + a.heads[1] : a.heads[0];
     p.pos = a.pos[side];
     return p;
 }
 
-// Sines and cosines of this lane's pairs; 0 and 1 past the table.  sincosf: its reduction keeps float32
-// accuracy for any angle (positions in metres reach hundreds of radians).
+// Cosine and sine of this lane's pairs of its token (1 and 0 past the table), through LDS: the workgroup's tokens
+// [t0, t0 + toks) have them computed once each.  sincosf: its reduction keeps float32 accuracy for any angle (positions in
+// metres reach hundreds of radians).
 template <int N>
-__device__ __forceinline__ void qn_angles(const QkNormArgs& a, const float* pos, int d, float (&c)[N], float (&s)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const int i = d / 2 + j;
-        c[j] = 1.0f;
-        s[j] = 0.0f;
-        if (i < a.pairs) {
-            float t = 0.0f;
-            for (int x = 0; x < a.axes; ++x) t = fmaf(pos[x], a.freqs[x * a.pairs + i], t);
-            sincosf(t, &s[j], &c[j]);
+__device__ __forceinline__ void qn_angles(const QkNormArgs& a, const QnSide& p, int64_t t0, int token, int d, float2* rot,
+                                          float2 (&f)[N / 2]) {
+    const int width = (N / 2) << a.shift, toks = kQnThreads >> (a.shift + a.heads_shift);
+    __syncthreads();    // the last tokens' are read
+    for (int e = threadIdx.x; e < toks * width; e += kQnThreads) {
+        const int t = e / width, i = e - t * width;
+        float c = 1.0f, s = 0.0f;
+        if (i < a.pairs && t0 + t < p.tokens) {
+            const float* pos = p.pos + (t0 + t) * a.axes;
+            float w = 0.0f;
+            for (int x = 0; x < a.axes; ++x) w = fmaf(pos[x], a.freqs[x * a.pairs + i], w);
+            sincosf(w, &s, &c);
         }
+        rot[e] = make_float2(c, s);
     }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) f[j] = rot[token * width + d / 2 + j];
+}
+
+// This lane's weights of both tensors (ones without).
+template <int N>
+__device__ __forceinline__ void qn_weights(const QkNormArgs& a, int d, float (&w)[2][N]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[k][j] = a.w[k] && d + j < a.dim ? a.w[k][d + j] : 1.0f;
+}
+
+// A thread's place in its workgroup: lane of a row, token, and which of the token's groups it is in.
+struct QnPlace {
+    int d, token, first, step;
+};
+template <int N>
+__device__ __forceinline__ QnPlace qn_place(const QkNormArgs& a) {
+    const int group = threadIdx.x >> a.shift;
+    QnPlace o;
+    o.d = (threadIdx.x & ((1 << a.shift) - 1)) * N;
+    o.step = 1 << a.heads_shift;
+    o.token = group >> a.heads_shift;
+    o.first = group & (o.step - 1);
+    return o;
 }
 
 template <typename T, bool AL>
 __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
     constexpr int N = QnVec<T>::n;
+    __shared__ float2 rot[kQnThreads * (N / 2)];
     const int side = blockIdx.x >= a.blocks0;
-    const QnPart p = qn_part(a, side);
-    const int lane = threadIdx.x & 63, slots = kQnThreads >> a.shift;
-    const int d = (lane & ((1 << a.shift) - 1)) * N;
-    const int64_t tok = (int64_t)(blockIdx.x - (side ? a.blocks0 : 0)) * slots + (threadIdx.x >> a.shift);
-    const int64_t t = tok < p.tokens ? tok : p.tokens - 1;      // lanes past the end repeat the last token, unstored
+    const QnSide p = qn_side(a, side);
+    const QnPlace o = qn_place<N>(a);
+    const int64_t t0 = (int64_t)(blockIdx.x - (side ? a.blocks0 : 0)) * (kQnThreads >> (a.shift + a.heads_shift));
+    const bool live = t0 + o.token < p.tokens;
+    const int64_t t = live ? t0 + o.token : p.tokens - 1;     // groups past the end repeat the last token, unstored
     const int64_t b = t / p.n, i = t - b * p.n;
-    float c[N / 2], s[N / 2];
-    qn_angles(a, p.pos + t * a.axes, d, c, s);
-    const int hb = p.h0 + (int)blockIdx.y * a.chunk;
-    const int he = hb + a.chunk < p.h1 ? hb + a.chunk : p.h1;
+    const T* xq = static_cast<const T*>(a.x[0]) + b * a.sb[0] + i * a.sn[0];
+    const T* xk = static_cast<const T*>(a.x[1]) + b * a.sb[1] + i * a.sn[1];
+    float w[2][N];
+    float2 f[N / 2];
+    qn_weights<N>(a, o.d, w);
+    qn_angles<N>(a, p, t0, o.token, o.d, rot, f);
     const float inv_d = 1.0f / (float)a.dim;
-    for (int h0 = hb; h0 < he; h0 += kQnUnroll) {
+    for (int h0 = p.h0 + o.first; h0 < p.h1; h0 += o.step * kQnUnroll) {
         typename QnVec<T>::raw x[kQnUnroll];
 #pragma unroll
         for (int u = 0; u < kQnUnroll; ++u) {
-            const int h = h0 + u < he ? h0 + u : he - 1, k = h >= a.heads[0];
-            const T* row = static_cast<const T*>(a.x[k]) + b * a.sb[k] + i * a.sn[k] +
-                           (int64_t)(h - (k ? a.heads[0] : 0)) * a.sh[k];
-            x[u] = qn_load<T, AL>(row, d, a.dim);
+            const int h = h0 + u * o.step;
+            const bool k = h >= a.heads[0];
+            if (h < p.h1) x[u] = qn_load<T, AL>(k ? xk + (h - a.heads[0]) * a.sh[1] : xq + h * a.sh[0], o.d, a.dim);
         }
 #pragma unroll
         for (int u = 0; u < kQnUnroll; ++u) {
-            if (h0 + u >= he) break;
-            const int h = h0 + u, k = h >= a.heads[0];
+            const int h = h0 + u * o.step;   // the same for all lanes of a group
+            if (h >= p.h1) break;
+            const bool k = h >= a.heads[0];
             float ss = 0.0f, y[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
@@ -143,144 +199,174 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
                 ss = fmaf(y[j], y[j], ss);
             }
             const float r = 1.0f / sqrtf(fmaf(token_sum(ss, a.shift), inv_d, a.eps));
-            const float* w = a.w[k];
 #pragma unroll
-            for (int j = 0; j < N; ++j) y[j] *= r * (w ? (d + j < a.dim ? w[d + j] : 0.0f) : 1.0f);
+            for (int j = 0; j < N; ++j) y[j] *= r * (k ? w[1][j] : w[0][j]);
 #pragma unroll
             for (int j = 0; j < N / 2; ++j) {
                 const float y0 = y[2 * j], y1 = y[2 * j + 1];
-                y[2 * j] = y0 * c[j] - y1 * s[j];
-                y[2 * j + 1] = y0 * s[j] + y1 * c[j];
+                y[2 * j] = y0 * f[j].x - y1 * f[j].y;
+                y[2 * j + 1] = y0 * f[j].y + y1 * f[j].x;
             }
-            T* row = static_cast<T*>(a.out[k]) + (t * a.heads[k] + (h - (k ? a.heads[0] : 0))) * a.dim;
-            if (tok < p.tokens) qn_store<T, AL>(row, d, a.dim, y);
+            T* row = k ? static_cast<T*>(a.out[1]) + (t * a.heads[1] + h - a.heads[0]) * a.dim
+                       : static_cast<T*>(a.out[0]) + (t * a.heads[0] + h) * a.dim;
+            if (live) qn_store<T, AL>(row, o.d, a.dim, y);
         }
     }
 }
 
-// Workgroups stride over the tokens of their side; a workgroup's sums of dL/dw go to dw_part, a head chunk's position
-// gradients to dpos_part (k_qk_norm_sums adds both in a fixed order).
+// Workgroups stride over the tokens of their side; a workgroup's sums of dL/dw go to dw_part (k_qk_norm_sums adds those, in a
+// fixed order).
 template <typename T, bool AL>
 __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a) {
     constexpr int N = QnVec<T>::n;
     __shared__ float red[kQnThreads * N];
+    float2* rot = reinterpret_cast<float2*>(red);
+    __shared__ float dcell[kQnThreads * kQnAxes];
     const int side = blockIdx.x >= a.blocks0;
-    const QnPart p = qn_part(a, side);
-    const int lane = threadIdx.x & 63, slots = kQnThreads >> a.shift;
-    const int d = (lane & ((1 << a.shift) - 1)) * N;
+    const QnSide p = qn_side(a, side);
+    const QnPlace o = qn_place<N>(a);
+    const int toks = kQnThreads >> (a.shift + a.heads_shift);
     const int blk = blockIdx.x - (side ? a.blocks0 : 0), nblk = side ? gridDim.x - a.blocks0 : a.blocks0;
-    const int hb = p.h0 + (int)blockIdx.y * a.chunk;
-    const int he = hb + a.chunk < p.h1 ? hb + a.chunk : p.h1;
     const float inv_d = 1.0f / (float)a.dim;
-    float dw[2][N];
+    float* dpos = a.dpos[side];
+    float w[2][N], dw[2][N];
+    float2 f[N / 2];
+    qn_weights<N>(a, o.d, w);
 #pragma unroll
     for (int j = 0; j < N; ++j) dw[0][j] = dw[1][j] = 0.0f;
-    for (int64_t t0 = (int64_t)blk * slots; t0 < p.tokens; t0 += (int64_t)nblk * slots) {
-        const int64_t tok = t0 + (threadIdx.x >> a.shift);
-        const bool live = tok < p.tokens;
-        const int64_t t = live ? tok : p.tokens - 1;
+    for (int64_t t0 = (int64_t)blk * toks; t0 < p.tokens; t0 += (int64_t)nblk * toks) {
+        const bool live = t0 + o.token < p.tokens;
+        const int64_t t = live ? t0 + o.token : p.tokens - 1;
         const int64_t b = t / p.n, i = t - b * p.n;
-        float c[N / 2], s[N / 2], dth[N / 2];
-        qn_angles(a, p.pos + t * a.axes, d, c, s);
+        const T* xq = static_cast<const T*>(a.x[0]) + b * a.sb[0] + i * a.sn[0];
+        const T* xk = static_cast<const T*>(a.x[1]) + b * a.sb[1] + i * a.sn[1];
+        const T* gq = static_cast<const T*>(a.g[0]) + b * a.gsb[0] + i * a.gsn[0];
+        const T* gk = static_cast<const T*>(a.g[1]) + b * a.gsb[1] + i * a.gsn[1];
+        float dth[N / 2];
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) dth[j] = 0.0f;
-        for (int h = hb; h < he; ++h) {
-            const int k = h >= a.heads[0], hk = h - (k ? a.heads[0] : 0);
-            const T* xr = static_cast<const T*>(a.x[k]) + b * a.sb[k] + i * a.sn[k] + (int64_t)hk * a.sh[k];
-            const T* gr = static_cast<const T*>(a.g[k]) + b * a.gsb[k] + i * a.gsn[k] + (int64_t)hk * a.gsh[k];
-            const auto xv = qn_load<T, AL>(xr, d, a.dim);
-            const auto gv = qn_load<T, AL>(gr, d, a.dim);
-            const float* w = a.w[k];
-            float x[N], dy[N], wv[N], ss = 0.0f, st = 0.0f;
+        qn_angles<N>(a, p, t0, o.token, o.d, rot, f);
+        for (int h0 = p.h0 + o.first; h0 < p.h1; h0 += o.step * kQnAhead) {
+            typename QnVec<T>::raw xv[kQnAhead], gv[kQnAhead];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                x[j] = (float)xv[j];
-                dy[j] = live ? (float)gv[j] : 0.0f;
-                wv[j] = w ? (d + j < a.dim ? w[d + j] : 0.0f) : 1.0f;
-                ss = fmaf(x[j], x[j], ss);
+            for (int u = 0; u < kQnAhead; ++u) {
+                const int h = h0 + u * o.step;
+                if (h >= p.h1) break;
+                const bool k = h >= a.heads[0];
+                xv[u] = qn_load<T, AL>(k ? xk + (h - a.heads[0]) * a.sh[1] : xq + h * a.sh[0], o.d, a.dim);
+                gv[u] = qn_load<T, AL>(k ? gk + (h - a.heads[0]) * a.gsh[1] : gq + h * a.gsh[0], o.d, a.dim);
             }
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) {
-                const float g0 = dy[2 * j], g1 = dy[2 * j + 1];
-                dy[2 * j] = g0 * c[j] + g1 * s[j];
-                dy[2 * j + 1] = g1 * c[j] - g0 * s[j];
-            }
+            for (int u = 0; u < kQnAhead; ++u) {
+                const int h = h0 + u * o.step;   // the same for all lanes of a group
+                if (h >= p.h1) break;
+                const bool k = h >= a.heads[0];
+                float x[N], dy[N], wv[N], ss = 0.0f, st = 0.0f;
 #pragma unroll
-            for (int j = 0; j < N; ++j) st = fmaf(wv[j] * dy[j], x[j], st);
-            ss = token_sum(ss, a.shift);
-            st = token_sum(st, a.shift);
-            const float r = 1.0f / sqrtf(fmaf(ss, inv_d, a.eps));
-            const float q = r * r * r * inv_d * st;
+                for (int j = 0; j < N; ++j) {
+                    x[j] = (float)xv[u][j];
+                    dy[j] = live ? (float)gv[u][j] : 0.0f;
+                    wv[j] = k ? w[1][j] : w[0][j];
+                    ss = fmaf(x[j], x[j], ss);
+                }
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) {
-                const float y0 = wv[2 * j] * x[2 * j] * r, y1 = wv[2 * j + 1] * x[2 * j + 1] * r;
-                dth[j] += dy[2 * j + 1] * y0 - dy[2 * j] * y1;
-            }
-            float dx[N];
+                for (int j = 0; j < N / 2; ++j) {
+                    const float g0 = dy[2 * j], g1 = dy[2 * j + 1];
+                    dy[2 * j] = g0 * f[j].x + g1 * f[j].y;
+                    dy[2 * j + 1] = g1 * f[j].x - g0 * f[j].y;
+                }
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float z = dy[j] * x[j] * r;
-                if (k) dw[1][j] += z;
-                else dw[0][j] += z;
-                dx[j] = r * wv[j] * dy[j] - x[j] * q;
+                for (int j = 0; j < N; ++j) st = fmaf(wv[j] * dy[j], x[j], st);
+                ss = token_sum(ss, a.shift);
+                st = token_sum(st, a.shift);
+                const float r = 1.0f / sqrtf(fmaf(ss, inv_d, a.eps));
+                const float q = r * r * r * inv_d * st;
+                float dx[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float xr = x[j] * r;
+                    const float z = dy[j] * xr;
+                    dw[0][j] += k ? 0.0f : z;
+                    dw[1][j] += k ? z : 0.0f;
+                    dx[j] = r * wv[j] * dy[j] - x[j] * q;
+                    x[j] = wv[j] * xr;
+                }
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) dth[j] += dy[2 * j + 1] * x[2 * j] - dy[2 * j] * x[2 * j + 1];
+                T* row = k ? static_cast<T*>(a.dx[1]) + (t * a.heads[1] + h - a.heads[0]) * a.dim
+                           : static_cast<T*>(a.dx[0]) + (t * a.heads[0] + h) * a.dim;
+                if (live) qn_store<T, AL>(row, o.d, a.dim, dx);
             }
-            T* row = static_cast<T*>(a.dx[k]) + (t * a.heads[k] + hk) * a.dim;
-            if (live) qn_store<T, AL>(row, d, a.dim, dx);
         }
-        if (a.dpos_part) {
-            float* out = a.dpos_part + ((int64_t)blockIdx.y * a.dpos_tokens + (side ? (int64_t)a.batch * a.n[0] : 0) + t) * a.axes;
-            for (int x = 0; x < a.axes; ++x) {
+        if (dpos) {   // of each of a token's groups, then of the token
+            for (int e = 0; e < a.axes; ++e) {
                 float v = 0.0f;
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j)
-                    if (d / 2 + j < a.pairs) v = fmaf(a.freqs[x * a.pairs + d / 2 + j], dth[j], v);
+                    if (o.d / 2 + j < a.pairs) v = fmaf(a.freqs[e * a.pairs + o.d / 2 + j], dth[j], v);
                 v = token_sum(v, a.shift);
-                if (live && d == 0) out[x] = v;
+                if (o.d == 0) dcell[(threadIdx.x >> a.shift) * a.axes + e] = v;
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < toks * a.axes; e += kQnThreads) {
+                const int tk = e / a.axes;
+                float v = 0.0f;
+                for (int g = 0; g < o.step; ++g) v += dcell[(tk * o.step + g) * a.axes + e - tk * a.axes];
+                if (t0 + tk < p.tokens) dpos[t0 * a.axes + e] = v;
             }
         }
     }
     if (!a.dw_part) return;
-    // the workgroup's sums: lanes of the same elements are 2^shift apart
+    // the workgroup's sums: lanes of the same elements are 2^shift apart.  Threads / width of them share an element's sum.
+    const int span = N << a.shift, parts = kQnThreads > span ? kQnThreads / span : 1, slots = kQnThreads >> a.shift;
+#pragma unroll
     for (int k = 0; k < 2; ++k) {
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < N; ++j) red[j * kQnThreads + threadIdx.x] = dw[k][j];
         __syncthreads();
-        const int width = N << a.shift;
-        for (int e = threadIdx.x; e < width; e += kQnThreads) {
+        for (int c = threadIdx.x; c < span * parts; c += kQnThreads) {
+            const int e = c % span;
             float v = 0.0f;
-            for (int o = 0; o < slots; ++o) v += red[(e % N) * kQnThreads + (o << a.shift) + e / N];
-            if (e < a.dim)
-                a.dw_part[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + k) * a.dim + e] = v;
+            for (int g = c / span; g < slots; g += parts) v += red[(e % N) * kQnThreads + (g << a.shift) + e / N];
+            if (parts == 1) {
+                if (e < a.dim) a.dw_part[((int64_t)blockIdx.x * 2 + k) * a.dim + e] = v;
+            } else {
+                dcell[c] = v;
+            }
+        }
+        if (parts == 1) continue;
+        __syncthreads();
+        for (int e = threadIdx.x; e < a.dim; e += kQnThreads) {
+            float v = 0.0f;
+            for (int g = 0; g < parts; ++g) v += dcell[g * span + e];
+            a.dw_part[((int64_t)blockIdx.x * 2 + k) * a.dim + e] = v;
         }
     }
 }
 
-// Sums of `rows` rows of `cols` values into out (cols), each column by 16 lanes in a fixed order.
-__global__ void __launch_bounds__(kQnThreads) k_qk_norm_sums(QkNormArgs a, int64_t rows, int col_blocks, int chunks) {
-    if ((int)blockIdx.x < col_blocks) {   // dL/dw of queries and keys, side by side
-        __shared__ float red[kQnThreads];
-        const int cols = 2 * a.dim;
-        const int col = blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
-        float v = 0.0f;
-        if (col < cols)
-            for (int64_t r = part; r < rows; r += 16) v += a.dw_part[r * cols + col];
-        red[threadIdx.x] = v;
-        __syncthreads();
-        if (part == 0 && col < cols) {
-            for (int o = 1; o < 16; ++o) v += red[o * 16 + (threadIdx.x & 15)];
-            float* dst = a.dw[col >= a.dim];
-            if (dst) dst[col >= a.dim ? col - a.dim : col] = v;
-        }
-        return;
-    }
-    const int64_t e = (int64_t)(blockIdx.x - col_blocks) * kQnThreads + threadIdx.x;
-    const int64_t nq = (int64_t)a.batch * a.n[0] * a.axes, all = a.dpos_tokens * a.axes;
-    if (e >= all) return;
+// dL/dw from the workgroups' parts (`rows` rows of both weights side by side): 16 columns a workgroup, 64 lanes a column,
+// a fixed order.
+constexpr int kQnSumThreads = 1024;
+__global__ void __launch_bounds__(kQnSumThreads) k_qk_norm_sums(QkNormArgs a, int rows) {
+    __shared__ float red[kQnSumThreads];
+    const int cols = 2 * a.dim;
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
     float v = 0.0f;
-    for (int y = 0; y < chunks; ++y) v += a.dpos_part[y * all + e];
-    float* dst = a.dpos[e >= nq];
-    if (dst) dst[e >= nq ? e - nq : e] = v;
+    if (col < cols) {
+#pragma unroll 8
+        for (int r = part; r < rows; r += 64) v += a.dw_part[(int64_t)r * cols + col];
+    }
+    red[threadIdx.x] = v;
+    __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) {
+        if (part < o) red[threadIdx.x] += red[threadIdx.x + 16 * o];
+        __syncthreads();
+    }
+    if (part == 0 && col < cols) {
+        float* dst = col >= a.dim ? a.dw[1] : a.dw[0];
+        if (dst) dst[col >= a.dim ? col - a.dim : col] = red[threadIdx.x];
+    }
 }
 
 template <typename T>
@@ -305,28 +391,30 @@ bool qn_aligned(const QkNormArgs& a, bool backward) {
     return ok;
 }
 
-// Lanes of a token (as a shift), heads of a workgroup and workgroups along the tokens.  A token's lanes cover its row
-// with 16 bytes each; heads are dealt to several workgroups only while the tokens alone leave most SIMDs without a wave.
+constexpr int kQnWant = 2048;   // workgroups that fill the card (8 waves a SIMD)
+
+// Lanes of a row and groups of a token (as shifts), and workgroups of each side.  A token's groups read neighbouring
+// rows: as many as make 512 bytes, more where the tokens would not fill the card, never more than heads.
 struct QnGrid {
-    int shift, chunk, chunks, blocks[2];
+    int shift, heads_shift, blocks[2];
 };
 QnGrid qn_grid(const QkNormArgs& a, bool bf16, bool backward) {
     QnGrid g;
     const int lanes = (int)ceil_div(a.dim, bf16 ? 8 : 4);
     g.shift = 0;
     while ((1 << g.shift) < lanes) ++g.shift;
-    const int slots = kQnThreads >> g.shift;
-    const int most = a.shared ? a.heads[0] + a.heads[1] : (a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1]);
-    const int64_t t[2] = {(int64_t)a.batch * a.n[0], a.shared ? 0 : (int64_t)a.batch * a.n[1]};
-    int64_t blocks = 0;
+    const int heads = a.shared ? a.heads[0] + a.heads[1] : (a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1]);
+    const int64_t t[2] = {a.heads[0] + (a.shared ? a.heads[1] : 0) > 0 ? (int64_t)a.batch * a.n[0] : 0,
+                          a.shared || a.heads[1] == 0 ? 0 : (int64_t)a.batch * a.n[1]};
+    auto blocks = [&](int side) { return ceil_div(t[side], kQnThreads >> (g.shift + g.heads_shift)); };
+    const int row = a.dim * (bf16 ? 2 : 4);
+    g.heads_shift = 0;
+    while (g.shift + g.heads_shift < 8 && (1 << g.heads_shift) < heads && ((row << g.heads_shift) < 512 || blocks(0) + blocks(1) < kQnWant))
+        ++g.heads_shift;
     for (int k = 0; k < 2; ++k) {
-        g.blocks[k] = (int)ceil_div(t[k], slots);
+        g.blocks[k] = (int)blocks(k);
         if (backward && g.blocks[k] > kQnBwdBlocks) g.blocks[k] = kQnBwdBlocks;
-        blocks += g.blocks[k];
     }
-    g.chunk = most;
-    while (g.chunk > kQnUnroll && blocks * ceil_div(most, g.chunk) < 1024) g.chunk = (int)ceil_div(g.chunk, 2);
-    g.chunks = g.chunk > 0 ? (int)ceil_div(most, g.chunk) : 0;
     return g;
 }
 
@@ -336,12 +424,11 @@ hipError_t launch_qk_norm_rotary(const QkNormArgs& args, int dtype, hipStream_t 
     QkNormArgs a = args;
     const bool bf16 = dtype == kDtBF16;
     const QnGrid g = qn_grid(a, bf16, false);
-    const int blocks = g.blocks[0] + g.blocks[1];
-    if (blocks == 0 || g.chunks == 0) return hipSuccess;
     a.shift = g.shift;
-    a.chunk = g.chunk;
+    a.heads_shift = g.heads_shift;
     a.blocks0 = g.blocks[0];
-    const dim3 grid(blocks, g.chunks), block(kQnThreads);
+    const dim3 grid(g.blocks[0] + g.blocks[1]), block(kQnThreads);
+    if (grid.x == 0) return hipSuccess;
     if (bf16) {
         if (qn_aligned<__bf16>(a, false)) G2V_LAUNCH((k_qk_norm_rotary<__bf16, true>), grid, block, 0, s, a);
         else G2V_LAUNCH((k_qk_norm_rotary<__bf16, false>), grid, block, 0, s, a);
@@ -355,8 +442,7 @@ hipError_t launch_qk_norm_rotary(const QkNormArgs& args, int dtype, hipStream_t 
 size_t qk_norm_bwd_workspace(const QkNormArgs& a, int dtype) {
     const QnGrid g = qn_grid(a, dtype == kDtBF16, true);
     Carver c(nullptr, (size_t)-1);
-    c.take<float>((size_t)(g.blocks[0] + g.blocks[1]) * g.chunks * 2 * a.dim);
-    c.take<float>((size_t)g.chunks * a.batch * ((size_t)a.n[0] + (a.shared ? 0 : a.n[1])) * a.axes);
+    c.take<float>((size_t)(g.blocks[0] + g.blocks[1]) * 2 * a.dim);
     return c.off + 256;
 }
 
@@ -364,19 +450,15 @@ hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& args, int dtype, void* ws
     QkNormArgs a = args;
     const bool bf16 = dtype == kDtBF16;
     const QnGrid g = qn_grid(a, bf16, true);
-    const int blocks = g.blocks[0] + g.blocks[1];
     a.shift = g.shift;
-    a.chunk = g.chunk;
+    a.heads_shift = g.heads_shift;
     a.blocks0 = g.blocks[0];
-    a.dpos_tokens = (int64_t)a.batch * ((int64_t)a.n[0] + (a.shared ? 0 : a.n[1]));
+    const bool want_w = a.dw[0] || a.dw[1];
+    const dim3 grid(g.blocks[0] + g.blocks[1]), block(kQnThreads);
     Carver c(ws, (size_t)-1);
-    float* wp = c.take<float>((size_t)blocks * g.chunks * 2 * a.dim);
-    float* pp = c.take<float>((size_t)g.chunks * a.dpos_tokens * a.axes);
-    const bool want_w = a.dw[0] || a.dw[1], want_p = a.dpos[0] || a.dpos[1];
-    a.dw_part = want_w ? wp : nullptr;
-    a.dpos_part = want_p ? pp : nullptr;
-    if (blocks > 0 && g.chunks > 0) {
-        const dim3 grid(blocks, g.chunks), block(kQnThreads);
+    float* part = c.take<float>((size_t)grid.x * 2 * a.dim);
+    a.dw_part = want_w ? part : nullptr;
+    if (grid.x > 0) {
         if (bf16) {
             if (qn_aligned<__bf16>(a, true)) G2V_LAUNCH((k_qk_norm_rotary_bwd<__bf16, true>), grid, block, 0, s, a);
             else G2V_LAUNCH((k_qk_norm_rotary_bwd<__bf16, false>), grid, block, 0, s, a);
@@ -385,11 +467,8 @@ hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& args, int dtype, void* ws
             else G2V_LAUNCH((k_qk_norm_rotary_bwd<float, false>), grid, block, 0, s, a);
         }
     }
-    const int col_blocks = want_w ? (int)ceil_div(2 * a.dim, 16) : 0;
-    const int64_t pos_blocks = want_p ? ceil_div(a.dpos_tokens * a.axes, kQnThreads) : 0;
-    if (col_blocks + pos_blocks > 0)
-        G2V_LAUNCH(k_qk_norm_sums, dim3((unsigned)(col_blocks + pos_blocks)), dim3(kQnThreads), 0, s, a,
-                   (int64_t)blocks * g.chunks, col_blocks, g.chunks);
+    if (want_w)
+        G2V_LAUNCH(k_qk_norm_sums, dim3((unsigned)ceil_div(2 * a.dim, 16)), dim3(kQnSumThreads), 0, s, a, (int)grid.x);
     return hipGetLastError();
 }
 
