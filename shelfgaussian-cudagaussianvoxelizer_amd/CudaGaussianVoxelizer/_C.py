@@ -7,6 +7,7 @@ caller's current HIP stream.  Outputs and workspaces come from PyTorch's caching
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -792,12 +793,26 @@ def covariance_from_scale_rotation_backward(scales, rotations, grad_cov):
     return gs, gq
 
 
+# ---- attention in front of the splat --------------------------------------------------------------
+# These calls are short, and a training step makes them from two threads (autograd runs backwards on its own), so their
+# host side is kept to one check a tensor: checked arguments serve the backward as they are.
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(device):
+    """The caller's current stream, as a number."""
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 def _heads_input(t, name, like=None):
     """(B, N, H, D) rows of float32 or bfloat16 on the GPU, in any layout with unit stride along D (others are
     copied); like: the tensor whose type and device it has to share."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name} must be a GPU tensor, got {t.device}")
     if t.dtype not in _FEAT_DTYPES:
         raise RuntimeError(f"expected scalar type Float or BFloat16 for {name} but found {t.dtype}")
@@ -805,63 +820,110 @@ def _heads_input(t, name, like=None):
         raise RuntimeError(f"{name} must be (B, N, H, D), got {tuple(t.shape)}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise RuntimeError(f"{name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
-    t = t.detach()
-    return t if t.stride(3) == 1 else t.contiguous()
+    return t if t.stride(3) == 1 else t.detach().contiguous()
+
+
+_Strides = ctypes.c_longlong * 3
 
 
 def _strides(t):
-    return None if t is None else (ctypes.c_longlong * 3)(*t.stride()[:3])
+    return None if t is None else _Strides(*t.stride()[:3])
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _plain_f32(t, name, shape, device):
     """A contiguous float32 tensor of this shape on this device (None passes)."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or tuple(t.shape) != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or t.shape != shape:
         got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
         raise RuntimeError(f"{name} must be float32 {shape} on {device}, got {got}")
-    return t.detach().contiguous()
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
-def _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions):
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(query, *args):
+    """What a *_workspace entry point of the library answers to these sizes (0: refused, by the call itself)."""
+    return max(1, getattr(_lib.load(), query)(*args))
+
+
+def _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions, eps):
+    """((q, k, positions, freqs, q_weight, k_weight, k_positions) as the kernels take them, what else a call takes)."""
     q = _heads_input(q, "q")
     B, nq, hq, D = q.shape
     dev = q.device
+    nk = hk = 0
     if k is not None:
         k = _heads_input(k, "k", q)
-        if k.shape[0] != B or k.shape[3] != D or (k_positions is None and k.shape[1] != nq):
+        Bk, nk, hk, Dk = k.shape
+        if Bk != B or Dk != D or (k_positions is None and nk != nq):
             raise RuntimeError(f"k {tuple(k.shape)} does not go with q {tuple(q.shape)}"
                                + ("" if k_positions is not None else " (without k_positions the tokens are the same)"))
-    nk, hk = (0, 0) if k is None else (k.shape[1], k.shape[2])
+    else:
+        k_positions = k_weight = None
+        nk = nq
     if not isinstance(freqs, torch.Tensor) or freqs.dim() != 2:
         raise RuntimeError("freqs must be (axes, pairs)")
     axes, pairs = freqs.shape
     freqs = _plain_f32(freqs, "freqs", (axes, pairs), dev)
-    positions = _plain_f32(positions, "positions", (B, nq, axes), dev)
     if positions is None:
         raise RuntimeError("positions must be a tensor")
-    k_positions = _plain_f32(k_positions, "k_positions", (B, nk, axes), dev) if k is not None else None
+    positions = _plain_f32(positions, "positions", (B, nq, axes), dev)
+    k_positions = _plain_f32(k_positions, "k_positions", (B, nk, axes), dev)
     q_weight = _plain_f32(q_weight, "q_weight", (D,), dev)
     k_weight = _plain_f32(k_weight, "k_weight", (D,), dev)
-    sizes = (B, nq, nk if k_positions is not None or k is None else nq, hq, hk, D, axes)
-    return q, k, positions, freqs, q_weight, k_weight, k_positions, sizes, pairs
+    call = ((B, nq, nk, hq, hk, D, axes), pairs, _FEAT_DTYPES[q.dtype], float(eps))
+    return (q, k, positions, freqs, q_weight, k_weight, k_positions), call
+
+
+def _qk_norm_forward(inputs, call):
+    q, k, pos, freqs, qw, kw, kpos = inputs
+    sizes, pairs, fdt, eps = call
+    dev = q.device
+    with _OnDevice(dev):
+        oq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        ok = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+        rc = _lib.load().g2v_qk_norm_rotary_forward(*sizes, pairs, _addr(q), _strides(q), _addr(k), _strides(k), fdt,
+                                                    _addr(qw), _addr(kw), _addr(pos), _addr(kpos), _addr(freqs), eps,
+                                                    _addr(oq), _addr(ok), _stream_of(dev))
+    if rc:
+        _lib.check(rc, "qk_norm_rotary_forward")
+    return oq, ok
+
+
+def _qk_norm_backward(gq, gk, inputs, call, want_weights, want_positions):
+    q, k, pos, freqs, qw, kw, kpos = inputs
+    sizes, pairs, fdt, eps = call
+    dev, f32 = q.device, torch.float32
+    if gq.shape != q.shape or (k is not None and gk.shape != k.shape):
+        raise RuntimeError(f"gradients must be {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
+    with _OnDevice(dev):
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+        dqw = torch.empty(sizes[5], dtype=f32, device=dev) if want_weights[0] else None
+        dkw = torch.empty(sizes[5], dtype=f32, device=dev) if want_weights[1] and k is not None else None
+        dpos = torch.empty(pos.shape, dtype=f32, device=dev) if want_positions[0] else None
+        dkpos = torch.empty(kpos.shape, dtype=f32, device=dev) if want_positions[1] and kpos is not None else None
+        nws = _workspace_bytes("g2v_qk_norm_rotary_backward_workspace", *sizes, fdt, 1 if kpos is None else 0)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        rc = _lib.load().g2v_qk_norm_rotary_backward(*sizes, pairs, _addr(q), _strides(q), _addr(k), _strides(k), fdt,
+                                                     _addr(qw), _addr(kw), _addr(pos), _addr(kpos), _addr(freqs), eps,
+                                                     _addr(gq), _strides(gq), _addr(gk), _strides(gk), _addr(dq),
+                                                     _addr(dk), _addr(dqw), _addr(dkw), _addr(dpos), _addr(dkpos),
+                                                     ws.data_ptr(), nws, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "qk_norm_rotary_backward")
+    return dq, dk, dqw, dkw, dpos, dkpos
 
 
 def qk_norm_rotary_forward(q, k, positions, freqs, q_weight=None, k_weight=None, k_positions=None, eps=1e-6):
     """(q', k'): the root-mean-square norm of every head of q (B, Nq, Hq, D) and k (B, Nk, Hk, D; or None), times
     q_weight / k_weight (D,), and its rotation by the token's position: pair i of a head turns by the angle
     sum_a positions[..., a] freqs[a, i].  k_positions None: the keys are the queries' tokens."""
-    lib = _lib.load()
-    q, k, pos, freqs, qw, kw, kpos, sizes, pairs = _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions)
-    dev = q.device
-    with _OnDevice(dev):
-        oq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        ok = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
-        _lib.check(lib.g2v_qk_norm_rotary_forward(*sizes, pairs, _ptr(q), _strides(q), _ptr(k), _strides(k),
-                                                  _FEAT_DTYPES[q.dtype], _ptr(qw), _ptr(kw), _ptr(pos), _ptr(kpos),
-                                                  _ptr(freqs), float(eps), _ptr(oq), _ptr(ok), _stream(dev)),
-                   "qk_norm_rotary_forward")
-    return oq, ok
+    return _qk_norm_forward(*_qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions, eps))
 
 
 def qk_norm_rotary_backward(grad_q_out, grad_k_out, q, k, positions, freqs, q_weight=None, k_weight=None,
@@ -869,41 +931,10 @@ def qk_norm_rotary_backward(grad_q_out, grad_k_out, q, k, positions, freqs, q_we
     """(grad_q, grad_k, grad_q_weight, grad_k_weight, grad_positions, grad_k_positions) of qk_norm_rotary_forward; the
     float32 weight and position gradients are None where not wanted (grad_k_positions also with shared positions,
     whose gradient is grad_positions)."""
-    lib = _lib.load()
-    q, k, pos, freqs, qw, kw, kpos, sizes, pairs = _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions)
-    dev = q.device
-    gq = _heads_input(grad_q_out, "grad_q_out", q)
-    gk = None if k is None else _heads_input(grad_k_out, "grad_k_out", q)
-    if gq.shape != q.shape or (k is not None and gk.shape != k.shape):
-        raise RuntimeError(f"gradients must be {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
-    D = q.shape[3]
-    with _OnDevice(dev):
-        f32 = dict(dtype=torch.float32, device=dev)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
-        dqw = torch.empty(D, **f32) if want_weights[0] else None
-        dkw = torch.empty(D, **f32) if want_weights[1] and k is not None else None
-        dpos = torch.empty(pos.shape, **f32) if want_positions[0] else None
-        dkpos = torch.empty(kpos.shape, **f32) if want_positions[1] and kpos is not None else None
-        ws = torch.empty(lib.g2v_qk_norm_rotary_backward_workspace(*sizes, _FEAT_DTYPES[q.dtype], 1 if kpos is None else 0),
-                         dtype=torch.uint8, device=dev)
-        _lib.check(lib.g2v_qk_norm_rotary_backward(*sizes, pairs, _ptr(q), _strides(q), _ptr(k), _strides(k),
-                                                   _FEAT_DTYPES[q.dtype], _ptr(qw), _ptr(kw), _ptr(pos), _ptr(kpos),
-                                                   _ptr(freqs), float(eps), _ptr(gq), _strides(gq), _ptr(gk),
-                                                   _strides(gk), _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(dpos),
-                                                   _ptr(dkpos), _ptr(ws), ws.numel(), _stream(dev)),
-                   "qk_norm_rotary_backward")
-    return dq, dk, dqw, dkw, dpos, dkpos
-
-
-def _attention_inputs(q, k, v, scale):
-    q = _heads_input(q, "q")
-    k, v = _heads_input(k, "k", q), _heads_input(v, "v", q)
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
-    B, nq, hq, D = q.shape
-    sizes = (B, nq, k.shape[1], hq, k.shape[2], D)
-    return q, k, v, sizes, float(D ** -0.5 if scale is None else scale)
+    inputs, call = _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
+    gq = _heads_input(grad_q_out, "grad_q_out", inputs[0])
+    gk = None if k is None else _heads_input(grad_k_out, "grad_k_out", inputs[0])
+    return _qk_norm_backward(gq, gk, inputs, call, want_weights, want_positions)
 
 
 def _in_place(*tensors):
@@ -915,63 +946,87 @@ def _in_place(*tensors):
     return 1
 
 
-def attention_forward(q, k, v, key_mask=None, scale=None, for_backward=False):
-    """(out, rest, lse, key_list): softmax(scale q k^T over the valid keys) v for q (B, Nq, Hq, D) and k, v (B, Nk, Hkv, D), Hq a
-    multiple of Hkv; scale None: D^-1/2.  key_mask (B, Nk) bool, False where a key is not attended to.  rest (what
-    rounding took from a bfloat16 out) and lse, None unless for_backward, and key_list, None without a mask, are what
-    attention_backward takes."""
-    lib = _lib.load()
-    q, k, v, sizes, scale = _attention_inputs(q, k, v, scale)
-    B, nq, nk, hq = sizes[:4]
-    dev, fdt = q.device, _FEAT_DTYPES[q.dtype]
+def _attention_inputs(q, k, v, key_mask, scale):
+    """((q, k, v, key_mask) as the kernels take them, what else a call takes)."""
+    q = _heads_input(q, "q")
+    k, v = _heads_input(k, "k", q), _heads_input(v, "v", q)
+    B, nq, hq, D = q.shape
+    Bk, nk, hk, Dk = k.shape
+    if k.shape != v.shape or Bk != B or Dk != D:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
     if key_mask is not None:
-        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype != torch.bool or key_mask.device != dev \
-                or tuple(key_mask.shape) != (B, nk):
-            raise RuntimeError(f"key_mask must be a bool tensor {(B, nk)} on {dev}")
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype != torch.bool or key_mask.device != q.device \
+                or key_mask.shape != (B, nk):
+            raise RuntimeError(f"key_mask must be a bool tensor {(B, nk)} on {q.device}")
         key_mask = key_mask.contiguous()
+    return (q, k, v, key_mask), ((B, nq, nk, hq, hk, D), _FEAT_DTYPES[q.dtype], float(D ** -0.5 if scale is None else scale))
+
+
+def _attention_forward(inputs, call, for_backward):
+    q, k, v, key_mask = inputs
+    sizes, fdt, scale = call
+    B, nq, nk, hq = sizes[:4]
+    dev = q.device
     with _OnDevice(dev):
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        rest = torch.empty_like(out) if for_backward and q.dtype == torch.bfloat16 else None
+        rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if for_backward and fdt == _lib.G2V_DTYPE_BF16 else None
         lse = torch.empty(B, hq, nq, dtype=torch.float32, device=dev) if for_backward else None
         lst = None if key_mask is None else torch.empty(B * (nk + 1), dtype=torch.int32, device=dev)
-        ws = torch.empty(lib.g2v_attention_forward_workspace(*sizes, fdt, _in_place(q, k, v), 0 if lst is None else 1),
-                         dtype=torch.uint8, device=dev)
-        _lib.check(lib.g2v_attention_forward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
-                                             _ptr(key_mask), scale, _ptr(out), _ptr(rest), _ptr(lse), _ptr(lst), _ptr(ws),
-                                             ws.numel(), _stream(dev)), "attention_forward")
+        nws = _workspace_bytes("g2v_attention_forward_workspace", *sizes, fdt, _in_place(q, k, v), 0 if lst is None else 1)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        rc = _lib.load().g2v_attention_forward(*sizes, _addr(q), _strides(q), _addr(k), _strides(k), _addr(v), _strides(v),
+                                               fdt, _addr(key_mask), scale, _addr(out), _addr(rest), _addr(lse), _addr(lst),
+                                               ws.data_ptr(), nws, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "attention_forward")
     return out, rest, lse, lst
+
+
+def _attention_backward(g, q, k, v, out, rest, lse, key_list, call, want_q, want_kv):
+    sizes, fdt, scale = call
+    dev = q.device
+    if g.shape != q.shape:
+        raise RuntimeError(f"grad_out must be {tuple(q.shape)}, got {tuple(g.shape)}")
+    with _OnDevice(dev):
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
+        dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
+        dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
+        nws = _workspace_bytes("g2v_attention_backward_workspace", *sizes, fdt, _in_place(q, k, v, g),
+                               0 if key_list is None else 1)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        rc = _lib.load().g2v_attention_backward(*sizes, _addr(q), _strides(q), _addr(k), _strides(k), _addr(v), _strides(v),
+                                                fdt, _addr(key_list), scale, _addr(out), _addr(rest), _addr(lse), _addr(g),
+                                                _strides(g), _addr(dq), _addr(dk), _addr(dv), ws.data_ptr(), nws,
+                                                _stream_of(dev))
+    if rc:
+        _lib.check(rc, "attention_backward")
+    return dq, dk, dv
+
+
+def attention_forward(q, k, v, key_mask=None, scale=None, for_backward=False):
+    """(out, rest, lse, key_list): softmax(scale q k^T over the valid keys) v for q (B, Nq, Hq, D) and k, v (B, Nk, Hkv, D),
+    Hq a multiple of Hkv; scale None: D^-1/2.  key_mask (B, Nk) bool, False where a key is not attended to.  rest (what
+    rounding took from a bfloat16 out) and lse, None unless for_backward, and key_list, None without a mask, are what
+    attention_backward takes."""
+    return _attention_forward(*_attention_inputs(q, k, v, key_mask, scale), for_backward)
 
 
 def attention_backward(grad_out, q, k, v, out, rest, lse, key_list=None, scale=None, want_q=True, want_kv=True):
     """(grad_q, grad_k, grad_v) of attention_forward from its results; None where not wanted."""
-    lib = _lib.load()
-    q, k, v, sizes, scale = _attention_inputs(q, k, v, scale)
-    B, nq, nk, hq = sizes[:4]
-    dev, fdt = q.device, _FEAT_DTYPES[q.dtype]
+    (q, k, v, _), call = _attention_inputs(q, k, v, None, scale)
+    B, nq, nk, hq = call[0][:4]
+    dev = q.device
     g = _heads_input(grad_out, "grad_out", q)
-    if g.shape != q.shape:
-        raise RuntimeError(f"grad_out must be {tuple(q.shape)}, got {tuple(g.shape)}")
     _check_saved(out, "out", q.dtype, dev)
     _check_saved(lse, "lse", torch.float32, dev)
     if rest is not None:
         _check_saved(rest, "rest", torch.bfloat16, dev)
         if rest.shape != out.shape:
             raise RuntimeError(f"rest must be {tuple(out.shape)}, got {tuple(rest.shape)}")
-    if out.shape != q.shape or tuple(lse.shape) != (B, hq, nq):
+    if out.shape != q.shape or lse.shape != (B, hq, nq):
         raise RuntimeError(f"out {tuple(out.shape)} and lse {tuple(lse.shape)} do not go with q {tuple(q.shape)}")
     if key_list is not None:
         _check_saved(key_list, "key_list", torch.int32, dev)
         if key_list.numel() != B * (nk + 1):
             raise RuntimeError(f"key_list must hold {B * (nk + 1)} values, got {key_list.numel()}")
-    with _OnDevice(dev):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
-        dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
-        dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
-        ws = torch.empty(lib.g2v_attention_backward_workspace(*sizes, fdt, _in_place(q, k, v, g),
-                                                              0 if key_list is None else 1),
-                         dtype=torch.uint8, device=dev)
-        _lib.check(lib.g2v_attention_backward(*sizes, _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), fdt,
-                                              _ptr(key_list), scale, _ptr(out), _ptr(rest), _ptr(lse), _ptr(g), _strides(g),
-                                              _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(dev)),
-                   "attention_backward")
-    return dq, dk, dv
+    return _attention_backward(g, q, k, v, out, rest, lse, key_list, call, want_q, want_kv)

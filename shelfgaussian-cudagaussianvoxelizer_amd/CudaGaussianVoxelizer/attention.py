@@ -18,14 +18,15 @@ def _needs_grad(*tensors):
 class _QkNormRotaryFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, freqs, q_weight, k_weight, k_positions, eps):
-        ctx.save_for_backward(q, k, positions, freqs, q_weight, k_weight, k_positions)
-        ctx.eps = eps
+        inputs, ctx.call = _C._qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
+        ctx.save_for_backward(*inputs)
         ctx.set_materialize_grads(False)
-        return _C.qk_norm_rotary_forward(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
+        return _C._qk_norm_forward(inputs, ctx.call)
 
     @staticmethod
     def backward(ctx, grad_q_out, grad_k_out):
-        q, k, positions, freqs, q_weight, k_weight, k_positions = ctx.saved_tensors
+        inputs = ctx.saved_tensors
+        q, k = inputs[:2]
         if grad_q_out is None and grad_k_out is None:
             return (None,) * 8
         if grad_q_out is None:
@@ -33,9 +34,11 @@ class _QkNormRotaryFunction(torch.autograd.Function):
         if grad_k_out is None and k is not None:
             grad_k_out = torch.zeros_like(k)
         need = ctx.needs_input_grad
-        dq, dk, dqw, dkw, dpos, dkpos = _C.qk_norm_rotary_backward(
-            grad_q_out, grad_k_out, q, k, positions, freqs, q_weight, k_weight, k_positions, ctx.eps,
-            want_weights=(need[4], need[5]), want_positions=(need[2], need[6]))
+        grad_q_out = _C._heads_input(grad_q_out, "grad_q_out", q)
+        if k is not None:
+            grad_k_out = _C._heads_input(grad_k_out, "grad_k_out", q)
+        dq, dk, dqw, dkw, dpos, dkpos = _C._qk_norm_backward(grad_q_out, grad_k_out, inputs, ctx.call,
+                                                             (need[4], need[5]), (need[2], need[6]))
         return dq, dk, dpos, None, dqw, dkw, dkpos, None
 
 
@@ -80,17 +83,16 @@ def rotary_frequencies(head_dim, axes=3, wavelengths=(0.8, 160.0), device="cuda"
 class _GaussianAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_mask, scale):
-        out, rest, lse, key_list = _C.attention_forward(q, k, v, key_mask, scale, for_backward=True)
-        ctx.save_for_backward(q, k, v, out, rest, lse, key_list)
-        ctx.scale = scale
+        inputs, ctx.call = _C._attention_inputs(q, k, v, key_mask, scale)
+        out, rest, lse, key_list = _C._attention_forward(inputs, ctx.call, True)
+        ctx.save_for_backward(*inputs[:3], out, rest, lse, key_list)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        q, k, v, out, rest, lse, key_list = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return _C.attention_backward(grad_out, q, k, v, out, rest, lse, key_list, ctx.scale, want_q=need[0],
-                                     want_kv=need[1] or need[2]) + (None, None)
+        saved, need = ctx.saved_tensors, ctx.needs_input_grad
+        grad_out = _C._heads_input(grad_out, "grad_out", saved[0])
+        return _C._attention_backward(grad_out, *saved, ctx.call, need[0], need[1] or need[2]) + (None, None)
 
 
 def gaussian_attention(q, k, v, key_mask=None, scale=None):
