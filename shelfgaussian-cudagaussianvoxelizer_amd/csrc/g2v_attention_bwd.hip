@@ -317,16 +317,35 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
     }
 }
 
-// Sums of the splits, in their order.
-template <int DP, typename T>
-__global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a) {
-    const int rows = a.group * a.nq;
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.bhs * rows;
-    const int64_t at = e / (DP / 4);
-    const int d = (int)(e % (DP / 4)) * 4;
-    if (at >= all) return;
+// Sums of the splits: each of `parts` threads every parts-th, then in their order.
+__device__ __forceinline__ f32x4 join_sum(const float* part, int64_t stride, int splits, int parts, bool live, float (*red)[256]) {
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) o += *reinterpret_cast<const f32x4*>(a.part + (s * all + at) * DP + d);
+    const int mine = threadIdx.x % parts;
+    if (live) {
+#pragma unroll 4
+        for (int s = mine; s < splits; s += parts) o += *reinterpret_cast<const f32x4*>(part + s * stride);
+    }
+    if (parts > 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[j][threadIdx.x] = o[j];
+        __syncthreads();
+        if (mine == 0)
+            for (int k = 1; k < parts; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] += red[j][threadIdx.x + k];
+    }
+    return o;
+}
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a, int parts) {
+    constexpr int kLanes = DP / 4;
+    __shared__ float red[4][256];
+    const int rows = a.group * a.nq, per = 256 / (kLanes * parts), e = threadIdx.x / parts, d = e % kLanes * 4;
+    const int64_t all = (int64_t)a.bhs * rows, at = (int64_t)blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < all;
+    const f32x4 o = join_sum(a.part + at * DP + d, all * DP, a.splits, parts, live, red);
+    if (!live || threadIdx.x % parts) return;
     const int bh = (int)(at / rows), r = (int)(at % rows);
     const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
     T* row = static_cast<T*>(a.dq) + (((int64_t)b * a.nq + tok) * a.hq + head) * a.dim;
@@ -334,16 +353,17 @@ __global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a) {
 }
 
 template <int DP, typename T>
-__global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.bhs * a.nk;
-    const int64_t at = e / (DP / 2);
-    const int d = (int)(e % (DP / 2)) * 4;    // dK, then dV
-    if (at >= all) return;
-    const int bh = (int)(at / a.nk), j = (int)(at % a.nk), b = bh / a.hk;
+__global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a, int parts) {
+    constexpr int kLanes = DP / 2;    // dK, then dV
+    __shared__ float red[4][256];
+    const int per = 256 / (kLanes * parts), e = threadIdx.x / parts, d = e % kLanes * 4;
+    const int64_t all = (int64_t)a.bhs * a.nk, at = (int64_t)blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < all;
+    const int bh = live ? (int)(at / a.nk) : 0, j = live ? (int)(at % a.nk) : 0, b = bh / a.hk;
     const int n = a.count ? a.count[b] : a.nk;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (j < n && (n > 1 || d >= DP))    // one key: its probability is 1 whatever k is
-        for (int s = 0; s < a.splits; ++s) o += *reinterpret_cast<const f32x4*>(a.part + (s * all + at) * (2 * DP) + d);
+    const bool some = j < n && (n > 1 || d >= DP);    // one key: its probability is 1 whatever k is
+    const f32x4 o = join_sum(a.part + at * (2 * DP) + d, all * (2 * DP), a.splits, parts, live && some, red);
+    if (!live || threadIdx.x % parts) return;
     const int64_t key = a.list ? a.list[(int64_t)b * a.nk + j] : j;
     const float f = d < DP ? a.scale : 1.0f;
     T* row = static_cast<T*>(d < DP ? a.dk : a.dv) + (((int64_t)b * a.nk + key) * a.hk + bh % a.hk) * a.dim;
@@ -379,8 +399,9 @@ template <int NP, int DP, int NQB, int NW, int KT, typename T>
 hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
     G2V_LAUNCH((k_attn_dq<NP, DP, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
     if (a.splits > 1) {
-        const int64_t threads = (int64_t)a.bhs * a.group * a.nq * (DP / 4);
-        G2V_LAUNCH((k_attn_dq_join<DP, T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, a);
+        const int64_t rows = (int64_t)a.bhs * a.group * a.nq;
+        const int parts = attn_join_parts(rows, DP / 4, a.splits);
+        G2V_LAUNCH((k_attn_dq_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 4 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();
 }
@@ -388,20 +409,28 @@ template <int NP, int DP, int NKB, int NW, int QT, typename T>
 hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
     G2V_LAUNCH((k_attn_dkv<NP, DP, NKB, NW, QT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
     if (a.splits > 1) {
-        const int64_t threads = (int64_t)a.bhs * a.nk * (DP / 2);
-        G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, a);
+        const int64_t rows = (int64_t)a.bhs * a.nk;
+        const int parts = attn_join_parts(rows, DP / 2, a.splits);
+        G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 2 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();
 }
 
+template <int NP, int DP, int NQB, int KT, typename T>
+hipError_t dq_waves(const AttnBwd& a, const AttnShape& g, hipStream_t s) {
+    if constexpr (NP == 1)
+        if (g.waves == 1) return dq_launch<NP, DP, 1, 1, KT, T>(a, s);
+    return dq_launch<NP, DP, NQB, 4, KT, T>(a, s);
+}
+
 }  // namespace
 
-AttnShape attn_dq_shape(bool f32, int dp) {
+AttnShape attn_dq_shape(bool f32, int dp, int64_t rows) {
     AttnShape g;
-    g.waves = 4;
-    g.blocks = !f32 && dp <= 64 ? 2 : 1;
+    g.waves = !f32 && rows <= 32 ? 1 : 4;    // as in attn_fwd_shape
+    g.blocks = g.waves == 4 && !f32 && dp <= 64 ? 2 : 1;
     g.tile = f32 && dp > 32 ? 32 : 64;
-    g.per_cu = f32 && dp > 32 ? 1 : 2;
+    g.per_cu = g.waves == 1 ? 4 : f32 && dp > 32 ? 1 : 2;
     return g;
 }
 AttnShape attn_dkv_shape(bool f32, int dp) {
@@ -414,19 +443,20 @@ AttnShape attn_dkv_shape(bool f32, int dp) {
 }
 
 hipError_t launch_attn_dq(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
+    const AttnShape g = attn_dq_shape(f32, dp, (int64_t)a.group * a.nq);
     if (f32) {
         switch (dp) {
-            case 32: return dq_launch<3, 32, 1, 4, 64, float>(a, s);
-            case 64: return dq_launch<3, 64, 1, 4, 32, float>(a, s);
-            case 96: return dq_launch<3, 96, 1, 4, 32, float>(a, s);
-            default: return dq_launch<3, 128, 1, 4, 32, float>(a, s);
+            case 32: return dq_waves<3, 32, 1, 64, float>(a, g, s);
+            case 64: return dq_waves<3, 64, 1, 32, float>(a, g, s);
+            case 96: return dq_waves<3, 96, 1, 32, float>(a, g, s);
+            default: return dq_waves<3, 128, 1, 32, float>(a, g, s);
         }
     }
     switch (dp) {
-        case 32: return dq_launch<1, 32, 2, 4, 64, __bf16>(a, s);
-        case 64: return dq_launch<1, 64, 2, 4, 64, __bf16>(a, s);
-        case 96: return dq_launch<1, 96, 1, 4, 64, __bf16>(a, s);
-        default: return dq_launch<1, 128, 1, 4, 64, __bf16>(a, s);
+        case 32: return dq_waves<1, 32, 2, 64, __bf16>(a, g, s);
+        case 64: return dq_waves<1, 64, 2, 64, __bf16>(a, g, s);
+        case 96: return dq_waves<1, 96, 1, 64, __bf16>(a, g, s);
+        default: return dq_waves<1, 128, 1, 64, __bf16>(a, g, s);
     }
 }
 

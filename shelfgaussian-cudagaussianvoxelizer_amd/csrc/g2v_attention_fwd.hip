@@ -201,28 +201,51 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
     }
 }
 
-// Joins the splits of a row: O = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M).  DP / 4 lanes a row.
+// Joins the splits of a row: O = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M).  DP / 4 lanes and `parts` threads of each to a
+// row: where rows are few their splits are many, and one thread after another's loads would take the time.  A
+// fixed order.
 template <int DP, typename T>
-__global__ void __launch_bounds__(256) k_attn_join(AttnFwd a) {
-    const int rows = a.group * a.nq;
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.bhs * rows;
-    const int64_t at = e / (DP / 4);
-    const int d = (int)(e % (DP / 4)) * 4;
-    if (at >= all) return;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * all + at)]);
-    float total = 0.0f;
+__global__ void __launch_bounds__(256) k_attn_join(AttnFwd a, int parts) {
+    constexpr int kLanes = DP / 4;
+    __shared__ float red[6][256];
+    const int rows = a.group * a.nq, per = 256 / (kLanes * parts);   // rows of a workgroup
+    const int part = threadIdx.x % parts, e = threadIdx.x / parts, d = e % kLanes * 4;
+    const int64_t all = (int64_t)a.bhs * rows, at = (int64_t)blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < all;
+    float top = -INFINITY, total = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t p = s * all + at;
-        const float l = a.part_ml[2 * p + 1];
-        if (l == 0.0f) continue;   // a split without keys (its maximum is the lowest value)
-        const float f = exp2_fast(a.part_ml[2 * p] - top);
-        total = fmaf(l, f, total);
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + p * DP + d);
+    if (live) {
+        for (int s = part; s < a.splits; s += parts) top = fmaxf(top, a.part_ml[2 * (s * all + at)]);
+#pragma unroll 4
+        for (int s = part; s < a.splits; s += parts) {
+            const int64_t p = s * all + at;
+            const float l = a.part_ml[2 * p + 1];
+            // a split without keys has no sum, and its maximum is the lowest value
+            const float f = l == 0.0f ? 0.0f : exp2_fast(a.part_ml[2 * p] - top);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + p * DP + d);
+            total = fmaf(l, f, total);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], f, o[j]);
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], f, o[j]);
+        }
     }
+    if (parts > 1) {
+        red[0][threadIdx.x] = top;
+        red[1][threadIdx.x] = total;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[2 + j][threadIdx.x] = o[j];
+        __syncthreads();
+        if (part > 0) return;
+        for (int k = 1; k < parts; ++k) {
+            const int i = threadIdx.x + k;
+            const float up = fmaxf(top, red[0][i]);
+            const float f = total == 0.0f ? 0.0f : exp2_fast(top - up), g = red[1][i] == 0.0f ? 0.0f : exp2_fast(red[0][i] - up);
+            top = up;
+            total = total * f + red[1][i] * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = o[j] * f + red[2 + j][i] * g;
+        }
+    }
+    if (!live) return;
     const int bh = (int)(at / rows), r = (int)(at % rows);
     const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
     const float inv = total > 0.0f ? 1.0f / total : 0.0f;
@@ -306,38 +329,49 @@ template <int NP, int DP, int NQB, int NW, int KT, typename T>
 hipError_t fwd_launch(const AttnFwd& a, hipStream_t s) {
     G2V_LAUNCH((k_attn_fwd<NP, DP, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
     if (a.splits > 1) {
-        const int64_t threads = (int64_t)a.bhs * a.group * a.nq * (DP / 4);
-        G2V_LAUNCH((k_attn_join<DP, T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, a);
+        const int64_t rows = (int64_t)a.bhs * a.group * a.nq;
+        const int parts = attn_join_parts(rows, DP / 4, a.splits);
+        G2V_LAUNCH((k_attn_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 4 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();
+}
+
+template <int NP, int DP, int NQB, int KT, typename T>
+hipError_t fwd_waves(const AttnFwd& a, const AttnShape& g, hipStream_t s) {
+    if constexpr (NP == 1)
+        if (g.waves == 1) return fwd_launch<NP, DP, 1, 1, KT, T>(a, s);
+    return fwd_launch<NP, DP, NQB, 4, KT, T>(a, s);
 }
 
 }  // namespace
 
 AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows) {
-    (void)rows;
     AttnShape g;
-    g.waves = 4;
-    g.blocks = !f32 && dp <= 64 ? 2 : 1;
+    // Rows that fit one wave's block: workgroups of that one wave, more of which fit a CU than of four (one query over
+    // 18000 keys x 16 heads x 64: 20 us instead of 25 with the same keys in flight).  float32 keys are packed first,
+    // which takes longer than either.
+    g.waves = !f32 && rows <= 32 ? 1 : 4;
+    g.blocks = g.waves == 4 && !f32 && dp <= 64 ? 2 : 1;
     g.tile = f32 && dp > 32 ? 32 : 64;
-    g.per_cu = f32 && dp > 64 ? 1 : 2;
+    g.per_cu = g.waves == 1 ? 4 : f32 && dp > 64 ? 1 : 2;
     return g;
 }
 
 hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s) {
+    const AttnShape g = attn_fwd_shape(f32, dp, (int64_t)a.group * a.nq);
     if (f32) {
         switch (dp) {
-            case 32: return fwd_launch<3, 32, 1, 4, 64, float>(a, s);
-            case 64: return fwd_launch<3, 64, 1, 4, 32, float>(a, s);
-            case 96: return fwd_launch<3, 96, 1, 4, 32, float>(a, s);
-            default: return fwd_launch<3, 128, 1, 4, 32, float>(a, s);
+            case 32: return fwd_waves<3, 32, 1, 64, float>(a, g, s);
+            case 64: return fwd_waves<3, 64, 1, 32, float>(a, g, s);
+            case 96: return fwd_waves<3, 96, 1, 32, float>(a, g, s);
+            default: return fwd_waves<3, 128, 1, 32, float>(a, g, s);
         }
     }
     switch (dp) {
-        case 32: return fwd_launch<1, 32, 2, 4, 64, __bf16>(a, s);
-        case 64: return fwd_launch<1, 64, 2, 4, 64, __bf16>(a, s);
-        case 96: return fwd_launch<1, 96, 1, 4, 64, __bf16>(a, s);
-        default: return fwd_launch<1, 128, 1, 4, 64, __bf16>(a, s);
+        case 32: return fwd_waves<1, 32, 2, 64, __bf16>(a, g, s);
+        case 64: return fwd_waves<1, 64, 2, 64, __bf16>(a, g, s);
+        case 96: return fwd_waves<1, 96, 1, 64, __bf16>(a, g, s);
+        default: return fwd_waves<1, 128, 1, 64, __bf16>(a, g, s);
     }
 }
 

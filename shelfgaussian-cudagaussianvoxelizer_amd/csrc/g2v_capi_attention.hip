@@ -81,16 +81,17 @@ int qn_fill(QkNormArgs& a, const void* q, const long long* qs, const void* k, co
 constexpr int kCus = 256;
 
 // Into how many workgroups the long axis (`units` tiles) of each of `wgs` workgroups goes.  unit_us: time of a tile in a
-// workgroup that shares its CU with another; join_us: writing and adding one split's partial results.  A CU runs
-// its workgroups two at a time; one without a partner takes about 0.65 of the time of two.
-int attn_splits(int64_t wgs, int units, double unit_us, double join_us) {
+// workgroup that shares its CU with as many others as fit (per_cu); join_us: writing and adding one split's partial
+// results.  A workgroup with fewer beside it is faster: alone it takes about 0.65 of the time of two.
+int attn_splits(int64_t wgs, int units, int per_cu, double unit_us, double join_us) {
     auto cost = [&](int s) {
-        const int64_t n = ceil_div(wgs * s, kCus);
-        const double us = (0.5 * n + 0.15 * (n & 1)) * (ceil_div(units, s) + 2) * unit_us;
+        const int64_t n = ceil_div(wgs * s, kCus);      // workgroups of the fullest CU
+        const double rounds = (double)(n / per_cu) + (n % per_cu ? 0.3 + 0.7 * (n % per_cu) / per_cu : 0.0);
+        const double us = rounds * (ceil_div(units, s) + 2) * unit_us;
         return s == 1 ? us : us + 5.0 + s * join_us;
     };
     int best = 1;
-    for (int s = 2; s <= 64 && s <= units; ++s)
+    for (int s = 2; s <= 128 && s <= units; ++s)
         if (cost(s) < cost(best)) best = s;
     return best;
 }
@@ -139,9 +140,9 @@ AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing,
     r.tiles = (int)ceil_div(mine, own);
     const int64_t units = ceil_div(passing, g.tile) * streams;
     const double flops = 2.0 * products * own * g.tile * z.dp;
-    const double unit_us = std::max(1.0, flops * 2.0 / ((z.f32 ? 0.12e9 : 0.7e9) / kCus));
+    const double unit_us = std::max(1.0, flops * g.per_cu / ((z.f32 ? 0.15e9 : 0.9e9) / kCus));
     const double join_us = 8.0 * mine * z.bhs * width / 3e6;
-    r.splits = attn_splits((int64_t)z.bhs * r.tiles, (int)std::min<int64_t>(units, 1 << 30), unit_us, join_us);
+    r.splits = attn_splits((int64_t)z.bhs * r.tiles, (int)std::min<int64_t>(units, 1 << 30), g.per_cu, unit_us, join_us);
     return r;
 }
 
@@ -204,7 +205,7 @@ hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool pa
 AttnRun attn_fwd_run(const AttnSizes& z) {
     return attn_run(z, attn_fwd_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 2, z.dp);
 }
-AttnRun attn_dq_run(const AttnSizes& z) { return attn_run(z, attn_dq_shape(z.f32, z.dp), z.rows(), z.nk, 1, 3, z.dp); }
+AttnRun attn_dq_run(const AttnSizes& z) { return attn_run(z, attn_dq_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 3, z.dp); }
 AttnRun attn_dkv_run(const AttnSizes& z) {
     return attn_run(z, attn_dkv_shape(z.f32, z.dp), z.nk, z.nq, z.group, 4, 2 * z.dp);
 }

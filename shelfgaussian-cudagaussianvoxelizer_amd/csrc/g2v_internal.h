@@ -286,9 +286,15 @@ struct AttnPack {
 struct AttnShape {
     int waves, blocks, tile, per_cu;
 };
+// Threads that share a row's splits in a join of `lanes` lanes a row: more while the rows leave the card empty.
+inline int attn_join_parts(int64_t rows, int lanes, int splits) {
+    int parts = 1;
+    while (2 * parts * lanes <= 256 && 2 * parts <= splits && rows * lanes * parts < 65536) parts *= 2;
+    return parts;
+}
 inline int attn_dp(int dim) { return (dim + 31) / 32 * 32; }
 AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows);
-AttnShape attn_dq_shape(bool f32, int dp);
+AttnShape attn_dq_shape(bool f32, int dp, int64_t rows);
 AttnShape attn_dkv_shape(bool f32, int dp);
 hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_attn_list(int batch, int nk, const unsigned char* mask, int* list, int* count, hipStream_t s);
