@@ -113,29 +113,37 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
     __syncthreads();
 }
 
-// A operand from a tile: rows 32 rb .. 32 rb + 31, contraction over d in 16 ks .. 16 ks + 15.
+// Reading a tile.  The slots are permuted by exclusive or, so a lane's address of any chunk is its address of chunk 0 with
+// bits flipped that are known when compiling (for DP = 96, whose rows are no power of two, only the lowest chunk bits are
+// permuted, and the rest is an offset): two registers a lane, whatever the number of chunks.
 template <int DP>
-__device__ __forceinline__ bf16x8 row_frag(const char* tile, int rb, int ks) {
-    const int l = threadIdx.x & 63, n = l & 31, g = l >> 5;
-    return *reinterpret_cast<const bf16x8*>(tile + (rb * 32 + n) * (DP * 2) + swz<DP>(n, 2 * ks + g) * 16);
-}
+struct Frags {
+    uint32_t row, tr;    // LDS offsets: row n's chunk g; the transposed reads' first row and chunk
 
-// A operand of the transposed tile: rows d = 32 t .. 32 t + 31, contraction over the tile's rows 32 rb + 16 s .. + 15 in
-// the order of a result's registers.  Each read transposes 4 x 16 values within 16 lanes.
-template <int DP>
-__device__ __forceinline__ bf16x8 tr_frag(const char* tile, int rb, int s, int t) {
-    const int l = threadIdx.x & 63, g = l >> 5, dh = (l >> 4) & 1, i = l & 15;
-    const int c = 4 * t + 2 * dh + ((i & 3) >> 1);
-    typedef __attribute__((address_space(3))) s16x4* p_t;
-    s16x4 x[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int r = 8 * j + 4 * g + (i >> 2);     // of 16: the swizzle looks at no higher bit
-        x[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (p_t)(tile + (rb * 32 + 16 * s + r) * (DP * 2) + swz<DP>(r, c) * 16 + (i & 1) * 8));
+    __device__ __forceinline__ void init(uint32_t lds) {
+        const int l = threadIdx.x & 63, n = l & 31, g = l >> 5, dh = (l >> 4) & 1, i = l & 15;
+        const int r = 4 * g + (i >> 2);
+        row = lds + n * (DP * 2) + swz<DP>(n, g) * 16;
+        tr = lds + r * (DP * 2) + swz<DP>(r, 2 * dh + ((i & 3) >> 1)) * 16 + (i & 1) * 8;
     }
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
-}
+    // A operand: rows 32 rb .. 32 rb + 31, contraction over d in 16 ks .. 16 ks + 15; `at` bytes into the buffer.
+    __device__ __forceinline__ bf16x8 rows(uint32_t buf, int at, int rb, int ks) const {
+        typedef const __attribute__((address_space(3))) bf16x8* p_t;
+        const uint32_t flip = DP == 96 ? (ks & 1) * 32 : ks * 32, off = DP == 96 ? (ks >> 1) * 64 : 0;
+        return *(p_t)(((row + buf) ^ flip) + at + rb * 32 * (DP * 2) + off);
+    }
+    // A operand of the transposed tile: rows d = 32 t .. 32 t + 31, contraction over the tile's rows 32 rb + 16 s .. + 15
+    // in the order of a result's registers.  Each read transposes 4 x 16 values within 16 lanes.
+    __device__ __forceinline__ bf16x8 cols(uint32_t buf, int at, int rb, int s, int t) const {
+        typedef __attribute__((address_space(3))) s16x4* p_t;
+        const uint32_t flip = DP == 96 ? 0 : t * 64, off = DP == 96 ? t * 64 : 0;
+        const uint32_t base = at + (rb * 32 + 16 * s) * (DP * 2) + off;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p_t)(((tr + buf) ^ flip) + base));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (p_t)(((tr + buf) ^ (flip ^ (DP == 64 ? 16 : 32))) + base + 8 * (DP * 2)));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
 
 // B operand from memory: this lane's row, contraction over d in 16 ks .. + 15 of plane pl; zero where there is none.
 template <int DP>

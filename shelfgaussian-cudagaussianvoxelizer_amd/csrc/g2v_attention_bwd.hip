@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
     constexpr int NS = NP == 1 ? 2 : NP;
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][TileT::kBytes];
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int rows = a.group * a.nq;
     const int r0 = (w.tile * NW + uniform(threadIdx.x >> 6)) * (NQB * 32) + (threadIdx.x & 31);
@@ -55,6 +55,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
 
     TileT tile;
     tile.init(a.k);
+    Frags<DP> frags;
+    frags.init(lds_off(lds));
     if (a.k.chunks < TileT::C) clear_lds<NT>(&lds[0][0][0], sizeof(lds));
     auto load = [&](int t, int buf) {
         if ((t + 1) * KT <= n) {
@@ -78,8 +80,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
         const int buf = (t - t0) & 1;
         tile_barrier();
         if (t + 1 < t1) load(t + 1, buf ^ 1);
-        const char* kt = lds[buf][0];
-        const char* vt = lds[buf][1];
+        const uint32_t at = buf * 2 * TileT::kBytes;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             f32x16 s[NQB], dp[NQB];
@@ -92,8 +93,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
                 bf16x8 fk[NP], fv[NP];
 #pragma unroll
                 for (int pl = 0; pl < NP; ++pl) {
-                    fk[pl] = row_frag<DP>(kt + pl * KT * DP * 2, kb, ks);
-                    fv[pl] = row_frag<DP>(vt + pl * KT * DP * 2, kb, ks);
+                    fk[pl] = frags.rows(at, pl * KT * DP * 2, kb, ks);
+                    fv[pl] = frags.rows(at, TileT::kBytes + pl * KT * DP * 2, kb, ks);
                 }
 #pragma unroll
                 for (int b = 0; b < NQB; ++b) {
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
                 for (int d = 0; d < DB; ++d) {
                     bf16x8 f[NP];
 #pragma unroll
-                    for (int pl = 0; pl < NP; ++pl) f[pl] = tr_frag<DP>(kt + pl * KT * DP * 2, kb, st, d);
+                    for (int pl = 0; pl < NP; ++pl) f[pl] = frags.cols(at, pl * KT * DP * 2, kb, st, d);
 #pragma unroll
                     for (int b = 0; b < NQB; ++b) dq[d][b] = mma(f, p[b], dq[d][b]);
                 }
@@ -157,10 +158,10 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
 // dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_dkv(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dkv(AttnBwd a) {
     constexpr int NT = NW * 64, QB = QT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, QT, NT> TileT;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][TileT::kBytes];
     __shared__ __attribute__((aligned(16))) float stat[2][2][64];   // lse and delta of the tile's rows
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int wave = uniform(threadIdx.x >> 6);
@@ -188,6 +189,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
 
     TileT tile;
     tile.init(a.q);
+    Frags<DP> frags;
+    frags.init(lds_off(lds));
     if (a.q.chunks < TileT::C) clear_lds<NT>(&lds[0][0][0], sizeof(lds));
     auto load = [&](int u, int buf) {
         const int hd = u / per, t = u - hd * per, head = w.h * a.group + hd;
@@ -219,8 +222,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
         const int buf = (u - u0) & 1;
         tile_barrier();
         if (u + 1 < u1) load(u + 1, buf ^ 1);
-        const char* qt = lds[buf][0];
-        const char* gt = lds[buf][1];
+        const uint32_t at = buf * 2 * TileT::kBytes;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
             f32x16 s[NKB], dp[NKB];
@@ -233,8 +235,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
                 bf16x8 fq[NP], fg[NP];
 #pragma unroll
                 for (int pl = 0; pl < NP; ++pl) {
-                    fq[pl] = row_frag<DP>(qt + pl * QT * DP * 2, qb, ks);
-                    fg[pl] = row_frag<DP>(gt + pl * QT * DP * 2, qb, ks);
+                    fq[pl] = frags.rows(at, pl * QT * DP * 2, qb, ks);
+                    fg[pl] = frags.rows(at, TileT::kBytes + pl * QT * DP * 2, qb, ks);
                 }
 #pragma unroll
                 for (int b = 0; b < NKB; ++b) {
@@ -268,8 +270,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP <= 96 ? 2 : 1) k_attn_d
                     bf16x8 fg[NP], fq[NP];
 #pragma unroll
                     for (int pl = 0; pl < NP; ++pl) {
-                        fg[pl] = tr_frag<DP>(gt + pl * QT * DP * 2, qb, st, d);
-                        fq[pl] = tr_frag<DP>(qt + pl * QT * DP * 2, qb, st, d);
+                        fg[pl] = frags.cols(at, TileT::kBytes + pl * QT * DP * 2, qb, st, d);
+                        fq[pl] = frags.cols(at, pl * QT * DP * 2, qb, st, d);
                     }
 #pragma unroll
                     for (int b = 0; b < NKB; ++b) {
@@ -437,8 +439,8 @@ AttnShape attn_dkv_shape(bool f32, int dp) {
     AttnShape g;
     g.waves = 4;
     g.blocks = 1;
-    g.tile = f32 && dp > 32 ? 32 : 64;
-    g.per_cu = (f32 && dp > 32) || dp > 96 ? 1 : 2;
+    g.tile = (f32 && dp > 32) || dp > 96 ? 32 : 64;
+    g.per_cu = f32 && dp > 32 ? 1 : 2;
     return g;
 }
 
@@ -473,7 +475,7 @@ hipError_t launch_attn_dkv(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
         case 32: return dkv_launch<1, 32, 1, 4, 64, __bf16>(a, s);
         case 64: return dkv_launch<1, 64, 1, 4, 64, __bf16>(a, s);
         case 96: return dkv_launch<1, 96, 1, 4, 64, __bf16>(a, s);
-        default: return dkv_launch<1, 128, 1, 4, 64, __bf16>(a, s);
+        default: return dkv_launch<1, 128, 1, 4, 32, __bf16>(a, s);
     }
 }
 

@@ -32,7 +32,7 @@ template <int NP, int DP, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a) {
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][TileT::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][TileT::kBytes];
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int lane = threadIdx.x & 63, rows = a.group * a.nq;
     const int r0 = (w.tile * NW + uniform(threadIdx.x >> 6)) * (NQB * 32) + (lane & 31);
@@ -56,6 +56,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
 
     TileT tile;
     tile.init(a.k);
+    Frags<DP> frags;
+    frags.init(lds_off(lds));
     if (a.k.chunks < TileT::C) clear_lds<NT>(&lds[0][0][0], sizeof(lds));
     auto load = [&](int t, int buf) {
         if ((t + 1) * KT <= n) {
@@ -83,8 +85,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
         const int buf = (t - t0) & 1;
         tile_barrier();
         if (t + 1 < t1) load(t + 1, buf ^ 1);
-        const char* kt = lds[buf][0];
-        const char* vt = lds[buf][1];
+        const uint32_t at = buf * 2 * TileT::kBytes;
         bf16x8 p[KB][2][NQB][NP];
         float sum[NQB];
         for (bool fresh = t == t0;; fresh = true) {
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
                 for (int ks = 0; ks < KS; ++ks) {
                     bf16x8 f[NP];
 #pragma unroll
-                    for (int pl = 0; pl < NP; ++pl) f[pl] = row_frag<DP>(kt + pl * KT * DP * 2, kb, ks);
+                    for (int pl = 0; pl < NP; ++pl) f[pl] = frags.rows(at, pl * KT * DP * 2, kb, ks);
 #pragma unroll
                     for (int b = 0; b < NQB; ++b) s[kb][b] = mma(f, q[b][ks], s[kb][b]);
                 }
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
                 for (int d = 0; d < DB; ++d) {
                     bf16x8 f[NP];
 #pragma unroll
-                    for (int pl = 0; pl < NP; ++pl) f[pl] = tr_frag<DP>(vt + pl * KT * DP * 2, kb, st, d);
+                    for (int pl = 0; pl < NP; ++pl) f[pl] = frags.cols(at, TileT::kBytes + pl * KT * DP * 2, kb, st, d);
 #pragma unroll
                     for (int b = 0; b < NQB; ++b) o[d][b] = mma(f, p[kb][st][b], o[d][b]);
                 }
