@@ -47,19 +47,41 @@ __device__ __forceinline__ uint32_t lds_off(const void* p) { return (uint32_t)(u
 
 // Direct-to-LDS loads: lane l's 16 (4) bytes land at lds + 16 l (4 l), whatever lanes are off.  Inline assembly, so that
 // the compiler ties no wait to them: tile_barrier waits.
+__device__ __forceinline__ const void* uniform(const void* p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return reinterpret_cast<const void*>((uintptr_t)((uint64_t)hi << 32 | lo));
+}
 __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 ::"v"(voff), "s"(uniform(sbase)), "s"(g2v::uniform((int)lds)) : "memory");
 }
 __device__ __forceinline__ void dma16(const void* addr, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 ::"v"(addr), "s"(g2v::uniform((int)lds)) : "memory");
 }
 __device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                 ::"v"(voff), "s"(uniform(sbase)), "s"(g2v::uniform((int)lds)) : "memory");
 }
 
-// Every load and LDS operation of this wave done, then the other waves met.
+// At most N loads of this wave outstanding (loads end in order) and its LDS operations done, then the other waves met.
+template <int N>
 __device__ __forceinline__ void tile_barrier() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Buffers of a kernel's tiles (pairs of `bytes`): three, loaded two tiles ahead, where the `groups` workgroups that the
+// kernel's registers allow a CU fit its 160 KB so, else two, loaded one ahead.  Three for two: 9000 x 12 heads x 64 float32
+// forward 1.33 -> 1.25 ms; bfloat16 at 96 channels dK and dV 0.395 -> 0.367 ms, but the forward there, whose
+// workgroups come three to a CU with two buffers, 0.22 -> 0.25 ms.  The barrier before tile t lets tile t + 1's loads go
+// on, if there are three buffers and that tile is whole: kLoads of them a wave (`counted`; in the last tile a wave's lanes
+// may be off altogether).  It also ends every wave's reads of tile t - 1, whose buffer is loaded next.
+constexpr int buffers(int groups, int bytes) { return 3 * 2 * bytes <= 160 * 1024 / groups ? 3 : 2; }
+template <int kBuffers, int kLoads>
+__device__ __forceinline__ void next_tile(bool counted) {
+    if (kBuffers == 3 && kLoads > 0 && counted) tile_barrier<kLoads>();
+    else tile_barrier<0>();
 }
 
 // A tile of ROWS rows of one tensor in LDS: [plane][row][DP], swizzled, filled by NT threads.
@@ -69,6 +91,7 @@ struct Tile {
     static constexpr int kChunks = NP * ROWS * C;
     static constexpr int kBytes = kChunks * 16;
     static constexpr int kIter = (kChunks + NT - 1) / NT;
+    static constexpr int kLoads = kChunks % NT ? 0 : kIter;    // of every wave; 0: not the same for all
 
     int row[kIter];         // this thread's row of each load
     uint32_t off[kIter];    // byte offset of its chunk in the row
@@ -86,7 +109,7 @@ struct Tile {
         }
     }
     __device__ __forceinline__ uint32_t dst(uint32_t lds, int it) const {
-        return lds + it * NT * 16 + (uint32_t)uniform(threadIdx.x >> 6) * 1024;
+        return lds + it * NT * 16 + (uint32_t)g2v::uniform(threadIdx.x >> 6) * 1024;
     }
     // Rows [j0, j0 + ROWS) of base, all of them there.
     __device__ __forceinline__ void load(const char* base, int64_t sn, int64_t j0, uint32_t lds) const {

@@ -15,17 +15,18 @@ using namespace attn;
 
 // dQ: rows in the lanes as in the forward, S^T = K Q^T and dP^T = V dO^T, dQ^T += K^T dS^T.
 template <int NP, int DP, int NQB, int NW, int KT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_dq(AttnBwd a) {
     // planes of dS in its product with K: two of bfloat16 for bfloat16 inputs.  The keys that a query attends to share
     // a direction, their dS sum to zero, and what is left of dQ is small beside the terms: rounding dS to 2^-9
     // alone puts dQ 3.0e-3 off (its own rounding: 1.7e-3), a second plane leaves 2.0e-3 for a third more products here
     constexpr int NS = NP == 1 ? 2 : NP;
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
-    __shared__ __attribute__((aligned(1024))) char lds[2][2][TileT::kBytes];
+    constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
+    __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int rows = a.group * a.nq;
-    const int r0 = (w.tile * NW + uniform(threadIdx.x >> 6)) * (NQB * 32) + (threadIdx.x & 31);
+    const int r0 = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32) + (threadIdx.x & 31);
     const int n = a.count ? a.count[w.b] : a.nk;
     const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
     const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
@@ -76,10 +77,10 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
     if (t0 < t1) load(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        tile_barrier();
-        if (t + 1 < t1) load(t + 1, buf ^ 1);
+    if (kAhead > 1 && t0 + 1 < t1) load(t0 + 1, 1);
+    for (int t = t0, buf = 0; t < t1; ++t, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
+        next_tile<kBuffers, 2 * TileT::kLoads>(t + 1 < t1 && (t + 2) * KT <= n);
+        if (t + kAhead < t1) load(t + kAhead, buf == 0 ? kBuffers - 1 : buf - 1);
         const uint32_t at = buf * 2 * TileT::kBytes;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -158,13 +159,15 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dq(AttnBwd a)
 // dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dkv(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 32 ? 2 : 1) k_attn_dkv(AttnBwd a) {
+    static_assert(NW % 2 == 0, "waves in pairs load the statistics");
     constexpr int NT = NW * 64, QB = QT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, QT, NT> TileT;
-    __shared__ __attribute__((aligned(1024))) char lds[2][2][TileT::kBytes];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][64];   // lse and delta of the tile's rows
+    constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
+    __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
+    __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and delta of the tile's rows
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
-    const int wave = uniform(threadIdx.x >> 6);
+    const int wave = g2v::uniform(threadIdx.x >> 6);
     const int j0 = (w.tile * NW + wave) * (NKB * 32) + (threadIdx.x & 31);
     const int n = a.count ? a.count[w.b] : a.nk;
     const int per = (a.nq + QT - 1) / QT;     // tiles of a query head
@@ -205,9 +208,9 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dkv(AttnBwd a
         }
         // rows past the end are there in the padded statistics: lse +inf makes their probabilities 0
         const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + t * QT;
+        // (even waves load lse and odd ones delta, each pair the same values: every wave has as many loads)
         const uint32_t lane = threadIdx.x & 63;
-        if (wave == 0 && lane < QT) dma4(a.lse + at, lane * 4, lds_off(stat[buf][0]));
-        if (wave == NW - 1 && lane < QT) dma4(a.delta + at, lane * 4, lds_off(stat[buf][1]));
+        if (lane < QT) dma4(((wave & 1) ? a.delta : a.lse) + at, lane * 4, lds_off(stat[buf][wave & 1]));
     };
 
     f32x16 dk[DB][NKB], dv[DB][NKB];
@@ -218,10 +221,10 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_dkv(AttnBwd a
 #pragma unroll
             for (int i = 0; i < 16; ++i) dk[d][b][i] = dv[d][b][i] = 0.0f;
     if (u0 < u1) load(u0, 0);
-    for (int u = u0; u < u1; ++u) {
-        const int buf = (u - u0) & 1;
-        tile_barrier();
-        if (u + 1 < u1) load(u + 1, buf ^ 1);
+    if (kAhead > 1 && u0 + 1 < u1) load(u0 + 1, 1);
+    for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
+        next_tile<kBuffers, TileT::kLoads ? 2 * TileT::kLoads + 1 : 0>(u + 1 < u1 && ((u + 1) % per + 1) * QT <= a.nq);
+        if (u + kAhead < u1) load(u + kAhead, buf == 0 ? kBuffers - 1 : buf - 1);
         const uint32_t at = buf * 2 * TileT::kBytes;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {

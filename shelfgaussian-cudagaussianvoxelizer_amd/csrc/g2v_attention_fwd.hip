@@ -29,13 +29,14 @@ __device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, f
 }
 
 template <int NP, int DP, int NQB, int NW, int KT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_fwd(AttnFwd a) {
     constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
-    __shared__ __attribute__((aligned(1024))) char lds[2][2][TileT::kBytes];
+    constexpr int kBuffers = buffers(NP == 1 && NQB == 1 ? 3 : 2, TileT::kBytes), kAhead = kBuffers - 1;
+    __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int lane = threadIdx.x & 63, rows = a.group * a.nq;
-    const int r0 = (w.tile * NW + uniform(threadIdx.x >> 6)) * (NQB * 32) + (lane & 31);
+    const int r0 = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32) + (lane & 31);
     const int n = a.count ? a.count[w.b] : a.nk;
     const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
     const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
@@ -81,10 +82,10 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 ? 2 : 1) k_attn_fwd(AttnFwd a
             for (int i = 0; i < 16; ++i) o[d][b][i] = 0.0f;
     }
     if (t0 < t1) load(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        tile_barrier();
-        if (t + 1 < t1) load(t + 1, buf ^ 1);
+    if (kAhead > 1 && t0 + 1 < t1) load(t0 + 1, 1);
+    for (int t = t0, buf = 0; t < t1; ++t, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
+        next_tile<kBuffers, 2 * TileT::kLoads>(t + 1 < t1 && (t + 2) * KT <= n);
+        if (t + kAhead < t1) load(t + kAhead, buf == 0 ? kBuffers - 1 : buf - 1);
         const uint32_t at = buf * 2 * TileT::kBytes;
         bf16x8 p[KB][2][NQB][NP];
         float sum[NQB];
@@ -354,7 +355,7 @@ AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows) {
     g.waves = !f32 && rows <= 32 ? 1 : 4;
     g.blocks = g.waves == 4 && !f32 && dp <= 64 ? 2 : 1;
     g.tile = f32 && dp > 32 ? 32 : 64;
-    g.per_cu = g.waves == 1 ? 4 : f32 && dp > 64 ? 1 : 2;
+    g.per_cu = g.waves == 1 ? 3 : f32 && dp > 64 ? 1 : 2;
     return g;
 }
 
