@@ -375,26 +375,36 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a, int parts) {
     store4<T>(row, d < DP ? d : d - DP, a.dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
 }
 
-// delta = sum_d dO O of a row and its lse, both padded to nqp rows of a head.  16 lanes a row.
+// delta = sum_d dO O of a row and its lse, both padded to nqp rows of a head.  2^shift lanes a row, 16 bytes each.
 template <typename T>
-__global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nqp, int heads, int dim, const T* out, const T* rest,
-                                                    const T* g, int64_t gsb, int64_t gsn, int64_t gsh, const float* lse, float* lse_p,
-                                                    float* delta) {
-    const int64_t e = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (e >= rows) return;
-    const int sub = threadIdx.x & 15;
+__global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nqp, int heads, int dim, int shift, const T* out,
+                                                    const T* rest, const T* g, int64_t gsb, int64_t gsn, int64_t gsh,
+                                                    const float* lse, float* lse_p, float* delta) {
+    constexpr int N = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    const int64_t e = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
+    if (e >= rows) return;      // the same for all lanes of a row
+    const int d = (threadIdx.x & ((1 << shift) - 1)) * N;
     const int64_t bh = e / nqp;
     const int i = (int)(e % nqp);
     const int64_t b = bh / heads, h = bh % heads;
     float v = 0.0f;
     if (i < nq) {
-        const T* o = out + ((b * nq + i) * heads + h) * dim;
-        const T* r = g + b * gsb + i * gsn + h * gsh;
-        const T* l = rest ? rest + (o - out) : nullptr;
-        for (int d = sub; d < dim; d += 16) v = fmaf(l ? (float)o[d] + (float)l[d] : (float)o[d], (float)r[d], v);
+        const int64_t at = ((b * nq + i) * heads + h) * dim + d;
+        const T* r = g + b * gsb + i * gsn + h * gsh + d;
+        if (d + N <= dim) {
+            const vec x = *reinterpret_cast<const vec*>(out + at), y = *reinterpret_cast<const vec*>(r);
+            vec l;
+            if (rest) l = *reinterpret_cast<const vec*>(rest + at);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v = fmaf(rest ? (float)x[j] + (float)l[j] : (float)x[j], (float)y[j], v);
+        } else {
+            for (int j = 0; d + j < dim; ++j)
+                v = fmaf(rest ? (float)out[at + j] + (float)rest[at + j] : (float)out[at + j], (float)r[j], v);
+        }
     }
-    for (int m = 8; m > 0; m >>= 1) v += __shfl_xor(v, m);
-    if (sub == 0) {
+    for (int m = (1 << shift) >> 1; m > 0; m >>= 1) v += __shfl_xor(v, m);
+    if (d == 0) {
         delta[e] = v;
         lse_p[e] = i < nq ? lse[bh * nq + i] : INFINITY;
     }
@@ -486,13 +496,16 @@ hipError_t launch_attn_delta(int batch, int nq, int nqp, int heads, int dim, con
                              int64_t gsb, int64_t gsn, int64_t gsh, bool f32, const float* lse, float* lse_p, float* delta, hipStream_t s) {
     const int64_t rows = (int64_t)batch * heads * nqp;
     if (rows == 0) return hipSuccess;
-    const dim3 grid((unsigned)ceil_div(rows, 16));
+    int shift = 0;
+    while ((f32 ? 4 : 8) << shift < dim) ++shift;
+    const dim3 grid((unsigned)ceil_div(rows, 256 >> shift));
     if (f32)
-        G2V_LAUNCH((k_attn_delta<float>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, static_cast<const float*>(out),
+        G2V_LAUNCH((k_attn_delta<float>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, shift, static_cast<const float*>(out),
                    static_cast<const float*>(nullptr), static_cast<const float*>(g), gsb, gsn, gsh, lse, lse_p, delta);
     else
-        G2V_LAUNCH((k_attn_delta<__bf16>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, static_cast<const __bf16*>(out),
-                   static_cast<const __bf16*>(rest), static_cast<const __bf16*>(g), gsb, gsn, gsh, lse, lse_p, delta);
+        G2V_LAUNCH((k_attn_delta<__bf16>), grid, dim3(256), 0, s, rows, nq, nqp, heads, dim, shift,
+                   static_cast<const __bf16*>(out), static_cast<const __bf16*>(rest), static_cast<const __bf16*>(g), gsb, gsn,
+                   gsh, lse, lse_p, delta);
     return hipGetLastError();
 }
 

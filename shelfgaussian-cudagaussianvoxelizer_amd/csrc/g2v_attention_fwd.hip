@@ -311,10 +311,24 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
         i = a.list[b * a.n[k] + i];
     }
     const T* src = static_cast<const T*>(a.src[k]) + bh / a.heads[k] * a.sb[k] + i * a.sn[k] + bh % a.heads[k] * a.sh[k];
+    // a whole chunk in one access or two, at any alignment (global memory takes it); a row's last elements one by one
+    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    constexpr int kPer = 16 / sizeof(T);
+    vec x[8 / kPer];
+#pragma unroll
+    for (int h = 0; h < 8 / kPer; ++h) {
+        const int d = c * 8 + h * kPer;
+        if (d + kPer <= a.dim) {
+            x[h] = *reinterpret_cast<const vec*>(src + d);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) x[h][j] = d + j < a.dim ? src[d + j] : (T)0.0f;
+        }
+    }
     bf16x8 o[NP];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float r = c * 8 + j < a.dim ? (float)src[c * 8 + j] : 0.0f;
+        float r = (float)x[j / kPer][j % kPer];
 #pragma unroll
         for (int pl = 0; pl < NP; ++pl) {
             const __bf16 h = (__bf16)r;
