@@ -298,7 +298,7 @@ struct AttnBwd {
     int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
     int nqp;             // nq rounded up to 64: rows of lse and delta, padded with +inf and 0
     float c, scale;
-    const float *lse, *delta;   // (batch, hq, nqp)
+    const float *lse, *delta;   // (batch, hq, nqp); -delta
     void *dq, *dk, *dv;
     float* part;         // dq: (splits, bhs, group nq, DP); dk and dv: (splits, bhs, 2, nk, DP)
 };

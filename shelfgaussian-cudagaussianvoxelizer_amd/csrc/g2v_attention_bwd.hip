@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
     if (n < 2) t1 = t0;    // one key: its probability is 1 whatever q is
 
     bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
-    float lse[NQB], delta[NQB];
+    float lse[NQB], delta[NQB];    // delta: negative, as it is stored
 #pragma unroll
     for (int b = 0; b < NQB; ++b) {
         const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
             for (int b = 0; b < NQB; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    s[b][i] = exp2_fast(fmaf(s[b][i], a.c, -lse[b])) * (dp[b][i] - delta[b]);
+                    s[b][i] = exp2_fast(fmaf(s[b][i], a.c, -lse[b])) * (dp[b][i] + delta[b]);
             if ((t + 1) * KT > n) {   // the last tile's rows past the end
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -159,13 +159,13 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
 // dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 32 ? 2 : 1) k_attn_dkv(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, NP == 1 && DP == 64 ? 3 : NP == 1 || DP <= 32 ? 2 : 1) k_attn_dkv(AttnBwd a) {
     static_assert(NW % 2 == 0, "waves in pairs load the statistics");
     constexpr int NT = NW * 64, QB = QT / 32, KS = DP / 16, DB = DP / 32;
     typedef Tile<NP, DP, QT, NT> TileT;
     constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
-    __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and delta of the tile's rows
+    __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and -delta of the tile's rows
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
     const int wave = g2v::uniform(threadIdx.x >> 6);
     const int j0 = (w.tile * NW + wave) * (NKB * 32) + (threadIdx.x & 31);
@@ -228,11 +228,19 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 32 ? 2 : 1) k_attn_d
         const uint32_t at = buf * 2 * TileT::kBytes;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-            f32x16 s[NKB], dp[NKB];
+            const int g4 = 4 * ((threadIdx.x >> 5) & 1);
+            f32x16 s[NKB], dp[NKB];    // dP begins at -delta
 #pragma unroll
-            for (int b = 0; b < NKB; ++b)
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[buf][1][qb * 32 + 2 * i + g4]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = dp[b][i] = 0.0f;
+                for (int b = 0; b < NKB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[b][i + j] = 0.0f;
+                        dp[b][i + j] = de[j];
+                    }
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 bf16x8 fq[NP], fg[NP];
@@ -247,17 +255,15 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 32 ? 2 : 1) k_attn_d
                     dp[b] = mma(fg, v[b][ks], dp[b]);
                 }
             }
-            const int g4 = 4 * ((threadIdx.x >> 5) & 1);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[buf][0][qb * 32 + 2 * i + g4]);
-                const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[buf][1][qb * 32 + 2 * i + g4]);
 #pragma unroll
                 for (int b = 0; b < NKB; ++b)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         s[b][i + j] = exp2_fast(fmaf(s[b][i + j], a.c, -ls[j]));
-                        dp[b][i + j] = s[b][i + j] * (dp[b][i + j] - de[j]);
+                        dp[b][i + j] *= s[b][i + j];
                     }
             }
 #pragma unroll
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a, int parts) {
     store4<T>(row, d < DP ? d : d - DP, a.dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
 }
 
-// delta = sum_d dO O of a row and its lse, both padded to nqp rows of a head.  2^shift lanes a row, 16 bytes each.
+// -delta = -sum_d dO O of a row and its lse, both padded to nqp rows of a head.  2^shift lanes a row, 16 bytes each.
 template <typename T>
 __global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nqp, int heads, int dim, int shift, const T* out,
                                                     const T* rest, const T* g, int64_t gsb, int64_t gsn, int64_t gsh,
@@ -405,7 +411,7 @@ __global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nq
     }
     for (int m = (1 << shift) >> 1; m > 0; m >>= 1) v += __shfl_xor(v, m);
     if (d == 0) {
-        delta[e] = v;
+        delta[e] = -v;
         lse_p[e] = i < nq ? lse[bh * nq + i] : INFINITY;
     }
 }
@@ -453,7 +459,7 @@ AttnShape attn_dkv_shape(bool f32, int dp) {
     g.waves = 4;
     g.blocks = 1;
     g.tile = (f32 && dp > 32) || dp > 96 ? 32 : 64;
-    g.per_cu = f32 && dp > 32 ? 1 : 2;
+    g.per_cu = f32 ? (dp > 32 ? 1 : 2) : dp == 32 ? 4 : dp == 64 ? 3 : 2;
     return g;
 }
 

@@ -367,9 +367,9 @@ AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows) {
     // 18000 keys x 16 heads x 64: 20 us instead of 25 with the same keys in flight).  float32 keys are packed first,
     // which takes longer than either.
     g.waves = !f32 && rows <= 32 ? 1 : 4;
-    g.blocks = g.waves == 4 && !f32 && dp <= 64 ? 2 : 1;
-    g.tile = f32 && dp > 32 ? 32 : 64;
-    g.per_cu = g.waves == 1 ? 3 : f32 && dp > 64 ? 1 : 2;
+    g.blocks = g.waves == 4 && !f32 && dp != 96 ? 2 : 1;
+    g.tile = (f32 && dp > 32) || dp > 96 ? 32 : 64;
+    g.per_cu = f32 ? (dp > 64 ? 1 : 2) : g.waves == 1 || dp == 32 || dp == 96 ? 3 : 2;
     return g;
 }
 
@@ -387,7 +387,7 @@ hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s) {
         case 32: return fwd_waves<1, 32, 2, 64, __bf16>(a, g, s);
         case 64: return fwd_waves<1, 64, 2, 64, __bf16>(a, g, s);
         case 96: return fwd_waves<1, 96, 1, 64, __bf16>(a, g, s);
-        default: return fwd_waves<1, 128, 1, 64, __bf16>(a, g, s);
+        default: return fwd_waves<1, 128, 2, 32, __bf16>(a, g, s);
     }
 }
 

@@ -86,7 +86,7 @@ constexpr int kCus = 256;
 int attn_splits(int64_t wgs, int units, int per_cu, double unit_us, double join_us) {
     auto cost = [&](int s) {
         const int64_t n = ceil_div(wgs * s, kCus);      // workgroups of the fullest CU
-        const double rounds = (double)(n / per_cu) + (n % per_cu ? 0.3 + 0.7 * (n % per_cu) / per_cu : 0.0);
+        const double rounds = (double)(n / per_cu) + (n % per_cu ? 0.2 + 0.8 * (n % per_cu) / per_cu : 0.0);
         const double us = rounds * (ceil_div(units, s) + 2) * unit_us;
         return s == 1 ? us : us + 5.0 + s * join_us;
     };
@@ -140,7 +140,7 @@ AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing,
     r.tiles = (int)ceil_div(mine, own);
     const int64_t units = ceil_div(passing, g.tile) * streams;
     const double flops = 2.0 * products * own * g.tile * z.dp;
-    const double unit_us = std::max(1.0, flops * g.per_cu / ((z.f32 ? 0.15e9 : 0.9e9) / kCus));
+    const double unit_us = std::max(1.0, flops * g.per_cu / ((z.f32 ? 0.15e9 : 1.0e9) / kCus));
     const double join_us = 8.0 * mine * z.bhs * width / 3e6;
     r.splits = attn_splits((int64_t)z.bhs * r.tiles, (int)std::min<int64_t>(units, 1 << 30), g.per_cu, unit_us, join_us);
     return r;

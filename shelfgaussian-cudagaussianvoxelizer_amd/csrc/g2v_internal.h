@@ -299,7 +299,7 @@ AttnShape attn_dkv_shape(bool f32, int dp);
 hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_attn_list(int batch, int nk, const unsigned char* mask, int* list, int* count, hipStream_t s);
 hipError_t launch_attn_pack(const AttnPack& a, bool f32, hipStream_t s);
-// lse and delta = sum_d g out of every row, padded to nqp rows of a head (+inf and 0); rest: see AttnFwd.
+// lse and -delta = -sum_d g out of every row, padded to nqp rows of a head (+inf and 0); rest: see AttnFwd.
 hipError_t launch_attn_delta(int batch, int nq, int nqp, int heads, int dim, const void* out, const void* rest, const void* g,
                              int64_t gsb, int64_t gsn, int64_t gsh, bool f32, const float* lse, float* lse_p, float* delta, hipStream_t s);
 hipError_t launch_attn_dq(const AttnBwd& a, bool f32, int dp, hipStream_t s);
