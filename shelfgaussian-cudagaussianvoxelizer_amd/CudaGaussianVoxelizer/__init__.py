@@ -12,12 +12,12 @@ import torch.nn as nn
 from . import _C
 from ._C import gaussian_voxelizer_forward, gaussian_voxelizer_backward
 from ._C import CudaFeatsCosinelossForward, CudaFeatsCosinelossBackward, gaussian_voxelizer_forward_batched
-from .attention import qk_norm_rotary, rotary_frequencies, gaussian_attention
+from .attention import PyGaussianAttention, gaussian_attention, qk_norm_rotary, rotary_frequencies
 
 __all__ = ["PyCudaGaussianVoxelizer", "PyCudaFeatsCosineLoss", "PyCudaGaussianVoxelizerCosineLoss", "_C",
            "gaussian_voxelizer_forward", "gaussian_voxelizer_backward", "gaussian_voxelizer_forward_batched",
            "CudaFeatsCosinelossForward", "CudaFeatsCosinelossBackward", "covariance_from_scale_rotation",
-           "qk_norm_rotary", "rotary_frequencies", "gaussian_attention"]
+           "PyGaussianAttention", "gaussian_attention", "qk_norm_rotary", "rotary_frequencies"]
 
 
 def _wants_backward(ctx, need_backward):

@@ -5,10 +5,11 @@ reached through ``_C`` on the caller's current stream.
 import math
 
 import torch
+import torch.nn as nn
 
 from . import _C
 
-__all__ = ["qk_norm_rotary", "rotary_frequencies", "gaussian_attention"]
+__all__ = ["qk_norm_rotary", "rotary_frequencies", "gaussian_attention", "PyGaussianAttention"]
 
 
 def _needs_grad(*tensors):
@@ -109,3 +110,45 @@ def gaussian_attention(q, k, v, key_mask=None, scale=None):
     if _needs_grad(q, k, v):
         return _GaussianAttentionFunction.apply(q, k, v, key_mask, scale)
     return _C.attention_forward(q, k, v, key_mask, scale)[0]
+
+
+class PyGaussianAttention(nn.Module):
+    """Multi-head attention of Gaussians to one another, or to other tokens at positions, with normed and rotated queries and
+    keys: the layer that makes the features that PyCudaGaussianVoxelizer splats.
+
+        q = rotate(norm(x Wq)),  k = rotate(norm(c Wk)),  v = c Wv,  y = attention(q, k, v) Wo
+
+    with c = x (self-attention) or the given context.  num_kv_heads key heads are shared by num_heads / num_kv_heads
+    query heads each.  ``wavelengths`` is the range over which the rotations turn, in the positions' unit (metres)."""
+
+    def __init__(self, embed_dim, num_heads, num_kv_heads=None, *, head_dim=None, axes=3, wavelengths=(0.8, 160.0), eps=1e-6,
+                 device="cuda", dtype=torch.float32):
+        super().__init__()
+        num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+        if head_dim is None:
+            if embed_dim % num_heads:
+                raise RuntimeError(f"embed_dim {embed_dim} is no multiple of num_heads {num_heads}: give head_dim")
+            head_dim = embed_dim // num_heads
+        if num_heads % num_kv_heads:
+            raise RuntimeError(f"num_heads {num_heads} is no multiple of num_kv_heads {num_kv_heads}")
+        self.heads, self.kv_heads, self.head_dim, self.eps = num_heads, num_kv_heads, head_dim, eps
+        kw = dict(bias=False, device=device, dtype=dtype)
+        self.to_q = nn.Linear(embed_dim, num_heads * head_dim, **kw)
+        self.to_kv = nn.Linear(embed_dim, 2 * num_kv_heads * head_dim, **kw)
+        self.to_out = nn.Linear(num_heads * head_dim, embed_dim, **kw)
+        self.q_weight = nn.Parameter(torch.ones(head_dim, device=device))
+        self.k_weight = nn.Parameter(torch.ones(head_dim, device=device))
+        self.register_buffer("freqs", rotary_frequencies(head_dim, axes, wavelengths, device), persistent=False)
+
+    def forward(self, x, positions, key_mask=None, *, context=None, context_positions=None):
+        """x (B, N, embed_dim) at positions (B, N, axes) float32; context (B, M, embed_dim) at context_positions (B, M, axes),
+        both or neither.  key_mask (B, N) or (B, M) bool, False at tokens that are not attended to.  Returns
+        (B, N, embed_dim); gradients flow to x, context, the weights and the positions."""
+        if (context is None) != (context_positions is None):
+            raise RuntimeError("context and context_positions go together")
+        c = x if context is None else context
+        q = self.to_q(x).unflatten(-1, (self.heads, self.head_dim))
+        k, v = self.to_kv(c).unflatten(-1, (2 * self.kv_heads, self.head_dim)).split(self.kv_heads, 2)
+        q, k = qk_norm_rotary(q, k, positions, self.freqs, self.q_weight, self.k_weight,
+                              k_positions=context_positions, eps=self.eps)
+        return self.to_out(gaussian_attention(q, k, v, key_mask).flatten(2))

@@ -1,0 +1,103 @@
+"""GPU tests of PyGaussianAttention: the layer against the same layer written in float64, gradients of every parameter, input
+and position included, and the example that trains through it and the voxelizer.
+
+Tolerance: the projections are float32 library products of at most 96 terms (2^-24 each, summed: below 1e-6), the
+operators' own bounds are 1e-5; together below 3e-5.
+"""
+import os
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def rel(x, y):
+    x, y = x.detach().double().cpu(), y.detach().double().cpu()
+    return float((x - y).norm() / y.norm())
+
+
+def plain_layer(layer, p, x, positions, mask, context, context_positions):
+    """The layer in float64 from its parameters p."""
+    H, K, D = layer.heads, layer.kv_heads, layer.head_dim
+    c, cpos = (x, positions) if context is None else (context, context_positions)
+    q = (x @ p["to_q.weight"].T).unflatten(-1, (H, D))
+    kv = (c @ p["to_kv.weight"].T).unflatten(-1, (2 * K, D))
+    k, v = kv[:, :, :K], kv[:, :, K:]
+    F = layer.freqs.double().cpu()
+
+    def turn(t, w, pos):
+        t = t * (t.square().mean(-1, keepdim=True) + layer.eps).rsqrt() * w
+        a = (pos @ F)[:, :, None]
+        n = 2 * F.shape[1]
+        z = torch.view_as_complex(t[..., :n].unflatten(-1, (-1, 2)).contiguous()) * torch.polar(torch.ones_like(a), a)
+        return torch.cat([torch.view_as_real(z).flatten(-2), t[..., n:]], -1)
+
+    q, k = turn(q, p["q_weight"], positions), turn(k, p["k_weight"], cpos)
+    k, v = k.repeat_interleave(H // K, 2), v.repeat_interleave(H // K, 2)
+    s = torch.matmul(q.transpose(1, 2), k.permute(0, 2, 3, 1)) * D ** -0.5
+    if mask is not None:
+        s = s.masked_fill(~mask[:, None, None], -torch.inf)
+    y = torch.matmul(s.softmax(-1), v.transpose(1, 2)).transpose(1, 2)
+    return y.flatten(2) @ p["to_out.weight"].T
+
+
+@pytest.mark.parametrize("cross", [False, True])
+@pytest.mark.parametrize("masked", [False, True])
+def test_layer(masked, cross):
+    from CudaGaussianVoxelizer import PyGaussianAttention
+    torch.manual_seed(3)
+    layer = PyGaussianAttention(96, 6, 2, wavelengths=(0.8, 40.0))
+    B, N, M = 2, 130, 77
+    g = torch.Generator().manual_seed(5)
+    ins = {"x": torch.randn(B, N, 96, generator=g), "positions": torch.rand(B, N, 3, generator=g) * 20 - 10}
+    if cross:
+        ins["context"] = torch.randn(B, M, 96, generator=g)
+        ins["context_positions"] = torch.rand(B, M, 3, generator=g) * 20 - 10
+    mask = torch.rand(B, M if cross else N, generator=g) < 0.7 if masked else None
+    go = torch.randn(B, N, 96, generator=g)
+    with torch.no_grad():   # weights that are not all ones
+        layer.q_weight += 0.2 * torch.randn(16, generator=g).cuda()
+        layer.k_weight += 0.2 * torch.randn(16, generator=g).cuda()
+    dev = {n: t.cuda().requires_grad_() for n, t in ins.items()}
+    y = layer(dev["x"], dev["positions"], None if mask is None else mask.cuda(), context=dev.get("context"),
+              context_positions=dev.get("context_positions"))
+    y.backward(go.cuda())
+    ref = {n: t.double().requires_grad_() for n, t in ins.items()}
+    p = {n: t.detach().double().cpu().requires_grad_() for n, t in layer.named_parameters()}
+    want = plain_layer(layer, p, ref["x"], ref["positions"], mask, ref.get("context"), ref.get("context_positions"))
+    want.backward(go.double())
+    assert rel(y, want) < 3e-5
+    for n, t in layer.named_parameters():
+        assert rel(t.grad, p[n].grad) < 3e-5, n
+    for n in ins:
+        assert rel(dev[n].grad, ref[n].grad) < 3e-5, n
+
+
+def test_layer_refusals():
+    from CudaGaussianVoxelizer import PyGaussianAttention
+    with pytest.raises(RuntimeError):
+        PyGaussianAttention(96, 7)
+    with pytest.raises(RuntimeError):
+        PyGaussianAttention(96, 6, 4)
+    with pytest.raises(RuntimeError):
+        PyGaussianAttention(8, 4)     # two values a head hold no pair for three axes
+    layer = PyGaussianAttention(96, 6)
+    with pytest.raises(RuntimeError):
+        layer(torch.zeros(1, 4, 96, device="cuda"), torch.zeros(1, 4, 3, device="cuda"),
+              context=torch.zeros(1, 4, 96, device="cuda"))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_example_trains(bf16):
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    try:
+        import gaussian_features_step as example
+    finally:
+        sys.path.pop(0)
+    losses = example.train(gaussians=600, scenes=2, channels=64, steps=6, bf16=bf16)
+    assert len(losses) == 6 and all(l == l for l in losses)
+    assert losses[-1] < losses[0] - 0.05
