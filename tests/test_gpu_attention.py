@@ -152,6 +152,35 @@ def test_large_scores(dtype):
 
 
 @pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk", [(70, 1000), (1, 5000), (300, 700)])
+@pytest.mark.parametrize("slope", [0.5, -0.5, 8.0])
+def test_references_far_from_the_maximum(slope, nq, nk, dtype):
+    """Scores that climb (or fall) by `slope` a key over the whole row, up to 40000: the first tile's reference is far off and
+    has to be renewed, and nearly all probabilities vanish.  Powers of two only, so the scores are exact in both types."""
+    d = 64
+    step = torch.arange(nk) // 64 * 64 if dtype == torch.bfloat16 else torch.arange(nk)   # 8 bits hold 64 * 0 .. 64 * 78
+    q, k = torch.zeros(1, nq, 1, d), torch.zeros(1, nk, 1, d)
+    q[..., 0] = slope
+    q[..., 1] = 1.0
+    k[..., 0] = step[None, :, None]
+    k[..., 1] = (torch.arange(nk) % 64 * abs(slope) / 16)[None, :, None]
+    g = torch.Generator().manual_seed(1)
+    v, go = torch.randn(1, nk, 1, d, generator=g), torch.randn(1, nq, 1, d, generator=g)
+    q, k, v, go = (t.to(dtype) for t in (q, k, v, go))
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    from CudaGaussianVoxelizer import gaussian_attention
+    out = gaussian_attention(*leaves, scale=1.0)
+    out.backward(go.cuda())
+    want = plain(q, k, v, None, go, 1.0)
+    # float32 scores of 40000 carry 2^-9 into the exponent at worst: 2^-24 x 40000 x log2(e), 3.4e-3
+    tol = 4e-3 if dtype == torch.float32 else 8e-3
+    assert rel(out, want[0]) < tol
+    for t, w in zip(leaves[1:], want[2:]):
+        assert torch.isfinite(t.grad).all()
+    assert rel(leaves[2].grad, want[3]) < tol
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
 @pytest.mark.parametrize("scale", [0.01, 1.0])
 def test_scale(scale, dtype):
     check(*make(1, 50, 200, 2, 2, 64, dtype, 9, size=0.7), None, dtype, scale)
@@ -207,6 +236,56 @@ def test_layouts(D, dtype):
             assert torch.equal(a, b)
     one = k[:1, :, :1].expand(B, n, h, D)
     assert torch.equal(_C.attention_forward(q, one, one)[0], _C.attention_forward(q, one.contiguous(), one.contiguous())[0])
+
+
+@pytest.mark.parametrize("stride", [40000, 1 << 24])
+def test_offsets_beyond_32_bits(stride):
+    """Keys whose rows lie further apart than 32 bits reach: views of a 5 GB buffer, read in place, and of wide strides, packed."""
+    from CudaGaussianVoxelizer import _C
+    n = (5 << 30) // 2 // stride + 2
+    buf = torch.empty(n * stride + 256, dtype=torch.bfloat16, device="cuda")
+    kv = torch.as_strided(buf, (1, n, 2, 64), (0, stride, 64, 1))
+    q, k, v, g = (t.cuda() for t in make(1, 40, n, 2, 2, 64, torch.bfloat16, 7))
+    kv.copy_(k)
+    want = _C.attention_forward(q, k, v, for_backward=True)
+    got = _C.attention_forward(q, kv, v, for_backward=True)
+    assert all(a is b is None or torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(_C.attention_backward(g, q, kv, v, *got[:3]), _C.attention_backward(g, q, k, v, *want[:3])):
+        assert torch.equal(a, b)
+    pos, fr = torch.rand(1, n, 3, device="cuda") * 80, torch.rand(3, 30, device="cuda")
+    assert torch.equal(_C.qk_norm_rotary_forward(kv, None, pos, fr)[0], _C.qk_norm_rotary_forward(k, None, pos, fr)[0])
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk,masked", [(1, 3000, False), (300, 300, True), (700, 900, False)])
+def test_graph_replays(nq, nk, masked, dtype):
+    """A captured step gives the eager step's results on every replay, with eager work and new inputs between the replays."""
+    from CudaGaussianVoxelizer import _C
+    q, k, v, g = (t.cuda() for t in make(2, nq, nk, 4, 2, 64, dtype, 5))
+    mask = random_mask(2, nk, 0.7, 3).cuda() if masked else None
+
+    def step(q, k, v, g):
+        out, rest, lse, lst = _C.attention_forward(q, k, v, mask, for_backward=True)
+        return (out,) + _C.attention_backward(g, q, k, v, out, rest, lse, lst)
+
+    static = [t.clone() for t in (q, k, v, g)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = step(*static)
+    for i in range(4):
+        new = [t.cuda() for t in make(2, nq, nk, 4, 2, 64, dtype, 20 + i)]
+        for a, b in zip(static, new):
+            a.copy_(b)
+        graph.replay()
+        want = step(*new)
+        torch.cuda.synchronize()
+        for a, b in zip(results, want):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
