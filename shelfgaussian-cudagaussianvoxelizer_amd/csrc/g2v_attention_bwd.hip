@@ -14,13 +14,14 @@ namespace {
 using namespace attn;
 
 // dQ: rows in the lanes as in the forward, S^T = K Q^T and dP^T = V dO^T, dQ^T += K^T dS^T.
-template <int NP, int DP, int NQB, int NW, int KT, typename T>
+// KS: see k_attn_fwd.
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_dq(AttnBwd a) {
     // planes of dS in its product with K: two of bfloat16 for bfloat16 inputs.  The keys that a query attends to share
     // a direction, their dS sum to zero, and what is left of dQ is small beside the terms: rounding dS to 2^-9
     // alone puts dQ 3.0e-3 off (its own rounding: 1.7e-3), a second plane leaves 2.0e-3 for a third more products here
     constexpr int NS = NP == 1 ? 2 : NP;
-    constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
+    constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
     constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
@@ -158,10 +159,10 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
 
 // dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
-template <int NP, int DP, int NKB, int NW, int QT, typename T>
+template <int NP, int DP, int KS, int NKB, int NW, int QT, typename T>
 __global__ void __launch_bounds__(NW * 64, NP == 1 && DP == 64 ? 3 : NP == 1 || DP <= 32 ? 2 : 1) k_attn_dkv(AttnBwd a) {
     static_assert(NW % 2 == 0, "waves in pairs load the statistics");
-    constexpr int NT = NW * 64, QB = QT / 32, KS = DP / 16, DB = DP / 32;
+    constexpr int NT = NW * 64, QB = QT / 32, DB = DP / 32;
     typedef Tile<NP, DP, QT, NT> TileT;
     constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
@@ -416,9 +417,9 @@ __global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nq
     }
 }
 
-template <int NP, int DP, int NQB, int NW, int KT, typename T>
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_dq<NP, DP, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
+    G2V_LAUNCH((k_attn_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
     if (a.splits > 1) {
         const int64_t rows = (int64_t)a.bhs * a.group * a.nq;
         const int parts = attn_join_parts(rows, DP / 4, a.splits);
@@ -426,9 +427,9 @@ hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
     }
     return hipGetLastError();
 }
-template <int NP, int DP, int NKB, int NW, int QT, typename T>
-hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_dkv<NP, DP, NKB, NW, QT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
+template <int NP, int DP, int KS, int NKB, int NW, int QT, typename T>
+hipError_t dkv_kernel(const AttnBwd& a, hipStream_t s) {
+    G2V_LAUNCH((k_attn_dkv<NP, DP, KS, NKB, NW, QT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
     if (a.splits > 1) {
         const int64_t rows = (int64_t)a.bhs * a.nk;
         const int parts = attn_join_parts(rows, DP / 2, a.splits);
@@ -439,9 +440,17 @@ hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
 
 template <int NP, int DP, int NQB, int KT, typename T>
 hipError_t dq_waves(const AttnBwd& a, const AttnShape& g, hipStream_t s) {
+    const bool full = a.dim > DP - 16;
     if constexpr (NP == 1)
-        if (g.waves == 1) return dq_launch<NP, DP, 1, 1, KT, T>(a, s);
-    return dq_launch<NP, DP, NQB, 4, KT, T>(a, s);
+        if (g.waves == 1)
+            return full ? dq_launch<NP, DP, DP / 16, 1, 1, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, 1, 1, KT, T>(a, s);
+    return full ? dq_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
+}
+
+template <int NP, int DP, int NKB, int NW, int QT, typename T>
+hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
+    return a.dim > DP - 16 ? dkv_kernel<NP, DP, DP / 16, NKB, NW, QT, T>(a, s)
+                           : dkv_kernel<NP, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
 }
 
 }  // namespace

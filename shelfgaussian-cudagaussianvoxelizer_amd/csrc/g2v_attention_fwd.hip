@@ -28,9 +28,10 @@ __device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, f
                       lost_by_rounding(x2), lost_by_rounding(x3));
 }
 
-template <int NP, int DP, int NQB, int NW, int KT, typename T>
+// KS: steps of 16 that the head's width takes in the scores' product (the last of DP / 16 may hold nothing but padding).
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_fwd(AttnFwd a) {
-    constexpr int NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
+    constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
     constexpr int kBuffers = buffers(NP == 1 && NQB == 1 ? 3 : 2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
@@ -341,9 +342,9 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
         *reinterpret_cast<bf16x8*>(static_cast<char*>(a.dst[k]) + ((row * NP + pl) * C + c) * 16) = o[pl];
 }
 
-template <int NP, int DP, int NQB, int NW, int KT, typename T>
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 hipError_t fwd_launch(const AttnFwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_fwd<NP, DP, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
+    G2V_LAUNCH((k_attn_fwd<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
     if (a.splits > 1) {
         const int64_t rows = (int64_t)a.bhs * a.group * a.nq;
         const int parts = attn_join_parts(rows, DP / 4, a.splits);
@@ -354,9 +355,11 @@ hipError_t fwd_launch(const AttnFwd& a, hipStream_t s) {
 
 template <int NP, int DP, int NQB, int KT, typename T>
 hipError_t fwd_waves(const AttnFwd& a, const AttnShape& g, hipStream_t s) {
+    const bool full = a.dim > DP - 16;
     if constexpr (NP == 1)
-        if (g.waves == 1) return fwd_launch<NP, DP, 1, 1, KT, T>(a, s);
-    return fwd_launch<NP, DP, NQB, 4, KT, T>(a, s);
+        if (g.waves == 1)
+            return full ? fwd_launch<NP, DP, DP / 16, 1, 1, KT, T>(a, s) : fwd_launch<NP, DP, DP / 16 - 1, 1, 1, KT, T>(a, s);
+    return full ? fwd_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : fwd_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
 }
 
 }  // namespace
