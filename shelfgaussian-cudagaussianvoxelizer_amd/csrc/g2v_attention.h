@@ -5,7 +5,7 @@
 //   C (32 x 32): column n, rows 8 (i / 4) + 4 g + i % 4 in registers i = 0 .. 15.
 // The contraction's order is free as long as A and B agree on it.  So a product's result C goes straight into the next
 // product as B, without leaving its lane: registers 8 s .. 8 s + 7 are the slots of step s, which stand for rows
-// 16 s + 4 g + {0..3} and 16 s + 8 + 4 g + {0..3}; the other operand reads its rows in that order (tr_frag).
+// 16 s + 4 g + {0..3} and 16 s + 8 + 4 g + {0..3}; the other operand reads its rows in that order (Frags::cols).
 // Scores are computed with the long axis in the registers and the workgroup's own rows in the lanes (S^T = K Q^T for the
 // forward and dQ, S = Q K^T for dK and dV): softmax statistics are one number a lane.
 //

@@ -6,7 +6,11 @@
 // The probabilities are recomputed, twice: once by workgroups that own keys (dK, dV; the queries pass by) and once by
 // workgroups that own queries (dQ; the keys pass by).  That is seven products of the scores' size instead of five, and
 // nothing is added to memory that another workgroup adds to: gradients are the same on every run, and shared key heads are
-// summed over their query heads in registers.
+// summed over their query heads in registers.  (Adding dQ up in memory would move 71 times dQ in float32 at 18000 keys,
+// 5 GB for 16 heads of 64; the two products recomputed take less.)
+//
+// Bound, like the forward, by matrix and vector work taking turns.  18000 x 8 heads x 64 bfloat16: dK and dV 1.32 ms (four
+// products, 1010 TFLOP/s), dQ 1.25 ms (three, and the one of dS twice for its two planes, 1060 TFLOP/s).
 #include "g2v_attention.h"
 
 namespace g2v {

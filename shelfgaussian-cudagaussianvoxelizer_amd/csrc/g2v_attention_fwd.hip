@@ -1,10 +1,16 @@
 // Attention over sets of Gaussians, forward: O = softmax(scale Q K^T) V over the valid keys of each scene.
 //
-// One pass over the keys with the running maximum and sum of the softmax.  The query heads that share a key head are rows
-// of one problem (row r = query r / group, head r % group), so K and V are read once for all of them.  A wave owns NQB
-// blocks of 32 rows: their Q stays in registers as B operands, K and V tiles come through LDS (direct loads, two tiles
-// deep), S^T = K Q^T lands with a lane per row and goes through exp2 straight into O^T += V^T P^T (no exchange of P).
-// Few rows: the keys are dealt to `splits` workgroups and k_attn_join joins them.
+// One pass over the keys with the running reference and sum of the softmax.  The query heads that share a key head are
+// rows of one problem (row r = query r / group, head r % group), so K and V are read once for all of them.  A wave owns NQB
+// blocks of 32 rows: their Q stays in registers as B operands, K and V tiles come through LDS by direct loads, S^T = K Q^T
+// lands with a lane per row and goes through exp2 straight into O^T += V^T P^T (no exchange of P).  Few rows, or a last
+// round of workgroups that leaves most of the card idle: the keys are dealt to `splits` workgroups and k_attn_join joins.
+//
+// Bound by the matrix and the vector unit of a SIMD taking turns: at 64 channels a row's 64 keys are 256 cycles of
+// products and, at 8.7 cycles for an exp2 of 64 lanes and 2.1 for anything else, about 220 of vector work; the counters show
+// 41 and 52 % of the kernel's cycles.  Two blocks of rows a wave halve what is read from LDS for each product (one block
+// and three or four waves a SIMD: 1.54 and 1.48 ms for 1.38).  18000 x 16 heads x 64 bfloat16: 1.38 ms, 960 TFLOP/s; 9000
+// x 12 x 64 float32: 1.25 ms, 199 TFLOP/s, 1190 of bfloat16 terms.
 #include "g2v_attention.h"
 
 namespace g2v {
@@ -366,8 +372,8 @@ hipError_t fwd_waves(const AttnFwd& a, const AttnShape& g, hipStream_t s) {
 
 AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows) {
     AttnShape g;
-    // Rows that fit one wave's block: workgroups of that one wave, more of which fit a CU than of four (one query over
-    // 18000 keys x 16 heads x 64: 20 us instead of 25 with the same keys in flight).  float32 keys are packed first,
+    // Rows that fit one wave's block: workgroups of that one wave, three to a CU with tiles of their own in flight (one
+    // query over 18000 keys x 16 heads x 64: 19 us; four waves, three of them idle, 29 us).  float32 keys are packed first,
     // which takes longer than either.
     g.waves = !f32 && rows <= 32 ? 1 : 4;
     g.blocks = g.waves == 4 && !f32 && dp != 96 ? 2 : 1;

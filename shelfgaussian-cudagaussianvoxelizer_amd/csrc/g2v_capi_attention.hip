@@ -29,9 +29,9 @@ int qn_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim
         return api_fail(G2V_ERR_INVALID, "dtype = %d (G2V_DTYPE_F32 or G2V_DTYPE_BF16)", dtype);
     if (shared && heads_k > 0 && n_k != n_q)
         return api_fail(G2V_ERR_INVALID, "shared positions need n_k == n_q, got %d and %d", n_k, n_q);
-    // workgroups along the tokens are counted in 32 bits
-    if ((double)batch * n_q > 1e9 || (double)batch * n_k > 1e9 || heads_q > 8192 || heads_k > 8192)
-        return api_fail(G2V_ERR_LIMIT, "batch %d x n %d / %d tokens (limit 1e9), heads %d / %d (limit 8192)", batch, n_q, n_k,
+    // workgroups and their threads are counted in 32 bits
+    if ((double)batch * n_q > 8388608.0 || (double)batch * n_k > 8388608.0 || heads_q > 8192 || heads_k > 8192)
+        return api_fail(G2V_ERR_LIMIT, "batch %d x n %d / %d tokens (limit 2^23), heads %d / %d (limit 8192)", batch, n_q, n_k,
                         heads_q, heads_k);
     return G2V_OK;
 }
@@ -82,17 +82,23 @@ constexpr int kCus = 256;
 
 // Into how many workgroups the long axis (`units` tiles) of each of `wgs` workgroups goes.  unit_us: time of a tile in a
 // workgroup that shares its CU with as many others as fit (per_cu); join_us: writing and adding one split's partial
-// results.  A workgroup with fewer beside it is faster: alone it takes about 0.65 of the time of two.
+// results.  A CU's last workgroups, fewer than fit, are faster: one of two takes 0.6 of the time of two.  Where a few
+// rounds fill the card more splits only add joins.  (18000 x 16 heads x 64 bfloat16 forward with 1 / 2 / 4 splits:
+// 1.51 / 1.40 / 1.44 ms; 18000 x 8 x 64 dQ with 1 / 2 / 4: 1.59 / 1.34 / 1.26 ms.)
 int attn_splits(int64_t wgs, int units, int per_cu, double unit_us, double join_us) {
-    auto cost = [&](int s) {
-        const int64_t n = ceil_div(wgs * s, kCus);      // workgroups of the fullest CU
-        const double rounds = (double)(n / per_cu) + (n % per_cu ? 0.2 + 0.8 * (n % per_cu) / per_cu : 0.0);
-        const double us = rounds * (ceil_div(units, s) + 2) * unit_us;
-        return s == 1 ? us : us + 5.0 + s * join_us;
-    };
+    const int64_t most = std::min<int64_t>(units, std::min<int64_t>(128, ceil_div(4 * kCus * per_cu, std::max<int64_t>(wgs, 1))));
     int best = 1;
-    for (int s = 2; s <= 128 && s <= units; ++s)
-        if (cost(s) < cost(best)) best = s;
+    double least = 0.0;
+    for (int s = 1; s == 1 || s <= most; ++s) {
+        const int n = (int)ceil_div(wgs * s, kCus);      // workgroups of the fullest CU
+        const double rounds = n / per_cu + (n % per_cu ? 0.2 + 0.8 * (n % per_cu) / per_cu : 0.0);
+        double us = rounds * ((units + s - 1) / s + 2) * unit_us;
+        if (s > 1) us += 5.0 + s * join_us;
+        if (s == 1 || us < least) {
+            best = s;
+            least = us;
+        }
+    }
     return best;
 }
 
@@ -118,24 +124,22 @@ int attn_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_d
     z.dp = attn_dp(head_dim);
     z.group = heads_q / heads_k;
     z.f32 = dtype == G2V_DTYPE_F32;
-    // rows of a key head and workgroups are counted in 32 bits
-    if ((double)heads_q / heads_k * n_q > 1e9 || n_k > 1000000000 || (double)batch * heads_q > 65535.0 ||
-        (double)batch * n_k > 2e9)
-        return api_fail(G2V_ERR_LIMIT, "batch %d x heads %d (limit 65535), rows %d x %d and keys %d (limit 1e9)", batch, heads_q,
-                        n_q, z.group, n_k);
+    // rows and workgroups are counted in 32 bits, and no launch has 2^32 threads
+    const double most = 33554432.0;
+    if ((double)batch * heads_q * ((double)n_q + 63.0) > most || (double)batch * heads_k * n_k > most || (double)batch * n_k > most)
+        return api_fail(G2V_ERR_LIMIT, "batch %d x heads %d / %d x n %d / %d rows (limit 2^25 of queries and of keys)", batch,
+                        heads_q, heads_k, n_q, n_k);
     z.bhs = batch * heads_k;
     return G2V_OK;
 }
 
 struct AttnRun {
-    AttnShape shape;
     int tiles, splits;
 };
 // Tiles of `mine` rows and splits of the `passing` rows (in `streams` runs that end inside a tile each); products: of
 // the scores' size that the kernel takes; width: values of a row's partial result.
 AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing, int streams, int products, int width) {
     AttnRun r;
-    r.shape = g;
     const int own = g.waves * g.blocks * 32;
     r.tiles = (int)ceil_div(mine, own);
     const int64_t units = ceil_div(passing, g.tile) * streams;
@@ -248,15 +252,15 @@ AttnBwdWs carve_attn_bwd(Carver& c, const AttnSizes& z, const AttnRun& dq, const
     return w;
 }
 
-size_t attn_fwd_bytes(const AttnSizes& z, bool packed, bool masked) {
+size_t attn_fwd_bytes(const AttnSizes& z, const AttnRun& r, bool packed, bool masked) {
     Carver c(nullptr, (size_t)-1);
-    carve_attn_fwd(c, z, attn_fwd_run(z));
+    carve_attn_fwd(c, z, r);
     carve_packed(c, z, packed, masked, false);
     return c.off + 256;
 }
-size_t attn_bwd_bytes(const AttnSizes& z, bool packed, bool masked) {
+size_t attn_bwd_bytes(const AttnSizes& z, const AttnRun& dq, const AttnRun& dkv, bool packed, bool masked) {
     Carver c(nullptr, (size_t)-1);
-    carve_attn_bwd(c, z, attn_dq_run(z), attn_dkv_run(z));
+    carve_attn_bwd(c, z, dq, dkv);
     carve_packed(c, z, packed, masked, true);
     return c.off + 256;
 }
@@ -275,7 +279,7 @@ size_t g2v_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q,
                                        int in_place, int masked) {
     AttnSizes z;
     if (attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z) != G2V_OK) return 0;
-    return attn_fwd_bytes(z, z.f32 || !in_place, masked != 0);
+    return attn_fwd_bytes(z, attn_fwd_run(z), z.f32 || !in_place, masked != 0);
 }
 
 int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -303,10 +307,10 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
                           {k, keys ? k_strides : none, n_k, heads_k, true},
                           {v, keys ? v_strides : none, n_k, heads_k, true}};
     const bool packed = !attn_in_place(z, t, 3);
-    const size_t need = attn_fwd_bytes(z, packed, list != nullptr);
+    const AttnRun r = attn_fwd_run(z);
+    const size_t need = attn_fwd_bytes(z, r, packed, list != nullptr);
     if (!workspace || workspace_bytes < need)
         return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
-    const AttnRun r = attn_fwd_run(z);
     Carver c(workspace, workspace_bytes);
     const AttnFwdWs w = carve_attn_fwd(c, z, r);
     attn::RowSrc src[3];
@@ -339,7 +343,7 @@ size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q
                                         int in_place, int masked) {
     AttnSizes z;
     if (attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z) != G2V_OK) return 0;
-    return attn_bwd_bytes(z, z.f32 || !in_place, masked != 0);
+    return attn_bwd_bytes(z, attn_dq_run(z), attn_dkv_run(z), z.f32 || !in_place, masked != 0);
 }
 
 int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -369,10 +373,10 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     const Strided t[4] = {{q, sq, n_q, heads_q, false}, {k, sk, n_k, heads_k, true}, {v, sv, n_k, heads_k, true},
                           {grad_out, sg, n_q, heads_q, false}};
     const bool packed = !attn_in_place(z, t, 4);
-    const size_t need = attn_bwd_bytes(z, packed, list != nullptr);
+    const AttnRun rq = attn_dq_run(z), rk = attn_dkv_run(z);
+    const size_t need = attn_bwd_bytes(z, rq, rk, packed, list != nullptr);
     if (!workspace || workspace_bytes < need)
         return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
-    const AttnRun rq = attn_dq_run(z), rk = attn_dkv_run(z);
     Carver c(workspace, workspace_bytes);
     const AttnBwdWs w = carve_attn_bwd(c, z, rq, rk);
     attn::RowSrc src[4];

@@ -66,7 +66,7 @@ def attention(lib, B=1, nq=4, nk=4, hq=2, hk=2, D=8, q=ONE, k=ONE, v=ONE, dt=BF1
     (dict(scale=float("inf")), 1, b"scale"), (dict(scale=float("nan")), 1, b"scale"), (dict(scale=3e38), 1, b"scale"),
     (dict(q=None), 1, b"null"), (dict(k=None), 1, b"null"), (dict(v=None), 1, b"null"), (dict(out=None), 1, b"null"),
     (dict(qs=None), 1, b"null"), (dict(mask=ONE), 1, b"key_list"), (dict(ws=None), 1, b"workspace"),
-    (dict(nws=1), 1, b"workspace"), (dict(B=40000, hq=2, hk=2), 3, b"limit"), (dict(nq=1 << 30, hq=2, hk=1), 3, b"limit"),
+    (dict(nws=1), 1, b"workspace"), (dict(B=1 << 20), 3, b"limit"), (dict(nk=1 << 25), 3, b"limit"), (dict(nq=1 << 30, hq=2, hk=1), 3, b"limit"),
 ])
 def test_attention_arguments(bad, code, word):
     lib = _lib()
