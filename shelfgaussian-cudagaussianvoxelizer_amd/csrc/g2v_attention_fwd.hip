@@ -299,25 +299,59 @@ __global__ void __launch_bounds__(kListThreads) k_attn_list(int nk, const unsign
 
 // Rows as NP bfloat16 planes of DP values each, contiguous (batch, heads, n): what the kernels cannot read in place
 // (float32, and rows that are not whole 16-byte chunks), and the valid keys of a mask one after another (9000 keys, a
-// fifth of them masked, 12 heads of 64: the forward takes 0.34 ms through an index in its loop, 0.25 ms on packed rows).
-// A thread writes one chunk of every plane.
-template <int NP, typename T>
+// fifth of them masked, 12 heads of 64: the forward takes 0.34 ms through an index in its loop, 0.28 ms on packed rows).
+// A workgroup packs neighbouring rows of one head, a thread one chunk of every plane.  MASK: the list of valid keys is
+// made here as well, each workgroup counting the mask before its rows and in all.
+template <int NP, bool MASK, typename T>
 __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
-    const int C = a.dp / 8;
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    int64_t row = e / C;
-    const int c = (int)(e % C);
+    __shared__ int counts[2][4];
+    __shared__ unsigned long long bits;
+    const int C = a.dp / 8, R = 256 / C;
+    int64_t id = blockIdx.x;
     int k = 0;
-    while (k < a.tensors && row >= a.rows[k]) row -= a.rows[k++];
-    if (k >= a.tensors) return;
-    const int64_t bh = row / a.n[k];
-    int64_t i = row % a.n[k];
-    if (a.count && a.keys[k]) {
-        const int64_t b = bh / a.heads[k];
-        if (i >= a.count[b]) return;     // never read
-        i = a.list[b * a.n[k] + i];
+    while (k < a.tensors - 1 && id >= a.blocks[k]) id -= a.blocks[k++];
+    const int per = (a.n[k] + R - 1) / R;
+    const int64_t bh = id / per, b = bh / a.heads[k];
+    const int r0 = (int)(id - bh * per) * R;
+    const int rr = threadIdx.x / C, c = threadIdx.x - rr * C;
+    int64_t i = r0 + rr, slot = i;
+    bool have = rr < R && i < a.n[k];
+    if (MASK && a.keys[k]) {
+        const unsigned char* mask = a.mask + b * a.n[k];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        int before = 0, total = 0;
+        for (int j0 = 0; j0 < a.n[k]; j0 += 256) {      // the same for all lanes
+            const int j = j0 + threadIdx.x;
+            const bool valid = j < a.n[k] && mask[j];
+            before += __popcll(__ballot(valid && j < r0));
+            total += __popcll(__ballot(valid));
+        }
+        if (lane == 0) {
+            counts[0][wave] = before;
+            counts[1][wave] = total;
+        }
+        if (wave == 0) {
+            const unsigned long long m = __ballot(r0 + lane < a.n[k] && mask[r0 + lane]);
+            if (lane == 0) bits = m;
+        }
+        __syncthreads();
+        before = counts[0][0] + counts[0][1] + counts[0][2] + counts[0][3];
+        total = counts[1][0] + counts[1][1] + counts[1][2] + counts[1][3];
+        const bool valid = have && (bits >> rr & 1);
+        const int rank = before + __popcll(bits & ((1ull << rr) - 1));
+        if (a.list_tensor == k && bh % a.heads[k] == 0) {    // valid keys in ascending order, then the others
+            if (have && c == 0) a.list_out[b * a.n[k] + (valid ? rank : total + (int)i - rank)] = (int)i;
+            if (r0 == 0 && threadIdx.x == 0) a.count_out[b] = total;
+        }
+        have = valid;
+        slot = rank;
+    } else if (a.count && a.keys[k]) {
+        have = have && i < a.count[b];     // what lies behind is never read
+        if (have) i = a.list[b * a.n[k] + i];
     }
-    const T* src = static_cast<const T*>(a.src[k]) + bh / a.heads[k] * a.sb[k] + i * a.sn[k] + bh % a.heads[k] * a.sh[k];
+    if (!have) return;
+    const T* src = static_cast<const T*>(a.src[k]) + b * a.sb[k] + i * a.sn[k] + bh % a.heads[k] * a.sh[k];
+    const int64_t row = bh * a.n[k] + slot;
     // a whole chunk in one access or two, at any alignment (global memory takes it); a row's last elements one by one
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
     constexpr int kPer = 16 / sizeof(T);
@@ -405,13 +439,23 @@ hipError_t launch_attn_list(int batch, int nk, const unsigned char* mask, int* l
     return hipGetLastError();
 }
 
-hipError_t launch_attn_pack(const AttnPack& a, bool f32, hipStream_t s) {
-    int64_t rows = 0;
-    for (int k = 0; k < a.tensors; ++k) rows += a.rows[k];
-    if (rows == 0) return hipSuccess;
-    const dim3 grid((unsigned)ceil_div(rows * (a.dp / 8), 256));
-    if (f32) G2V_LAUNCH((k_attn_pack<3, float>), grid, dim3(256), 0, s, a);
-    else G2V_LAUNCH((k_attn_pack<1, __bf16>), grid, dim3(256), 0, s, a);
+hipError_t launch_attn_pack(const AttnPack& args, bool f32, hipStream_t s) {
+    AttnPack a = args;
+    const int R = 256 / (a.dp / 8);
+    int64_t blocks = 0;
+    for (int k = 0; k < a.tensors; ++k) {
+        a.blocks[k] = ceil_div(a.n[k], R) * a.batch * a.heads[k];
+        blocks += a.blocks[k];
+    }
+    if (blocks == 0) return hipSuccess;
+    const dim3 grid((unsigned)blocks), block(256);
+    if (a.mask) {
+        if (f32) G2V_LAUNCH((k_attn_pack<3, true, float>), grid, block, 0, s, a);
+        else G2V_LAUNCH((k_attn_pack<1, true, __bf16>), grid, block, 0, s, a);
+    } else {
+        if (f32) G2V_LAUNCH((k_attn_pack<3, false, float>), grid, block, 0, s, a);
+        else G2V_LAUNCH((k_attn_pack<1, false, __bf16>), grid, block, 0, s, a);
+    }
     return hipGetLastError();
 }
 

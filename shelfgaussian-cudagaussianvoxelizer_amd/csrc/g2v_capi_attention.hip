@@ -173,16 +173,35 @@ size_t attn_packed_bytes(const AttnSizes& z, int64_t n, int heads) {
     return (size_t)z.batch * heads * n * (z.f32 ? 3 : 1) * z.dp * 2;
 }
 
+// Keys up to which packing makes the list of valid keys by itself, every workgroup reading its scene's mask: a launch less
+// (6 x 300 keys x 8 heads x 32 float32 forward: 21.6 -> 19.1 us a pass), but work that grows with the keys (4096 keys x 8
+// heads x 64 float32: 20.8 us in one launch, 6.6 + 13.6 in two).
+constexpr int kListInPack = 2048;
+
 // The tensors as the kernels read them.  What cannot be read in place is packed into c's space (all of a call, or none),
-// and the keys of a masked call are: the valid ones one after another.
-hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool packed, const int* key_list, Carver& c,
-                        attn::RowSrc* out, hipStream_t s) {
+// and the keys of a masked call are: the valid ones one after another.  key_list: (batch, nk) and (batch); with mask it
+// is made first.
+hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool packed, const unsigned char* mask, int* key_list,
+                        Carver& c, attn::RowSrc* out, hipStream_t s) {
     AttnPack a = {};
+    a.batch = z.batch;
     a.dim = z.dim;
     a.dp = z.dp;
+    a.list_tensor = -1;
     if (key_list) {
-        a.list = key_list;
-        a.count = key_list + (int64_t)z.batch * z.nk;
+        int* counts = key_list + (int64_t)z.batch * z.nk;
+        if (mask && z.nk <= kListInPack) {
+            a.mask = mask;
+            a.list_out = key_list;
+            a.count_out = counts;
+        } else {
+            if (mask) {
+                const hipError_t e = launch_attn_list(z.batch, z.nk, mask, key_list, counts, s);
+                if (e != hipSuccess) return e;
+            }
+            a.list = key_list;
+            a.count = counts;
+        }
     }
     for (int i = 0; i < count; ++i) {
         if (!packed && !(key_list && t[i].keys)) {
@@ -198,8 +217,8 @@ hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool pa
         a.sh[k] = t[i].s[2];
         a.n[k] = t[i].n;
         a.heads[k] = t[i].heads;
-        a.rows[k] = (int64_t)z.batch * t[i].heads * t[i].n;
         a.keys[k] = t[i].keys;
+        if (t[i].keys && a.list_tensor < 0) a.list_tensor = k;
         a.dst[k] = dst;
         out[i] = {dst, row * t[i].n * t[i].heads, row, row * t[i].n, z.dp / 8};
     }
@@ -294,15 +313,16 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
     if (rc != G2V_OK) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool keys = (int64_t)batch * n_k > 0;
-    if (keys && key_mask) {   // also without queries: the backward writes the keys' gradients by this list
-        if (!key_list) return api_fail(G2V_ERR_INVALID, "key_mask without key_list");
-        G2V_HIP(launch_attn_list(batch, n_k, key_mask, key_list, key_list + (int64_t)batch * n_k, s));
+    if (keys && key_mask && !key_list) return api_fail(G2V_ERR_INVALID, "key_mask without key_list");
+    if ((int64_t)batch * n_q == 0) {
+        // without queries too: the backward writes the keys' gradients by this list
+        if (keys && key_mask) G2V_HIP(launch_attn_list(batch, n_k, key_mask, key_list, key_list + (int64_t)batch * n_k, s));
+        return G2V_OK;
     }
-    if ((int64_t)batch * n_q == 0) return G2V_OK;
     if (!out || !q || !q_strides || (keys && (!k || !v || !k_strides || !v_strides)))
         return api_fail(G2V_ERR_INVALID, "null q, k, v, strides or out");
     static const long long none[3] = {0, 0, 0};
-    const int* list = keys && key_mask ? key_list : nullptr;
+    int* list = keys && key_mask ? key_list : nullptr;
     const Strided t[3] = {{q, q_strides, n_q, heads_q, false},
                           {k, keys ? k_strides : none, n_k, heads_k, true},
                           {v, keys ? v_strides : none, n_k, heads_k, true}};
@@ -314,7 +334,7 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
     Carver c(workspace, workspace_bytes);
     const AttnFwdWs w = carve_attn_fwd(c, z, r);
     attn::RowSrc src[3];
-    G2V_HIP(attn_sources(z, t, 3, packed, list, c, src, s));
+    G2V_HIP(attn_sources(z, t, 3, packed, key_mask, list, c, src, s));
     AttnFwd a = {};
     a.q = src[0];
     a.k = src[1];
@@ -380,7 +400,7 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     Carver c(workspace, workspace_bytes);
     const AttnBwdWs w = carve_attn_bwd(c, z, rq, rk);
     attn::RowSrc src[4];
-    G2V_HIP(attn_sources(z, t, 4, packed, list, c, src, s));
+    G2V_HIP(attn_sources(z, t, 4, packed, nullptr, const_cast<int*>(list), c, src, s));
     G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, out_rest, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
                               w.delta, s));
     AttnBwd a = {};

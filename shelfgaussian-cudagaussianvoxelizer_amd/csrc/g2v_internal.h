@@ -273,14 +273,19 @@ struct AttnFwd;
 struct AttnBwd;
 // Up to four tensors (batch, n, heads, dim) at element strides sb, sn, sh, packed as bfloat16 planes of dp values.
 struct AttnPack {
-    int tensors, dim, dp;
+    int tensors, batch, dim, dp;
     const void* src[4];
     int64_t sb[4], sn[4], sh[4];
     int n[4], heads[4];
-    int64_t rows[4];   // batch heads n
-    bool keys[4];      // of the keys: with count, the valid ones in list's order
-    const int *count, *list;
+    bool keys[4];      // of the keys: the valid ones alone, one after another
     void* dst[4];
+    // the valid keys, (batch) and (batch, n) of launch_attn_list; or the mask they are counted from here, and where
+    // count and list go (beside tensor list_tensor)
+    const int *count, *list;
+    const unsigned char* mask;
+    int *count_out, *list_out;
+    int list_tensor;
+    int64_t blocks[4];   // set by the launch
 };
 // A kernel's workgroup: waves, blocks of 32 rows of a wave, rows of a tile of the long axis, workgroups that fit a CU.
 struct AttnShape {
