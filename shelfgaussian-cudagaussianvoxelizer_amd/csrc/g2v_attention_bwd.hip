@@ -163,8 +163,10 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
 
 // dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
-template <int NP, int DP, int KS, int NKB, int NW, int QT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 && DP == 64 ? 3 : NP == 1 || DP <= 32 ? 2 : 1) k_attn_dkv(AttnBwd a) {
+// NS: planes of P and dS in their products.
+template <int NP, int NS, int DP, int KS, int NKB, int NW, int QT, typename T>
+__global__ void __launch_bounds__(NW * 64, NS > NP ? (DP <= 96 ? 2 : 1) : NP == 1 && DP == 64 ? 3 : NP == 1 || DP <= 32 ? 2 : 1)
+    k_attn_dkv(AttnBwd a) {
     static_assert(NW % 2 == 0, "waves in pairs load the statistics");
     constexpr int NT = NW * 64, QB = QT / 32, DB = DP / 32;
     typedef Tile<NP, DP, QT, NT> TileT;
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 && DP == 64 ? 3 : NP == 1 || 
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                bf16x8 p[NKB][NP], ds[NKB][NP];
+                bf16x8 p[NKB][NS], ds[NKB][NS];
 #pragma unroll
                 for (int b = 0; b < NKB; ++b) {
                     to_operand(s[b], st, p[b]);
@@ -431,9 +433,9 @@ hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
     }
     return hipGetLastError();
 }
-template <int NP, int DP, int KS, int NKB, int NW, int QT, typename T>
+template <int NP, int NS, int DP, int KS, int NKB, int NW, int QT, typename T>
 hipError_t dkv_kernel(const AttnBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_dkv<NP, DP, KS, NKB, NW, QT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
+    G2V_LAUNCH((k_attn_dkv<NP, NS, DP, KS, NKB, NW, QT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
     if (a.splits > 1) {
         const int64_t rows = (int64_t)a.bhs * a.nk;
         const int parts = attn_join_parts(rows, DP / 2, a.splits);
@@ -451,10 +453,19 @@ hipError_t dq_waves(const AttnBwd& a, const AttnShape& g, hipStream_t s) {
     return full ? dq_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
 }
 
+// Keys up to which bfloat16 P and dS go into dV and dK as two planes: with few keys delta takes away most of dP, and rounding
+// what is left to 2^-9 puts dK up to 2.7e-3 off (its own rounding: 1.7e-3; 2.4e-3 with many keys).  A half more products, of
+// problems whose launches take longer; 18000 queries x 300 keys x 8 heads x 64: 65 -> 74 us.
+constexpr int kFewKeys = 1024;
+
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
 hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
-    return a.dim > DP - 16 ? dkv_kernel<NP, DP, DP / 16, NKB, NW, QT, T>(a, s)
-                           : dkv_kernel<NP, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
+    const bool full = a.dim > DP - 16;
+    if constexpr (NP == 1)
+        if (a.nk <= kFewKeys)
+            return full ? dkv_kernel<NP, 2, DP, DP / 16, NKB, NW, QT, T>(a, s)
+                        : dkv_kernel<NP, 2, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
+    return full ? dkv_kernel<NP, NP, DP, DP / 16, NKB, NW, QT, T>(a, s) : dkv_kernel<NP, NP, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
 }
 
 }  // namespace
