@@ -82,16 +82,18 @@ constexpr int kCus = 256;
 
 // Into how many workgroups the long axis (`units` tiles) of each of `wgs` workgroups goes.  unit_us: time of a tile in a
 // workgroup that shares its CU with as many others as fit (per_cu); join_us: writing and adding one split's partial
-// results.  A CU's last workgroups, fewer than fit, are faster: one of two takes 0.6 of the time of two.  Where a few
-// rounds fill the card more splits only add joins.  (18000 x 16 heads x 64 bfloat16 forward with 1 / 2 / 4 splits:
-// 1.51 / 1.40 / 1.44 ms; 18000 x 8 x 64 dQ with 1 / 2 / 4: 1.59 / 1.34 / 1.26 ms.)
+// results.  A CU's last workgroups, fewer than fit, are only a little faster, a tile's loads and barriers taking their time
+// alone too: one of two is counted 0.8 of the time of two.  (3000 x 8 x 64 bfloat16 dK and dV with their join 65 us,
+// dQ 60, forward 48; counted 0.6: 92, 69 and 52.)  Where a few rounds fill the card more splits only add joins.
+// (18000 x 16 heads x 64 bfloat16 forward with 1 / 2 / 4 splits: 1.51 / 1.40 / 1.44 ms; 18000 x 8 x 64 dQ with 1 / 2 / 4:
+// 1.59 / 1.34 / 1.26 ms.)
 int attn_splits(int64_t wgs, int units, int per_cu, double unit_us, double join_us) {
     const int64_t most = std::min<int64_t>(units, std::min<int64_t>(128, ceil_div(4 * kCus * per_cu, std::max<int64_t>(wgs, 1))));
     int best = 1;
     double least = 0.0;
     for (int s = 1; s == 1 || s <= most; ++s) {
         const int n = (int)ceil_div(wgs * s, kCus);      // workgroups of the fullest CU
-        const double rounds = n / per_cu + (n % per_cu ? 0.2 + 0.8 * (n % per_cu) / per_cu : 0.0);
+        const double rounds = n / per_cu + (n % per_cu ? 0.6 + 0.4 * (n % per_cu) / per_cu : 0.0);
         double us = rounds * ((units + s - 1) / s + 2) * unit_us;
         if (s > 1) us += 5.0 + s * join_us;
         if (s == 1 || us < least) {
