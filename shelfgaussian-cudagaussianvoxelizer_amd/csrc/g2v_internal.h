@@ -263,7 +263,7 @@ struct QkNormArgs {
     float* dw_part;
 };
 constexpr int kQnAxes = 8;           // most coordinates of a position
-constexpr int kQnBwdBlocks = 2048;   // most workgroups of a side in the backward: the rows of dL/dw's partial sums
+constexpr int kQnBwdBlocks = 1024;   // most workgroups of a tensor in the backward (what the card holds): rows of dL/dw's parts
 hipError_t launch_qk_norm_rotary(const QkNormArgs& a, int dtype, hipStream_t s);
 size_t qk_norm_bwd_workspace(const QkNormArgs& a, int dtype);
 hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& a, int dtype, void* ws, hipStream_t s);

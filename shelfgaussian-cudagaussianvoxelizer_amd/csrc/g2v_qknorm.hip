@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kQnThreads = 256;
 constexpr int kQnUnroll = 4;       // rows whose loads a thread has in flight, forward
-constexpr int kQnAhead = 2;        // the same, backward (two tensors)
+constexpr int kQnAhead = 1;        // the same, backward (two tensors), the next loaded while one is computed
 
 template <typename T>
 struct QnVec;
@@ -78,21 +78,33 @@ __device__ __forceinline__ void qn_store(T* row, int d, int D, const float (&o)[
     }
 }
 
-// Sum over the 2^shift lanes of a token.  Within 16 lanes by data-parallel moves: after the steps before it every
+// Sums over the 2^shift lanes of a row.  Within 16 lanes by data-parallel moves: after the steps before it every
 // lane of a mirrored half holds the same sum, so a mirror serves as the exchange of the next size.
 template <int kCtrl>
 __device__ __forceinline__ float dpp_add(float v) {
     const int o = __builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xF, 0xF, true);
     return v + __int_as_float(o);
 }
-__device__ __forceinline__ float token_sum(float v, int shift) {
-    if (shift > 0) v = dpp_add<0xB1>(v);     // quad_perm 1 0 3 2
-    if (shift > 1) v = dpp_add<0x4E>(v);     // quad_perm 2 3 0 1
-    if (shift > 2) v = dpp_add<0x141>(v);    // row_half_mirror
-    if (shift > 3) v = dpp_add<0x140>(v);    // row_mirror
-    if (shift > 4) v += __shfl_xor(v, 16);
-    if (shift > 5) v += __shfl_xor(v, 32);
-    return v;
+template <int M>
+__device__ __forceinline__ void row_sums(float (&v)[M], int shift) {
+    if (shift > 0)    // quad_perm 1 0 3 2
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = dpp_add<0xB1>(v[m]);
+    if (shift > 1)    // quad_perm 2 3 0 1
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = dpp_add<0x4E>(v[m]);
+    if (shift > 2)    // row_half_mirror
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = dpp_add<0x141>(v[m]);
+    if (shift > 3)    // row_mirror
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = dpp_add<0x140>(v[m]);
+    if (shift > 4)
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] += __shfl_xor(v[m], 16);
+    if (shift > 5)
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] += __shfl_xor(v[m], 32);
 }
 
 // A workgroup's side of the problem: queries, keys, or both when they share positions.
@@ -117,15 +129,15 @@ __device__ __forceinline__ QnSide qn_side(const QkNormArgs& a, int side) {
 // [t0, t0 + toks) have them computed once each.  sincosf: its reduction keeps float32 accuracy for any angle (positions in
 // metres reach hundreds of radians).
 template <int N>
-__device__ __forceinline__ void qn_angles(const QkNormArgs& a, const QnSide& p, int64_t t0, int token, int d, float2* rot,
-                                          float2 (&f)[N / 2]) {
+__device__ __forceinline__ void qn_angles(const QkNormArgs& a, const float* positions, int64_t tokens, int64_t t0, int token, int d,
+                                          float2* rot, float2 (&f)[N / 2]) {
     const int width = (N / 2) << a.shift, toks = kQnThreads >> (a.shift + a.heads_shift);
     __syncthreads();    // the last tokens' are read
     for (int e = threadIdx.x; e < toks * width; e += kQnThreads) {
         const int t = e / width, i = e - t * width;
         float c = 1.0f, s = 0.0f;
-        if (i < a.pairs && t0 + t < p.tokens) {
-            const float* pos = p.pos + (t0 + t) * a.axes;
+        if (i < a.pairs && t0 + t < tokens) {
+            const float* pos = positions + (t0 + t) * a.axes;
             float w = 0.0f;
             for (int x = 0; x < a.axes; ++x) w = fmaf(pos[x], a.freqs[x * a.pairs + i], w);
             sincosf(w, &s, &c);
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
     float w[2][N];
     float2 f[N / 2];
     qn_weights<N>(a, o.d, w);
-    qn_angles<N>(a, p, t0, o.token, o.d, rot, f);
+    qn_angles<N>(a, p.pos, p.tokens, t0, o.token, o.d, rot, f);
     const float inv_d = 1.0f / (float)a.dim;
     for (int h0 = p.h0 + o.first; h0 < p.h1; h0 += o.step * kQnUnroll) {
         typename QnVec<T>::raw x[kQnUnroll];
@@ -192,13 +204,14 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
             const int h = h0 + u * o.step;   // the same for all lanes of a group
             if (h >= p.h1) break;
             const bool k = h >= a.heads[0];
-            float ss = 0.0f, y[N];
+            float ss[1] = {0.0f}, y[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 y[j] = (float)x[u][j];
-                ss = fmaf(y[j], y[j], ss);
+                ss[0] = fmaf(y[j], y[j], ss[0]);
             }
-            const float r = 1.0f / sqrtf(fmaf(token_sum(ss, a.shift), inv_d, a.eps));
+            row_sums(ss, a.shift);
+            const float r = 1.0f / sqrtf(fmaf(ss[0], inv_d, a.eps));
 #pragma unroll
             for (int j = 0; j < N; ++j) y[j] *= r * (k ? w[1][j] : w[0][j]);
 #pragma unroll
@@ -214,148 +227,155 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
     }
 }
 
-// Workgroups stride over the tokens of their side; a workgroup's sums of dL/dw go to dw_part (k_qk_norm_sums adds those, in a
-// fixed order).
+// Workgroups stride over the tokens of one tensor (queries, then keys: a workgroup of both holds the addresses, weights and
+// sums of both: 139 registers instead of 112, and 70 us instead of 60 at 18000 tokens x 16 + 16 heads x 64 bfloat16, 221 MB
+// at 3.7 TB/s; two rows ahead 62, five waves a SIMD with spills 74).  A workgroup's sums of dL/dw go to dw_part, and where the keys share the
+// queries' positions their parts of dL/dp to a.dpos[1]; k_qk_norm_sums adds those, in a fixed order.  The first rows are
+// asked for before the angles.
 template <typename T, bool AL>
 __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a) {
     constexpr int N = QnVec<T>::n;
     __shared__ float red[kQnThreads * N];
     float2* rot = reinterpret_cast<float2*>(red);
     __shared__ float dcell[kQnThreads * kQnAxes];
-    const int side = blockIdx.x >= a.blocks0;
-    const QnSide p = qn_side(a, side);
+    const int k = blockIdx.x >= a.blocks0;
     const QnPlace o = qn_place<N>(a);
-    const int toks = kQnThreads >> (a.shift + a.heads_shift);
-    const int blk = blockIdx.x - (side ? a.blocks0 : 0), nblk = side ? gridDim.x - a.blocks0 : a.blocks0;
+    const int toks = kQnThreads >> (a.shift + a.heads_shift), heads = a.heads[k];
+    const int blk = blockIdx.x - (k ? a.blocks0 : 0), nblk = k ? gridDim.x - a.blocks0 : a.blocks0;
+    const int64_t tokens = (int64_t)a.batch * a.n[k], sh = a.sh[k], gsh = a.gsh[k];
+    const float* pos = a.pos[a.shared ? 0 : k];
+    const float* weight = a.w[k];
     const float inv_d = 1.0f / (float)a.dim;
-    float* dpos = a.dpos[side];
-    float w[2][N], dw[2][N];
+    float* dpos = a.dpos[k];
+    float w[N], dw[N];
     float2 f[N / 2];
-    qn_weights<N>(a, o.d, w);
 #pragma unroll
-    for (int j = 0; j < N; ++j) dw[0][j] = dw[1][j] = 0.0f;
-    for (int64_t t0 = (int64_t)blk * toks; t0 < p.tokens; t0 += (int64_t)nblk * toks) {
-        const bool live = t0 + o.token < p.tokens;
-        const int64_t t = live ? t0 + o.token : p.tokens - 1;
-        const int64_t b = t / p.n, i = t - b * p.n;
-        const T* xq = static_cast<const T*>(a.x[0]) + b * a.sb[0] + i * a.sn[0];
-        const T* xk = static_cast<const T*>(a.x[1]) + b * a.sb[1] + i * a.sn[1];
-        const T* gq = static_cast<const T*>(a.g[0]) + b * a.gsb[0] + i * a.gsn[0];
-        const T* gk = static_cast<const T*>(a.g[1]) + b * a.gsb[1] + i * a.gsn[1];
+    for (int j = 0; j < N; ++j) {
+        w[j] = weight && o.d + j < a.dim ? weight[o.d + j] : 1.0f;
+        dw[j] = 0.0f;
+    }
+    for (int64_t t0 = (int64_t)blk * toks; t0 < tokens; t0 += (int64_t)nblk * toks) {
+        const bool live = t0 + o.token < tokens;
+        const int64_t t = live ? t0 + o.token : tokens - 1;   // groups past the end repeat the last token, unstored
+        const int64_t b = t / a.n[k], i = t - b * a.n[k];
+        const T* x0 = static_cast<const T*>(a.x[k]) + b * a.sb[k] + i * a.sn[k];
+        const T* g0 = static_cast<const T*>(a.g[k]) + b * a.gsb[k] + i * a.gsn[k];
+        T* row = static_cast<T*>(a.dx[k]) + t * heads * a.dim;
+        typename QnVec<T>::raw xv[kQnAhead], gv[kQnAhead];
         float dth[N / 2];
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) dth[j] = 0.0f;
-        qn_angles<N>(a, p, t0, o.token, o.d, rot, f);
-        for (int h0 = p.h0 + o.first; h0 < p.h1; h0 += o.step * kQnAhead) {
-            typename QnVec<T>::raw xv[kQnAhead], gv[kQnAhead];
 #pragma unroll
-            for (int u = 0; u < kQnAhead; ++u) {
-                const int h = h0 + u * o.step;
-                if (h >= p.h1) break;
-                const bool k = h >= a.heads[0];
-                xv[u] = qn_load<T, AL>(k ? xk + (h - a.heads[0]) * a.sh[1] : xq + h * a.sh[0], o.d, a.dim);
-                gv[u] = qn_load<T, AL>(k ? gk + (h - a.heads[0]) * a.gsh[1] : gq + h * a.gsh[0], o.d, a.dim);
-            }
+        for (int u = 0; u < kQnAhead; ++u) {
+            const int h = o.first + u * o.step;
+            if (h >= heads) break;
+            xv[u] = qn_load<T, AL>(x0 + h * sh, o.d, a.dim);
+            gv[u] = qn_load<T, AL>(g0 + h * gsh, o.d, a.dim);
+        }
+        qn_angles<N>(a, pos, tokens, t0, o.token, o.d, rot, f);
+        for (int h0 = o.first; h0 < heads; h0 += o.step * kQnAhead) {
 #pragma unroll
             for (int u = 0; u < kQnAhead; ++u) {
                 const int h = h0 + u * o.step;   // the same for all lanes of a group
-                if (h >= p.h1) break;
-                const bool k = h >= a.heads[0];
-                float x[N], dy[N], wv[N], ss = 0.0f, st = 0.0f;
+                if (h >= heads) break;
+                float x[N], dy[N], s[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     x[j] = (float)xv[u][j];
                     dy[j] = live ? (float)gv[u][j] : 0.0f;
-                    wv[j] = k ? w[1][j] : w[0][j];
-                    ss = fmaf(x[j], x[j], ss);
+                    s[0] = fmaf(x[j], x[j], s[0]);
+                }
+                const int next = h + o.step * kQnAhead;
+                if (next < heads) {
+                    xv[u] = qn_load<T, AL>(x0 + next * sh, o.d, a.dim);
+                    gv[u] = qn_load<T, AL>(g0 + next * gsh, o.d, a.dim);
                 }
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j) {
-                    const float g0 = dy[2 * j], g1 = dy[2 * j + 1];
-                    dy[2 * j] = g0 * f[j].x + g1 * f[j].y;
-                    dy[2 * j + 1] = g1 * f[j].x - g0 * f[j].y;
+                    const float c = dy[2 * j], d = dy[2 * j + 1];
+                    dy[2 * j] = c * f[j].x + d * f[j].y;
+                    dy[2 * j + 1] = d * f[j].x - c * f[j].y;
                 }
 #pragma unroll
-                for (int j = 0; j < N; ++j) st = fmaf(wv[j] * dy[j], x[j], st);
-                ss = token_sum(ss, a.shift);
-                st = token_sum(st, a.shift);
-                const float r = 1.0f / sqrtf(fmaf(ss, inv_d, a.eps));
-                const float q = r * r * r * inv_d * st;
+                for (int j = 0; j < N; ++j) s[1] = fmaf(w[j] * dy[j], x[j], s[1]);
+                row_sums(s, a.shift);
+                const float r = 1.0f / sqrtf(fmaf(s[0], inv_d, a.eps));
+                const float q = r * r * inv_d * s[1];
                 float dx[N];
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    const float xr = x[j] * r;
-                    const float z = dy[j] * xr;
-                    dw[0][j] += k ? 0.0f : z;
-                    dw[1][j] += k ? z : 0.0f;
-                    dx[j] = r * wv[j] * dy[j] - x[j] * q;
-                    x[j] = wv[j] * xr;
+                    const float xr = x[j] * r, wdy = w[j] * dy[j];
+                    dw[j] = fmaf(dy[j], xr, dw[j]);
+                    dx[j] = r * wdy - xr * q;
+                    x[j] = w[j] * xr;
                 }
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j) dth[j] += dy[2 * j + 1] * x[2 * j] - dy[2 * j] * x[2 * j + 1];
-                T* row = k ? static_cast<T*>(a.dx[1]) + (t * a.heads[1] + h - a.heads[0]) * a.dim
-                           : static_cast<T*>(a.dx[0]) + (t * a.heads[0] + h) * a.dim;
-                if (live) qn_store<T, AL>(row, o.d, a.dim, dx);
+                if (live) qn_store<T, AL>(row + (int64_t)h * a.dim, o.d, a.dim, dx);
             }
         }
         if (dpos) {   // of each of a token's groups, then of the token
             for (int e = 0; e < a.axes; ++e) {
-                float v = 0.0f;
+                float v[1] = {0.0f};
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j)
-                    if (o.d / 2 + j < a.pairs) v = fmaf(a.freqs[e * a.pairs + o.d / 2 + j], dth[j], v);
-                v = token_sum(v, a.shift);
-                if (o.d == 0) dcell[(threadIdx.x >> a.shift) * a.axes + e] = v;
+                    if (o.d / 2 + j < a.pairs) v[0] = fmaf(a.freqs[e * a.pairs + o.d / 2 + j], dth[j], v[0]);
+                row_sums(v, a.shift);
+                if (o.d == 0) dcell[(threadIdx.x >> a.shift) * a.axes + e] = v[0];
             }
             __syncthreads();
             for (int e = threadIdx.x; e < toks * a.axes; e += kQnThreads) {
                 const int tk = e / a.axes;
                 float v = 0.0f;
                 for (int g = 0; g < o.step; ++g) v += dcell[(tk * o.step + g) * a.axes + e - tk * a.axes];
-                if (t0 + tk < p.tokens) dpos[t0 * a.axes + e] = v;
+                if (t0 + tk < tokens) dpos[t0 * a.axes + e] = v;
             }
         }
     }
     if (!a.dw_part) return;
     // the workgroup's sums: lanes of the same elements are 2^shift apart.  Threads / width of them share an element's sum.
     const int span = N << a.shift, parts = kQnThreads > span ? kQnThreads / span : 1, slots = kQnThreads >> a.shift;
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < N; ++j) red[j * kQnThreads + threadIdx.x] = dw[k][j];
-        __syncthreads();
-        for (int c = threadIdx.x; c < span * parts; c += kQnThreads) {
-            const int e = c % span;
-            float v = 0.0f;
-            for (int g = c / span; g < slots; g += parts) v += red[(e % N) * kQnThreads + (g << a.shift) + e / N];
-            if (parts == 1) {
-                if (e < a.dim) a.dw_part[((int64_t)blockIdx.x * 2 + k) * a.dim + e] = v;
-            } else {
-                dcell[c] = v;
-            }
+    for (int j = 0; j < N; ++j) red[j * kQnThreads + threadIdx.x] = dw[j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < span * parts; c += kQnThreads) {
+        const int e = c % span;
+        float v = 0.0f;
+        for (int g = c / span; g < slots; g += parts) v += red[(e % N) * kQnThreads + (g << a.shift) + e / N];
+        if (parts == 1) {
+            if (e < a.dim) a.dw_part[(int64_t)blockIdx.x * a.dim + e] = v;
+        } else {
+            dcell[c] = v;
         }
-        if (parts == 1) continue;
-        __syncthreads();
-        for (int e = threadIdx.x; e < a.dim; e += kQnThreads) {
-            float v = 0.0f;
-            for (int g = 0; g < parts; ++g) v += dcell[g * span + e];
-            a.dw_part[((int64_t)blockIdx.x * 2 + k) * a.dim + e] = v;
-        }
+    }
+    if (parts == 1) return;
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.dim; e += kQnThreads) {
+        float v = 0.0f;
+        for (int g = 0; g < parts; ++g) v += dcell[g * span + e];
+        a.dw_part[(int64_t)blockIdx.x * a.dim + e] = v;
     }
 }
 
-// dL/dw from the workgroups' parts (`rows` rows of both weights side by side): 16 columns a workgroup, 64 lanes a column,
-// a fixed order.
+// dL/dw from the workgroups' parts (`rows` rows, the queries' before the keys'): 16 columns a workgroup, 64 lanes a column,
+// a fixed order.  Workgroups from `sums` on add the keys' parts of shared positions to the queries'.
 constexpr int kQnSumThreads = 1024;
-__global__ void __launch_bounds__(kQnSumThreads) k_qk_norm_sums(QkNormArgs a, int rows) {
+__global__ void __launch_bounds__(kQnSumThreads) k_qk_norm_sums(QkNormArgs a, int rows, int sums) {
     __shared__ float red[kQnSumThreads];
+    if ((int)blockIdx.x >= sums) {
+        const int64_t e = (int64_t)(blockIdx.x - sums) * kQnSumThreads + threadIdx.x;
+        if (e < (int64_t)a.batch * a.n[0] * a.axes) a.dpos[0][e] += a.dpos[1][e];
+        return;
+    }
     const int cols = 2 * a.dim;
     const int col = blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
+    const int k = col >= a.dim, e = k ? col - a.dim : col;
+    const int last = k ? rows : a.blocks0;
     float v = 0.0f;
     if (col < cols) {
 #pragma unroll 8
-        for (int r = part; r < rows; r += 64) v += a.dw_part[(int64_t)r * cols + col];
+        for (int r = (k ? a.blocks0 : 0) + part; r < last; r += 64) v += a.dw_part[(int64_t)r * a.dim + e];
     }
     red[threadIdx.x] = v;
     __syncthreads();
@@ -364,8 +384,8 @@ __global__ void __launch_bounds__(kQnSumThreads) k_qk_norm_sums(QkNormArgs a, in
         __syncthreads();
     }
     if (part == 0 && col < cols) {
-        float* dst = col >= a.dim ? a.dw[1] : a.dw[0];
-        if (dst) dst[col >= a.dim ? col - a.dim : col] = red[threadIdx.x];
+        float* dst = k ? a.dw[1] : a.dw[0];
+        if (dst) dst[e] = red[threadIdx.x];
     }
 }
 
@@ -403,9 +423,10 @@ QnGrid qn_grid(const QkNormArgs& a, bool bf16, bool backward) {
     const int lanes = (int)ceil_div(a.dim, bf16 ? 8 : 4);
     g.shift = 0;
     while ((1 << g.shift) < lanes) ++g.shift;
-    const int heads = a.shared ? a.heads[0] + a.heads[1] : (a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1]);
+    const bool both = a.shared && !backward;     // a workgroup's tokens have queries and keys
+    const int heads = both ? a.heads[0] + a.heads[1] : std::max(a.heads[0], a.heads[1]);
     const int64_t t[2] = {a.heads[0] + (a.shared ? a.heads[1] : 0) > 0 ? (int64_t)a.batch * a.n[0] : 0,
-                          a.shared || a.heads[1] == 0 ? 0 : (int64_t)a.batch * a.n[1]};
+                          both || a.heads[1] == 0 ? 0 : (int64_t)a.batch * a.n[1]};
     auto blocks = [&](int side) { return ceil_div(t[side], kQnThreads >> (g.shift + g.heads_shift)); };
     const int row = a.dim * (bf16 ? 2 : 4);
     g.heads_shift = 0;
@@ -442,7 +463,8 @@ hipError_t launch_qk_norm_rotary(const QkNormArgs& args, int dtype, hipStream_t 
 size_t qk_norm_bwd_workspace(const QkNormArgs& a, int dtype) {
     const QnGrid g = qn_grid(a, dtype == kDtBF16, true);
     Carver c(nullptr, (size_t)-1);
-    c.take<float>((size_t)(g.blocks[0] + g.blocks[1]) * 2 * a.dim);
+    c.take<float>((size_t)(g.blocks[0] + g.blocks[1]) * a.dim);
+    if (a.shared) c.take<float>((size_t)a.batch * a.n[1] * a.axes);
     return c.off + 256;
 }
 
@@ -456,8 +478,10 @@ hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& args, int dtype, void* ws
     const bool want_w = a.dw[0] || a.dw[1];
     const dim3 grid(g.blocks[0] + g.blocks[1]), block(kQnThreads);
     Carver c(ws, (size_t)-1);
-    float* part = c.take<float>((size_t)grid.x * 2 * a.dim);
+    float* part = c.take<float>((size_t)grid.x * a.dim);
     a.dw_part = want_w ? part : nullptr;
+    const bool add_pos = a.shared && a.dpos[0] && g.blocks[1] > 0;
+    if (a.shared) a.dpos[1] = add_pos ? c.take<float>((size_t)a.batch * a.n[1] * a.axes) : nullptr;
     if (grid.x > 0) {
         if (bf16) {
             if (qn_aligned<__bf16>(a, true)) G2V_LAUNCH((k_qk_norm_rotary_bwd<__bf16, true>), grid, block, 0, s, a);
@@ -467,8 +491,10 @@ hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& args, int dtype, void* ws
             else G2V_LAUNCH((k_qk_norm_rotary_bwd<float, false>), grid, block, 0, s, a);
         }
     }
-    if (want_w)
-        G2V_LAUNCH(k_qk_norm_sums, dim3((unsigned)ceil_div(2 * a.dim, 16)), dim3(kQnSumThreads), 0, s, a, (int)grid.x);
+    const int sums = want_w ? (int)ceil_div(2 * a.dim, 16) : 0;
+    const int adds = add_pos ? (int)ceil_div((int64_t)a.batch * a.n[0] * a.axes, kQnSumThreads) : 0;
+    if (sums + adds > 0)
+        G2V_LAUNCH(k_qk_norm_sums, dim3((unsigned)(sums + adds)), dim3(kQnSumThreads), 0, s, a, (int)grid.x, sums);
     return hipGetLastError();
 }
 
