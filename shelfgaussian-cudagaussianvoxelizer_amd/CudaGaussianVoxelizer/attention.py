@@ -6,6 +6,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _C
 
@@ -25,6 +26,7 @@ class _QkNormRotaryFunction(torch.autograd.Function):
         return _C._qk_norm_forward(inputs, ctx.call)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_q_out, grad_k_out):
         inputs = ctx.saved_tensors
         q, k = inputs[:2]
@@ -53,7 +55,7 @@ def qk_norm_rotary(q, k, positions, freqs, q_weight=None, k_weight=None, *, k_po
     sum_a positions[..., a] freqs[a, i], what is left of D stays (rotary_frequencies makes the usual table).
     q_weight and k_weight (D,) scale the normed rows.  Returns (q', k') of q's type, contiguous.
 
-    Gradients flow to q, k, the weights and the positions; freqs is a constant."""
+    Gradients flow to q, k, the weights and the positions (once: their own gradients are refused); freqs is a constant."""
     if isinstance(freqs, torch.Tensor) and freqs.requires_grad:
         raise RuntimeError("freqs is a constant of qk_norm_rotary: it gets no gradient")
     if q_weight is not None and q_weight.dtype == torch.bfloat16:
@@ -90,6 +92,7 @@ class _GaussianAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         saved, need = ctx.saved_tensors, ctx.needs_input_grad
         grad_out = _C._heads_input(grad_out, "grad_out", saved[0])
@@ -106,7 +109,8 @@ def gaussian_attention(q, k, v, key_mask=None, scale=None):
     q's type, contiguous.  Any number of queries and keys, zero and one included: a single query that pools a scene has its
     keys split over the GPU.
 
-    Gradients flow to q, k and v; the backward recomputes the probabilities and gives the same bits on every run."""
+    Gradients flow to q, k and v; the backward recomputes the probabilities and gives the same bits on every run.  Gradients
+    of gradients are refused."""
     if _needs_grad(q, k, v):
         return _GaussianAttentionFunction.apply(q, k, v, key_mask, scale)
     return _C.attention_forward(q, k, v, key_mask, scale)[0]

@@ -101,3 +101,17 @@ def test_example_trains(bf16):
     losses = example.train(gaussians=600, scenes=2, channels=64, steps=6, bf16=bf16)
     assert len(losses) == 6 and all(l == l for l in losses)
     assert losses[-1] < losses[0] - 0.05
+
+
+def test_gradients_of_gradients_are_refused():
+    from CudaGaussianVoxelizer import gaussian_attention, qk_norm_rotary, rotary_frequencies
+    x = torch.randn(1, 9, 2, 8, device="cuda", requires_grad=True)
+    y = gaussian_attention(x, x, x)
+    (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    pos = torch.rand(1, 9, 3, device="cuda")
+    q, k = qk_norm_rotary(x, x, pos, rotary_frequencies(8))
+    (g,) = torch.autograd.grad((q * k).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
