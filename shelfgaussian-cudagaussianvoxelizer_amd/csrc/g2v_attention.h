@@ -253,17 +253,54 @@ __device__ __forceinline__ void store4(T* row, int d, int D, float x0, float x1,
 // The same for what bfloat16 rounding leaves of the values.
 __device__ __forceinline__ float lost_by_rounding(float x) { return x - (float)(__bf16)x; }
 
-// A workgroup's item: head (scene b, key head h), tile and split, heads fastest, so that with 8 heads or a multiple the
-// workgroups of a head share an XCD's L2 (workgroups go to the 8 XCDs in turn).
-struct Item {
-    int b, h, bh, tile, split;
+// Into which workgroups the tiles of the heads go: the first `head` tiles of each (row0 rows) to head_splits each, the others
+// to `splits` each.  A tile's only workgroup writes its result; more write partial results, which are joined: rows [0, row0)
+// as (head_splits, bhs, row0, ..) where they are split, behind them (splits, bhs, rows - row0, ..).
+struct Parts {
+    int tiles, head, head_splits, splits, row0;
 };
-__device__ __forceinline__ Item item_of(int id, int bhs, int hk, int tiles) {
+inline int64_t workgroups(const Parts& p, int bhs) {
+    return bhs * ((int64_t)p.head * p.head_splits + (int64_t)(p.tiles - p.head) * p.splits);
+}
+// Rows of a head that a join does not see, and those of all heads' partial results.
+__host__ __device__ __forceinline__ int joined_from(const Parts& p, int rows) {
+    return p.head_splits > 1 ? 0 : p.splits > 1 ? p.row0 : rows;
+}
+inline int64_t part_rows(const Parts& p, int bhs, int64_t rows) {
+    return bhs * ((p.head_splits > 1 ? p.head_splits * (int64_t)p.row0 : 0) + (p.splits > 1 ? p.splits * (rows - p.row0) : 0));
+}
+
+// Where row r of head bh has its partial results: the first, and from one split to the next.
+struct PartRow {
+    int64_t at, step;
+    int splits;
+};
+__device__ __forceinline__ PartRow part_row(const Parts& p, int bhs, int bh, int rows, int r) {
+    PartRow o;
+    if (r < p.row0) {
+        o.splits = p.head_splits;
+        o.step = (int64_t)bhs * p.row0;
+        o.at = (int64_t)bh * p.row0 + r;
+    } else {
+        o.splits = p.splits;
+        o.step = (int64_t)bhs * (rows - p.row0);
+        o.at = (int64_t)bh * (rows - p.row0) + r - p.row0 + (p.head_splits > 1 ? (int64_t)bhs * p.head_splits * p.row0 : 0);
+    }
+    return o;
+}
+
+// A workgroup's item: head (scene b, key head h), tile and split of how many, heads fastest, so that with 8 heads or a
+// multiple the workgroups of a head share an XCD's L2 (workgroups go to the 8 XCDs in turn).
+struct Item {
+    int b, h, bh, tile, split, splits;
+};
+__device__ __forceinline__ Item item_of(int id, int bhs, int hk, const Parts& p) {
     Item w;
     w.bh = id % bhs;
-    const int rest = id / bhs;
-    w.tile = rest % tiles;
-    w.split = rest / tiles;
+    const int at = id / bhs, over = at - p.head * p.head_splits, tail = p.tiles - p.head;
+    w.tile = over < 0 ? at % p.head : p.head + over % tail;
+    w.split = over < 0 ? at / p.head : over / tail;
+    w.splits = over < 0 ? p.head_splits : p.splits;
     w.b = w.bh / hk;
     w.h = w.bh % hk;
     return w;
@@ -282,25 +319,27 @@ __device__ __forceinline__ void split_range(int all, int split, int splits, int&
 struct AttnFwd {
     attn::RowSrc q, k, v;
     const int* count;   // (batch) valid keys, the first rows of k and v; null: nk
-    int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
+    int nq, nk, hq, hk, group, dim, bhs;
+    attn::Parts parts;
     float c;            // scale log2(e)
     void* out;          // (batch, nq, hq, dim)
     void* rest;         // like out: what rounding to bfloat16 left of it, or null
     float* lse;         // (batch, hq, nq) log2 of the sum of 2^(c s); +inf for a row without keys
-    float* part_o;      // (splits, bhs, group nq, DP)
-    float* part_ml;     // (splits, bhs, group nq, 2)
+    float* part_o;      // partial results, DP values each
+    float* part_ml;     // and their maximum and sum
 };
 
 struct AttnBwd {
     attn::RowSrc q, k, v, g;
     const int* count;    // as in AttnFwd
     const int* list;     // (batch, nk) the keys that the rows of k and v are, valid ones first; null: in order
-    int nq, nk, hq, hk, group, dim, bhs, tiles, splits;
+    int nq, nk, hq, hk, group, dim, bhs;
+    attn::Parts parts;
     int nqp;             // nq rounded up to 64: rows of lse and delta, padded with +inf and 0
     float c, scale;
     const float *lse, *delta;   // (batch, hq, nqp); -delta
     void *dq, *dk, *dv;
-    float* part;         // dq: (splits, bhs, group nq, DP); dk and dv: (splits, bhs, 2, nk, DP)
+    float* part;         // partial results: dq: DP values each; dk and dv: 2 DP
 };
 
 }  // namespace g2v

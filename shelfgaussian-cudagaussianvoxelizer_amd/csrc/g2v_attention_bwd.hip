@@ -29,14 +29,14 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
     typedef Tile<NP, DP, KT, NT> TileT;
     constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
-    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int rows = a.group * a.nq;
     const int r0 = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32) + (threadIdx.x & 31);
     const int n = a.count ? a.count[w.b] : a.nk;
     const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
     const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
     int t0, t1;
-    split_range((n + KT - 1) / KT, w.split, a.splits, t0, t1);
+    split_range((n + KT - 1) / KT, w.split, w.splits, t0, t1);
     if (n < 2) t1 = t0;    // one key: its probability is 1 whatever q is
 
     bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
@@ -140,8 +140,9 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
     for (int b = 0; b < NQB; ++b) {
         const int r = r0 + 32 * b;
         if (r >= rows) continue;
-        if (a.splits > 1) {
-            float* out = a.part + (((int64_t)w.split * a.bhs + w.bh) * rows + r) * DP;
+        if (w.splits > 1) {
+            const PartRow pr = part_row(a.parts, a.bhs, w.bh, rows, r);
+            float* out = a.part + (pr.at + w.split * pr.step) * DP;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -173,13 +174,13 @@ __global__ void __launch_bounds__(NW * 64, NS > NP ? (DP <= 96 ? 2 : 1) : NP == 
     constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and -delta of the tile's rows
-    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int wave = g2v::uniform(threadIdx.x >> 6);
     const int j0 = (w.tile * NW + wave) * (NKB * 32) + (threadIdx.x & 31);
     const int n = a.count ? a.count[w.b] : a.nk;
     const int per = (a.nq + QT - 1) / QT;     // tiles of a query head
     int u0, u1;
-    split_range(per * a.group, w.split, a.splits, u0, u1);
+    split_range(per * a.group, w.split, w.splits, u0, u1);
     if (w.tile * (NW * NKB * 32) >= n) u1 = u0;    // no valid key: nothing to add up
 
     bf16x8 k[NKB][KS][NP], v[NKB][KS][NP];
@@ -302,9 +303,10 @@ __global__ void __launch_bounds__(NW * 64, NS > NP ? (DP <= 96 ? 2 : 1) : NP == 
     for (int b = 0; b < NKB; ++b) {
         const int j = j0 + 32 * b;
         if (j >= a.nk) continue;
-        if (a.splits > 1) {
+        if (w.splits > 1) {
             if (j >= n) continue;   // k_attn_dkv_join writes zeros without looking
-            float* out = a.part + (((int64_t)w.split * a.bhs + w.bh) * a.nk + j) * (2 * DP);
+            const PartRow pr = part_row(a.parts, a.bhs, w.bh, a.nk, j);
+            float* out = a.part + (pr.at + w.split * pr.step) * (2 * DP);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -359,12 +361,14 @@ template <int DP, typename T>
 __global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a, int parts) {
     constexpr int kLanes = DP / 4;
     __shared__ float red[4][256];
-    const int rows = a.group * a.nq, per = 256 / (kLanes * parts), e = threadIdx.x / parts, d = e % kLanes * 4;
-    const int64_t all = (int64_t)a.bhs * rows, at = (int64_t)blockIdx.x * per + e / kLanes;
-    const bool live = e / kLanes < per && at < all;
-    const f32x4 o = join_sum(a.part + at * DP + d, all * DP, a.splits, parts, live, red);
+    const int rows = a.group * a.nq, from = joined_from(a.parts, rows), own = rows - from, per = 256 / (kLanes * parts);
+    const int e = threadIdx.x / parts, d = e % kLanes * 4;
+    const int64_t at = (int64_t)blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < (int64_t)a.bhs * own;
+    const int bh = live ? (int)(at / own) : 0, r = live ? from + (int)(at % own) : from;
+    const PartRow pr = part_row(a.parts, a.bhs, bh, rows, r);
+    const f32x4 o = join_sum(a.part + pr.at * DP + d, pr.step * DP, pr.splits, parts, live, red);
     if (!live || threadIdx.x % parts) return;
-    const int bh = (int)(at / rows), r = (int)(at % rows);
     const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
     T* row = static_cast<T*>(a.dq) + (((int64_t)b * a.nq + tok) * a.hq + head) * a.dim;
     store4<T>(row, d, a.dim, o[0] * a.scale, o[1] * a.scale, o[2] * a.scale, o[3] * a.scale);
@@ -374,13 +378,15 @@ template <int DP, typename T>
 __global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a, int parts) {
     constexpr int kLanes = DP / 2;    // dK, then dV
     __shared__ float red[4][256];
-    const int per = 256 / (kLanes * parts), e = threadIdx.x / parts, d = e % kLanes * 4;
-    const int64_t all = (int64_t)a.bhs * a.nk, at = (int64_t)blockIdx.x * per + e / kLanes;
-    const bool live = e / kLanes < per && at < all;
-    const int bh = live ? (int)(at / a.nk) : 0, j = live ? (int)(at % a.nk) : 0, b = bh / a.hk;
+    const int from = joined_from(a.parts, a.nk), own = a.nk - from, per = 256 / (kLanes * parts);
+    const int e = threadIdx.x / parts, d = e % kLanes * 4;
+    const int64_t at = (int64_t)blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < (int64_t)a.bhs * own;
+    const int bh = live ? (int)(at / own) : 0, j = live ? from + (int)(at % own) : from, b = bh / a.hk;
     const int n = a.count ? a.count[b] : a.nk;
     const bool some = j < n && (n > 1 || d >= DP);    // one key: its probability is 1 whatever k is
-    const f32x4 o = join_sum(a.part + at * (2 * DP) + d, all * (2 * DP), a.splits, parts, live && some, red);
+    const PartRow pr = part_row(a.parts, a.bhs, bh, a.nk, j);
+    const f32x4 o = join_sum(a.part + pr.at * (2 * DP) + d, pr.step * (2 * DP), pr.splits, parts, live && some, red);
     if (!live || threadIdx.x % parts) return;
     const int64_t key = a.list ? a.list[(int64_t)b * a.nk + j] : j;
     const float f = d < DP ? a.scale : 1.0f;
@@ -425,20 +431,20 @@ __global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nq
 
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
-    if (a.splits > 1) {
-        const int64_t rows = (int64_t)a.bhs * a.group * a.nq;
-        const int parts = attn_join_parts(rows, DP / 4, a.splits);
+    G2V_LAUNCH((k_attn_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    const int64_t rows = (int64_t)a.bhs * (a.group * a.nq - joined_from(a.parts, a.group * a.nq));
+    if (rows > 0) {
+        const int parts = attn_join_parts(rows, DP / 4, std::max(a.parts.head_splits, a.parts.splits));
         G2V_LAUNCH((k_attn_dq_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 4 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();
 }
 template <int NP, int NS, int DP, int KS, int NKB, int NW, int QT, typename T>
 hipError_t dkv_kernel(const AttnBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_dkv<NP, NS, DP, KS, NKB, NW, QT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
-    if (a.splits > 1) {
-        const int64_t rows = (int64_t)a.bhs * a.nk;
-        const int parts = attn_join_parts(rows, DP / 2, a.splits);
+    G2V_LAUNCH((k_attn_dkv<NP, NS, DP, KS, NKB, NW, QT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    const int64_t rows = (int64_t)a.bhs * (a.nk - joined_from(a.parts, a.nk));
+    if (rows > 0) {
+        const int parts = attn_join_parts(rows, DP / 2, std::max(a.parts.head_splits, a.parts.splits));
         G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 2 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();

@@ -41,14 +41,14 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_f
     typedef Tile<NP, DP, KT, NT> TileT;
     constexpr int kBuffers = buffers(NP == 1 && NQB == 1 ? 3 : 2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
-    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.tiles);
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int lane = threadIdx.x & 63, rows = a.group * a.nq;
     const int r0 = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32) + (lane & 31);
     const int n = a.count ? a.count[w.b] : a.nk;
     const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
     const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
     int t0, t1;
-    split_range((n + KT - 1) / KT, w.split, a.splits, t0, t1);
+    split_range((n + KT - 1) / KT, w.split, w.splits, t0, t1);
 
     bf16x8 q[NQB][KS][NP];
 #pragma unroll
@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_f
         const int r = r0 + 32 * b;
         const float total = half_sum(l[b]);
         if (r >= rows) continue;
-        if (a.splits > 1) {
-            const int64_t at = ((int64_t)w.split * a.bhs + w.bh) * rows + r;
+        if (w.splits > 1) {
+            const PartRow pr = part_row(a.parts, a.bhs, w.bh, rows, r);
+            const int64_t at = pr.at + w.split * pr.step;
             if (lane < 32) {
                 a.part_ml[2 * at] = m[b] * a.c;
                 a.part_ml[2 * at + 1] = total;
@@ -217,17 +218,19 @@ template <int DP, typename T>
 __global__ void __launch_bounds__(256) k_attn_join(AttnFwd a, int parts) {
     constexpr int kLanes = DP / 4;
     __shared__ float red[6][256];
-    const int rows = a.group * a.nq, per = 256 / (kLanes * parts);   // rows of a workgroup
+    const int rows = a.group * a.nq, from = joined_from(a.parts, rows), own = rows - from, per = 256 / (kLanes * parts);
     const int part = threadIdx.x % parts, e = threadIdx.x / parts, d = e % kLanes * 4;
-    const int64_t all = (int64_t)a.bhs * rows, at = (int64_t)blockIdx.x * per + e / kLanes;
-    const bool live = e / kLanes < per && at < all;
+    const int64_t row = (int64_t)blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && row < (int64_t)a.bhs * own;
+    const int bh = live ? (int)(row / own) : 0, r = live ? from + (int)(row % own) : from;
+    const PartRow pr = part_row(a.parts, a.bhs, bh, rows, r);
     float top = -INFINITY, total = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     if (live) {
-        for (int s = part; s < a.splits; s += parts) top = fmaxf(top, a.part_ml[2 * (s * all + at)]);
+        for (int s = part; s < pr.splits; s += parts) top = fmaxf(top, a.part_ml[2 * (pr.at + s * pr.step)]);
 #pragma unroll 4
-        for (int s = part; s < a.splits; s += parts) {
-            const int64_t p = s * all + at;
+        for (int s = part; s < pr.splits; s += parts) {
+            const int64_t p = pr.at + s * pr.step;
             const float l = a.part_ml[2 * p + 1];
             // a split without keys has no sum, and its maximum is the lowest value
             const float f = l == 0.0f ? 0.0f : exp2_fast(a.part_ml[2 * p] - top);
@@ -255,7 +258,6 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnFwd a, int parts) {
         }
     }
     if (!live) return;
-    const int bh = (int)(at / rows), r = (int)(at % rows);
     const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
     const float inv = total > 0.0f ? 1.0f / total : 0.0f;
     if (a.lse && d == 0) a.lse[((int64_t)b * a.hq + head) * a.nq + tok] = total > 0.0f ? top + log2f(total) : INFINITY;
@@ -384,10 +386,10 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
 
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 hipError_t fwd_launch(const AttnFwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_fwd<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)(a.bhs * a.tiles * a.splits)), dim3(NW * 64), 0, s, a);
-    if (a.splits > 1) {
-        const int64_t rows = (int64_t)a.bhs * a.group * a.nq;
-        const int parts = attn_join_parts(rows, DP / 4, a.splits);
+    G2V_LAUNCH((k_attn_fwd<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    const int64_t rows = (int64_t)a.bhs * (a.group * a.nq - joined_from(a.parts, a.group * a.nq));
+    if (rows > 0) {
+        const int parts = attn_join_parts(rows, DP / 4, std::max(a.parts.head_splits, a.parts.splits));
         G2V_LAUNCH((k_attn_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 4 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();

@@ -87,10 +87,10 @@ constexpr int kCus = 256;
 // dQ 60, forward 48; counted 0.6: 92, 69 and 52.)  Where a few rounds fill the card more splits only add joins.
 // (18000 x 16 heads x 64 bfloat16 forward with 1 / 2 / 4 splits: 1.51 / 1.40 / 1.44 ms; 18000 x 8 x 64 dQ with 1 / 2 / 4:
 // 1.59 / 1.34 / 1.26 ms.)
-int attn_splits(int64_t wgs, int units, int per_cu, double unit_us, double join_us) {
+int attn_splits(int64_t wgs, int units, int per_cu, double unit_us, double join_us, double& least) {
     const int64_t most = std::min<int64_t>(units, std::min<int64_t>(128, ceil_div(4 * kCus * per_cu, std::max<int64_t>(wgs, 1))));
     int best = 1;
-    double least = 0.0;
+    least = 0.0;
     for (int s = 1; s == 1 || s <= most; ++s) {
         const int n = (int)ceil_div(wgs * s, kCus);      // workgroups of the fullest CU
         const double rounds = n / per_cu + (n % per_cu ? 0.6 + 0.4 * (n % per_cu) / per_cu : 0.0);
@@ -135,21 +135,47 @@ int attn_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_d
     return G2V_OK;
 }
 
+// The tiles of `mine` rows and the workgroups that share the `passing` rows (in `streams` runs that end inside a tile each);
+// products: of the scores' size that the kernel takes; width: values of a row's partial result.  Where all tiles with as many
+// splits would leave the card's last round half empty, the first tiles have as few splits as fill whole rounds, and the others
+// as many as fill one more, short one, together; `even`: not so, as how many tiles have work is known on the GPU only (the key
+// tiles of a masked call).  The space is that of either plan, so that masks only add to a workspace.  (9000 x
+// 8 x 128 bfloat16 dK and dV, 568 tiles on 512 places, with their join: 851 us with 3 splits each, 714 with 512 tiles whole and 56
+// in 9; its forward, 288 tiles, 400 us with 3 splits, 357 with 256 tiles in 2 and 32 in 16.)
 struct AttnRun {
-    int tiles, splits;
+    attn::Parts parts;
+    int64_t part_rows;
 };
-// Tiles of `mine` rows and splits of the `passing` rows (in `streams` runs that end inside a tile each); products: of
-// the scores' size that the kernel takes; width: values of a row's partial result.
-AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing, int streams, int products, int width) {
-    AttnRun r;
-    const int own = g.waves * g.blocks * 32;
+AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing, int streams, int products, int width, bool even) {
+    attn::Parts r = {};
+    const int own = g.waves * g.blocks * 32, slots = kCus * g.per_cu;
     r.tiles = (int)ceil_div(mine, own);
-    const int64_t units = ceil_div(passing, g.tile) * streams;
+    r.head_splits = 1;
+    const int units = (int)std::min<int64_t>(ceil_div(passing, g.tile) * streams, 1 << 30);
     const double flops = 2.0 * products * own * g.tile * z.dp;
     const double unit_us = std::max(1.0, flops * g.per_cu / ((z.f32 ? 0.15e9 : 1.0e9) / kCus));
     const double join_us = 8.0 * mine * z.bhs * width / 3e6;
-    r.splits = attn_splits((int64_t)z.bhs * r.tiles, (int)std::min<int64_t>(units, 1 << 30), g.per_cu, unit_us, join_us);
-    return r;
+    const int64_t all = (int64_t)z.bhs * r.tiles;
+    double least;
+    r.splits = attn_splits(all, units, g.per_cu, unit_us, join_us, least);
+    const AttnRun same = {r, part_rows(r, z.bhs, mine)};
+    if (least <= 1.05 * all * units * unit_us / slots) return same;
+    for (int first = 1; first <= std::min(4, units); ++first) {
+        const int64_t rounds = all * first / slots, head = rounds * slots / ((int64_t)z.bhs * first), tail = r.tiles - head;
+        if (head == 0 || tail == 0) continue;
+        double us;
+        const int splits = attn_splits(z.bhs * tail, units, g.per_cu, unit_us, join_us * tail / r.tiles, us);
+        if (splits == 1) continue;
+        us += rounds * (ceil_div(units, first) + 2) * unit_us + (first > 1 ? first * join_us * head / r.tiles : 0.0);
+        if (us < least) {
+            least = us;
+            r.head = (int)head;
+            r.head_splits = first;
+            r.splits = splits;
+            r.row0 = r.head * own;
+        }
+    }
+    return {even ? same.parts : r, std::max(same.part_rows, part_rows(r, z.bhs, mine))};
 }
 
 struct Strided {
@@ -228,11 +254,13 @@ hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool pa
 }
 
 AttnRun attn_fwd_run(const AttnSizes& z) {
-    return attn_run(z, attn_fwd_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 2, z.dp);
+    return attn_run(z, attn_fwd_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 2, z.dp, false);
 }
-AttnRun attn_dq_run(const AttnSizes& z) { return attn_run(z, attn_dq_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 3, z.dp); }
-AttnRun attn_dkv_run(const AttnSizes& z) {
-    return attn_run(z, attn_dkv_shape(z.f32, z.dp), z.nk, z.nq, z.group, 4, 2 * z.dp);
+AttnRun attn_dq_run(const AttnSizes& z) {
+    return attn_run(z, attn_dq_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 3, z.dp, false);
+}
+AttnRun attn_dkv_run(const AttnSizes& z, bool masked) {
+    return attn_run(z, attn_dkv_shape(z.f32, z.dp), z.nk, z.nq, z.group, 4, 2 * z.dp, masked);
 }
 
 struct AttnFwdWs {
@@ -240,8 +268,7 @@ struct AttnFwdWs {
 };
 AttnFwdWs carve_attn_fwd(Carver& c, const AttnSizes& z, const AttnRun& r) {
     AttnFwdWs w = {nullptr, nullptr};
-    if (r.splits > 1) {
-        const size_t rows = (size_t)r.splits * z.bhs * z.rows();
+    if (const int64_t rows = r.part_rows) {
         w.part_o = c.take<float>(rows * z.dp);
         w.part_ml = c.take<float>(rows * 2);
     }
@@ -266,9 +293,8 @@ AttnBwdWs carve_attn_bwd(Carver& c, const AttnSizes& z, const AttnRun& dq, const
     w.lse = c.take<float>((size_t)z.batch * z.hq * w.nqp);
     w.delta = c.take<float>((size_t)z.batch * z.hq * w.nqp);
     // one area: the two kernels run one after the other
-    size_t part = 0;
-    if (dq.splits > 1) part = (size_t)dq.splits * z.bhs * z.rows() * z.dp;
-    if (dkv.splits > 1) part = std::max(part, (size_t)dkv.splits * z.bhs * z.nk * 2 * z.dp);
+    size_t part = (size_t)dq.part_rows * z.dp;
+    part = std::max(part, (size_t)dkv.part_rows * 2 * z.dp);
     w.part = part ? c.take<float>(part) : nullptr;
     return w;
 }
@@ -349,8 +375,7 @@ int g2v_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k,
     a.group = z.group;
     a.dim = head_dim;
     a.bhs = z.bhs;
-    a.tiles = r.tiles;
-    a.splits = r.splits;
+    a.parts = r.parts;
     a.c = scale * attn::kLog2e;
     a.out = out;
     a.rest = out_rest;
@@ -365,7 +390,7 @@ size_t g2v_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q
                                         int in_place, int masked) {
     AttnSizes z;
     if (attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, z) != G2V_OK) return 0;
-    return attn_bwd_bytes(z, attn_dq_run(z), attn_dkv_run(z), z.f32 || !in_place, masked != 0);
+    return attn_bwd_bytes(z, attn_dq_run(z), attn_dkv_run(z, masked != 0), z.f32 || !in_place, masked != 0);
 }
 
 int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -395,7 +420,7 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     const Strided t[4] = {{q, sq, n_q, heads_q, false}, {k, sk, n_k, heads_k, true}, {v, sv, n_k, heads_k, true},
                           {grad_out, sg, n_q, heads_q, false}};
     const bool packed = !attn_in_place(z, t, 4);
-    const AttnRun rq = attn_dq_run(z), rk = attn_dkv_run(z);
+    const AttnRun rq = attn_dq_run(z), rk = attn_dkv_run(z, list != nullptr);
     const size_t need = attn_bwd_bytes(z, rq, rk, packed, list != nullptr);
     if (!workspace || workspace_bytes < need)
         return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
@@ -429,13 +454,11 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     a.dv = grad_v;
     a.part = w.part;
     if (grad_k && keys) {
-        a.tiles = rk.tiles;
-        a.splits = rk.splits;
+        a.parts = rk.parts;
         G2V_HIP(launch_attn_dkv(a, z.f32, z.dp, s));
     }
     if (grad_q && queries) {
-        a.tiles = rq.tiles;
-        a.splits = rq.splits;
+        a.parts = rq.parts;
         G2V_HIP(launch_attn_dq(a, z.f32, z.dp, s));
     }
     return G2V_OK;

@@ -354,3 +354,13 @@ def test_refusals():
     for b in bad:
         with pytest.raises(RuntimeError):
             gaussian_attention(**dict(good, **b))
+
+
+@pytest.mark.parametrize("nq,nk,H,D,dtype,keep", [
+    (99, 1301, 24, 64, torch.float32, 1.0), (641, 1299, 12, 64, torch.float32, 1.0), (641, 1299, 12, 64, torch.float32, 0.6),
+    (300, 201, 88, 64, torch.float32, 1.0), (401, 640, 36, 64, torch.float32, 1.0), (699, 641, 44, 64, torch.float32, 0.9),
+    (700, 200, 88, 64, torch.float32, 1.0), (700, 640, 44, 64, torch.float32, 1.0),
+    (500, 1300, 48, 128, torch.bfloat16, 1.0), (401, 3000, 68, 128, torch.bfloat16, 1.0)])
+def test_rounds_of_workgroups(nq, nk, H, D, dtype, keep):
+    """Tiles that fill the card once and a little: the first ones whole or in two splits, the rest in more."""
+    check(*make(1, nq, nk, H, H, D, dtype, nq + nk), None if keep == 1.0 else random_mask(1, nk, keep, nk), dtype)
