@@ -296,13 +296,19 @@ struct Item {
 };
 __device__ __forceinline__ Item item_of(int id, int bhs, int hk, const Parts& p) {
     Item w;
-    w.bh = id % bhs;
-    const int at = id / bhs, over = at - p.head * p.head_splits, tail = p.tiles - p.head;
-    w.tile = over < 0 ? at % p.head : p.head + over % tail;
-    w.split = over < 0 ? at / p.head : over / tail;
-    w.splits = over < 0 ? p.head_splits : p.splits;
-    w.b = w.bh / hk;
-    w.h = w.bh % hk;
+    int at = g2v::uniform(id / bhs), first = 0, tiles = p.head;    // (divisions run in vector registers)
+    w.bh = id - at * bhs;
+    w.splits = p.head_splits;
+    if (at >= p.head * p.head_splits) {
+        at -= p.head * p.head_splits;
+        first = p.head;
+        tiles = p.tiles - p.head;
+        w.splits = p.splits;
+    }
+    w.split = g2v::uniform(at / tiles);
+    w.tile = first + at - w.split * tiles;
+    w.b = g2v::uniform(w.bh / hk);
+    w.h = w.bh - w.b * hk;
     return w;
 }
 

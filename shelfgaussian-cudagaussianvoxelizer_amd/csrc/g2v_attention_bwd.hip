@@ -363,9 +363,9 @@ __global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a, int parts) {
     __shared__ float red[4][256];
     const int rows = a.group * a.nq, from = joined_from(a.parts, rows), own = rows - from, per = 256 / (kLanes * parts);
     const int e = threadIdx.x / parts, d = e % kLanes * 4;
-    const int64_t at = (int64_t)blockIdx.x * per + e / kLanes;
-    const bool live = e / kLanes < per && at < (int64_t)a.bhs * own;
-    const int bh = live ? (int)(at / own) : 0, r = live ? from + (int)(at % own) : from;
+    const int at = blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < a.bhs * own;
+    const int bh = live ? at / own : 0, r = live ? from + at - bh * own : from;
     const PartRow pr = part_row(a.parts, a.bhs, bh, rows, r);
     const f32x4 o = join_sum(a.part + pr.at * DP + d, pr.step * DP, pr.splits, parts, live, red);
     if (!live || threadIdx.x % parts) return;
@@ -380,9 +380,9 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a, int parts) {
     __shared__ float red[4][256];
     const int from = joined_from(a.parts, a.nk), own = a.nk - from, per = 256 / (kLanes * parts);
     const int e = threadIdx.x / parts, d = e % kLanes * 4;
-    const int64_t at = (int64_t)blockIdx.x * per + e / kLanes;
-    const bool live = e / kLanes < per && at < (int64_t)a.bhs * own;
-    const int bh = live ? (int)(at / own) : 0, j = live ? from + (int)(at % own) : from, b = bh / a.hk;
+    const int at = blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < a.bhs * own;
+    const int bh = live ? at / own : 0, j = live ? from + at - bh * own : from, b = bh / a.hk;
     const int n = a.count ? a.count[b] : a.nk;
     const bool some = j < n && (n > 1 || d >= DP);    // one key: its probability is 1 whatever k is
     const PartRow pr = part_row(a.parts, a.bhs, bh, a.nk, j);

@@ -220,9 +220,9 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnFwd a, int parts) {
     __shared__ float red[6][256];
     const int rows = a.group * a.nq, from = joined_from(a.parts, rows), own = rows - from, per = 256 / (kLanes * parts);
     const int part = threadIdx.x % parts, e = threadIdx.x / parts, d = e % kLanes * 4;
-    const int64_t row = (int64_t)blockIdx.x * per + e / kLanes;
-    const bool live = e / kLanes < per && row < (int64_t)a.bhs * own;
-    const int bh = live ? (int)(row / own) : 0, r = live ? from + (int)(row % own) : from;
+    const int row = blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && row < a.bhs * own;
+    const int bh = live ? row / own : 0, r = live ? from + row - bh * own : from;
     const PartRow pr = part_row(a.parts, a.bhs, bh, rows, r);
     float top = -INFINITY, total = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
