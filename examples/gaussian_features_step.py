@@ -71,7 +71,8 @@ def train(gaussians=2000, scenes=2, channels=64, steps=5, bf16=False, seed=0):
             seen = density.detach() > 1e-3
         loss = sum(cosine(label, seen[b], grid[b], target)[0] for b in range(scenes)) / scenes
         optimizer.zero_grad()
-        loss.backward()
+        with torch.autograd.set_multithreading_enabled(False):   # one GPU: no waiting for the engine's thread
+            loss.backward()
         optimizer.step()
         losses.append(float(loss.detach()))
     return losses

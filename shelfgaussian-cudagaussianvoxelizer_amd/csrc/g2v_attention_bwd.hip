@@ -9,8 +9,8 @@
 // summed over their query heads in registers.  (Adding dQ up in memory would move 71 times dQ in float32 at 18000 keys,
 // 5 GB for 16 heads of 64; the two products recomputed take less.)
 //
-// Bound, like the forward, by matrix and vector work taking turns.  18000 x 8 heads x 64 bfloat16: dK and dV 1.32 ms (four
-// products, 1010 TFLOP/s), dQ 1.25 ms (three, and the one of dS twice for its two planes, 1060 TFLOP/s).
+// Bound, like the forward, by matrix and vector work taking turns.  18000 x 8 heads x 64 bfloat16: dK and dV 1.27 ms (four
+// products, 1050 TFLOP/s), dQ 1.17 ms (three, and the one of dS twice for its two planes, 1150 TFLOP/s).
 #include "g2v_attention.h"
 
 namespace g2v {

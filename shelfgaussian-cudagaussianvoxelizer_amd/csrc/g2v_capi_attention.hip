@@ -85,8 +85,8 @@ constexpr int kCus = 256;
 // results.  A CU's last workgroups, fewer than fit, are only a little faster, a tile's loads and barriers taking their time
 // alone too: one of two is counted 0.8 of the time of two.  (3000 x 8 x 64 bfloat16 dK and dV with their join 65 us,
 // dQ 60, forward 48; counted 0.6: 92, 69 and 52.)  Where a few rounds fill the card more splits only add joins.
-// (18000 x 16 heads x 64 bfloat16 forward with 1 / 2 / 4 splits: 1.51 / 1.40 / 1.44 ms; 18000 x 8 x 64 dQ with 1 / 2 / 4:
-// 1.59 / 1.34 / 1.26 ms.)
+// (18000 x 16 heads x 64 bfloat16 forward with 1 / 2 / 4 splits of every tile: 1.51 / 1.40 / 1.44 ms; 18000 x 8 x 64 dQ with
+// 1 / 2 / 4: 1.59 / 1.34 / 1.26 ms; attn_run goes on from there.)
 int attn_splits(int64_t wgs, int units, int per_cu, double unit_us, double join_us, double& least) {
     const int64_t most = std::min<int64_t>(units, std::min<int64_t>(128, ceil_div(4 * kCus * per_cu, std::max<int64_t>(wgs, 1))));
     int best = 1;

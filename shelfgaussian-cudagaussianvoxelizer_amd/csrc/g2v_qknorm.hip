@@ -227,11 +227,11 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
     }
 }
 
-// Workgroups stride over the tokens of one tensor (queries, then keys: a workgroup of both holds the addresses, weights and
-// sums of both: 139 registers instead of 112, and 70 us instead of 60 at 18000 tokens x 16 + 16 heads x 64 bfloat16, 221 MB
-// at 3.7 TB/s; two rows ahead 62, five waves a SIMD with spills 74).  A workgroup's sums of dL/dw go to dw_part, and where the keys share the
-// queries' positions their parts of dL/dp to a.dpos[1]; k_qk_norm_sums adds those, in a fixed order.  The first rows are
-// asked for before the angles.
+// Workgroups stride over the tokens of one tensor, queries or keys: a workgroup of both holds the addresses, weights and sums
+// of both (139 registers instead of 112, and 70 us instead of 60 at 18000 tokens x 16 + 16 heads x 64 bfloat16, 221 MB at
+// 3.8 TB/s; two rows ahead 62, five waves a SIMD with spills 74).  A workgroup's sums of dL/dw go to dw_part, and where
+// the keys share the queries' positions their parts of dL/dp to a.dpos[1]; k_qk_norm_sums adds those, in a fixed order.  The
+// first rows are asked for before the angles.
 template <typename T, bool AL>
 __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a) {
     constexpr int N = QnVec<T>::n;
