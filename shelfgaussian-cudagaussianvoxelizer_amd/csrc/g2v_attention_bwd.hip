@@ -481,7 +481,7 @@ AttnShape attn_dq_shape(bool f32, int dp, int64_t rows) {
     g.waves = !f32 && rows <= 32 ? 1 : 4;    // as in attn_fwd_shape
     g.blocks = g.waves == 4 && !f32 && dp <= 64 ? 2 : 1;
     g.tile = f32 && dp > 32 ? 32 : 64;
-    g.per_cu = g.waves == 1 ? 4 : f32 && dp > 32 ? 1 : 2;
+    g.per_cu = g.waves == 1 ? 4 : f32 && dp > 64 ? 1 : 2;
     return g;
 }
 AttnShape attn_dkv_shape(bool f32, int dp) {
