@@ -879,13 +879,18 @@ def _qk_norm_inputs(q, k, positions, freqs, q_weight, k_weight, k_positions, eps
     return (q, k, positions, freqs, q_weight, k_weight, k_positions), call
 
 
+def _empty_rows(t):
+    """A contiguous tensor like t (a microsecond less of host time than naming shape, type and device)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _qk_norm_forward(inputs, call):
     q, k, pos, freqs, qw, kw, kpos = inputs
     sizes, pairs, fdt, eps = call
     dev = q.device
     with _OnDevice(dev):
-        oq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        ok = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+        oq = _empty_rows(q)
+        ok = None if k is None else _empty_rows(k)
         rc = _lib.load().g2v_qk_norm_rotary_forward(*sizes, pairs, _addr(q), _strides(q), _addr(k), _strides(k), fdt,
                                                     _addr(qw), _addr(kw), _addr(pos), _addr(kpos), _addr(freqs), eps,
                                                     _addr(oq), _addr(ok), _stream_of(dev))
@@ -901,8 +906,8 @@ def _qk_norm_backward(gq, gk, inputs, call, want_weights, want_positions):
     if gq.shape != q.shape or (k is not None and gk.shape != k.shape):
         raise RuntimeError(f"gradients must be {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
     with _OnDevice(dev):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+        dq = _empty_rows(q)
+        dk = None if k is None else _empty_rows(k)
         dqw = torch.empty(sizes[5], dtype=f32, device=dev) if want_weights[0] else None
         dkw = torch.empty(sizes[5], dtype=f32, device=dev) if want_weights[1] and k is not None else None
         dpos = torch.empty(pos.shape, dtype=f32, device=dev) if want_positions[0] else None
@@ -968,8 +973,8 @@ def _attention_forward(inputs, call, for_backward):
     B, nq, nk, hq = sizes[:4]
     dev = q.device
     with _OnDevice(dev):
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if for_backward and fdt == _lib.G2V_DTYPE_BF16 else None
+        out = _empty_rows(q)
+        rest = _empty_rows(q) if for_backward and fdt == _lib.G2V_DTYPE_BF16 else None
         lse = torch.empty(B, hq, nq, dtype=torch.float32, device=dev) if for_backward else None
         lst = None if key_mask is None else torch.empty(B * (nk + 1), dtype=torch.int32, device=dev)
         nws = _workspace_bytes("g2v_attention_forward_workspace", *sizes, fdt, _in_place(q, k, v), 0 if lst is None else 1)
@@ -988,9 +993,9 @@ def _attention_backward(g, q, k, v, out, rest, lse, key_list, call, want_q, want
     if g.shape != q.shape:
         raise RuntimeError(f"grad_out must be {tuple(q.shape)}, got {tuple(g.shape)}")
     with _OnDevice(dev):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
-        dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
-        dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if want_kv else None
+        dq = _empty_rows(q) if want_q else None
+        dk = _empty_rows(k) if want_kv else None
+        dv = _empty_rows(k) if want_kv else None
         nws = _workspace_bytes("g2v_attention_backward_workspace", *sizes, fdt, _in_place(q, k, v, g),
                                0 if key_list is None else 1)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev)
