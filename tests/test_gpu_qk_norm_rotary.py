@@ -195,3 +195,43 @@ def test_refusals():
         args = dict(dict(q=q, k=None, positions=pos, freqs=fr), **b)
         with pytest.raises(RuntimeError):
             qk_norm_rotary(**args)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+@pytest.mark.parametrize("wanted", ["pos", "qw", "kw", "q", "k"])
+def test_single_gradients(wanted, shared):
+    """One input alone wants a gradient: it is the one of the call that gives all, bit for bit."""
+    from CudaGaussianVoxelizer import qk_norm_rotary
+    d, _ = make(2, 70, 130, 6, 3, 24, 3, 12, torch.float32, 5, shared)
+    d = {n: None if t is None else t.cuda() for n, t in d.items()}
+    g = torch.Generator().manual_seed(9)
+    go = [torch.randn(t.shape, generator=g).cuda() for t in (d["q"], d["k"])]
+    grads = []
+    for names in ([n for n, t in d.items() if t is not None and n != "freqs"], [wanted]):
+        leaves = {n: None if t is None else t.detach().clone().requires_grad_(n in names) for n, t in d.items()}
+        out = qk_norm_rotary(leaves["q"], leaves["k"], leaves["pos"], leaves["freqs"], leaves["qw"], leaves["kw"],
+                             k_positions=leaves["kpos"])
+        torch.autograd.backward(out, go)
+        grads.append(leaves[wanted].grad)
+    assert grads[0] is not None and torch.equal(*grads)
+
+
+def test_no_query_heads():
+    """Keys alone with the queries' positions: their gradient is the keys'."""
+    from CudaGaussianVoxelizer import qk_norm_rotary
+    d, _ = make(2, 40, 40, 4, 2, 16, 3, 8, torch.float32, 6, False)
+    g = torch.Generator().manual_seed(10)
+    go = torch.randn(2, 40, 2, 16, generator=g).cuda()
+    res = []
+    for empty in (True, False):
+        k, pos = d["k"].cuda().requires_grad_(), d["kpos"].cuda().requires_grad_()
+        fr, kw = d["freqs"].cuda(), d["kw"].cuda()
+        if empty:
+            q, out = qk_norm_rotary(torch.empty(2, 40, 0, 16, device="cuda"), k, pos, fr, None, kw)
+            assert q.shape == (2, 40, 0, 16)
+        else:
+            out, _ = qk_norm_rotary(k, None, pos, fr, kw)
+        out.backward(go)
+        res.append((out.detach(), k.grad, pos.grad))
+    for x, y in zip(*res):
+        assert torch.equal(x, y)
