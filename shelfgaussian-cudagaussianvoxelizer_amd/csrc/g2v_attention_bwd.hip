@@ -459,16 +459,17 @@ hipError_t dq_waves(const AttnBwd& a, const AttnShape& g, hipStream_t s) {
     return full ? dq_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
 }
 
-// Keys up to which bfloat16 P and dS go into dV and dK as two planes: with few keys delta takes away most of dP, and rounding
-// what is left to 2^-9 puts dK up to 2.7e-3 off (its own rounding: 1.7e-3; 2.4e-3 with many keys).  A half more products, of
-// problems whose launches take longer; 18000 queries x 300 keys x 8 heads x 64: 65 -> 74 us.
-constexpr int kFewKeys = 1024;
+// Keys, and query rows of a key head, up to which bfloat16 P and dS go into dV and dK as two planes.  With few keys delta takes
+// away most of dP, and rounding what is left to 2^-9 puts dK up to 2.7e-3 off (its own rounding: 1.7e-3; 2.4e-3 with many
+// keys); with few rows it does not average out (30 rows, 3035 keys: 2.5e-3).  A half more products, of problems whose
+// launches and bytes take longer: 18000 queries x 300 keys x 8 heads x 64 65 -> 74 us, 10 queries x 18000 keys 28 -> 33.
+constexpr int kFewKeys = 1024, kFewRows = 64;
 
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
 hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
     const bool full = a.dim > DP - 16;
     if constexpr (NP == 1)
-        if (a.nk <= kFewKeys)
+        if (a.nk <= kFewKeys || a.group * a.nq <= kFewRows)
             return full ? dkv_kernel<NP, 2, DP, DP / 16, NKB, NW, QT, T>(a, s)
                         : dkv_kernel<NP, 2, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
     return full ? dkv_kernel<NP, NP, DP, DP / 16, NKB, NW, QT, T>(a, s) : dkv_kernel<NP, NP, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
