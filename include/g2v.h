@@ -370,10 +370,12 @@ int g2v_qk_norm_rotary_backward(int batch, int n_q, int n_k, int heads_q, int he
  * heads h heads_q / heads_k ... share key head h); dtype G2V_DTYPE_F32 or G2V_DTYPE_BF16 for all; strides in elements
  * along batch, tokens and heads, unit stride along head_dim; out contiguous.  head_dim <= 128, scale > 0.
  * key_mask (batch, n_k) bytes: 0 where a key is not attended to (NULL: none); what such a key's rows hold is never read.
- * A query without any key gives 0.  out_rest (like out, NULL where not wanted, unused for float32) receives what
- * rounding to bfloat16 took from out, for a backward whose row sums of grad_out out are not off by it.  lse (batch, heads_q, n_q) float32, NULL where no backward follows: the base-2
- * logarithm of the sum of 2^(scale log2(e) q.k), +inf for a query without keys.  key_list (batch n_k + batch ints,
- * needed with key_mask) receives the valid keys of every scene and their number, for the backward.
+ * A query without any key gives 0.  float32 values of valid rows have to be finite: they are split into three bfloat16
+ * planes, and an infinity times a plane of zeros is NaN.  out_rest (like out, NULL where not wanted, unused for float32)
+ * receives what rounding to bfloat16 took from out, for a backward whose row sums of grad_out out are not off by it.
+ * lse (batch, heads_q, n_q) float32, NULL where no backward follows: the base-2 logarithm of the sum of
+ * 2^(scale log2(e) q.k), +inf for a query without keys.  key_list (batch n_k + batch ints, needed with key_mask)
+ * receives the valid keys of every scene and their number, for the backward.
  * Sums and softmax statistics are float32; bfloat16 probabilities are rounded to nearest even for their product.
  * in_place: whether every tensor is bfloat16 with head_dim and strides multiples of 8 and 16-byte aligned data (others
  * are packed into the workspace first; pass 0 when unsure).  masked: whether key_mask / key_list will be given (valid

@@ -22,6 +22,10 @@ using namespace attn;
 // (a tenth of the vector instructions; matrix and vector work of a SIMD take their time one after the other).
 constexpr float kFar = 1048576.0f;
 
+// The reference (times c) of a row whose scores were all -inf so far: any other one passes kFar from it
+// (or, where c is so small that the reference itself is at float32's lowest values, is in its reach).
+constexpr float kLowest = -1e37f;
+
 // Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
 // to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
 // the same error on all of them, which their sum dS K does not average out (dQ then 3.2e-3 off instead of 2.2e-3).
@@ -131,7 +135,8 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_f
 #pragma unroll
                         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][b][i]);
                     top = half_max(top);
-                    const float f = m[b] == top ? 1.0f : exp2_fast((m[b] - top) * a.c);
+                    if (top == -INFINITY) top = fmaxf(kLowest / a.c, -3e38f);
+                    const float f = exp2_fast((m[b] - top) * a.c);
                     m[b] = top;
                     l[b] *= f;
 #pragma unroll
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_f
             bool over = false;
 #pragma unroll
             for (int b = 0; b < NQB; ++b) {
-                const float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;
+                const float mc = m[b] * a.c;
                 sum[b] = 0.0f;
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {

@@ -180,6 +180,23 @@ def test_references_far_from_the_maximum(slope, nq, nk, dtype):
     assert rel(leaves[2].grad, want[3]) < tol
 
 
+@pytest.mark.parametrize("D", [32, 64, 100, 128])
+@pytest.mark.parametrize("nq,nk", [(70, 1000), (1, 5000), (300, 700)])
+def test_first_keys_with_scores_of_minus_infinity(nq, nk, D):
+    """bfloat16 keys whose scores are -inf fill the first tiles, and the others' scores are about -200 (2^-288 without a
+    reference): the result is that of the other keys alone."""
+    q, k, v, _ = make(1, nq, nk, 2, 2, D, torch.bfloat16, 21, size=0.3)
+    q[..., 0], q[..., 1] = 1.0, 1.0
+    k[:, :150, :, 0] = -float("inf")
+    k[:, 150:, :, 0] = 0.0
+    k[..., 1] = -200.0
+    mask = (torch.arange(nk) >= 150)[None]
+    from CudaGaussianVoxelizer import gaussian_attention
+    out = gaussian_attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)
+    # scores of 200 carry 200 x 2^-24 into the exponent, far below the rounding of bfloat16 probabilities and outputs
+    assert rel(out, plain(q, k, v, mask, scale=1.0)[0]) < TOL[torch.bfloat16][0]
+
+
 @pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
 @pytest.mark.parametrize("scale", [0.01, 1.0])
 def test_scale(scale, dtype):
