@@ -344,7 +344,8 @@ int g2v_covariance_from_scale_rotation_backward(int n, const float* scales, cons
  *
  * The backward maps the upstream gradients (strided like q and k) to grad_q, grad_k (contiguous, dtype) and, where
  * not NULL, float32 grad_q_weight, grad_k_weight (head_dim) and grad_q_positions, grad_k_positions (with shared
- * positions grad_q_positions holds the sum and grad_k_positions is unused).  Deterministic: fixed summation order. */
+ * positions grad_q_positions holds the sum and grad_k_positions is unused); those of a side without heads are
+ * zeros.  Deterministic: fixed summation order. */
 int g2v_qk_norm_rotary_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int num_axes,
                                int num_pairs, const void* q, const long long q_strides[3], const void* k,
                                const long long k_strides[3], int dtype, const float* q_weight,

@@ -527,7 +527,13 @@ int g2v_qk_norm_rotary_backward(int batch, int n_q, int n_k, int heads_q, int he
     a.dw[1] = grad_k_weight;
     a.dpos[0] = grad_q_positions;
     a.dpos[1] = a.shared ? nullptr : grad_k_positions;
-    G2V_HIP(launch_qk_norm_rotary_bwd(a, dtype, workspace, static_cast<hipStream_t>(stream)));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    G2V_HIP(launch_qk_norm_rotary_bwd(a, dtype, workspace, s));
+    // no workgroup runs over positions that turn no head
+    if (grad_q_positions && heads_q == 0 && (k_positions || heads_k == 0))
+        G2V_HIP(launch_fill_i32((int64_t)batch * n_q * num_axes, 0, reinterpret_cast<int*>(grad_q_positions), s));
+    if (grad_k_positions && heads_k == 0 && k_positions)
+        G2V_HIP(launch_fill_i32((int64_t)batch * n_k * num_axes, 0, reinterpret_cast<int*>(grad_k_positions), s));
     return G2V_OK;
 }
 

@@ -235,3 +235,37 @@ def test_no_query_heads():
         res.append((out.detach(), k.grad, pos.grad))
     for x, y in zip(*res):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("hq,hk,shared", [(0, 2, False), (3, 0, False), (0, 0, False), (0, 0, True)])
+def test_positions_of_a_side_without_heads(hq, hk, shared, dtype):
+    """A side without heads: its positions and weights turn and scale nothing, so their gradients are zeros (and not what their
+    memory held), and the other side's are those of the call without it."""
+    from CudaGaussianVoxelizer import _C, qk_norm_rotary
+    B, nq, nk, D = 2, 700, 700 if shared else 900, 16
+    d, r = make(B, nq, nk, max(hq, 1), max(hk, 1), D, 3, 8, dtype, 11, shared)
+    fr = d["freqs"].cuda()
+    leaf = lambda t: t.cuda().requires_grad_()   # noqa: E731
+    q, k = leaf(d["q"][:, :, :hq]), leaf(d["k"][:, :, :hk])
+    pos, kpos, qw, kw = leaf(d["pos"]), None if shared else leaf(d["kpos"]), leaf(d["qw"]), leaf(d["kw"])
+    go = [r(*t.shape).to(dtype).cuda() for t in (q, k)]
+    out = qk_norm_rotary(q, k, pos, fr, qw, kw, k_positions=kpos)
+    wrt = [q, k, pos, qw, kw] + ([] if shared else [kpos])
+    used = [torch.full_like(t, float("nan")) for t in (pos, pos, qw, kw) + (() if shared else (kpos, kpos))]
+    torch.cuda.synchronize()
+    del used      # whose memory the gradients may get
+    dq, dk, dpos, dqw, dkw, *dkpos = torch.autograd.grad(out, wrt, go)
+    assert dq.shape == q.shape and dk.shape == k.shape
+    if hq == 0:
+        assert torch.count_nonzero(dqw) == 0
+        assert hk > 0 and shared or torch.count_nonzero(dpos) == 0
+    else:
+        want = _C.qk_norm_rotary_backward(go[0], None, q, None, pos, fr, qw)
+        assert torch.equal(dq, want[0]) and torch.equal(dqw, want[2]) and torch.equal(dpos, want[4])
+    if hk == 0:
+        assert torch.count_nonzero(dkw) == 0
+        assert all(torch.count_nonzero(t) == 0 for t in dkpos)
+    else:
+        want = _C.qk_norm_rotary_backward(go[1], None, k, None, kpos, fr, kw)
+        assert torch.equal(dk, want[0]) and torch.equal(dkw, want[2]) and torch.equal(dkpos[0], want[4])
