@@ -5,6 +5,7 @@ reached through ``_C`` on the caller's current stream.
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
@@ -13,8 +14,17 @@ from . import _C
 __all__ = ["qk_norm_rotary", "rotary_frequencies", "gaussian_attention", "PyGaussianAttention"]
 
 
-def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _tangents(*tensors):
+    """Whether one of these carries a forward-mode derivative (which has no requires_grad, and flows under no_grad too).  None
+    does outside of a dual level, which is looked at first: unpacking three tensors takes 3 us of a call's 12."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _differentiated(*tensors):
+    """Whether a derivative in either mode is asked for: the call then goes through its autograd.Function, which has the
+    backward and refuses tangents.  Others save its bookkeeping."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _tangents(*tensors)
 
 
 class _QkNormRotaryFunction(torch.autograd.Function):
@@ -55,14 +65,15 @@ def qk_norm_rotary(q, k, positions, freqs, q_weight=None, k_weight=None, *, k_po
     sum_a positions[..., a] freqs[a, i], what is left of D stays (rotary_frequencies makes the usual table).
     q_weight and k_weight (D,) scale the normed rows.  Returns (q', k') of q's type, contiguous.
 
-    Gradients flow to q, k, the weights and the positions (once: their own gradients are refused); freqs is a constant."""
-    if isinstance(freqs, torch.Tensor) and freqs.requires_grad:
+    Gradients flow to q, k, the weights and the positions (once: their own gradients, and forward-mode derivatives, are
+    refused); freqs is a constant."""
+    if isinstance(freqs, torch.Tensor) and (freqs.requires_grad or _tangents(freqs)):
         raise RuntimeError("freqs is a constant of qk_norm_rotary: it gets no gradient")
     if q_weight is not None and q_weight.dtype == torch.bfloat16:
         q_weight = q_weight.float()
     if k_weight is not None and k_weight.dtype == torch.bfloat16:
         k_weight = k_weight.float()
-    if _needs_grad(q, k, positions, q_weight, k_weight, k_positions):
+    if _differentiated(q, k, positions, q_weight, k_weight, k_positions):
         return _QkNormRotaryFunction.apply(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
     return _C.qk_norm_rotary_forward(q, k, positions, freqs, q_weight, k_weight, k_positions, eps)
 
@@ -111,8 +122,8 @@ def gaussian_attention(q, k, v, key_mask=None, scale=None):
     keys split over the GPU.
 
     Gradients flow to q, k and v; the backward recomputes the probabilities and gives the same bits on every run.  Gradients
-    of gradients are refused."""
-    if _needs_grad(q, k, v):
+    of gradients and forward-mode derivatives are refused."""
+    if _differentiated(q, k, v):
         return _GaussianAttentionFunction.apply(q, k, v, key_mask, scale)
     return _C.attention_forward(q, k, v, key_mask, scale)[0]
 

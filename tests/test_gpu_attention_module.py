@@ -115,3 +115,34 @@ def test_gradients_of_gradients_are_refused():
     (g,) = torch.autograd.grad((q * k).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+def test_forward_mode_is_refused():
+    """A tangent of any differentiable input is refused instead of being dropped, with or without gradients enabled; inside a dual
+    level inputs without tangents give what they give outside."""
+    import torch.autograd.forward_ad as fwad
+    from CudaGaussianVoxelizer import gaussian_attention, qk_norm_rotary, rotary_frequencies
+    q, k, v = (torch.randn(1, 9, 2, 8, device="cuda") for _ in range(3))
+    w = torch.ones(8, device="cuda")
+    attn = dict(q=q, k=k, v=v)
+    norm = dict(q=q, k=k, positions=torch.rand(1, 9, 3, device="cuda"), freqs=rotary_frequencies(8), q_weight=w, k_weight=w,
+                k_positions=torch.rand(1, 9, 3, device="cuda"))
+    layer = PyGaussianAttentionOf8()
+    want = gaussian_attention(**attn), qk_norm_rotary(**norm)[1], layer(q.flatten(2), norm["positions"])
+    with fwad.dual_level():
+        assert torch.equal(gaussian_attention(**attn), want[0]) and torch.equal(qk_norm_rotary(**norm)[1], want[1])
+        for call, args in ((gaussian_attention, attn), (qk_norm_rotary, norm)):
+            for name, t in args.items():
+                for enabled in (True, False):
+                    dual = fwad.make_dual(t, torch.ones_like(t))
+                    with torch.set_grad_enabled(enabled), pytest.raises((RuntimeError, NotImplementedError)):
+                        call(**dict(args, **{name: dual}))
+        x = fwad.make_dual(q.flatten(2), torch.ones_like(q.flatten(2)))
+        with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+            layer(x, norm["positions"])
+    assert torch.equal(layer(q.flatten(2), norm["positions"]), want[2])
+
+
+def PyGaussianAttentionOf8():
+    from CudaGaussianVoxelizer import PyGaussianAttention
+    return PyGaussianAttention(16, 2)
