@@ -135,7 +135,8 @@ class PyGaussianAttention(nn.Module):
         q = rotate(norm(x Wq)),  k = rotate(norm(c Wk)),  v = c Wv,  y = attention(q, k, v) Wo
 
     with c = x (self-attention) or the given context.  num_kv_heads key heads are shared by num_heads / num_kv_heads
-    query heads each.  ``wavelengths`` is the range over which the rotations turn, in the positions' unit (metres)."""
+    query heads each.  ``wavelengths`` is the range over which the rotations turn, in the positions' unit (metres).  A conversion
+    (``layer.bfloat16()``) takes the weights along and leaves the table of angles, ``freqs``, in float32."""
 
     def __init__(self, embed_dim, num_heads, num_kv_heads=None, *, head_dim=None, axes=3, wavelengths=(0.8, 160.0), eps=1e-6,
                  device="cuda", dtype=torch.float32):
@@ -155,6 +156,15 @@ class PyGaussianAttention(nn.Module):
         self.q_weight = nn.Parameter(torch.ones(head_dim, device=device))
         self.k_weight = nn.Parameter(torch.ones(head_dim, device=device))
         self.register_buffer("freqs", rotary_frequencies(head_dim, axes, wavelengths, device), persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        """Moves and conversions of a module's tensors.  The table of angles only moves: at 40 m from the origin one rounded to
+        8 bits would turn by tenths of a radian less or more."""
+        table = self.freqs
+        super()._apply(fn, recurse)
+        if self.freqs.dtype != table.dtype:
+            self.freqs = table.to(self.freqs.device)
+        return self
 
     def forward(self, x, positions, key_mask=None, *, context=None, context_positions=None):
         """x (B, N, embed_dim) at positions (B, N, axes) float32; context (B, M, embed_dim) at context_positions (B, M, axes),

@@ -146,3 +146,25 @@ def test_forward_mode_is_refused():
 def PyGaussianAttentionOf8():
     from CudaGaussianVoxelizer import PyGaussianAttention
     return PyGaussianAttention(16, 2)
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+def test_converted_layer(where):
+    """A layer converted to bfloat16 (and moved) is the one built in bfloat16: outputs and gradients bit for bit."""
+    from CudaGaussianVoxelizer import PyGaussianAttention
+    torch.manual_seed(4)
+    built = PyGaussianAttention(96, 6, 2, wavelengths=(0.8, 40.0), dtype=torch.bfloat16)
+    layer = PyGaussianAttention(96, 6, 2, wavelengths=(0.8, 40.0), device=where)
+    layer.load_state_dict(built.state_dict())
+    layer = layer.bfloat16().cuda()
+    g = torch.Generator().manual_seed(6)
+    x, go = (torch.randn(2, 70, 96, generator=g).bfloat16().cuda() for _ in range(2))
+    pos = (torch.rand(2, 70, 3, generator=g) * 80 - 40).cuda()
+    results = []
+    for m in (built, layer):
+        xi, pi = x.clone().requires_grad_(), pos.clone().requires_grad_()
+        y = m(xi, pi)
+        y.backward(go)
+        results.append([y.detach(), xi.grad, pi.grad, m.to_q.weight.grad, m.q_weight.grad.bfloat16()])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
