@@ -117,7 +117,7 @@ def gaussian_attention(q, k, v, key_mask=None, scale=None):
     multiple of Hkv (consecutive query heads share a key head), D at most 128.  key_mask (B, Nk) bool is False at keys
     that are not attended to (padding of a batch, pruned Gaussians): what their rows hold, NaN included, reaches no result
     and they get zero gradients; a query without any key gives zeros.  float32 values of valid rows have to be finite (an
-    infinity gives NaN, as they are split into three bfloat16 planes).  scale None: D^-1/2.  Returns (B, Nq, Hq, D) of
+    infinity gives NaN, as they are split into three bfloat16 planes), and sums within float32's range (include/g2v.h says which).  scale None: D^-1/2.  Returns (B, Nq, Hq, D) of
     q's type, contiguous.  Any number of queries and keys, zero and one included: a single query that pools a scene has its
     keys split over the GPU.
 

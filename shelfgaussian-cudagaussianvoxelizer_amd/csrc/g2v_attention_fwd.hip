@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnFwd a, int parts) {
 // ---- what both directions prepare -----------------------------------------------------------------------------------
 
 constexpr int kListThreads = 1024;
+constexpr float kMaxBf16 = 0x1.fep127f;
 
 // Valid keys of a scene in ascending order, then the others; their number in count.  One workgroup a scene.
 __global__ void __launch_bounds__(kListThreads) k_attn_list(int nk, const unsigned char* mask, int* list, int* count) {
@@ -379,9 +380,12 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
         float r = (float)x[j / kPer][j % kPer];
 #pragma unroll
         for (int pl = 0; pl < NP; ++pl) {
-            const __bf16 h = (__bf16)r;
-            o[pl][j] = h;
-            r = __builtin_isfinite((float)h) ? r - (float)h : 0.0f;   // an infinity is its first plane alone
+            // a finite value above the largest bfloat16 starts with that (what is left is small); an infinity is its first
+            // plane alone
+            float h = (float)(__bf16)r;
+            if (NP > 1 && pl == 0 && !__builtin_isfinite(h) && __builtin_isfinite(r)) h = copysignf(kMaxBf16, r);
+            o[pl][j] = (__bf16)h;
+            r = __builtin_isfinite(h) ? r - h : 0.0f;
         }
     }
 #pragma unroll

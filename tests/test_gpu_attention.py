@@ -381,3 +381,22 @@ def test_refusals():
 def test_rounds_of_workgroups(nq, nk, H, D, dtype, keep):
     """Tiles that fill the card once and a little: the first ones whole or in two splits, the rest in more."""
     check(*make(1, nq, nk, H, H, D, dtype, nq + nk), None if keep == 1.0 else random_mask(1, nk, keep, nk), dtype)
+
+
+def _largest_keys():
+    """Keys of up to the largest float32 in one channel, where queries are 2^-125: scores of a few units."""
+    top = torch.finfo(torch.float32).max
+    q, k, v, g = make(1, 70, 300, 2, 2, 32, torch.float32, 13)
+    sign = torch.where(torch.arange(300) % 3 == 0, -1.0, 1.0)[None, :, None]
+    k[..., 0] = sign * top * torch.linspace(0.9975, 1.0, 300)[None, :, None]
+    q[..., 0] = 2.0 ** -125
+    return q, k, v, g
+
+
+def test_largest_finite_values():
+    """float32 values beyond the largest bfloat16 (3.39e38) are finite like any other.  Products keep 24 bits as ever: 1e-5."""
+    from CudaGaussianVoxelizer import gaussian_attention
+    q, k, v, _ = _largest_keys()
+    assert rel(gaussian_attention(q.cuda(), k.cuda(), v.cuda()), plain(q, k, v, None)[0]) < 1e-5
+    v[..., 3] = float("inf")      # infinities stay what they are
+    assert not torch.isfinite(gaussian_attention(q.cuda(), k.cuda(), v.cuda())[..., 3]).any()
