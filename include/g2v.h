@@ -373,8 +373,8 @@ int g2v_qk_norm_rotary_backward(int batch, int n_q, int n_k, int heads_q, int he
  * key_mask (batch, n_k) bytes: 0 where a key is not attended to (NULL: none); what such a key's rows hold is never read.
  * A query without any key gives 0.  float32 values of valid rows have to be finite: they are split into three bfloat16
  * planes, and an infinity times a plane of zeros is NaN.  Sums are float32 in either type: scores times log2(e), the sum
- * of v times probabilities of up to 2^20 before it is divided by theirs, and gradients of q and k before they are
- * multiplied by scale have to stay in its range.  out_rest (like out, NULL where not wanted, unused for float32)
+ * of v times probabilities of up to 2^20 before it is divided by theirs, and dK before it is multiplied by scale have to
+ * stay in its range.  out_rest (like out, NULL where not wanted, unused for float32)
  * receives what rounding to bfloat16 took from out, for a backward whose row sums of grad_out out are not off by it.
  * lse (batch, heads_q, n_q) float32, NULL where no backward follows: the base-2 logarithm of the sum of
  * 2^(scale log2(e) q.k), +inf for a query without keys.  key_list (batch n_k + batch ints, needed with key_mask)

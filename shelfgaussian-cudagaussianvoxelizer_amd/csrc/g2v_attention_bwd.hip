@@ -17,7 +17,8 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-// dQ: rows in the lanes as in the forward, S^T = K Q^T and dP^T = V dO^T, dQ^T += K^T dS^T.
+// dQ: rows in the lanes as in the forward, S^T = K Q^T and dP^T = V dO^T, dQ^T += K^T (scale dS)^T.  (Scaled before the sum
+// over the keys, which then overflows only where dQ does; the factor turns an addition into a fused one and takes no time.)
 // KS: see k_attn_fwd.
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_dq(AttnBwd a) {
@@ -40,7 +41,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
     if (n < 2) t1 = t0;    // one key: its probability is 1 whatever q is
 
     bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
-    float lse[NQB], delta[NQB];    // delta: negative, as it is stored
+    float lse[NQB], delta[NQB];    // delta: negative, as it is stored, and times scale
 #pragma unroll
     for (int b = 0; b < NQB; ++b) {
         const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
@@ -56,7 +57,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
             }
         const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
         lse[b] = a.lse[at];
-        delta[b] = a.delta[at];
+        delta[b] = a.delta[at] * a.scale;
     }
 
     TileT tile;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
             for (int b = 0; b < NQB; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    s[b][i] = exp2_fast(fmaf(s[b][i], a.c, -lse[b])) * (dp[b][i] + delta[b]);
+                    s[b][i] = exp2_fast(fmaf(s[b][i], a.c, -lse[b])) * fmaf(dp[b][i], a.scale, delta[b]);   // scale dS
             if ((t + 1) * KT > n) {   // the last tile's rows past the end
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -157,8 +158,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                store4<T>(row, 32 * d + reg_row(i), a.dim, dq[d][b][i] * a.scale, dq[d][b][i + 1] * a.scale,
-                          dq[d][b][i + 2] * a.scale, dq[d][b][i + 3] * a.scale);
+                store4<T>(row, 32 * d + reg_row(i), a.dim, dq[d][b][i], dq[d][b][i + 1], dq[d][b][i + 2], dq[d][b][i + 3]);
     }
 }
 
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a, int parts) {
     if (!live || threadIdx.x % parts) return;
     const int b = bh / a.hk, tok = r / a.group, head = (bh % a.hk) * a.group + r % a.group;
     T* row = static_cast<T*>(a.dq) + (((int64_t)b * a.nq + tok) * a.hq + head) * a.dim;
-    store4<T>(row, d, a.dim, o[0] * a.scale, o[1] * a.scale, o[2] * a.scale, o[3] * a.scale);
+    store4<T>(row, d, a.dim, o[0], o[1], o[2], o[3]);
 }
 
 template <int DP, typename T>

@@ -400,3 +400,13 @@ def test_largest_finite_values():
     assert rel(gaussian_attention(q.cuda(), k.cuda(), v.cuda()), plain(q, k, v, None)[0]) < 1e-5
     v[..., 3] = float("inf")      # infinities stay what they are
     assert not torch.isfinite(gaussian_attention(q.cuda(), k.cuda(), v.cuda())[..., 3]).any()
+
+
+def test_gradients_of_largest_finite_values():
+    """dQ is a sum over the keys times scale: it is finite wherever that product is, also where the sum alone would not be."""
+    from CudaGaussianVoxelizer import gaussian_attention
+    q, k, v, g = _largest_keys()
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    gaussian_attention(*leaves).backward(g.cuda())
+    for t, w in zip(leaves, plain(q, k, v, None, g)[1:]):
+        assert torch.isfinite(t.grad).all() and rel(t.grad, w) < 1e-5
