@@ -54,15 +54,15 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 }
 __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 ::"v"(voff), "s"(uniform(sbase)), "s"(g2v::uniform((int)lds)) : "memory");
+                 ::"v"(voff), "s"(uniform(sbase)), "s"(g2v::uniform((int)lds)) : "memory", "m0");
 }
 __device__ __forceinline__ void dma16(const void* addr, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                 ::"v"(addr), "s"(g2v::uniform((int)lds)) : "memory");
+                 ::"v"(addr), "s"(g2v::uniform((int)lds)) : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
-                 ::"v"(voff), "s"(uniform(sbase)), "s"(g2v::uniform((int)lds)) : "memory");
+                 ::"v"(voff), "s"(uniform(sbase)), "s"(g2v::uniform((int)lds)) : "memory", "m0");
 }
 
 // At most N loads of this wave outstanding (loads end in order) and its LDS operations done, then the other waves met.
