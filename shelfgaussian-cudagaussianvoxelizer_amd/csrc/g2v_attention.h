@@ -341,6 +341,7 @@ struct AttnBwd {
     const int* list;     // (batch, nk) the keys that the rows of k and v are, valid ones first; null: in order
     int nq, nk, hq, hk, group, dim, bhs;
     attn::Parts parts;
+    bool by_count;       // set by launch_attn_dkv
     int nqp;             // nq rounded up to 64: rows of lse and delta, padded with +inf and 0
     float c, scale;
     const float *lse, *delta;   // (batch, hq, nqp); -delta

@@ -162,9 +162,17 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
     }
 }
 
+// Valid keys, and query rows of a key head, up to which bfloat16 P and dS go into dV and dK as two planes.  With few keys delta
+// takes away most of dP, and rounding what is left to 2^-9 puts dK up to 2.7e-3 off (its own rounding: 1.7e-3; 2.4e-3 with many
+// keys); with few rows it does not average out (30 rows, 3035 keys: 2.5e-3).  A half more products, of problems whose
+// launches and bytes take longer: 18000 queries x 300 keys x 8 heads x 64 65 -> 74 us, 10 queries x 18000 keys 28 -> 33.
+constexpr int kFewKeys = 1024, kFewRows = 64;
+
 // dK and dV: keys in the lanes (a wave owns NKB blocks of 32), S = Q K^T and dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  The queries of each query head that shares the key head pass by, head after head.
-// NS: planes of P and dS in their products.
+// NS: planes of P and dS in their products.  Where the mask decides on them (a.by_count: how many keys of a scene are valid is
+// known here only) both kernels are launched, and a scene's workgroups of the one that it does not belong to end at once (the
+// second launch: 4 us of 9000 x 12 x 64's step of 1210; 6 scenes with 300 valid keys of 3000, 8 x 64: 228 -> 239).
 template <int NP, int NS, int DP, int KS, int NKB, int NW, int QT, typename T>
 __global__ void __launch_bounds__(NW * 64, NS > NP ? (DP <= 96 ? 2 : 1) : NP == 1 && DP == 64 ? 3 : NP == 1 || DP <= 32 ? 2 : 1)
     k_attn_dkv(AttnBwd a) {
@@ -178,6 +186,7 @@ __global__ void __launch_bounds__(NW * 64, NS > NP ? (DP <= 96 ? 2 : 1) : NP == 
     const int wave = g2v::uniform(threadIdx.x >> 6);
     const int j0 = (w.tile * NW + wave) * (NKB * 32) + (threadIdx.x & 31);
     const int n = a.count ? a.count[w.b] : a.nk;
+    if (NP == 1 && a.by_count && (n <= kFewKeys) != (NS > NP)) return;
     const int per = (a.nq + QT - 1) / QT;     // tiles of a query head
     int u0, u1;
     split_range(per * a.group, w.split, w.splits, u0, u1);
@@ -439,15 +448,11 @@ hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
     }
     return hipGetLastError();
 }
-template <int NP, int NS, int DP, int KS, int NKB, int NW, int QT, typename T>
-hipError_t dkv_kernel(const AttnBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_dkv<NP, NS, DP, KS, NKB, NW, QT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
-    const int64_t rows = (int64_t)a.bhs * (a.nk - joined_from(a.parts, a.nk));
-    if (rows > 0) {
-        const int parts = attn_join_parts(rows, DP / 2, std::max(a.parts.head_splits, a.parts.splits));
-        G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 2 * parts))), dim3(256), 0, s, a, parts);
-    }
-    return hipGetLastError();
+template <int NP, int NS, int DP, int NKB, int NW, int QT, typename T>
+void dkv_kernel(const AttnBwd& a, hipStream_t s) {
+    const dim3 grid((unsigned)workgroups(a.parts, a.bhs)), block(NW * 64);
+    if (a.dim > DP - 16) G2V_LAUNCH((k_attn_dkv<NP, NS, DP, DP / 16, NKB, NW, QT, T>), grid, block, 0, s, a);
+    else G2V_LAUNCH((k_attn_dkv<NP, NS, DP, DP / 16 - 1, NKB, NW, QT, T>), grid, block, 0, s, a);
 }
 
 template <int NP, int DP, int NQB, int KT, typename T>
@@ -459,20 +464,19 @@ hipError_t dq_waves(const AttnBwd& a, const AttnShape& g, hipStream_t s) {
     return full ? dq_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
 }
 
-// Keys, and query rows of a key head, up to which bfloat16 P and dS go into dV and dK as two planes.  With few keys delta takes
-// away most of dP, and rounding what is left to 2^-9 puts dK up to 2.7e-3 off (its own rounding: 1.7e-3; 2.4e-3 with many
-// keys); with few rows it does not average out (30 rows, 3035 keys: 2.5e-3).  A half more products, of problems whose
-// launches and bytes take longer: 18000 queries x 300 keys x 8 heads x 64 65 -> 74 us, 10 queries x 18000 keys 28 -> 33.
-constexpr int kFewKeys = 1024, kFewRows = 64;
-
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
-hipError_t dkv_launch(const AttnBwd& a, hipStream_t s) {
-    const bool full = a.dim > DP - 16;
+hipError_t dkv_launch(AttnBwd& a, hipStream_t s) {
+    const bool few = a.nk <= kFewKeys || (int64_t)a.group * a.nq <= kFewRows;
+    a.by_count = NP == 1 && a.count && !few;
     if constexpr (NP == 1)
-        if (a.nk <= kFewKeys || a.group * a.nq <= kFewRows)
-            return full ? dkv_kernel<NP, 2, DP, DP / 16, NKB, NW, QT, T>(a, s)
-                        : dkv_kernel<NP, 2, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
-    return full ? dkv_kernel<NP, NP, DP, DP / 16, NKB, NW, QT, T>(a, s) : dkv_kernel<NP, NP, DP, DP / 16 - 1, NKB, NW, QT, T>(a, s);
+        if (few || a.by_count) dkv_kernel<NP, 2, DP, NKB, NW, QT, T>(a, s);
+    if (NP > 1 || !few) dkv_kernel<NP, NP, DP, NKB, NW, QT, T>(a, s);
+    const int64_t rows = (int64_t)a.bhs * (a.nk - joined_from(a.parts, a.nk));
+    if (rows > 0) {
+        const int parts = attn_join_parts(rows, DP / 2, std::max(a.parts.head_splits, a.parts.splits));
+        G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 2 * parts))), dim3(256), 0, s, a, parts);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -512,7 +516,8 @@ hipError_t launch_attn_dq(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
     }
 }
 
-hipError_t launch_attn_dkv(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
+hipError_t launch_attn_dkv(const AttnBwd& args, bool f32, int dp, hipStream_t s) {
+    AttnBwd a = args;
     if (f32) {
         switch (dp) {
             case 32: return dkv_launch<3, 32, 1, 4, 64, float>(a, s);

@@ -410,3 +410,32 @@ def test_gradients_of_largest_finite_values():
     gaussian_attention(*leaves).backward(g.cuda())
     for t, w in zip(leaves, plain(q, k, v, None, g)[1:]):
         assert torch.isfinite(t.grad).all() and rel(t.grad, w) < 1e-5
+
+
+@pytest.mark.parametrize("D", [24, 32, 64, 72, 96, 128])
+def test_padding_does_not_cost_accuracy(D):
+    """Scenes of few valid keys in a batch that is padded to many: dK and dV of each scene are as near to 64 bits as those of its
+    valid keys alone.  The number of planes of P and dS is the same in both then, and with it every rounding but those of float32
+    sums (2^-24 each) and of the bfloat16 outputs, which are as large in both: the two errors agree within a few percent, where one
+    plane instead of two adds a quarter or more.  (dQ takes two planes always.)"""
+    from CudaGaussianVoxelizer import _C
+    nk, counts = 3663, [440, 2, 1024, 1025, 3663, 90, 0]
+    q, k, v, g = (t.cuda() for t in make(len(counts), 150, nk, 4, 2, D, torch.bfloat16, D))
+    # keys of a scene share a direction (the mean of the scores' gradients is what delta takes away)
+    k = (k + torch.randn(len(counts), 1, 2, D, generator=torch.Generator().manual_seed(1)).cuda()).bfloat16()
+    order = torch.rand(len(counts), nk, generator=torch.Generator().manual_seed(2)).argsort(1).argsort(1)
+    mask = order < torch.tensor(counts)[:, None]
+    out, rest, lse, lst = _C.attention_forward(q, k, v, mask.cuda(), for_backward=True)
+    grads = _C.attention_backward(g, q, k, v, out, rest, lse, lst)
+    for b, n in enumerate(counts):
+        at, keys = slice(b, b + 1), mask[b].nonzero()[:, 0].cuda()
+        assert torch.count_nonzero(grads[1][b][~mask[b].cuda()]) == 0 and torch.count_nonzero(grads[2][b][~mask[b].cuda()]) == 0
+        if n < 2:
+            continue
+        alone = q[at], k[at, keys].contiguous(), v[at, keys].contiguous()
+        o, r, l, _ = _C.attention_forward(*alone, for_backward=True)
+        lone = _C.attention_backward(g[at], *alone, o, r, l)
+        want = plain(*alone, None, g[at])[1:]
+        errs = [(rel(x[at, keys], w), rel(y, w)) for x, y, w in zip(grads[1:], lone[1:], want[1:])]
+        say(D, n, " ".join(f"{e:.2e}/{f:.2e}" for e, f in errs))
+        assert all(e <= 1.05 * f for e, f in errs), (n, errs)
