@@ -71,13 +71,30 @@ __device__ __forceinline__ void tile_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// Workgroups of a kernel that share a CU: its launch bound (so that its registers fit), checked against its LDS, and what the
+// splits of the long axis are planned by.  np, ns: planes of the inputs and of P and dS; waves: of a workgroup.  (Of one-wave
+// workgroups at 32 channels six would fit, but the splits that fill so many places take the join longer: one query over 18000
+// keys x 16 heads x 32 26.3 -> 27.3 us.  At one wave a SIMD four fit whatever their registers; their bound stays at two, with
+// which the compiler keeps more of them out of the accumulation file: at 32 channels 4 queries x 9000 keys 20.3 -> 19.5 us.)
+constexpr int kLdsBytes = 160 * 1024;
+constexpr int launch_bound(int waves, int per_cu) { return waves == 1 ? 2 : per_cu; }
+constexpr int fwd_per_cu(int np, int dp, int waves) {
+    return np > 1 ? (dp > 64 ? 1 : 2) : waves == 1 || dp == 32 || dp == 96 ? 3 : 2;
+}
+constexpr int dq_per_cu(int np, int dp, int waves) {
+    return np > 1 ? (dp > 64 ? 1 : 2) : waves == 1 && dp <= 64 ? 3 : 2;
+}
+constexpr int dkv_per_cu(int np, int ns, int dp) {
+    return np > 1 ? (dp > 32 ? 1 : 2) : dp == 32 ? 4 : dp == 64 && ns == 1 ? 3 : dp == 128 && ns > 1 ? 1 : 2;
+}
+
 // Buffers of a kernel's tiles (pairs of `bytes`): three, loaded two tiles ahead, where the `groups` workgroups that the
 // kernel's registers allow a CU fit its 160 KB so, else two, loaded one ahead.  Three for two: 9000 x 12 heads x 64 float32
 // forward 1.33 -> 1.25 ms; bfloat16 at 96 channels dK and dV 0.395 -> 0.367 ms, but the forward there, whose
 // workgroups come three to a CU with two buffers, 0.22 -> 0.25 ms.  The barrier before tile t lets tile t + 1's loads go
 // on, if there are three buffers and that tile is whole: kLoads of them a wave (`counted`; in the last tile a wave's lanes
 // may be off altogether).  It also ends every wave's reads of tile t - 1, whose buffer is loaded next.
-constexpr int buffers(int groups, int bytes) { return 3 * 2 * bytes <= 160 * 1024 / groups ? 3 : 2; }
+constexpr int buffers(int groups, int bytes) { return 3 * 2 * bytes <= kLdsBytes / groups ? 3 : 2; }
 template <int kBuffers, int kLoads>
 __device__ __forceinline__ void next_tile(bool counted) {
     if (kBuffers == 3 && kLoads > 0 && counted) tile_barrier<kLoads>();

@@ -21,7 +21,7 @@ using namespace attn;
 // over the keys, which then overflows only where dQ does; the factor turns an addition into a fused one and takes no time.)
 // KS: see k_attn_fwd.
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_dq(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, launch_bound(NW, dq_per_cu(NP, DP, NW))) k_attn_dq(AttnBwd a) {
     // planes of dS in its product with K: two of bfloat16 for bfloat16 inputs.  The keys that a query attends to share
     // a direction, their dS sum to zero, and what is left of dQ is small beside the terms: rounding dS to 2^-9
     // alone puts dQ 3.0e-3 off (its own rounding: 1.7e-3), a second plane leaves 2.0e-3 for a third more products here
@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_d
     typedef Tile<NP, DP, KT, NT> TileT;
     constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
+    static_assert(dq_per_cu(NP, DP, NW) * sizeof(lds) <= kLdsBytes, "planned by more workgroups than fit");
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int rows = a.group * a.nq;
     const int r0 = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32) + (threadIdx.x & 31);
@@ -174,14 +175,14 @@ constexpr int kFewKeys = 1024, kFewRows = 64;
 // known here only) both kernels are launched, and a scene's workgroups of the one that it does not belong to end at once (the
 // second launch: 4 us of 9000 x 12 x 64's step of 1210; 6 scenes with 300 valid keys of 3000, 8 x 64: 228 -> 239).
 template <int NP, int NS, int DP, int KS, int NKB, int NW, int QT, typename T>
-__global__ void __launch_bounds__(NW * 64, NS > NP ? (DP <= 96 ? 2 : 1) : NP == 1 && DP == 64 ? 3 : NP == 1 || DP <= 32 ? 2 : 1)
-    k_attn_dkv(AttnBwd a) {
+__global__ void __launch_bounds__(NW * 64, dkv_per_cu(NP, NS, DP)) k_attn_dkv(AttnBwd a) {
     static_assert(NW % 2 == 0, "waves in pairs load the statistics");
     constexpr int NT = NW * 64, QB = QT / 32, DB = DP / 32;
     typedef Tile<NP, DP, QT, NT> TileT;
     constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and -delta of the tile's rows
+    static_assert(dkv_per_cu(NP, NS, DP) * (sizeof(lds) + sizeof(stat)) <= kLdsBytes, "planned by more workgroups than fit");
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int wave = g2v::uniform(threadIdx.x >> 6);
     const int j0 = (w.tile * NW + wave) * (NKB * 32) + (threadIdx.x & 31);
@@ -466,11 +467,11 @@ hipError_t dq_waves(const AttnBwd& a, const AttnShape& g, hipStream_t s) {
 
 template <int NP, int DP, int NKB, int NW, int QT, typename T>
 hipError_t dkv_launch(AttnBwd& a, hipStream_t s) {
-    const bool few = a.nk <= kFewKeys || (int64_t)a.group * a.nq <= kFewRows;
-    a.by_count = NP == 1 && a.count && !few;
+    const int planes = attn_dkv_planes(NP > 1, a.nk, (int64_t)a.group * a.nq);
+    a.by_count = planes == 1 && a.count;
     if constexpr (NP == 1)
-        if (few || a.by_count) dkv_kernel<NP, 2, DP, NKB, NW, QT, T>(a, s);
-    if (NP > 1 || !few) dkv_kernel<NP, NP, DP, NKB, NW, QT, T>(a, s);
+        if (planes == 2 || a.by_count) dkv_kernel<NP, 2, DP, NKB, NW, QT, T>(a, s);
+    if (planes == NP) dkv_kernel<NP, NP, DP, NKB, NW, QT, T>(a, s);
     const int64_t rows = (int64_t)a.bhs * (a.nk - joined_from(a.parts, a.nk));
     if (rows > 0) {
         const int parts = attn_join_parts(rows, DP / 2, std::max(a.parts.head_splits, a.parts.splits));
@@ -486,15 +487,20 @@ AttnShape attn_dq_shape(bool f32, int dp, int64_t rows) {
     g.waves = !f32 && rows <= 32 ? 1 : 4;    // as in attn_fwd_shape
     g.blocks = g.waves == 4 && !f32 && dp <= 64 ? 2 : 1;
     g.tile = f32 && dp > 32 ? 32 : 64;
-    g.per_cu = g.waves == 1 ? 4 : f32 && dp > 64 ? 1 : 2;
+    g.per_cu = dq_per_cu(f32 ? 3 : 1, dp, g.waves);
+    g.products = f32 ? 3 : 4;    // bfloat16: dS as two planes
     return g;
 }
-AttnShape attn_dkv_shape(bool f32, int dp) {
+int attn_dkv_planes(bool f32, int64_t nk, int64_t rows) {
+    return f32 ? 3 : nk <= kFewKeys || rows <= kFewRows ? 2 : 1;
+}
+AttnShape attn_dkv_shape(bool f32, int dp, int planes) {
     AttnShape g;
     g.waves = 4;
     g.blocks = 1;
     g.tile = (f32 && dp > 32) || dp > 96 ? 32 : 64;
-    g.per_cu = f32 ? (dp > 32 ? 1 : 2) : dp == 32 ? 4 : dp == 64 ? 3 : 2;
+    g.per_cu = dkv_per_cu(f32 ? 3 : 1, planes, dp);
+    g.products = f32 ? 4 : 2 + 2 * planes;
     return g;
 }
 

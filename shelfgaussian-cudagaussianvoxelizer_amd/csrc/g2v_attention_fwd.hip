@@ -40,11 +40,12 @@ __device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, f
 
 // KS: steps of 16 that the head's width takes in the scores' product (the last of DP / 16 may hold nothing but padding).
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
-__global__ void __launch_bounds__(NW * 64, NP == 1 || DP <= 64 ? 2 : 1) k_attn_fwd(AttnFwd a) {
+__global__ void __launch_bounds__(NW * 64, launch_bound(NW, fwd_per_cu(NP, DP, NW))) k_attn_fwd(AttnFwd a) {
     constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
     typedef Tile<NP, DP, KT, NT> TileT;
     constexpr int kBuffers = buffers(NP == 1 && NQB == 1 ? 3 : 2, TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
+    static_assert(fwd_per_cu(NP, DP, NW) * sizeof(lds) <= kLdsBytes, "planned by more workgroups than fit");
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int lane = threadIdx.x & 63, rows = a.group * a.nq;
     const int r0 = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32) + (lane & 31);
@@ -423,7 +424,8 @@ AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows) {
     g.waves = !f32 && rows <= 32 ? 1 : 4;
     g.blocks = g.waves == 4 && !f32 && dp != 96 ? 2 : 1;
     g.tile = (f32 && dp > 32) || dp > 96 ? 32 : 64;
-    g.per_cu = f32 ? (dp > 64 ? 1 : 2) : g.waves == 1 || dp == 32 || dp == 96 ? 3 : 2;
+    g.per_cu = fwd_per_cu(f32 ? 3 : 1, dp, g.waves);
+    g.products = 2;
     return g;
 }
 

@@ -146,13 +146,13 @@ struct AttnRun {
     attn::Parts parts;
     int64_t part_rows;
 };
-AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing, int streams, int products, int width, bool even) {
+AttnRun attn_run(const AttnSizes& z, AttnShape g, int64_t mine, int64_t passing, int streams, int width, bool even) {
     attn::Parts r = {};
     const int own = g.waves * g.blocks * 32, slots = kCus * g.per_cu;
     r.tiles = (int)ceil_div(mine, own);
     r.head_splits = 1;
     const int units = (int)std::min<int64_t>(ceil_div(passing, g.tile) * streams, 1 << 30);
-    const double flops = 2.0 * products * own * g.tile * z.dp;
+    const double flops = 2.0 * g.products * own * g.tile * z.dp;
     const double unit_us = std::max(1.0, flops * g.per_cu / ((z.f32 ? 0.15e9 : 1.0e9) / kCus));
     const double join_us = 8.0 * mine * z.bhs * width / 3e6;
     const int64_t all = (int64_t)z.bhs * r.tiles;
@@ -254,13 +254,14 @@ hipError_t attn_sources(const AttnSizes& z, const Strided* t, int count, bool pa
 }
 
 AttnRun attn_fwd_run(const AttnSizes& z) {
-    return attn_run(z, attn_fwd_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 2, z.dp, false);
+    return attn_run(z, attn_fwd_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, z.dp, false);
 }
 AttnRun attn_dq_run(const AttnSizes& z) {
-    return attn_run(z, attn_dq_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, 3, z.dp, false);
+    return attn_run(z, attn_dq_shape(z.f32, z.dp, z.rows()), z.rows(), z.nk, 1, z.dp, false);
 }
 AttnRun attn_dkv_run(const AttnSizes& z, bool masked) {
-    return attn_run(z, attn_dkv_shape(z.f32, z.dp), z.nk, z.nq, z.group, 4, 2 * z.dp, masked);
+    const AttnShape g = attn_dkv_shape(z.f32, z.dp, attn_dkv_planes(z.f32, z.nk, z.rows()));
+    return attn_run(z, g, z.nk, z.nq, z.group, 2 * z.dp, masked);
 }
 
 struct AttnFwdWs {

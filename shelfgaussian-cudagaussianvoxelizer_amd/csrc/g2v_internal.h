@@ -287,9 +287,10 @@ struct AttnPack {
     int list_tensor;
     int64_t blocks[4];   // set by the launch
 };
-// A kernel's workgroup: waves, blocks of 32 rows of a wave, rows of a tile of the long axis, workgroups that fit a CU.
+// A kernel's workgroup: waves, blocks of 32 rows of a wave, rows of a tile of the long axis, workgroups that fit a CU; and
+// the products of the scores' size that the kernel takes (float32's six terms count as one).
 struct AttnShape {
-    int waves, blocks, tile, per_cu;
+    int waves, blocks, tile, per_cu, products;
 };
 // Threads that share a row's splits in a join of `lanes` lanes a row: more while the rows leave the card empty.
 inline int attn_join_parts(int64_t rows, int lanes, int splits) {
@@ -300,7 +301,8 @@ inline int attn_join_parts(int64_t rows, int lanes, int splits) {
 inline int attn_dp(int dim) { return (dim + 31) / 32 * 32; }
 AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows);
 AttnShape attn_dq_shape(bool f32, int dp, int64_t rows);
-AttnShape attn_dkv_shape(bool f32, int dp);
+int attn_dkv_planes(bool f32, int64_t nk, int64_t rows);    // of P and dS; rows: of queries of a key head
+AttnShape attn_dkv_shape(bool f32, int dp, int planes);
 hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_attn_list(int batch, int nk, const unsigned char* mask, int* list, int* count, hipStream_t s);
 hipError_t launch_attn_pack(const AttnPack& a, bool f32, hipStream_t s);
