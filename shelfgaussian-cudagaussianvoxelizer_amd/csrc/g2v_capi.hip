@@ -16,14 +16,6 @@ namespace {
 
 thread_local char g_err[512] = "";
 
-int fail(int code, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
 }  // namespace
 
 namespace g2v {
@@ -38,6 +30,8 @@ int api_fail(int code, const char* fmt, ...) {
 }  // namespace g2v
 
 namespace {
+
+int (*const fail)(int, const char*, ...) = api_fail;
 
 int hip_fail(hipError_t e, const char* where) {
     return fail(G2V_ERR_HIP, "%s: %s", where, hipGetErrorString(e));
