@@ -439,3 +439,73 @@ def test_padding_does_not_cost_accuracy(D):
         errs = [(rel(x[at, keys], w), rel(y, w)) for x, y, w in zip(grads[1:], lone[1:], want[1:])]
         say(D, n, " ".join(f"{e:.2e}/{f:.2e}" for e, f in errs))
         assert all(e <= 1.05 * f for e, f in errs), (n, errs)
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("nq", [11, 130])
+@pytest.mark.parametrize("nk", [2048, 2049, 5000])
+def test_masks_of_many_keys(nk, nq, dtype):
+    """Masks on both sides of the number of keys up to which packing makes their list: an empty scene, a single key, a valid prefix
+    (padding), a valid suffix, a random share, few keys, all; rows of NaN where nothing is attended to."""
+    B = 7
+    q, k, v, g = make(B, nq, nk, 4, 2, 64, dtype, nk + nq)
+    at = torch.arange(nk)
+    mask = torch.stack([torch.zeros(nk, dtype=torch.bool), at == nk - 1, at < 1300, at >= nk - 700, random_mask(1, nk, 0.8, 1)[0],
+                        random_mask(1, nk, 0.02, 2)[0], torch.ones(nk, dtype=torch.bool)])
+    check(q, k, v, g, mask, dtype)
+    from CudaGaussianVoxelizer import gaussian_attention
+    results = []
+    for bad in (0.0, float("nan")):
+        kb, vb = (torch.where(mask[:, :, None, None], t, torch.full_like(t, bad)) for t in (k, v))
+        leaves = [t.cuda().requires_grad_() for t in (q, kb, vb)]
+        out = gaussian_attention(*leaves, key_mask=mask.cuda())
+        out.backward(g.cuda())
+        results.append([out.detach()] + [t.grad for t in leaves])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("nq,nk", [(10, 1500), (200, 300), (200, 1500)])
+def test_backward_without_the_rounding_lost(nq, nk):
+    """A bfloat16 backward whose caller did not keep what rounding took from the output: delta is off by that rounding, within the
+    bound of gradients."""
+    from CudaGaussianVoxelizer import _C
+    q, k, v, g = make(1, nq, nk, 4, 2, 64, torch.bfloat16, nk)
+    dev = [t.cuda() for t in (q, k, v)]
+    out, rest, lse, _ = _C.attention_forward(*dev, for_backward=True)
+    assert rest is not None
+    got = _C.attention_backward(g.cuda(), *dev, out, None, lse)
+    for x, y in zip(got, plain(q, k, v, None, g)[1:]):
+        assert rel(x, y) < TOL[torch.bfloat16][1]
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk", [(70, 1000), (1, 5000), (300, 700)])
+@pytest.mark.parametrize("slope", [0.5, -0.5])
+def test_gradients_far_from_the_maximum(slope, nq, nk, dtype):
+    """dQ and dK where scores climb over the whole row.  Their terms cancel (keys lie far from 0, and one or a few of them have all
+    the probability), so errors are measured against the sums of the terms' magnitudes: a float32 score of 2500 carries at
+    most 2500 x 2^-24 x log2(e) into the exponent, 2.1e-4 of a probability, bfloat16 rounds outputs to 2^-9 (and P and dS, or their
+    second planes).  A term takes P twice (its own and delta's): 1e-3 and 8e-3."""
+    d = 64
+    step = torch.arange(nk) // 64 * 64 if dtype == torch.bfloat16 else torch.arange(nk)
+    q, k = torch.zeros(1, nq, 1, d), torch.zeros(1, nk, 1, d)
+    q[..., 0] = slope
+    q[..., 1] = 1.0
+    k[..., 0] = step[None, :, None]
+    k[..., 1] = (torch.arange(nk) % 64 * abs(slope) / 16)[None, :, None]
+    gen = torch.Generator().manual_seed(1)
+    v, go = torch.randn(1, nk, 1, d, generator=gen), torch.randn(1, nq, 1, d, generator=gen)
+    q, k, v, go = (t.to(dtype) for t in (q, k, v, go))
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    from CudaGaussianVoxelizer import gaussian_attention
+    gaussian_attention(*leaves, scale=1.0).backward(go.cuda())
+    _, dq, dk, _ = plain(q, k, v, None, go, 1.0)
+    Q, K, V, G = (t[0, :, 0].double() for t in (q, k, v, go))
+    p, dp = torch.softmax(Q @ K.T, -1), G @ V.T
+    size = p * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True))
+    tol = 1e-3 if dtype == torch.float32 else 8e-3
+    for got, want, most in ((leaves[0].grad, dq, size @ K.abs()), (leaves[1].grad, dk, size.T @ Q.abs())):
+        err = float((got.double().cpu()[0, :, 0] - want[0, :, 0]).norm() / most.norm())
+        say(f"{err:.1e}")
+        assert err < tol

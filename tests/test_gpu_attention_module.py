@@ -168,3 +168,29 @@ def test_converted_layer(where):
         results.append([y.detach(), xi.grad, pi.grad, m.to_q.weight.grad, m.q_weight.grad.bfloat16()])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_bfloat16_layer(masked):
+    """The bfloat16 layer against 64 bits.  On its way an output is rounded eight times (q, k, v, the two normed and turned, the
+    probabilities, the attention's output, the last projection), by at most 2^-9 each, 2e-3 added up linearly: below 1.6e-2; a
+    gradient passes as many roundings again on its way back: below 3.2e-2."""
+    from CudaGaussianVoxelizer import PyGaussianAttention
+    torch.manual_seed(8)
+    layer = PyGaussianAttention(96, 6, 2, wavelengths=(0.8, 40.0), dtype=torch.bfloat16)
+    B, N = 2, 130
+    g = torch.Generator().manual_seed(9)
+    x, go = (torch.randn(B, N, 96, generator=g).bfloat16() for _ in range(2))
+    pos = torch.rand(B, N, 3, generator=g) * 20 - 10
+    mask = torch.rand(B, N, generator=g) < 0.7 if masked else None
+    xd, pd = x.cuda().requires_grad_(), pos.cuda().requires_grad_()
+    y = layer(xd, pd, None if mask is None else mask.cuda())
+    y.backward(go.cuda())
+    xr, pr = x.double().requires_grad_(), pos.double().requires_grad_()
+    p = {n: t.detach().double().cpu().requires_grad_() for n, t in layer.named_parameters()}
+    want = plain_layer(layer, p, xr, pr, mask, None, None)
+    want.backward(go.double())
+    assert y.dtype == torch.bfloat16 and rel(y, want) < 1.6e-2
+    assert rel(xd.grad, xr.grad) < 3.2e-2 and rel(pd.grad, pr.grad) < 3.2e-2
+    for n, t in layer.named_parameters():
+        assert rel(t.grad, p[n].grad) < 3.2e-2, n
