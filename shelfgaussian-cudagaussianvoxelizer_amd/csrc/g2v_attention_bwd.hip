@@ -6,11 +6,13 @@
 // The probabilities are recomputed, twice: once by workgroups that own keys (dK, dV; the queries pass by) and once by
 // workgroups that own queries (dQ; the keys pass by).  That is seven products of the scores' size instead of five, and
 // nothing is added to memory that another workgroup adds to: gradients are the same on every run, and shared key heads are
-// summed over their query heads in registers.  (Adding dQ up in memory would move 71 times dQ in float32 at 18000 keys,
-// 5 GB for 16 heads of 64; the two products recomputed take less.)
+// summed over their query heads in registers.  (Adding dQ up in memory, not built, would move dQ in float32 once for each
+// 128 keys of a workgroup: 141 times at 18000 keys, 10 GB for 16 heads of 64, 2 ms at a copy's rate and more with atomics; the two
+// products recomputed are 1.3e12 flop there, 1.2 ms.)
 //
 // Bound, like the forward, by matrix and vector work taking turns.  18000 x 8 heads x 64 bfloat16: dK and dV 1.27 ms (four
-// products, 1050 TFLOP/s), dQ 1.17 ms (three, and the one of dS twice for its two planes, 1150 TFLOP/s).
+// products, 1050 TFLOP/s; at that launch bound 7 of its registers are spilled, 32 bytes a lane), dQ 1.17 ms (three, and the one of
+// dS twice for its two planes, 1150 TFLOP/s).
 #include "g2v_attention.h"
 
 namespace g2v {

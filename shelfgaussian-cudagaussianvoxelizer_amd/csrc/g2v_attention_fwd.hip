@@ -9,8 +9,9 @@
 // Bound by the matrix and the vector unit of a SIMD taking turns: at 64 channels a row's 64 keys are 256 cycles of
 // products and, at 8.7 cycles for an exp2 of 64 lanes and 2.1 for anything else, about 220 of vector work; the counters show
 // 44 and about 50 % of the kernel's cycles.  Two blocks of rows a wave halve what is read from LDS for each product (one block
-// and three or four waves a SIMD: 1.54 and 1.48 ms for 1.38).  18000 x 16 heads x 64 bfloat16: 1.33 ms, 1000 TFLOP/s; 9000
-// x 12 x 64 float32: 1.21 ms, 205 TFLOP/s, 1250 of bfloat16 terms.
+// and three or four waves a SIMD: 1.54 and 1.48 ms for 1.38; at 128 channels two blocks spill 12 registers, 52 bytes a lane, and
+// are faster than one all the same).  18000 x 16 heads x 64 bfloat16: 1.32 to 1.38 ms by card, 970 to 1000 TFLOP/s; 9000
+// x 12 x 64 float32: 1.21 to 1.23 ms, 205 TFLOP/s, 1250 of bfloat16 terms.
 #include "g2v_attention.h"
 
 namespace g2v {

@@ -334,6 +334,7 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a)
     }
     if (!a.dw_part) return;
     // the workgroup's sums: lanes of the same elements are 2^shift apart.  Threads / width of them share an element's sum.
+    // (N neighbouring lanes read one bank here, for a few reads once a workgroup.)
     const int span = N << a.shift, parts = kQnThreads > span ? kQnThreads / span : 1, slots = kQnThreads >> a.shift;
     __syncthreads();
 #pragma unroll
