@@ -301,7 +301,9 @@ inline int attn_join_parts(int64_t rows, int lanes, int splits) {
 inline int attn_dp(int dim) { return (dim + 31) / 32 * 32; }
 AttnShape attn_fwd_shape(bool f32, int dp, int64_t rows);
 AttnShape attn_dq_shape(bool f32, int dp, int64_t rows);
-int attn_dkv_planes(bool f32, int64_t nk, int64_t rows);    // of P and dS; rows: of queries of a key head
+// Planes of P and dS by all keys (rows: of queries of a key head).  What a mask leaves is known on the GPU only: a scene of few
+// valid keys among many takes two planes by the plan of one.
+int attn_dkv_planes(bool f32, int64_t nk, int64_t rows);
 AttnShape attn_dkv_shape(bool f32, int dp, int planes);
 hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_attn_list(int batch, int nk, const unsigned char* mask, int* list, int* count, hipStream_t s);
