@@ -401,6 +401,32 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
                            const void* out_rest, const float* lse, const void* grad_out, const long long grad_out_strides[3], void* grad_q,
                            void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention within a window ---------------------------------------------------------------
+ * The attention above over a part of the keys: the scene's Gaussians in an order in which neighbours are near (along a
+ * space-filling curve, or by time).  No counterpart in the reference.  Query i stands at key place p = i + n_k - n_q (queries
+ * and keys of one length: p = i; one query: the last key's) and sees key j if it is valid and
+ *     j <= p + right  and  (j >= p - left  or  j < sinks).
+ * left, right: -1 for no bound.  right = 0 with a bound to the left is the window of a causal order, whose first `sinks`
+ * keys stay visible.  p may be negative (n_q > n_k).  A query that sees no key gives 0 and no gradient.  Arguments, types and
+ * limits as above; the mask is given to the backward again (no key_list); what a masked key's rows hold is never read.  A forward
+ * reads none of the keys between the sinks and the first query's window: one query costs what its window holds.
+ * The gradients of the first `sinks` keys are sums over all queries that see them, in a fixed order.  Asynchronous. */
+size_t g2v_window_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                              int left, int right, int sinks, int in_place, int masked);
+int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                                 const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                                 const long long v_strides[3], int dtype, const unsigned char* key_mask, int left, int right,
+                                 int sinks, float scale, void* out, void* out_rest, float* lse, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+size_t g2v_window_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                               int left, int right, int sinks, int in_place, int masked);
+int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                                  const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                                  const long long v_strides[3], int dtype, const unsigned char* key_mask, int left, int right,
+                                  int sinks, float scale, const void* out, const void* out_rest, const float* lse,
+                                  const void* grad_out, const long long grad_out_strides[3], void* grad_q, void* grad_k,
+                                  void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- per-kernel timing (benchmarks) --------------------------------------------------------
  * No counterpart in the reference (which times the whole forward/backward with one CUDA event
  * pair, src/cuda_gaussian_voxelizer.cu:1549-1555, :1905-1913).  While enabled, every kernel launch

@@ -1035,3 +1035,89 @@ def attention_backward(grad_out, q, k, v, out, rest, lse, key_list=None, scale=N
         if key_list.numel() != B * (nk + 1):
             raise RuntimeError(f"key_list must hold {B * (nk + 1)} values, got {key_list.numel()}")
     return _attention_backward(g, q, k, v, out, rest, lse, key_list, call, want_q, want_kv)
+
+
+# ---- attention within a window ----------------------------------------------------------------------
+
+def _window_side(side, name):
+    """A side of a window as the library takes it: places, -1 without a bound."""
+    if side is None:
+        return -1
+    if isinstance(side, bool) or not isinstance(side, int) or side < 0:
+        raise RuntimeError(f"window: {name} must be a number of places or None, got {side!r}")
+    return min(side, 1 << 30)
+
+
+def _window(window, sinks):
+    """(left, right, sinks) as the library takes them."""
+    if not isinstance(window, (tuple, list)) or len(window) != 2:
+        raise RuntimeError(f"window must be (left, right), got {window!r}")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise RuntimeError(f"sinks must be a number of keys, got {sinks!r}")
+    return _window_side(window[0], "left"), _window_side(window[1], "right"), min(sinks, 1 << 30)
+
+
+def _window_attention_forward(inputs, call, window, for_backward):
+    q, k, v, key_mask = inputs
+    sizes, fdt, scale = call
+    B, nq, nk, hq = sizes[:4]
+    dev = q.device
+    with _OnDevice(dev):
+        out = _empty_rows(q)
+        rest = _empty_rows(q) if for_backward and fdt == _lib.G2V_DTYPE_BF16 else None
+        lse = torch.empty(B, hq, nq, dtype=torch.float32, device=dev) if for_backward else None
+        nws = _workspace_bytes("g2v_window_attention_forward_workspace", *sizes, fdt, *window, _in_place(q, k, v),
+                               0 if key_mask is None else 1)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        rc = _lib.load().g2v_window_attention_forward(*sizes, _addr(q), _strides(q), _addr(k), _strides(k), _addr(v), _strides(v),
+                                                      fdt, _addr(key_mask), *window, scale, _addr(out), _addr(rest), _addr(lse),
+                                                      ws.data_ptr(), nws, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "window_attention_forward")
+    return out, rest, lse
+
+
+def _window_attention_backward(g, q, k, v, key_mask, out, rest, lse, call, window, want_q, want_kv):
+    sizes, fdt, scale = call
+    dev = q.device
+    if g.shape != q.shape:
+        raise RuntimeError(f"grad_out must be {tuple(q.shape)}, got {tuple(g.shape)}")
+    with _OnDevice(dev):
+        dq = _empty_rows(q) if want_q else None
+        dk = _empty_rows(k) if want_kv else None
+        dv = _empty_rows(k) if want_kv else None
+        nws = _workspace_bytes("g2v_window_attention_backward_workspace", *sizes, fdt, *window, _in_place(q, k, v, g),
+                               0 if key_mask is None else 1)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        rc = _lib.load().g2v_window_attention_backward(*sizes, _addr(q), _strides(q), _addr(k), _strides(k), _addr(v),
+                                                       _strides(v), fdt, _addr(key_mask), *window, scale, _addr(out),
+                                                       _addr(rest), _addr(lse), _addr(g), _strides(g), _addr(dq), _addr(dk),
+                                                       _addr(dv), ws.data_ptr(), nws, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "window_attention_backward")
+    return dq, dk, dv
+
+
+def window_attention_forward(q, k, v, window, sinks=0, key_mask=None, scale=None, for_backward=False):
+    """(out, rest, lse): attention_forward over the keys that each query sees.  Query i stands at key place p = i + Nk - Nq and
+    sees key j if j <= p + right and (j >= p - left or j < sinks), with window = (left, right), None for no bound.  rest and lse,
+    None unless for_backward, are what window_attention_backward takes."""
+    return _window_attention_forward(*_attention_inputs(q, k, v, key_mask, scale), _window(window, sinks), for_backward)
+
+
+def window_attention_backward(grad_out, q, k, v, out, rest, lse, window, sinks=0, key_mask=None, scale=None, want_q=True,
+                              want_kv=True):
+    """(grad_q, grad_k, grad_v) of window_attention_forward from its results; None where not wanted."""
+    (q, k, v, key_mask), call = _attention_inputs(q, k, v, key_mask, scale)
+    B, nq, _, hq = call[0][:4]
+    dev = q.device
+    g = _heads_input(grad_out, "grad_out", q)
+    _check_saved(out, "out", q.dtype, dev)
+    _check_saved(lse, "lse", torch.float32, dev)
+    if rest is not None:
+        _check_saved(rest, "rest", torch.bfloat16, dev)
+        if rest.shape != out.shape:
+            raise RuntimeError(f"rest must be {tuple(out.shape)}, got {tuple(rest.shape)}")
+    if out.shape != q.shape or lse.shape != (B, hq, nq):
+        raise RuntimeError(f"out {tuple(out.shape)} and lse {tuple(lse.shape)} do not go with q {tuple(q.shape)}")
+    return _window_attention_backward(g, q, k, v, key_mask, out, rest, lse, call, _window(window, sinks), want_q, want_kv)

@@ -110,8 +110,26 @@ class _GaussianAttentionFunction(torch.autograd.Function):
         return _C._attention_backward(grad_out, *saved, ctx.call, need[0], need[1] or need[2]) + (None, None)
 
 
-def gaussian_attention(q, k, v, key_mask=None, scale=None):
-    """softmax(scale q k^T over the valid keys) v, without an order among queries or keys.
+class _WindowAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, scale, window, sinks):
+        inputs, ctx.call = _C._attention_inputs(q, k, v, key_mask, scale)
+        ctx.window = _C._window(window, sinks)
+        out, rest, lse = _C._window_attention_forward(inputs, ctx.call, ctx.window, True)
+        ctx.save_for_backward(*inputs, out, rest, lse)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        saved, need = ctx.saved_tensors, ctx.needs_input_grad
+        grad_out = _C._heads_input(grad_out, "grad_out", saved[0])
+        return _C._window_attention_backward(grad_out, *saved, ctx.call, ctx.window, need[0], need[1] or need[2]) + (None,) * 4
+
+
+def gaussian_attention(q, k, v, key_mask=None, scale=None, *, window=None, sinks=0):
+    """softmax(scale q k^T over the valid keys) v, without an order among queries or keys; with a window, over the keys near
+    each query in theirs.
 
     q (B, Nq, Hq, D) and k, v (B, Nk, Hkv, D) are float32 or bfloat16 in any layout with unit stride along D; Hq is a
     multiple of Hkv (consecutive query heads share a key head), D at most 128.  key_mask (B, Nk) bool is False at keys
@@ -121,12 +139,24 @@ def gaussian_attention(q, k, v, key_mask=None, scale=None):
     q's type, contiguous.  Any number of queries and keys, zero and one included: a single query that pools a scene has its
     keys split over the GPU.
 
+    window (left, right): query i stands at place p = i + Nk - Nq of the keys (of its own, where queries and keys are the same
+    tokens; of the last one, if it is alone) and sees the places p - left to p + right, None for no bound, and the first
+    ``sinks`` places up to p + right, however far.  Time and memory go with the window, not with the square of the scene:
+    Gaussians sorted along a space-filling curve see their neighbours and a few global tokens in front, those of a stream
+    (right = 0) what came before them.  A query may see no key.
+
     Scores and sums are float32.  With bfloat16 inputs the probabilities are rounded to bfloat16 before their product with v, and
     the backward's factors likewise (as two such planes where keys or queries are few): outputs and gradients are off by 1.7e-3 to
     2.4e-3 of their norm, where rounding exact ones would put them 1.7e-3 off.  float32 keeps 24 bits throughout.
 
     Gradients flow to q, k and v; the backward recomputes the probabilities and gives the same bits on every run.  Gradients
     of gradients and forward-mode derivatives are refused."""
+    if window is None and sinks:
+        raise RuntimeError("sinks without a window: every key is visible")
+    if window is not None:
+        if _differentiated(q, k, v):
+            return _WindowAttentionFunction.apply(q, k, v, key_mask, scale, window, sinks)
+        return _C.window_attention_forward(q, k, v, window, sinks, key_mask, scale)[0]
     if _differentiated(q, k, v):
         return _GaussianAttentionFunction.apply(q, k, v, key_mask, scale)
     return _C.attention_forward(q, k, v, key_mask, scale)[0]
@@ -139,12 +169,18 @@ class PyGaussianAttention(nn.Module):
         q = rotate(norm(x Wq)),  k = rotate(norm(c Wk)),  v = c Wv,  y = attention(q, k, v) Wo
 
     with c = x (self-attention) or the given context.  num_kv_heads key heads are shared by num_heads / num_kv_heads
-    query heads each.  ``wavelengths`` is the range over which the rotations turn, in the positions' unit (metres).  A conversion
+    query heads each.  With ``window`` (left, right) and ``sinks`` a token sees those near it in the tokens' order (see
+    gaussian_attention).  ``wavelengths`` is the range over which the rotations turn, in the positions' unit (metres).  A conversion
     (``layer.bfloat16()``) takes the weights along and leaves the table of angles, ``freqs``, in float32."""
 
     def __init__(self, embed_dim, num_heads, num_kv_heads=None, *, head_dim=None, axes=3, wavelengths=(0.8, 160.0), eps=1e-6,
-                 device="cuda", dtype=torch.float32):
+                 window=None, sinks=0, device="cuda", dtype=torch.float32):
         super().__init__()
+        if window is not None:
+            _C._window(window, sinks)
+        elif sinks:
+            raise RuntimeError("sinks without a window: every key is visible")
+        self.window, self.sinks = window, sinks
         num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
         if head_dim is None:
             if embed_dim % num_heads:
@@ -181,4 +217,4 @@ class PyGaussianAttention(nn.Module):
         k, v = self.to_kv(c).unflatten(-1, (2 * self.kv_heads, self.head_dim)).split(self.kv_heads, 2)
         q, k = qk_norm_rotary(q, k, positions, self.freqs, self.q_weight, self.k_weight,
                               k_positions=context_positions, eps=self.eps)
-        return self.to_out(gaussian_attention(q, k, v, key_mask).flatten(2))
+        return self.to_out(gaussian_attention(q, k, v, key_mask, window=self.window, sinks=self.sinks).flatten(2))

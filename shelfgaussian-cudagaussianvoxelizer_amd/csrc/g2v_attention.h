@@ -105,6 +105,7 @@ __device__ __forceinline__ void next_tile(bool counted) {
 template <int NP, int DP, int ROWS, int NT>
 struct Tile {
     static constexpr int C = DP / 8;                    // chunks of a row
+    static constexpr int kThreads = NT;
     static constexpr int kChunks = NP * ROWS * C;
     static constexpr int kBytes = kChunks * 16;
     static constexpr int kIter = (kChunks + NT - 1) / NT;
@@ -270,6 +271,15 @@ __device__ __forceinline__ void store4(T* row, int d, int D, float x0, float x1,
 // The same for what bfloat16 rounding leaves of the values.
 __device__ __forceinline__ float lost_by_rounding(float x) { return x - (float)(__bf16)x; }
 
+// The maximum in use is that of a wave's first tile, and is taken anew from a tile in which a row's sum of probabilities
+// passes this: any finite reference does in float32 as long as nothing overflows, so that most tiles skip the maximum
+// (a tenth of the vector instructions; matrix and vector work of a SIMD take their time one after the other).
+constexpr float kFar = 1048576.0f;
+
+// The reference (times c) of a row whose scores were all -inf so far: any other one passes kFar from it
+// (or, where c is so small that the reference itself is at float32's lowest values, is in its reach).
+constexpr float kLowest = -1e37f;
+
 // Into which workgroups the tiles of the heads go: the first `head` tiles of each (row0 rows) to head_splits each, the others
 // to `splits` each.  A tile's only workgroup writes its result; more write partial results, which are joined: rows [0, row0)
 // as (head_splits, bhs, row0, ..) where they are split, behind them (splits, bhs, rows - row0, ..).
@@ -337,6 +347,26 @@ __device__ __forceinline__ void split_range(int all, int split, int splits, int&
     hi = lo + per < all ? lo + per : all;
 }
 
+// Sums of the splits: each of `parts` threads every parts-th, then in their order.
+__device__ __forceinline__ f32x4 join_sum(const float* part, int64_t stride, int splits, int parts, bool live, float (*red)[256]) {
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int mine = threadIdx.x % parts;
+    if (live) {
+#pragma unroll 4
+        for (int s = mine; s < splits; s += parts) o += *reinterpret_cast<const f32x4*>(part + s * stride);
+    }
+    if (parts > 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[j][threadIdx.x] = o[j];
+        __syncthreads();
+        if (mine == 0)
+            for (int k = 1; k < parts; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] += red[j][threadIdx.x + k];
+    }
+    return o;
+}
+
 }  // namespace attn
 
 struct AttnFwd {
@@ -364,6 +394,36 @@ struct AttnBwd {
     const float *lse, *delta;   // (batch, hq, nqp); -delta
     void *dq, *dk, *dv;
     float* part;         // partial results: dq: DP values each; dk and dv: 2 DP
+};
+
+namespace attn {
+// Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
+// to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
+// the same error on all of them, which their sum dS K does not average out (dQ then 3.2e-3 off instead of 2.2e-3).
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, float x0, float x1, float x2, float x3) {
+    store4<T>(static_cast<T*>(a.out) + at, d, a.dim, x0, x1, x2, x3);
+    if constexpr (sizeof(T) == 2)
+        if (a.rest)
+            store4<T>(static_cast<T*>(a.rest) + at, d, a.dim, lost_by_rounding(x0), lost_by_rounding(x1),
+                      lost_by_rounding(x2), lost_by_rounding(x3));
+}
+}  // namespace attn
+
+// What a query sees of its scene's keys (g2v_attention_window.hip).  Query i stands at key place i + shift and sees key j if
+// j <= i + shift + right and (j >= i + shift - left or j < sinks), and bit j of the scene is set.  Rows of k and v in place skip
+// `gap` rows behind the sinks, which no query sees (those of the backward and packed ones skip none).
+struct AttnWindow {
+    int left, right, sinks, shift, gap;
+    const uint64_t* bits;   // (batch, words), null: all keys are valid
+    int words;
+};
+struct WinFwd : AttnFwd {
+    AttnWindow win;
+};
+struct WinBwd : AttnBwd {
+    AttnWindow win;
+    bool all_queries;    // dK and dV: of the sinks, from every query that sees them (else of all keys, from those within the window)
 };
 
 }  // namespace g2v

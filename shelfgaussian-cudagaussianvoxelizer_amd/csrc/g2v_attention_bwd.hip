@@ -349,26 +349,6 @@ __global__ void __launch_bounds__(NW * 64, dkv_per_cu(NP, NS, DP)) k_attn_dkv(At
     }
 }
 
-// Sums of the splits: each of `parts` threads every parts-th, then in their order.
-__device__ __forceinline__ f32x4 join_sum(const float* part, int64_t stride, int splits, int parts, bool live, float (*red)[256]) {
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int mine = threadIdx.x % parts;
-    if (live) {
-#pragma unroll 4
-        for (int s = mine; s < splits; s += parts) o += *reinterpret_cast<const f32x4*>(part + s * stride);
-    }
-    if (parts > 1) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) red[j][threadIdx.x] = o[j];
-        __syncthreads();
-        if (mine == 0)
-            for (int k = 1; k < parts; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] += red[j][threadIdx.x + k];
-    }
-    return o;
-}
-
 template <int DP, typename T>
 __global__ void __launch_bounds__(256) k_attn_dq_join(AttnBwd a, int parts) {
     constexpr int kLanes = DP / 4;
@@ -441,15 +421,29 @@ __global__ void __launch_bounds__(256) k_attn_delta(int64_t rows, int nq, int nq
     }
 }
 
-template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
-hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+template <int DP, typename T>
+hipError_t dq_join_launch(const AttnBwd& a, hipStream_t s) {
     const int64_t rows = (int64_t)a.bhs * (a.group * a.nq - joined_from(a.parts, a.group * a.nq));
     if (rows > 0) {
         const int parts = attn_join_parts(rows, DP / 4, std::max(a.parts.head_splits, a.parts.splits));
         G2V_LAUNCH((k_attn_dq_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 4 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();
+}
+template <int DP, typename T>
+hipError_t dkv_join_launch(const AttnBwd& a, hipStream_t s) {
+    const int64_t rows = (int64_t)a.bhs * (a.nk - joined_from(a.parts, a.nk));
+    if (rows > 0) {
+        const int parts = attn_join_parts(rows, DP / 2, std::max(a.parts.head_splits, a.parts.splits));
+        G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 2 * parts))), dim3(256), 0, s, a, parts);
+    }
+    return hipGetLastError();
+}
+
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+hipError_t dq_launch(const AttnBwd& a, hipStream_t s) {
+    G2V_LAUNCH((k_attn_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    return dq_join_launch<DP, T>(a, s);
 }
 template <int NP, int NS, int DP, int NKB, int NW, int QT, typename T>
 void dkv_kernel(const AttnBwd& a, hipStream_t s) {
@@ -474,12 +468,7 @@ hipError_t dkv_launch(AttnBwd& a, hipStream_t s) {
     if constexpr (NP == 1)
         if (planes == 2 || a.by_count) dkv_kernel<NP, 2, DP, NKB, NW, QT, T>(a, s);
     if (planes == NP) dkv_kernel<NP, NP, DP, NKB, NW, QT, T>(a, s);
-    const int64_t rows = (int64_t)a.bhs * (a.nk - joined_from(a.parts, a.nk));
-    if (rows > 0) {
-        const int parts = attn_join_parts(rows, DP / 2, std::max(a.parts.head_splits, a.parts.splits));
-        G2V_LAUNCH((k_attn_dkv_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 2 * parts))), dim3(256), 0, s, a, parts);
-    }
-    return hipGetLastError();
+    return dkv_join_launch<DP, T>(a, s);
 }
 
 }  // namespace
@@ -539,6 +528,24 @@ hipError_t launch_attn_dkv(const AttnBwd& args, bool f32, int dp, hipStream_t s)
         case 64: return dkv_launch<1, 64, 1, 4, 64, __bf16>(a, s);
         case 96: return dkv_launch<1, 96, 1, 4, 64, __bf16>(a, s);
         default: return dkv_launch<1, 128, 1, 4, 32, __bf16>(a, s);
+    }
+}
+
+hipError_t launch_attn_dq_join(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
+    switch (dp) {
+        case 32: return f32 ? dq_join_launch<32, float>(a, s) : dq_join_launch<32, __bf16>(a, s);
+        case 64: return f32 ? dq_join_launch<64, float>(a, s) : dq_join_launch<64, __bf16>(a, s);
+        case 96: return f32 ? dq_join_launch<96, float>(a, s) : dq_join_launch<96, __bf16>(a, s);
+        default: return f32 ? dq_join_launch<128, float>(a, s) : dq_join_launch<128, __bf16>(a, s);
+    }
+}
+
+hipError_t launch_attn_dkv_join(const AttnBwd& a, bool f32, int dp, hipStream_t s) {
+    switch (dp) {
+        case 32: return f32 ? dkv_join_launch<32, float>(a, s) : dkv_join_launch<32, __bf16>(a, s);
+        case 64: return f32 ? dkv_join_launch<64, float>(a, s) : dkv_join_launch<64, __bf16>(a, s);
+        case 96: return f32 ? dkv_join_launch<96, float>(a, s) : dkv_join_launch<96, __bf16>(a, s);
+        default: return f32 ? dkv_join_launch<128, float>(a, s) : dkv_join_launch<128, __bf16>(a, s);
     }
 }
 

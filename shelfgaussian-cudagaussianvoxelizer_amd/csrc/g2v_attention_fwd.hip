@@ -18,27 +18,6 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-// The maximum in use is that of a wave's first tile, and is taken anew from a tile in which a row's sum of probabilities
-// passes this: any finite reference does in float32 as long as nothing overflows, so that most tiles skip the maximum
-// (a tenth of the vector instructions; matrix and vector work of a SIMD take their time one after the other).
-constexpr float kFar = 1048576.0f;
-
-// The reference (times c) of a row whose scores were all -inf so far: any other one passes kFar from it
-// (or, where c is so small that the reference itself is at float32's lowest values, is in its reach).
-constexpr float kLowest = -1e37f;
-
-// Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
-// to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
-// the same error on all of them, which their sum dS K does not average out (dQ then 3.2e-3 off instead of 2.2e-3).
-template <typename T>
-__device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, float x0, float x1, float x2, float x3) {
-    store4<T>(static_cast<T*>(a.out) + at, d, a.dim, x0, x1, x2, x3);
-    if constexpr (sizeof(T) == 2)
-        if (a.rest)
-            store4<T>(static_cast<T*>(a.rest) + at, d, a.dim, lost_by_rounding(x0), lost_by_rounding(x1),
-                      lost_by_rounding(x2), lost_by_rounding(x3));
-}
-
 // KS: steps of 16 that the head's width takes in the scores' product (the last of DP / 16 may hold nothing but padding).
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, launch_bound(NW, fwd_per_cu(NP, DP, NW))) k_attn_fwd(AttnFwd a) {
@@ -360,6 +339,11 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
         if (have) i = a.list[b * a.n[k] + i];
     }
     if (!have) return;
+    bool zero = false;
+    if (a.keys[k]) {
+        if (a.bits) zero = !(a.bits[b * a.words + (i >> 6)] >> (i & 63) & 1);
+        if (a.gap && i >= a.sinks) i += a.gap;
+    }
     const T* src = static_cast<const T*>(a.src[k]) + b * a.sb[k] + i * a.sn[k] + bh % a.heads[k] * a.sh[k];
     const int64_t row = bh * a.n[k] + slot;
     // a whole chunk in one access or two, at any alignment (global memory takes it); a row's last elements one by one
@@ -369,7 +353,10 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
 #pragma unroll
     for (int h = 0; h < 8 / kPer; ++h) {
         const int d = c * 8 + h * kPer;
-        if (d + kPer <= a.dim) {
+        if (zero) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) x[h][j] = (T)0.0f;
+        } else if (d + kPer <= a.dim) {
             x[h] = *reinterpret_cast<const vec*>(src + d);
         } else {
 #pragma unroll
@@ -395,15 +382,20 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
         *reinterpret_cast<bf16x8*>(static_cast<char*>(a.dst[k]) + ((row * NP + pl) * C + c) * 16) = o[pl];
 }
 
-template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
-hipError_t fwd_launch(const AttnFwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_attn_fwd<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+template <int DP, typename T>
+hipError_t join_launch(const AttnFwd& a, hipStream_t s) {
     const int64_t rows = (int64_t)a.bhs * (a.group * a.nq - joined_from(a.parts, a.group * a.nq));
     if (rows > 0) {
         const int parts = attn_join_parts(rows, DP / 4, std::max(a.parts.head_splits, a.parts.splits));
         G2V_LAUNCH((k_attn_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 4 * parts))), dim3(256), 0, s, a, parts);
     }
     return hipGetLastError();
+}
+
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+hipError_t fwd_launch(const AttnFwd& a, hipStream_t s) {
+    G2V_LAUNCH((k_attn_fwd<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    return join_launch<DP, T>(a, s);
 }
 
 template <int NP, int DP, int NQB, int KT, typename T>
@@ -445,6 +437,15 @@ hipError_t launch_attn_fwd(const AttnFwd& a, bool f32, int dp, hipStream_t s) {
         case 64: return fwd_waves<1, 64, 2, 64, __bf16>(a, g, s);
         case 96: return fwd_waves<1, 96, 1, 64, __bf16>(a, g, s);
         default: return fwd_waves<1, 128, 2, 32, __bf16>(a, g, s);
+    }
+}
+
+hipError_t launch_attn_join(const AttnFwd& a, bool f32, int dp, hipStream_t s) {
+    switch (dp) {
+        case 32: return f32 ? join_launch<32, float>(a, s) : join_launch<32, __bf16>(a, s);
+        case 64: return f32 ? join_launch<64, float>(a, s) : join_launch<64, __bf16>(a, s);
+        case 96: return f32 ? join_launch<96, float>(a, s) : join_launch<96, __bf16>(a, s);
+        default: return f32 ? join_launch<128, float>(a, s) : join_launch<128, __bf16>(a, s);
     }
 }
 

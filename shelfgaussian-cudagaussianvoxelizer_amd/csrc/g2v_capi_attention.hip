@@ -313,6 +313,163 @@ size_t attn_bwd_bytes(const AttnSizes& z, const AttnRun& dq, const AttnRun& dkv,
     return c.off + 256;
 }
 
+// ---- attention within a window -----------------------------------------------------------------
+
+// Sizes and window as the kernels take them: z.nk without the keys between the sinks and the first window (forward only; in
+// steps of 64, the mask's words).
+struct WinSizes {
+    AttnSizes z;
+    AttnWindow w;
+    int64_t span;    // keys of a query's window
+};
+int win_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype, int left, int right, int sinks,
+              bool forward, WinSizes& x) {
+    const int rc = attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, x.z);
+    if (rc != G2V_OK) return rc;
+    if (left < -1 || right < -1 || sinks < 0)
+        return api_fail(G2V_ERR_INVALID, "left = %d, right = %d, sinks = %d (not negative; left, right -1: no bound)", left, right, sinks);
+    constexpr int kFarAway = 1 << 28;    // places are below 2^26
+    x.w = {};
+    x.w.left = left < 0 ? kFarAway : std::min(left, kFarAway);
+    x.w.right = right < 0 ? kFarAway : std::min(right, kFarAway);
+    x.w.sinks = std::min(sinks, n_k);
+    x.w.shift = n_k - n_q;
+    x.span = (int64_t)x.w.left + x.w.right + 1;
+    if (forward) {
+        const int first = std::max(0, x.w.shift - x.w.left);
+        x.w.gap = first > x.w.sinks ? (first - x.w.sinks) / 64 * 64 : 0;
+        x.z.nk -= x.w.gap;
+        x.w.shift -= x.w.gap;
+    }
+    x.w.words = (int)ceil_div(x.z.nk, 64);
+    return G2V_OK;
+}
+
+// A workgroup's rows see a window longer by themselves, and the sinks.
+int64_t win_keys(const WinSizes& x, AttnShape g) {
+    return std::min<int64_t>(x.z.nk, x.span + g.waves * g.blocks * 32 / x.z.group + (x.w.sinks ? g.tile : 0));
+}
+AttnRun win_fwd_run(const WinSizes& x) {
+    const AttnShape g = window_fwd_shape(x.z.f32, x.z.dp, x.z.rows());
+    return attn_run(x.z, g, x.z.rows(), win_keys(x, g), 1, x.z.dp, false);
+}
+AttnRun win_dq_run(const WinSizes& x) {
+    const AttnShape g = window_dq_shape(x.z.f32, x.z.dp, x.z.rows());
+    return attn_run(x.z, g, x.z.rows(), win_keys(x, g), 1, x.z.dp, false);
+}
+// Planes of P and dS by the keys that a query sees (see attn_dkv_planes); two where a mask leaves fewer, how many is known on the
+// GPU only.
+int win_dkv_planes(const WinSizes& x, bool masked) {
+    return attn_dkv_planes(x.z.f32, masked ? 1 : std::min<int64_t>(x.z.nk, x.span + x.w.sinks), x.z.rows());
+}
+AttnRun win_dkv_run(const WinSizes& x, int planes) {
+    const AttnShape g = window_dkv_shape(x.z.f32, x.z.dp, planes, false);
+    return attn_run(x.z, g, x.z.nk, std::min<int64_t>(x.z.nq, x.span + g.waves * 32), x.z.group, 2 * x.z.dp, false);
+}
+// The sinks' queries beyond their windows: whether there are any, and the splits of all queries for each tile of sinks.
+bool win_has_far(const WinSizes& x) { return x.w.sinks > 0 && (int64_t)x.w.left - x.w.shift + 1 < x.z.nq; }
+AttnRun win_sinks_run(const WinSizes& x, int planes) {
+    attn::Parts r = {};
+    if (!win_has_far(x)) return {r, 0};
+    const AttnShape g = window_dkv_shape(x.z.f32, x.z.dp, planes, true);
+    r.tiles = r.head = (int)ceil_div(x.w.sinks, 32);
+    r.row0 = x.w.sinks;
+    r.splits = 1;
+    const int units = (int)std::min<int64_t>(ceil_div(x.z.nq, g.tile) * x.z.group, 1 << 30);
+    const double unit_us = std::max(1.0, 2.0 * g.products * 32 * g.tile * x.z.dp * g.per_cu / ((x.z.f32 ? 0.15e9 : 1.0e9) / kCus));
+    double least;
+    r.head_splits = attn_splits((int64_t)x.z.bhs * r.tiles, units, g.per_cu, unit_us, 8.0 * x.w.sinks * x.z.bhs * 2 * x.z.dp / 3e6, least);
+    return {r, part_rows(r, x.z.bhs, x.w.sinks)};
+}
+
+struct WinFwdWs {
+    uint64_t* bits;
+    float *part_o, *part_ml;
+};
+WinFwdWs carve_win_fwd(Carver& c, const WinSizes& x, const AttnRun& r, bool masked) {
+    WinFwdWs w;
+    const AttnFwdWs f = carve_attn_fwd(c, x.z, r);
+    w.part_o = f.part_o;
+    w.part_ml = f.part_ml;
+    w.bits = masked ? c.take<uint64_t>((size_t)x.z.batch * x.w.words) : nullptr;
+    return w;
+}
+struct WinBwdRuns {
+    int planes;
+    AttnRun dq, dkv, sinks;
+};
+WinBwdRuns win_bwd_runs(const WinSizes& x, bool masked) {
+    WinBwdRuns r;
+    r.planes = win_dkv_planes(x, masked);
+    r.dq = win_dq_run(x);
+    r.dkv = win_dkv_run(x, r.planes);
+    r.sinks = win_sinks_run(x, r.planes);
+    return r;
+}
+struct WinBwdWs {
+    int nqp;
+    float *lse, *delta, *part;
+    uint64_t* bits;
+};
+WinBwdWs carve_win_bwd(Carver& c, const WinSizes& x, const WinBwdRuns& r, bool masked) {
+    WinBwdWs w;
+    AttnRun dkv = r.dkv;    // the sinks' partial results take the area of the others' after them
+    dkv.part_rows = std::max(dkv.part_rows, r.sinks.part_rows);
+    const AttnBwdWs f = carve_attn_bwd(c, x.z, r.dq, dkv);
+    w.nqp = f.nqp;
+    w.lse = f.lse;
+    w.delta = f.delta;
+    w.part = f.part;
+    w.bits = masked ? c.take<uint64_t>((size_t)x.z.batch * x.w.words) : nullptr;
+    return w;
+}
+size_t win_fwd_bytes(const WinSizes& x, const AttnRun& r, bool packed, bool masked) {
+    Carver c(nullptr, (size_t)-1);
+    carve_win_fwd(c, x, r, masked);
+    carve_packed(c, x.z, packed, false, false);
+    return c.off + 256;
+}
+size_t win_bwd_bytes(const WinSizes& x, const WinBwdRuns& r, bool packed, bool masked) {
+    Carver c(nullptr, (size_t)-1);
+    carve_win_bwd(c, x, r, masked);
+    carve_packed(c, x.z, packed, false, true);
+    return c.off + 256;
+}
+
+// The tensors as the kernels read them: all in place, or all packed without the gap and with zeros in masked keys' rows.
+hipError_t win_sources(const WinSizes& x, const Strided* t, int count, bool packed, const uint64_t* bits, Carver& c,
+                       attn::RowSrc* out, hipStream_t s) {
+    const AttnSizes& z = x.z;
+    AttnPack a = {};
+    a.batch = z.batch;
+    a.dim = z.dim;
+    a.dp = z.dp;
+    a.list_tensor = -1;
+    a.sinks = x.w.sinks;
+    a.gap = x.w.gap;
+    a.words = x.w.words;
+    a.bits = bits;
+    for (int i = 0; i < count; ++i) {
+        if (!packed) {
+            out[i] = {static_cast<const char*>(t[i].p), t[i].s[0] * 2, t[i].s[1] * 2, t[i].s[2] * 2, z.dim / 8};
+            continue;
+        }
+        const int64_t row = (int64_t)(z.f32 ? 3 : 1) * z.dp * 2;
+        char* dst = c.take<char>(attn_packed_bytes(z, t[i].n, t[i].heads));
+        const int k = a.tensors++;
+        a.src[k] = t[i].p;
+        a.sb[k] = t[i].s[0];
+        a.sn[k] = t[i].s[1];
+        a.sh[k] = t[i].s[2];
+        a.n[k] = t[i].n;
+        a.heads[k] = t[i].heads;
+        a.keys[k] = t[i].keys;
+        a.dst[k] = dst;
+        out[i] = {dst, row * t[i].n * t[i].heads, row, row * t[i].n, z.dp / 8};
+    }
+    return a.tensors ? launch_attn_pack(a, z.f32, s) : hipSuccess;
+}
+
 int attn_scale(float scale) {
     if (!(scale > 0.0f) || !isfinite(scale * attn::kLog2e))
         return api_fail(G2V_ERR_INVALID, "scale = %g (positive and finite)", (double)scale);
@@ -461,6 +618,155 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
     if (grad_q && queries) {
         a.parts = rq.parts;
         G2V_HIP(launch_attn_dq(a, z.f32, z.dp, s));
+    }
+    return G2V_OK;
+}
+
+size_t g2v_window_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                              int left, int right, int sinks, int in_place, int masked) {
+    WinSizes x;
+    if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, true, x) != G2V_OK) return 0;
+    return win_fwd_bytes(x, win_fwd_run(x), x.z.f32 || !in_place, masked != 0);
+}
+
+int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                                 const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                                 const long long v_strides[3], int dtype, const unsigned char* key_mask, int left, int right,
+                                 int sinks, float scale, void* out, void* out_rest, float* lse, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+    api_begin();
+    WinSizes x;
+    int rc = win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, true, x);
+    if (rc != G2V_OK) return rc;
+    rc = attn_scale(scale);
+    if (rc != G2V_OK) return rc;
+    if ((int64_t)batch * n_q == 0) return G2V_OK;
+    const bool keys = (int64_t)batch * n_k > 0;
+    if (!out || !q || !q_strides || (keys && (!k || !v || !k_strides || !v_strides)))
+        return api_fail(G2V_ERR_INVALID, "null q, k, v, strides or out");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    static const long long none[3] = {0, 0, 0};
+    const AttnSizes& z = x.z;
+    const Strided t[3] = {{q, q_strides, n_q, heads_q, false},
+                          {k, keys ? k_strides : none, z.nk, heads_k, true},
+                          {v, keys ? v_strides : none, z.nk, heads_k, true}};
+    const bool packed = !attn_in_place(z, t, 3), masked = keys && key_mask;
+    const AttnRun r = win_fwd_run(x);
+    const size_t need = win_fwd_bytes(x, r, packed, masked);
+    if (!workspace || workspace_bytes < need)
+        return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
+    Carver c(workspace, workspace_bytes);
+    const WinFwdWs w = carve_win_fwd(c, x, r, masked);
+    if (masked) G2V_HIP(launch_window_bits(batch, z.nk, x.w.sinks, x.w.gap, key_mask, x.w.words, w.bits, s));
+    attn::RowSrc src[3];
+    G2V_HIP(win_sources(x, t, 3, packed, w.bits, c, src, s));
+    WinFwd a = {};
+    a.q = src[0];
+    a.k = src[1];
+    a.v = src[2];
+    a.nq = n_q;
+    a.nk = z.nk;
+    a.hq = heads_q;
+    a.hk = heads_k;
+    a.group = z.group;
+    a.dim = head_dim;
+    a.bhs = z.bhs;
+    a.parts = r.parts;
+    a.c = scale * attn::kLog2e;
+    a.out = out;
+    a.rest = out_rest;
+    a.lse = lse;
+    a.part_o = w.part_o;
+    a.part_ml = w.part_ml;
+    a.win = x.w;
+    a.win.bits = w.bits;
+    if (packed) a.win.gap = 0;
+    G2V_HIP(launch_window_fwd(a, z.f32, z.dp, s));
+    return G2V_OK;
+}
+
+size_t g2v_window_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
+                                               int left, int right, int sinks, int in_place, int masked) {
+    WinSizes x;
+    if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, false, x) != G2V_OK) return 0;
+    return win_bwd_bytes(x, win_bwd_runs(x, masked != 0), x.z.f32 || !in_place, masked != 0);
+}
+
+int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
+                                  const long long q_strides[3], const void* k, const long long k_strides[3], const void* v,
+                                  const long long v_strides[3], int dtype, const unsigned char* key_mask, int left, int right,
+                                  int sinks, float scale, const void* out, const void* out_rest, const float* lse,
+                                  const void* grad_out, const long long grad_out_strides[3], void* grad_q, void* grad_k,
+                                  void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
+    api_begin();
+    WinSizes x;
+    int rc = win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, false, x);
+    if (rc != G2V_OK) return rc;
+    rc = attn_scale(scale);
+    if (rc != G2V_OK) return rc;
+    const bool queries = (int64_t)batch * n_q > 0, keys = (int64_t)batch * n_k > 0;
+    if (!queries && !keys) return G2V_OK;
+    if ((grad_k == nullptr) != (grad_v == nullptr)) return api_fail(G2V_ERR_INVALID, "grad_k and grad_v go together");
+    if ((queries && (!q || !q_strides || !out || !lse || !grad_out || !grad_out_strides)) ||
+        (keys && (!k || !v || !k_strides || !v_strides)))
+        return api_fail(G2V_ERR_INVALID, "null q, k, v, out, lse, grad_out or strides");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    static const long long none[3] = {0, 0, 0};
+    const long long* sg = queries ? grad_out_strides : none;
+    const Strided t[4] = {{q, queries ? q_strides : none, n_q, heads_q, false},
+                          {k, keys ? k_strides : none, n_k, heads_k, true},
+                          {v, keys ? v_strides : none, n_k, heads_k, true},
+                          {grad_out, sg, n_q, heads_q, false}};
+    const AttnSizes& z = x.z;
+    const bool packed = !attn_in_place(z, t, 4), masked = keys && key_mask;
+    const WinBwdRuns r = win_bwd_runs(x, masked);
+    const size_t need = win_bwd_bytes(x, r, packed, masked);
+    if (!workspace || workspace_bytes < need)
+        return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
+    Carver c(workspace, workspace_bytes);
+    const WinBwdWs w = carve_win_bwd(c, x, r, masked);
+    if (masked) G2V_HIP(launch_window_bits(batch, n_k, x.w.sinks, 0, key_mask, x.w.words, w.bits, s));
+    attn::RowSrc src[4];
+    G2V_HIP(win_sources(x, t, 4, packed, w.bits, c, src, s));
+    G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, out_rest, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
+                              w.delta, s));
+    WinBwd a = {};
+    a.q = src[0];
+    a.k = src[1];
+    a.v = src[2];
+    a.g = src[3];
+    a.nq = n_q;
+    a.nk = n_k;
+    a.hq = heads_q;
+    a.hk = heads_k;
+    a.group = z.group;
+    a.dim = head_dim;
+    a.bhs = z.bhs;
+    a.nqp = w.nqp;
+    a.c = scale * attn::kLog2e;
+    a.scale = scale;
+    a.lse = w.lse;
+    a.delta = w.delta;
+    a.dq = grad_q;
+    a.dk = grad_k;
+    a.dv = grad_v;
+    a.part = w.part;
+    a.win = x.w;
+    a.win.bits = w.bits;
+    if (grad_k && keys) {
+        WinBwd kv = a;
+        if (n_k == 1 || (x.span == 1 && x.w.sinks == 0)) kv.scale = 0.0f;    // a query's only key: its probability is 1
+        kv.parts = r.dkv.parts;
+        G2V_HIP(launch_window_dkv(kv, z.f32, z.dp, r.planes, s));
+        if (queries && win_has_far(x)) {    // written anew behind them
+            kv.all_queries = true;
+            kv.parts = r.sinks.parts;
+            G2V_HIP(launch_window_dkv(kv, z.f32, z.dp, r.planes, s));
+        }
+    }
+    if (grad_q && queries) {
+        a.parts = r.dq.parts;
+        G2V_HIP(launch_window_dq(a, z.f32, z.dp, s));
     }
     return G2V_OK;
 }

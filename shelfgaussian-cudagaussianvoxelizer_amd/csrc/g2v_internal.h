@@ -285,6 +285,10 @@ struct AttnPack {
     const unsigned char* mask;
     int *count_out, *list_out;
     int list_tensor;
+    // rows of the keys from `sinks` on are `gap` rows further in src, and those whose bit is not set are packed as zeros,
+    // unread (64 keys a word; null: all)
+    int sinks, gap, words;
+    const uint64_t* bits;
     int64_t blocks[4];   // set by the launch
 };
 // A kernel's workgroup: waves, blocks of 32 rows of a wave, rows of a tile of the long axis, workgroups that fit a CU; and
@@ -313,6 +317,25 @@ hipError_t launch_attn_delta(int batch, int nq, int nqp, int heads, int dim, con
                              int64_t gsb, int64_t gsn, int64_t gsh, bool f32, const float* lse, float* lse_p, float* delta, hipStream_t s);
 hipError_t launch_attn_dq(const AttnBwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_attn_dkv(const AttnBwd& a, bool f32, int dp, hipStream_t s);
+// The joins of the splits by a's plan, which the launches above make themselves.
+hipError_t launch_attn_join(const AttnFwd& a, bool f32, int dp, hipStream_t s);
+hipError_t launch_attn_dq_join(const AttnBwd& a, bool f32, int dp, hipStream_t s);
+hipError_t launch_attn_dkv_join(const AttnBwd& a, bool f32, int dp, hipStream_t s);
+
+// ---- attention within a window (g2v_attention_window.hip) -----------------------------------
+struct WinFwd;
+struct WinBwd;
+// Bits of the valid keys of each scene, 64 keys a word, by mask (batch, nk + gap); key j of the words is key j + gap of the mask
+// behind the sinks.
+hipError_t launch_window_bits(int batch, int nk, int sinks, int gap, const unsigned char* mask, int words, uint64_t* bits,
+                              hipStream_t s);
+AttnShape window_fwd_shape(bool f32, int dp, int64_t rows);
+AttnShape window_dq_shape(bool f32, int dp, int64_t rows);
+AttnShape window_dkv_shape(bool f32, int dp, int planes, bool all_queries);
+hipError_t launch_window_fwd(const WinFwd& a, bool f32, int dp, hipStream_t s);
+hipError_t launch_window_dq(const WinBwd& a, bool f32, int dp, hipStream_t s);
+// planes: of P and dS.  With a.all_queries a.parts splits all tiles of the sinks alike.
+hipError_t launch_window_dkv(const WinBwd& a, bool f32, int dp, int planes, hipStream_t s);
 
 // Brackets one kernel launch with HIP events when profiling is enabled (g2v_profile.hip).
 class ProfMark {
