@@ -427,6 +427,42 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
                                   const void* grad_out, const long long grad_out_strides[3], void* grad_q, void* grad_k,
                                   void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- layer norm ------------------------------------------------------------------------------
+ * The norm around an attention layer, with the residual sum before it in the same pass.  No counterpart in the reference.
+ *     s = x + residual  (rounded to dtype),  y = (s - mean s) (var s + eps)^-1/2 weight + bias
+ * x, residual (NULL: s = x), y and sum (batch, n, channels) of dtype (G2V_DTYPE_F32 or G2V_DTYPE_BF16): inputs with strides in
+ * elements along batch and n and unit stride along channels, y and sum (needed with residual) contiguous.  weight and
+ * bias (channels) of weight_dtype, NULL for ones and zeros.  stats (batch n, 2) float32 receives mean and (var + eps)^-1/2 of each
+ * row, for the backward (NULL where none follows).  channels <= 8192.  Sums are float32, the variance is that of the
+ * differences to the mean.  Asynchronous.
+ *
+ * The backward maps the gradients of y and of sum (grad_sum NULL: none) to grad_x, the gradient of x and of residual alike
+ * (contiguous, dtype), and, where not NULL, grad_weight and grad_bias (weight_dtype; summed in float32); x is what was normed: the
+ * forward's sum, where it had a residual.  Deterministic: fixed summation order. */
+int g2v_layer_norm_forward(int batch, int n, int channels, const void* x, const long long x_strides[2], const void* residual,
+                           const long long residual_strides[2], int dtype, const void* weight, const void* bias,
+                           int weight_dtype, float eps, void* y, void* sum, float* stats, void* stream);
+size_t g2v_layer_norm_backward_workspace(int batch, int n, int channels, int dtype);
+int g2v_layer_norm_backward(int batch, int n, int channels, const void* x, const long long x_strides[2], int dtype,
+                            const void* weight, int weight_dtype, const float* stats, const void* grad_y,
+                            const long long grad_y_strides[2], const void* grad_sum, const long long grad_sum_strides[2],
+                            void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* ---- gradient norm and clipping ---------------------------------------------------------------
+ * The norm of `count` gradient tensors taken together, and their clipping by it, at the end of a training step's backward.  No
+ * counterpart in the reference.
+ *     norm = (sum over tensors and elements of g^2)^1/2,   out = min(1, max_norm / (norm + 1e-6)) g
+ * The arrays (grads, outs, their dtypes, numels) are on the host and read before the call returns; grads[i] and outs[i] hold
+ * numels[i] contiguous elements of grad_dtypes[i] and out_dtypes[i], outs[i] may be grads[i] with the same type (in place; where
+ * nothing is clipped it is not written).  Other memory that is written must not be shared (checked).  norm is a device float.
+ * Squares are summed in 64 bits, in a fixed order, and products are rounded to float32, and from that to a bfloat16 output.  A NaN or infinity
+ * among the gradients makes norm one and every output c g of it, as the formula says.  Asynchronous, any number of tensors. */
+size_t g2v_clip_gradients_workspace(int count);
+int g2v_clip_gradients(int count, const void* const* grads, const int* grad_dtypes, void* const* outs, const int* out_dtypes,
+                       const long long* numels, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 /* ---- per-kernel timing (benchmarks) --------------------------------------------------------
  * No counterpart in the reference (which times the whole forward/backward with one CUDA event
  * pair, src/cuda_gaussian_voxelizer.cu:1549-1555, :1905-1913).  While enabled, every kernel launch

@@ -6,6 +6,7 @@ caller's current HIP stream.  Outputs and workspaces come from PyTorch's caching
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 
@@ -1121,3 +1122,176 @@ def window_attention_backward(grad_out, q, k, v, out, rest, lse, window, sinks=0
     if out.shape != q.shape or lse.shape != (B, hq, nq):
         raise RuntimeError(f"out {tuple(out.shape)} and lse {tuple(lse.shape)} do not go with q {tuple(q.shape)}")
     return _window_attention_backward(g, q, k, v, key_mask, out, rest, lse, call, _window(window, sinks), want_q, want_kv)
+
+
+# ---- layer norm --------------------------------------------------------------------------------------
+
+def _rows_input(t, name, like=None):
+    """(rows as (B, N, C) with unit stride along C, their strides along B and N); like: the tensor whose type, device and shape it
+    has to share.  Leading dimensions are taken together where their strides allow it, others are copied."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a GPU tensor, got {t.device}")
+    if t.dtype not in _FEAT_DTYPES:
+        raise RuntimeError(f"expected scalar type Float or BFloat16 for {name} but found {t.dtype}")
+    if t.dim() < 1:
+        raise RuntimeError(f"{name} must be (..., C), got a scalar")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape != like.shape):
+        raise RuntimeError(f"{name} is {t.dtype} {tuple(t.shape)} on {t.device}, expected {like.dtype} {tuple(like.shape)} on "
+                           f"{like.device}")
+    C = t.shape[-1]
+    if C and t.numel() // C >= 1 << 31:
+        raise RuntimeError(f"{name} has {t.numel() // C} rows (limit 2^31)")
+    if t.is_contiguous():
+        n = t.numel() // C if C else 0
+        return t, (1, n, C), (n * C, C)
+    if t.dim() == 3 and t.stride(2) == 1:
+        return t, tuple(t.shape), t.stride()[:2]
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, (1,) + tuple(t.shape), (0, t.stride(0))
+    return _rows_input(t.detach().contiguous(), name)
+
+
+_RowStrides = ctypes.c_longlong * 2
+
+
+def _row_strides(rows):
+    return None if rows is None else _RowStrides(*rows[2])
+
+
+def _norm_weight(t, name, C, device, like=None):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in _FEAT_DTYPES or t.device != device or t.shape != (C,):
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise RuntimeError(f"{name} must be float32 or bfloat16 {(C,)} on {device}, got {got}")
+    if like is not None and t.dtype != like.dtype:
+        raise RuntimeError(f"{name} is {t.dtype}, weight {like.dtype}")
+    return t if t.is_contiguous() else t.detach().contiguous()
+
+
+def _same_rows(rows, other):
+    """Two inputs' rows with one split of their leading dimensions (that of the one that is not contiguous)."""
+    if rows[1] == other[1]:
+        return rows, other
+    if rows[1][0] == 1 and rows[0].is_contiguous():
+        B, n, C = other[1]
+        return (rows[0], other[1], (n * C, C)), other
+    if other[1][0] == 1 and other[0].is_contiguous():
+        return _same_rows(other, rows)[::-1]
+    return _same_rows(rows, _rows_input(other[0].detach().contiguous(), "rows"))
+
+
+def layer_norm_forward(x, weight=None, bias=None, residual=None, eps=1e-5, for_backward=False):
+    """(y, sum, stats): the layer norm of the rows of x (..., C), or of sum = x + residual, with weight and bias (C,).  sum is None
+    without residual; stats, None unless for_backward, holds the rows' mean and (variance + eps)^-1/2 for layer_norm_backward."""
+    rows, other = _rows_input(x, "x"), None
+    if residual is not None:
+        rows, other = _same_rows(rows, _rows_input(residual, "residual", x))
+    C, dev = x.shape[-1], x.device
+    weight = _norm_weight(weight, "weight", C, dev)
+    bias = _norm_weight(bias, "bias", C, dev, weight)
+    wdt = next((_FEAT_DTYPES[t.dtype] for t in (weight, bias) if t is not None), _lib.G2V_DTYPE_F32)
+    with _OnDevice(dev):
+        y = _empty_rows(x)
+        total = None if residual is None else _empty_rows(x)
+        stats = torch.empty(x.numel() // C if C else 0, 2, dtype=torch.float32, device=dev) if for_backward else None
+        rc = _lib.load().g2v_layer_norm_forward(*rows[1], rows[0].data_ptr(), _row_strides(rows),
+                                                None if other is None else other[0].data_ptr(), _row_strides(other),
+                                                _FEAT_DTYPES[x.dtype], _addr(weight), _addr(bias), wdt, float(eps), y.data_ptr(),
+                                                _addr(total), _addr(stats), _stream_of(dev))
+    if rc:
+        _lib.check(rc, "layer_norm_forward")
+    return y, total, stats
+
+
+def layer_norm_backward(grad_y, x, weight, stats, grad_sum=None, want_weights=(True, True), bias_dtype=None):
+    """(grad_x, grad_weight, grad_bias) of layer_norm_forward from what it normed (x, or the sum with the residual, whose gradient is
+    grad_x as well) and its stats; grad_sum: the gradient that reaches the sum besides.  Weight gradients have the weight's type
+    (without one bias_dtype, None: float32) and are None where not wanted."""
+    rows, gy = _rows_input(x, "x"), _rows_input(grad_y, "grad_y", x)
+    C, dev = x.shape[-1], x.device
+    weight = _norm_weight(weight, "weight", C, dev)
+    _check_saved(stats, "stats", torch.float32, dev)
+    if stats.shape != (x.numel() // C if C else 0, 2):
+        raise RuntimeError(f"stats {tuple(stats.shape)} do not go with x {tuple(x.shape)}")
+    rows, gy = _same_rows(rows, gy)
+    gs = None
+    if grad_sum is not None:
+        gs = _rows_input(grad_sum, "grad_sum", x)
+        if gs[1] != rows[1]:      # three layouts that share no split of the leading dimensions
+            rows, gy, gs = (_rows_input(t[0].detach().contiguous(), "rows") for t in (rows, gy, gs))
+    wdtype = weight.dtype if weight is not None else bias_dtype or torch.float32
+    with _OnDevice(dev):
+        dx = _empty_rows(x)
+        dw = torch.empty(C, dtype=wdtype, device=dev) if want_weights[0] else None
+        db = torch.empty(C, dtype=wdtype, device=dev) if want_weights[1] else None
+        nws = _workspace_bytes("g2v_layer_norm_backward_workspace", *rows[1], _FEAT_DTYPES[x.dtype])
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        rc = _lib.load().g2v_layer_norm_backward(*rows[1], rows[0].data_ptr(), _row_strides(rows), _FEAT_DTYPES[x.dtype],
+                                                 _addr(weight), _FEAT_DTYPES[wdtype], stats.data_ptr(), gy[0].data_ptr(),
+                                                 _row_strides(gy), None if gs is None else gs[0].data_ptr(), _row_strides(gs),
+                                                 dx.data_ptr(), _addr(dw), _addr(db), ws.data_ptr(), nws, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "layer_norm_backward")
+    return dx, dw, db
+
+
+# ---- gradient norm and clipping ----------------------------------------------------------------------
+
+def _dense(t):
+    """Whether a tensor's elements are one piece of memory, each once, in some order of its dimensions."""
+    return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
+
+
+def clip_gradients(grads, max_norm, outs=None):
+    """The norm (a 0-dim float32 GPU tensor) of a list of gradient tensors taken together, float32 or bfloat16 on one GPU; each is
+    scaled by min(1, max_norm / (norm + 1e-6)), in place or into outs, tensors of the same shapes (float32 or bfloat16)."""
+    lib = _lib.load()
+    if not grads:
+        raise RuntimeError("clip_gradients: no tensors")
+    dev = grads[0].device
+    if dev.type != "cuda":
+        raise RuntimeError(f"gradients must be GPU tensors, got {dev}")
+    if outs is not None and len(outs) != len(grads):
+        raise RuntimeError(f"{len(grads)} gradients, but {len(outs)} outputs")
+    into = grads if outs is None else outs
+    back = []       # (tensor, contiguous copy of its result)
+    src, dst = [], []
+    for i, (g, o) in enumerate(zip(grads, into)):
+        if g.device != dev or g.layout != torch.strided or g.dtype not in _FEAT_DTYPES:
+            raise RuntimeError(f"gradient {i} must be float32 or bfloat16 on {dev}, got {g.dtype} ({g.layout}) on {g.device}")
+        if o is not g:
+            if o.device != dev or o.layout != torch.strided or o.dtype not in _FEAT_DTYPES or o.shape != g.shape:
+                raise RuntimeError(f"output {i} must be float32 or bfloat16 {tuple(g.shape)} on {dev}, got {o.dtype} "
+                                   f"{tuple(o.shape)} ({o.layout}) on {o.device}")
+            if not (g.is_contiguous() and o.is_contiguous()):
+                if g.stride() != o.stride() or not _dense(g):
+                    g = g.contiguous()
+                    if not o.is_contiguous():
+                        back.append((o, torch.empty(o.shape, dtype=o.dtype, device=dev)))
+                        o = back[-1][1]
+        elif not _dense(g):
+            back.append((g, g.contiguous()))
+            g = o = back[-1][1]
+        src.append(g)
+        dst.append(o)
+    with _OnDevice(dev):
+        n = len(src)
+        numels = array.array("q", [g.numel() for g in src])
+        gp = array.array("Q", [g.data_ptr() for g in src])
+        gd = array.array("i", [_FEAT_DTYPES[g.dtype] for g in src])
+        op, od = (gp, gd) if outs is None else (array.array("Q", [o.data_ptr() for o in dst]),
+                                                array.array("i", [_FEAT_DTYPES[o.dtype] for o in dst]))
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        nws = _workspace_bytes("g2v_clip_gradients_workspace", n)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        rc = lib.g2v_clip_gradients(n, gp.buffer_info()[0], gd.buffer_info()[0], op.buffer_info()[0], od.buffer_info()[0],
+                                    numels.buffer_info()[0], float(max_norm), norm.data_ptr(), ws.data_ptr(), nws, _stream_of(dev))
+        if rc:
+            _lib.check(rc, "clip_gradients")
+        for t, result in back:
+            t.copy_(result)
+    torch.autograd.graph.increment_version(into)
+    return norm

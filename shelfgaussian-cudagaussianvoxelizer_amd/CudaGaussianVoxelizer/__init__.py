@@ -13,11 +13,14 @@ from . import _C
 from ._C import gaussian_voxelizer_forward, gaussian_voxelizer_backward
 from ._C import CudaFeatsCosinelossForward, CudaFeatsCosinelossBackward, gaussian_voxelizer_forward_batched
 from .attention import PyGaussianAttention, gaussian_attention, qk_norm_rotary, rotary_frequencies
+from .clip import clip_grad_norm_
+from .norm import PyLayerNorm, layer_norm
 
 __all__ = ["PyCudaGaussianVoxelizer", "PyCudaFeatsCosineLoss", "PyCudaGaussianVoxelizerCosineLoss", "_C",
            "gaussian_voxelizer_forward", "gaussian_voxelizer_backward", "gaussian_voxelizer_forward_batched",
            "CudaFeatsCosinelossForward", "CudaFeatsCosinelossBackward", "covariance_from_scale_rotation",
-           "PyGaussianAttention", "gaussian_attention", "qk_norm_rotary", "rotary_frequencies"]
+           "PyGaussianAttention", "gaussian_attention", "qk_norm_rotary", "rotary_frequencies", "PyLayerNorm", "layer_norm",
+           "clip_grad_norm_"]
 
 
 def _wants_backward(ctx, need_backward):

@@ -85,6 +85,11 @@ SIGNATURES = {
     "g2v_window_attention_backward_workspace": (_sz, [_i] * 12),
     "g2v_window_attention_backward": (_i, [_i] * 6 + [_vp, _llp, _vp, _llp, _vp, _llp, _i, _vp, _i, _i, _i, ctypes.c_float, _vp,
                                                       _vp, _vp, _vp, _llp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "g2v_layer_norm_forward": (_i, [_i, _i, _i, _vp, _llp, _vp, _llp, _i, _vp, _vp, _i, ctypes.c_float, _vp, _vp, _vp, _vp]),
+    "g2v_layer_norm_backward_workspace": (_sz, [_i] * 4),
+    "g2v_layer_norm_backward": (_i, [_i, _i, _i, _vp, _llp, _i, _vp, _i, _vp, _vp, _llp, _vp, _llp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "g2v_clip_gradients_workspace": (_sz, [_i]),
+    "g2v_clip_gradients": (_i, [_i, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _sz, _vp]),
     "g2v_profile_enable": (_i, [_i]),
     "g2v_profile_reset": (_i, []),
     "g2v_profile_collect": (_i, []),

@@ -24,7 +24,7 @@ def _tangents(*tensors):
 def _differentiated(*tensors):
     """Whether a derivative in either mode is asked for: the call then goes through its autograd.Function, which has the
     backward and refuses tangents.  Others save its bookkeeping."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _tangents(*tensors)
+    return (torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)) or _tangents(*tensors)
 
 
 class _QkNormRotaryFunction(torch.autograd.Function):

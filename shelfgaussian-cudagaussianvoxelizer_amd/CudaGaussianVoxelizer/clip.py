@@ -1,0 +1,41 @@
+"""The norm of a training step's gradients and their clipping.  No counterpart in the reference, which leaves training to its
+caller; the kernels live in libg2v_hip.so and are reached through ``_C`` on the caller's current stream.
+"""
+import torch
+
+from . import _C
+
+__all__ = ["clip_grad_norm_"]
+
+
+@torch.no_grad()
+def clip_grad_norm_(tensors, max_norm, *, out=None):
+    """Scales gradients by min(1, max_norm / (norm + 1e-6)), norm the 2-norm of all of them taken together, and returns the norm, a
+    0-dim float32 GPU tensor (nothing waits for it).
+
+    tensors: parameters (a module's ``parameters()``), whose .grad is clipped and which are skipped where they have none, or
+    gradients themselves, tensors that require no gradient.  float32 and bfloat16 may be mixed, on one GPU; one tensor may come alone.
+    A tensor must not be there twice, nor two that share memory.  In place; with ``out``, a list of as many float32 or bfloat16 tensors of
+    the same shapes, the scaled gradients go there and the gradients stay (the float32 gradients of an optimizer's main weights from
+    a bfloat16 layer's).  Squares are summed in 64 bits: the norm is finite where float32 holds it.  NaN or infinite
+    gradients give a norm that is, and outputs as the formula says: nothing is skipped.  Two launches for up to 120 tensors, two more for
+    every 120; they may be captured into a graph, which keeps the tensors' addresses."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not all(isinstance(t, torch.Tensor) for t in tensors):
+        raise RuntimeError("tensors must be parameters or gradients")
+    if not float(max_norm) >= 0.0:
+        raise RuntimeError(f"max_norm must not be negative, got {max_norm}")
+    if out is not None:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(out) != len(tensors) or not all(isinstance(t, torch.Tensor) for t in out):
+            raise RuntimeError(f"out must hold {len(tensors)} tensors")
+    grads, into = [], []
+    for i, t in enumerate(tensors):
+        g = t.grad if t.requires_grad else t
+        if g is not None:
+            grads.append(g)
+            if out is not None:
+                into.append(out[i])
+    if not grads:    # nothing to clip
+        return torch.zeros((), device=tensors[0].device if tensors else "cuda")
+    return _C.clip_gradients(grads, max_norm, None if out is None else into)

@@ -268,6 +268,45 @@ hipError_t launch_qk_norm_rotary(const QkNormArgs& a, int dtype, hipStream_t s);
 size_t qk_norm_bwd_workspace(const QkNormArgs& a, int dtype);
 hipError_t launch_qk_norm_rotary_bwd(const QkNormArgs& a, int dtype, void* ws, hipStream_t s);
 
+// ---- layer norm (g2v_layernorm.hip) ----------------------------------------------------------
+// Rows (batch, n, dim): inputs at element strides sb, sn, outputs contiguous.
+struct LayerNormArgs {
+    int64_t rows;                  // batch n
+    int n, dim;
+    const void* in[3];             // forward: x, residual (or null); backward: x (or the sum), dy, ds (or null)
+    int64_t sb[3], sn[3];
+    const void *w, *b;             // (dim) float32 or bfloat16 (wbf16), null: ones, zeros
+    int wbf16;
+    float eps;
+    void* y;                       // backward: dx
+    void* sum;                     // x + residual
+    float* stats;                  // (rows, 2) mean and (variance + eps)^-1/2; forward: null where no backward follows
+    void *dw, *db;                 // (dim) of the weights' type, null: not wanted
+    // set by the launches
+    int shift;
+    float* part;
+};
+hipError_t launch_layer_norm(const LayerNormArgs& a, int dtype, hipStream_t s);
+size_t layer_norm_bwd_workspace(int64_t rows, int dim, int dtype);
+hipError_t launch_layer_norm_bwd(const LayerNormArgs& a, int dtype, void* ws, hipStream_t s);
+
+// ---- gradient norm and clipping (g2v_clip.hip) ------------------------------------------------
+// A launch's tensors, as kernel arguments.
+constexpr int kClipTensors = 120;
+struct ClipArgs {
+    int count, chunks;
+    int64_t chunk;                       // elements of a chunk
+    const void* g[kClipTensors];
+    void* out[kClipTensors];
+    int64_t n[kClipTensors];
+    int start[kClipTensors];             // a tensor's first chunk
+    unsigned char bf16[kClipTensors];    // 1: of g, 2: of out
+};
+static_assert(sizeof(ClipArgs) <= 4000, "kernel arguments are 4 KB");
+size_t clip_workspace(int64_t count);
+hipError_t launch_clip(int64_t count, const void* const* g, void* const* out, const int64_t* numels, const int* g_bf16,
+                       const int* out_bf16, float max_norm, float* norm, void* ws, hipStream_t s);
+
 // ---- attention (g2v_attention_fwd.hip, g2v_attention_bwd.hip) -------------------------------
 struct AttnFwd;
 struct AttnBwd;

@@ -18,6 +18,7 @@
 // to the token (its angles, the sum of their gradients over its heads) stays in registers.
 #include "../../include/g2v.h"
 #include "g2v_internal.h"
+#include "g2v_rows.h"
 
 namespace g2v {
 namespace {
@@ -25,87 +26,6 @@ namespace {
 constexpr int kQnThreads = 256;
 constexpr int kQnUnroll = 4;       // rows whose loads a thread has in flight, forward
 constexpr int kQnAhead = 1;        // the same, backward (two tensors), the next loaded while one is computed
-
-template <typename T>
-struct QnVec;
-template <>
-struct QnVec<float> {
-    static constexpr int n = 4;
-    typedef f32x4 raw;
-};
-template <>
-struct QnVec<__bf16> {
-    static constexpr int n = 8;
-    typedef bf16x8 raw;
-};
-
-// Elements [d, d + n) of a row, zero past the end.  AL: rows and D are whole 16-byte vectors; else a vector within the row
-// is still one access (global memory takes any alignment), and only the row's last elements go one by one.
-template <typename T, bool AL>
-__device__ __forceinline__ typename QnVec<T>::raw qn_load(const T* row, int d, int D) {
-    typedef typename QnVec<T>::raw raw;
-    typedef raw raw_any __attribute__((aligned(sizeof(T))));
-    raw v;
-#pragma unroll
-    for (int j = 0; j < QnVec<T>::n; ++j) v[j] = (T)0.0f;
-    if constexpr (AL) {
-        if (d < D) v = *reinterpret_cast<const raw*>(row + d);
-    } else if (d + QnVec<T>::n <= D) {
-        v = *reinterpret_cast<const raw_any*>(row + d);
-    } else {
-#pragma unroll
-        for (int j = 0; j < QnVec<T>::n; ++j)
-            if (d + j < D) v[j] = row[d + j];
-    }
-    return v;
-}
-template <typename T, bool AL>
-__device__ __forceinline__ void qn_store(T* row, int d, int D, const float (&o)[QnVec<T>::n]) {
-    constexpr int n = QnVec<T>::n;
-    typedef typename QnVec<T>::raw raw;
-    typedef raw raw_any __attribute__((aligned(sizeof(T))));
-    raw v;
-#pragma unroll
-    for (int j = 0; j < n; ++j) v[j] = (T)o[j];
-    if constexpr (AL) {
-        if (d < D) *reinterpret_cast<raw*>(row + d) = v;
-    } else if (d + n <= D) {
-        *reinterpret_cast<raw_any*>(row + d) = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < n; ++j)
-            if (d + j < D) row[d + j] = v[j];
-    }
-}
-
-// Sums over the 2^shift lanes of a row.  Within 16 lanes by data-parallel moves: after the steps before it every
-// lane of a mirrored half holds the same sum, so a mirror serves as the exchange of the next size.
-template <int kCtrl>
-__device__ __forceinline__ float dpp_add(float v) {
-    const int o = __builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xF, 0xF, true);
-    return v + __int_as_float(o);
-}
-template <int M>
-__device__ __forceinline__ void row_sums(float (&v)[M], int shift) {
-    if (shift > 0)    // quad_perm 1 0 3 2
-#pragma unroll
-        for (int m = 0; m < M; ++m) v[m] = dpp_add<0xB1>(v[m]);
-    if (shift > 1)    // quad_perm 2 3 0 1
-#pragma unroll
-        for (int m = 0; m < M; ++m) v[m] = dpp_add<0x4E>(v[m]);
-    if (shift > 2)    // row_half_mirror
-#pragma unroll
-        for (int m = 0; m < M; ++m) v[m] = dpp_add<0x141>(v[m]);
-    if (shift > 3)    // row_mirror
-#pragma unroll
-        for (int m = 0; m < M; ++m) v[m] = dpp_add<0x140>(v[m]);
-    if (shift > 4)
-#pragma unroll
-        for (int m = 0; m < M; ++m) v[m] += __shfl_xor(v[m], 16);
-    if (shift > 5)
-#pragma unroll
-        for (int m = 0; m < M; ++m) v[m] += __shfl_xor(v[m], 32);
-}
 
 // A workgroup's side of the problem: queries, keys, or both when they share positions.
 struct QnSide {
@@ -175,7 +95,7 @@ __device__ __forceinline__ QnPlace qn_place(const QkNormArgs& a) {
 
 template <typename T, bool AL>
 __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
-    constexpr int N = QnVec<T>::n;
+    constexpr int N = RowVec<T>::n;
     __shared__ float2 rot[kQnThreads * (N / 2)];
     const int side = blockIdx.x >= a.blocks0;
     const QnSide p = qn_side(a, side);
@@ -192,12 +112,12 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
     qn_angles<N>(a, p.pos, p.tokens, t0, o.token, o.d, rot, f);
     const float inv_d = 1.0f / (float)a.dim;
     for (int h0 = p.h0 + o.first; h0 < p.h1; h0 += o.step * kQnUnroll) {
-        typename QnVec<T>::raw x[kQnUnroll];
+        typename RowVec<T>::raw x[kQnUnroll];
 #pragma unroll
         for (int u = 0; u < kQnUnroll; ++u) {
             const int h = h0 + u * o.step;
             const bool k = h >= a.heads[0];
-            if (h < p.h1) x[u] = qn_load<T, AL>(k ? xk + (h - a.heads[0]) * a.sh[1] : xq + h * a.sh[0], o.d, a.dim);
+            if (h < p.h1) x[u] = row_load<T, AL>(k ? xk + (h - a.heads[0]) * a.sh[1] : xq + h * a.sh[0], o.d, a.dim);
         }
 #pragma unroll
         for (int u = 0; u < kQnUnroll; ++u) {
@@ -222,7 +142,7 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
             }
             T* row = k ? static_cast<T*>(a.out[1]) + (t * a.heads[1] + h - a.heads[0]) * a.dim
                        : static_cast<T*>(a.out[0]) + (t * a.heads[0] + h) * a.dim;
-            if (live) qn_store<T, AL>(row, o.d, a.dim, y);
+            if (live) row_store<T, AL>(row, o.d, a.dim, y);
         }
     }
 }
@@ -234,7 +154,7 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary(QkNormArgs a) {
 // first rows are asked for before the angles.
 template <typename T, bool AL>
 __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a) {
-    constexpr int N = QnVec<T>::n;
+    constexpr int N = RowVec<T>::n;
     __shared__ float red[kQnThreads * N];
     float2* rot = reinterpret_cast<float2*>(red);
     __shared__ float dcell[kQnThreads * kQnAxes];
@@ -261,7 +181,7 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a)
         const T* x0 = static_cast<const T*>(a.x[k]) + b * a.sb[k] + i * a.sn[k];
         const T* g0 = static_cast<const T*>(a.g[k]) + b * a.gsb[k] + i * a.gsn[k];
         T* row = static_cast<T*>(a.dx[k]) + t * heads * a.dim;
-        typename QnVec<T>::raw xv[kQnAhead], gv[kQnAhead];
+        typename RowVec<T>::raw xv[kQnAhead], gv[kQnAhead];
         float dth[N / 2];
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) dth[j] = 0.0f;
@@ -269,8 +189,8 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a)
         for (int u = 0; u < kQnAhead; ++u) {
             const int h = o.first + u * o.step;
             if (h >= heads) break;
-            xv[u] = qn_load<T, AL>(x0 + h * sh, o.d, a.dim);
-            gv[u] = qn_load<T, AL>(g0 + h * gsh, o.d, a.dim);
+            xv[u] = row_load<T, AL>(x0 + h * sh, o.d, a.dim);
+            gv[u] = row_load<T, AL>(g0 + h * gsh, o.d, a.dim);
         }
         qn_angles<N>(a, pos, tokens, t0, o.token, o.d, rot, f);
         for (int h0 = o.first; h0 < heads; h0 += o.step * kQnAhead) {
@@ -287,8 +207,8 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a)
                 }
                 const int next = h + o.step * kQnAhead;
                 if (next < heads) {
-                    xv[u] = qn_load<T, AL>(x0 + next * sh, o.d, a.dim);
-                    gv[u] = qn_load<T, AL>(g0 + next * gsh, o.d, a.dim);
+                    xv[u] = row_load<T, AL>(x0 + next * sh, o.d, a.dim);
+                    gv[u] = row_load<T, AL>(g0 + next * gsh, o.d, a.dim);
                 }
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j) {
@@ -311,7 +231,7 @@ __global__ void __launch_bounds__(kQnThreads) k_qk_norm_rotary_bwd(QkNormArgs a)
                 }
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j) dth[j] += dy[2 * j + 1] * x[2 * j] - dy[2 * j] * x[2 * j + 1];
-                if (live) qn_store<T, AL>(row + (int64_t)h * a.dim, o.d, a.dim, dx);
+                if (live) row_store<T, AL>(row + (int64_t)h * a.dim, o.d, a.dim, dx);
             }
         }
         if (dpos) {   // of each of a token's groups, then of the token
@@ -392,7 +312,7 @@ __global__ void __launch_bounds__(kQnSumThreads) k_qk_norm_sums(QkNormArgs a, in
 
 template <typename T>
 bool qn_aligned(const QkNormArgs& a, bool backward) {
-    const int64_t n = QnVec<T>::n;
+    const int64_t n = RowVec<T>::n;
     bool ok = a.dim % n == 0;
     auto row = [&](const void* p, const int64_t* s) {
         if (!p) return;
