@@ -9,6 +9,7 @@ from __future__ import annotations
 import array
 import ctypes
 import functools
+import operator
 
 import torch
 
@@ -1245,6 +1246,28 @@ def _dense(t):
     return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
 
 
+def _clip_checked(grads, outs, dev):
+    """(gradients, outputs, results to copy back) as flat memory: tensors of other layouts go through contiguous copies."""
+    src, dst, back = [], [], []
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        for t, what in ((g, "gradient"), (o, "output")):
+            if t.device != dev or t.layout != torch.strided or t.dtype not in _FEAT_DTYPES or t.shape != g.shape:
+                raise RuntimeError(f"{what} {i} must be float32 or bfloat16 {tuple(g.shape)} on {dev}, got {t.dtype} "
+                                   f"{tuple(t.shape)} ({t.layout}) on {t.device}")
+        if not (g.stride() == o.stride() and _dense(g)):
+            same = o is g
+            g = g.contiguous()
+            if same or not o.is_contiguous():
+                back.append((o, g if same else torch.empty(o.shape, dtype=o.dtype, device=dev)))
+                o = back[-1][1]
+        src.append(g)
+        dst.append(o)
+    return src, dst, back
+
+
+_tensor_dtype, _tensor_shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
+
+
 def clip_gradients(grads, max_norm, outs=None):
     """The norm (a 0-dim float32 GPU tensor) of a list of gradient tensors taken together, float32 or bfloat16 on one GPU; each is
     scaled by min(1, max_norm / (norm + 1e-6)), in place or into outs, tensors of the same shapes (float32 or bfloat16)."""
@@ -1257,33 +1280,26 @@ def clip_gradients(grads, max_norm, outs=None):
     if outs is not None and len(outs) != len(grads):
         raise RuntimeError(f"{len(grads)} gradients, but {len(outs)} outputs")
     into = grads if outs is None else outs
-    back = []       # (tensor, contiguous copy of its result)
-    src, dst = [], []
-    for i, (g, o) in enumerate(zip(grads, into)):
-        if g.device != dev or g.layout != torch.strided or g.dtype not in _FEAT_DTYPES:
-            raise RuntimeError(f"gradient {i} must be float32 or bfloat16 on {dev}, got {g.dtype} ({g.layout}) on {g.device}")
-        if o is not g:
-            if o.device != dev or o.layout != torch.strided or o.dtype not in _FEAT_DTYPES or o.shape != g.shape:
-                raise RuntimeError(f"output {i} must be float32 or bfloat16 {tuple(g.shape)} on {dev}, got {o.dtype} "
-                                   f"{tuple(o.shape)} ({o.layout}) on {o.device}")
-            if not (g.is_contiguous() and o.is_contiguous()):
-                if g.stride() != o.stride() or not _dense(g):
-                    g = g.contiguous()
-                    if not o.is_contiguous():
-                        back.append((o, torch.empty(o.shape, dtype=o.dtype, device=dev)))
-                        o = back[-1][1]
-        elif not _dense(g):
-            back.append((g, g.contiguous()))
-            g = o = back[-1][1]
-        src.append(g)
-        dst.append(o)
+    # a model's hundreds of tensors are looked over by a few passes, half a microsecond each; whatever is out of line is named by
+    # the slower way
+    T, src, dst, back = torch.Tensor, grads, into, ()
+    kinds = set(map(_tensor_dtype, grads))
+    plain = set(map(T.get_device, grads)) == {dev.index} and all(map(T.is_contiguous, grads))
+    if plain and outs is not None:
+        kinds |= set(map(_tensor_dtype, outs))
+        plain = set(map(T.get_device, outs)) == {dev.index} and all(map(T.is_contiguous, outs)) \
+            and list(map(_tensor_shape, grads)) == list(map(_tensor_shape, outs))
+    if not (plain and kinds <= _FEAT_DTYPES.keys()):
+        src, dst, back = _clip_checked(grads, into, dev)
+
+    def arrays(tensors):
+        return (array.array("Q", map(T.data_ptr, tensors)), array.array("i", map(_FEAT_DTYPES.__getitem__, map(_tensor_dtype, tensors))))
+
     with _OnDevice(dev):
         n = len(src)
-        numels = array.array("q", [g.numel() for g in src])
-        gp = array.array("Q", [g.data_ptr() for g in src])
-        gd = array.array("i", [_FEAT_DTYPES[g.dtype] for g in src])
-        op, od = (gp, gd) if outs is None else (array.array("Q", [o.data_ptr() for o in dst]),
-                                                array.array("i", [_FEAT_DTYPES[o.dtype] for o in dst]))
+        numels = array.array("q", map(T.numel, src))
+        gp, gd = arrays(src)
+        op, od = (gp, gd) if dst is src else arrays(dst)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         nws = _workspace_bytes("g2v_clip_gradients_workspace", n)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev)

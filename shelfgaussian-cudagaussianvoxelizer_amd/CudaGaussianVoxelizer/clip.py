@@ -7,6 +7,8 @@ from . import _C
 
 __all__ = ["clip_grad_norm_"]
 
+_TYPES = {torch.Tensor, torch.nn.Parameter}
+
 
 @torch.no_grad()
 def clip_grad_norm_(tensors, max_norm, *, out=None):
@@ -21,7 +23,7 @@ def clip_grad_norm_(tensors, max_norm, *, out=None):
     gradients give a norm that is, and outputs as the formula says: nothing is skipped.  Two launches for up to 120 tensors, two more for
     every 120; they may be captured into a graph, which keeps the tensors' addresses."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not all(isinstance(t, torch.Tensor) for t in tensors):
+    if not set(map(type, tensors)) <= _TYPES and not all(isinstance(t, torch.Tensor) for t in tensors):
         raise RuntimeError("tensors must be parameters or gradients")
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"max_norm must not be negative, got {max_norm}")
@@ -29,13 +31,11 @@ def clip_grad_norm_(tensors, max_norm, *, out=None):
         out = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(out) != len(tensors) or not all(isinstance(t, torch.Tensor) for t in out):
             raise RuntimeError(f"out must hold {len(tensors)} tensors")
-    grads, into = [], []
-    for i, t in enumerate(tensors):
-        g = t.grad if t.requires_grad else t
-        if g is not None:
-            grads.append(g)
-            if out is not None:
-                into.append(out[i])
+    grads = [t.grad if t.requires_grad else t for t in tensors]
+    if any(g is None for g in grads):
+        if out is not None:
+            out = [o for o, g in zip(out, grads) if g is not None]
+        grads = [g for g in grads if g is not None]
     if not grads:    # nothing to clip
         return torch.zeros((), device=tensors[0].device if tensors else "cuda")
-    return _C.clip_gradients(grads, max_norm, None if out is None else into)
+    return _C.clip_gradients(grads, max_norm, out)

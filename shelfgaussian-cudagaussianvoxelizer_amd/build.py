@@ -18,7 +18,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "CudaGaussianVoxelizer", "libg2v_hip.so")
 SOURCES = ["g2v_csr.hip", "g2v_forward.hip", "g2v_backward.hip", "g2v_cosine.hip", "g2v_covariance.hip",
-           "g2v_qknorm.hip", "g2v_attention_fwd.hip", "g2v_attention_bwd.hip", "g2v_attention_window.hip",
+           "g2v_qknorm.hip", "g2v_attention_fwd.hip", "g2v_attention_bwd.hip", "g2v_attention_window_fwd.hip",
+           "g2v_attention_window_bwd.hip",
            "g2v_layernorm.hip", "g2v_clip.hip", "g2v_capi_training.hip", "g2v_capi_attention.hip", "g2v_capi.hip", "g2v_profile.hip"]
 ARCH = os.environ.get("G2V_OFFLOAD_ARCH", "gfx950")
 

@@ -268,6 +268,38 @@ __device__ __forceinline__ void store4(T* row, int d, int D, float x0, float x1,
     }
 }
 
+// A result's 32 values d0 .. d0 + 31 of a row, its registers of two lanes 32 apart (both here, or neither).  bfloat16 rows whose
+// 16-byte chunks are whole and aligned: the lanes exchange halves, so that each stores 16 bytes that lie together.
+template <typename T>
+__device__ __forceinline__ void store_block(T* row, int d0, int D, const float (&x)[16]) {
+    if constexpr (sizeof(T) == 2) {
+        if ((D & 7) == 0 && ((uintptr_t)row & 15) == 0) {
+#pragma unroll
+            for (int h = 0; h < 16; h += 8) {
+                uint32_t lo[2], hi[2];    // d0 + 2 h + 4 g .., and 8 further
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    lo[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)x[h + 2 * j], (__bf16)x[h + 2 * j + 1]});
+                    hi[j] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)x[h + 4 + 2 * j], (__bf16)x[h + 4 + 2 * j + 1]});
+                }
+                uint32_t v[4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const auto r = __builtin_amdgcn_permlane32_swap(lo[j], hi[j], false, false);
+                    v[j] = r[0];
+                    v[2 + j] = r[1];
+                }
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                const int d = d0 + 2 * h + 8 * ((threadIdx.x >> 5) & 1);
+                if (d < D) *reinterpret_cast<u32x4*>(row + d) = u32x4{v[0], v[1], v[2], v[3]};
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) store4<T>(row, d0 + reg_row(i), D, x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+
 // The same for what bfloat16 rounding leaves of the values.
 __device__ __forceinline__ float lost_by_rounding(float x) { return x - (float)(__bf16)x; }
 
@@ -410,7 +442,7 @@ __device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, f
 }
 }  // namespace attn
 
-// What a query sees of its scene's keys (g2v_attention_window.hip).  Query i stands at key place i + shift and sees key j if
+// What a query sees of its scene's keys (g2v_attention_window.h).  Query i stands at key place i + shift and sees key j if
 // j <= i + shift + right and (j >= i + shift - left or j < sinks), and bit j of the scene is set.  Rows of k and v in place skip
 // `gap` rows behind the sinks, which no query sees (those of the backward and packed ones skip none).
 struct AttnWindow {

@@ -1,0 +1,173 @@
+// Attention within a window: query i, at key place p = i + shift, sees the keys
+//
+//   [0, min(sinks, p + right + 1))  and  [p - left, p + right],
+//
+// those among them whose bit is set, and O, dQ, dK and dV are those of g2v_attention_fwd.hip and g2v_attention_bwd.hip over
+// these keys.  A wave's 32 or 64 rows see a range of keys little longer than a window, so a workgroup walks the tiles of the
+// sinks and then those of its rows' ranges, and a wave skips the tiles that none of its rows sees.  Where a tile lies inside
+// every row's range no score is looked at; at the range's ends a lane makes 32 bits of what its row sees of a block of 32 keys, and
+// an operation spreads one of them over a register (v_bfe) and another lets the score through or not (v_bfi).  Masked keys are
+// not packed away: the word of a tile's 64 valid keys is in a scalar register, their rows alone are loaded, and zeros stand in
+// the other rows' place, as what they hold may be NaN.
+//
+// For dK and dV keys are in the lanes and a key's queries are a range, too: p - right .. p + left, and for a sink all from
+// p - right on.  As that would have one workgroup walk all queries, the sinks' gradients are computed again by one-wave
+// workgroups that share out the queries, and joined.
+#pragma once
+#include "g2v_attention.h"
+
+namespace g2v {
+namespace attn {
+
+// Keys [lo, hi) that a query sees beside the sinks.
+struct KeyRange {
+    int lo, hi;
+};
+__device__ __forceinline__ KeyRange key_range(const AttnWindow& w, int nk, int tok) {
+    const int p = tok + w.shift;
+    KeyRange r;
+    r.hi = min(max(p + w.right + 1, 0), nk);
+    r.lo = min(max(p - w.left, 0), r.hi);
+    return r;
+}
+
+// The lowest x of 32 bits, none to all.
+__device__ __forceinline__ uint32_t bits_below(int x) { return (uint32_t)((1ull << min(max(x, 0), 32)) - 1); }
+// Bit j: whether a row sees key base + j.
+__device__ __forceinline__ uint32_t seen_bits(const KeyRange& r, int sinks, int base) {
+    return bits_below(r.hi - base) & (~bits_below(r.lo - base) | bits_below(sinks - base));
+}
+// Bit j of x in all bits.
+__device__ __forceinline__ uint32_t spread_bit(uint32_t x, int j) { return (uint32_t)((int32_t)(x << (31 - j)) >> 31); }
+// x where the mask's bits are set, else -inf; or else 0.
+__device__ __forceinline__ float or_lowest(uint32_t mask, float x) {
+    return __uint_as_float((mask & __float_as_uint(x)) | (~mask & 0xff800000u));
+}
+__device__ __forceinline__ float or_zero(uint32_t mask, float x) { return __uint_as_float(mask & __float_as_uint(x)); }
+
+// The tiles of KT keys that a workgroup's tokens [first, last] see: those of the sinks, then those of the ranges.
+template <int KT>
+struct KeyTiles {
+    int sinks, from, all;
+    __device__ __forceinline__ void init(const AttnWindow& w, int nk, int first, int last) {
+        const int hi = key_range(w, nk, last).hi, lo = key_range(w, nk, first).lo;
+        sinks = (min(w.sinks, hi) + KT - 1) / KT;
+        from = max(sinks, lo / KT);
+        all = sinks + max(0, (hi + KT - 1) / KT - from);
+    }
+    __device__ __forceinline__ int at(int u) const { return u < sinks ? u : from + u - sinks; }
+};
+
+// Which keys of a tile are valid, bit j for the tile's key j: all of them in the tiles of one range, by which most tiles are told;
+// else a lane holds the word of one of 64 units, so that the loop over the units reads no memory for them.
+template <int KT>
+struct TileWords {
+    static constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
+    int whole0, whole;    // the range's first tile and its number of tiles
+    uint64_t held;
+    int from;
+    __device__ __forceinline__ void init(const AttnWindow& w, int nk) {
+        // keys between the sinks and the first query's window are seen by no query; with a gap the sinks' rows lie elsewhere
+        const int unseen = w.shift - w.left;
+        whole0 = unseen > w.sinks || w.gap ? (max(unseen, w.sinks) + KT - 1) / KT : 0;
+        whole = w.bits ? 0 : max(0, nk / KT - whole0);
+        from = -64;
+    }
+    __device__ __forceinline__ bool all(int t) const { return (uint32_t)(t - whole0) < (uint32_t)whole; }
+    // The word of unit u, tile t, which is none of the range's.
+    __device__ __forceinline__ uint64_t at(const AttnWindow& w, const KeyTiles<KT>& tiles, int nk, int b, int u, int u1) {
+        if ((uint32_t)(u - from) >= 64u) {
+            from = u;
+            const int mine = u + (int)(threadIdx.x & 63);
+            held = 0;
+            if (mine < u1) {
+                const int t = tiles.at(mine), left = nk - t * KT, unseen = min(w.shift - w.left - t * KT, KT);
+                const int sinks = min(max(w.sinks - t * KT, 0), KT);
+                held = left >= KT ? kAll : (1ull << left) - 1;
+                if (unseen > sinks) held &= ~((unseen == 64 ? ~0ull : (1ull << unseen) - 1) & ~((1ull << sinks) - 1));
+                if (w.bits) {
+                    const uint64_t* row = w.bits + (int64_t)b * w.words;
+                    held &= KT == 64 ? row[t] : row[t >> 1] >> (32 * (t & 1));
+                }
+            }
+        }
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)held, u - from);
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(held >> 32), u - from);
+        return (uint64_t)hi << 32 | lo;
+    }
+};
+
+// A tile in LDS as Tile's ([plane][row][DP], swizzled), with less to do for each load: chunks past the rows' end repeat the last
+// one instead of being left out (the other operand is zero there, or the product's row is not stored), and offsets are kept.
+template <int NP, int DP, int ROWS, int NT>
+struct WinTile {
+    static constexpr int C = DP / 8;
+    static constexpr int kChunks = NP * ROWS * C;
+    static constexpr int kBytes = kChunks * 16;
+    static constexpr int kIter = (kChunks + NT - 1) / NT;
+    static constexpr int kLoads = kChunks % NT ? 0 : kIter;    // of every wave; 0: not the same for all
+
+    __device__ __forceinline__ static int row(int it) { return (it * NT + (int)threadIdx.x) % (ROWS * C) / C; }
+    __device__ __forceinline__ static bool on(int it) { return kChunks % NT == 0 || it < kIter - 1 || it * NT + (int)threadIdx.x < kChunks; }
+    // Byte offset of this thread's chunk in its row.
+    __device__ __forceinline__ static uint32_t chunk(int it, int chunks) {
+        const int L = it * NT + threadIdx.x, pl = L / (ROWS * C), c = swz<DP>(row(it), L % C);
+        return (uint32_t)(pl * C + min(c, chunks - 1)) * 16;
+    }
+    __device__ __forceinline__ static uint32_t dst(uint32_t lds, int it) {
+        return lds + it * NT * 16 + (uint32_t)g2v::uniform(threadIdx.x >> 6) * 1024;
+    }
+    uint32_t off[kIter];    // of its chunk from the tile's first row
+    __device__ __forceinline__ void init(const RowSrc& s) {
+#pragma unroll
+        for (int it = 0; it < kIter; ++it) off[it] = (uint32_t)row(it) * (uint32_t)s.sn + chunk(it, s.chunks);
+    }
+    // The rows from p on, all of them there.
+    __device__ __forceinline__ void load(const char* p, uint32_t lds) const {
+#pragma unroll
+        for (int it = 0; it < kIter; ++it)
+            if (on(it)) dma16(p, off[it], dst(lds, it));
+    }
+    // Rows j0 .. of base, those of the word's bits; zeros in the others' place, nothing where there are none.  Rows from `sinks` on
+    // are `gap` rows further.
+    __device__ __forceinline__ static void load_some(const RowSrc& s, const char* base, int j0, uint64_t word, int sinks, int gap, char* lds) {
+        if (word == 0) return;
+#pragma unroll
+        for (int it = 0; it < kIter; ++it) {
+            if (!on(it)) continue;
+            const int j = j0 + row(it);
+            if (word >> row(it) & 1) dma16(base + ((int64_t)j + (j >= sinks ? gap : 0)) * s.sn + chunk(it, s.chunks), dst(lds_off(lds), it));
+            else *reinterpret_cast<f32x4*>(lds + (it * NT + threadIdx.x) * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    // Rows j0 .. n - 1 of base, the last one repeated.
+    __device__ __forceinline__ static void load_tail(const RowSrc& s, const char* base, int j0, int n, uint32_t lds) {
+#pragma unroll
+        for (int it = 0; it < kIter; ++it)
+            if (on(it)) dma16(base + (int64_t)min(j0 + row(it), n - 1) * s.sn + chunk(it, s.chunks), dst(lds, it));
+    }
+};
+
+// A wave's rows: blocks of 32 keys of which any row sees one, and those that every row sees, as ranges of the blocks' first keys, for
+// the tiles of the sinks and for those behind them (the first may hold too many blocks, the second too few).
+struct WaveBlocks {
+    struct Range {
+        int at;
+        uint32_t n;
+        __device__ __forceinline__ bool has(int j) const { return (uint32_t)(j - at) < n; }
+    };
+    Range any, every, any_far, every_far;    // of the window; of the sinks' tiles
+    __device__ __forceinline__ void init(const AttnWindow& w, int nk, int group, int rows, int first, int count, int sinks_end) {
+        any = every = any_far = every_far = {0, 0u};
+        if (first >= rows) return;
+        const KeyRange a = key_range(w, nk, first / group), b = key_range(w, nk, (min(first + count, rows) - 1) / group);
+        const int lo0 = g2v::uniform(a.lo), lo1 = g2v::uniform(b.lo), hi0 = g2v::uniform(a.hi), hi1 = g2v::uniform(b.hi);
+        if (hi1 > lo0) any = {lo0 - 31, (uint32_t)(hi1 - lo0 + 31)};
+        if (hi0 - 31 > lo1) every = {lo1, (uint32_t)(hi0 - 31 - lo1)};
+        any_far = {0, (uint32_t)(lo0 < sinks_end ? hi1 : min(hi1, w.sinks))};
+        every_far = {0, (uint32_t)max(0, min(hi0, w.sinks) - 31)};
+    }
+};
+
+}  // namespace attn
+}  // namespace g2v

@@ -1,0 +1,514 @@
+// Attention within a window, backward (g2v_attention_window.h).
+#include <algorithm>
+
+#include "g2v_attention_window.h"
+
+namespace g2v {
+namespace {
+using namespace attn;
+
+#ifndef V_DQB64
+#define V_DQB64 1
+#endif
+#ifndef V_DQP64
+#define V_DQP64 3
+#endif
+constexpr int window_dq_per_cu(int np, int dp, int waves) {
+    return np == 1 && dp == 64 && waves > 1 ? V_DQP64 : dq_per_cu(np, dp, waves);
+}
+
+// As k_attn_dq.
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+__global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP, DP, NW))) k_window_dq(WinBwd a) {
+    constexpr int NS = NP == 1 ? 2 : NP;    // planes of dS, see k_attn_dq
+    constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
+    typedef WinTile<NP, DP, KT, NT> TileT;
+    typedef TileWords<KT> Words;
+    constexpr int kBuffers = buffers(window_dq_per_cu(NP, DP, NW), TileT::kBytes), kAhead = kBuffers - 1;
+    __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
+    static_assert(window_dq_per_cu(NP, DP, NW) * sizeof(lds) <= kLdsBytes, "planned by more workgroups than fit");
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
+    const int rows = a.group * a.nq, half = (threadIdx.x >> 5) & 1;
+    const int first = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32), r0 = first + (threadIdx.x & 31);
+    const int g0 = w.tile * (NW * NQB * 32), g1 = min(g0 + NW * NQB * 32, rows) - 1;
+    const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
+    const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
+    KeyTiles<KT> tiles;
+    tiles.init(a.win, a.nk, g2v::uniform(g0 / a.group), g2v::uniform(g1 / a.group));
+    int u0, u1;
+    split_range(tiles.all, w.split, w.splits, u0, u1);
+    WaveBlocks blocks;
+    blocks.init(a.win, a.nk, a.group, rows, first, NQB * 32, tiles.sinks * KT);
+
+    bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
+    KeyRange see[NQB];
+    float lse[NQB], delta[NQB];    // delta: negative, as it is stored, and times scale
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
+        const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
+        const char* qrow = a.q.p + w.b * a.q.sb + tok * a.q.sn + head * a.q.sh;
+        const char* grow = a.g.p + w.b * a.g.sb + tok * a.g.sn + head * a.g.sh;
+        see[b] = key_range(a.win, a.nk, tok);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl) {
+                q[b][ks][pl] = mem_frag<DP>(qrow, r < rows, a.q.chunks, pl, ks);
+                g[b][ks][pl] = mem_frag<DP>(grow, r < rows, a.g.chunks, pl, ks);
+            }
+        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
+        lse[b] = a.lse[at];
+        delta[b] = a.delta[at] * a.scale;
+    }
+
+    TileT ktile, vtile;
+    ktile.init(a.k);
+    vtile.init(a.v);
+    Frags<DP> frags;
+    frags.init(lds_off(lds));
+    Words words;
+    words.init(a.win, a.nk);
+    auto load = [&](int u, int buf) {
+        const int t = tiles.at(u), j0 = t * KT;
+        if (words.all(t)) {
+            ktile.load(kbase + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
+            vtile.load(vbase + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
+            return Words::kAll;
+        }
+        const uint64_t word = words.at(a.win, tiles, a.nk, w.b, u, u1);
+        TileT::load_some(a.k, kbase, j0, word, a.win.sinks, 0, lds[buf][0]);
+        TileT::load_some(a.v, vbase, j0, word, a.win.sinks, 0, lds[buf][1]);
+        return word;
+    };
+
+    f32x16 dq[DB][NQB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < NQB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
+    uint64_t word = 0, next = 0, after = 0;
+    if (u0 < u1) word = load(u0, 0);
+    if (kAhead > 1 && u0 + 1 < u1) next = load(u0 + 1, 1);
+    for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
+        next_tile<kBuffers, 2 * TileT::kLoads>(u + 1 < u1 && words.all(tiles.at(u + 1)));
+        after = 0;
+        if (u + kAhead < u1) {
+            const uint64_t x = load(u + kAhead, buf == 0 ? kBuffers - 1 : buf - 1);
+            if (kAhead > 1) after = x;
+            else next = x;
+        }
+        const uint32_t at = buf * 2 * TileT::kBytes;
+        const int j0 = tiles.at(u) * KT;
+        const bool far = u < tiles.sinks;
+        const WaveBlocks::Range some = far ? blocks.any_far : blocks.any, every = far ? blocks.every_far : blocks.every;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const uint32_t part = (uint32_t)(word >> (32 * kb));
+            const int jb = j0 + 32 * kb;
+            if (!some.has(jb) || !part) continue;
+            f32x16 s[NQB], dp[NQB];
+#pragma unroll
+            for (int b = 0; b < NQB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = dp[b][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 fk[NP], fv[NP];
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) {
+                    fk[pl] = frags.rows(at, pl * KT * DP * 2, kb, ks);
+                    fv[pl] = frags.rows(at, TileT::kBytes + pl * KT * DP * 2, kb, ks);
+                }
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) {
+                    s[b] = mma(fk, q[b][ks], s[b]);
+                    dp[b] = mma(fv, g[b][ks], dp[b]);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NQB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[b][i] = exp2_fast(fmaf(s[b][i], a.c, -lse[b])) * fmaf(dp[b][i], a.scale, delta[b]);   // scale dS
+            if (!every.has(jb) || part != ~0u) {
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) {
+                    const uint32_t x = (seen_bits(see[b], a.win.sinks, jb) & part) >> (4 * half);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][i] = or_zero(spread_bit(x, 8 * (i >> 2) + (i & 3)), s[b][i]);
+                }
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                bf16x8 p[NQB][NS];
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) to_operand(s[b], st, p[b]);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    bf16x8 f[NP];
+#pragma unroll
+                    for (int pl = 0; pl < NP; ++pl) f[pl] = frags.cols(at, pl * KT * DP * 2, kb, st, d);
+#pragma unroll
+                    for (int b = 0; b < NQB; ++b) dq[d][b] = mma(f, p[b], dq[d][b]);
+                }
+            }
+        }
+        word = next;
+        next = after;
+    }
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        const int r = r0 + 32 * b;
+        if (r >= rows) continue;
+        // one key: its probability is 1 whatever q is
+        const bool one = see[b].hi - see[b].lo + min(a.win.sinks, see[b].lo) < 2;
+        if (one)
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
+        if (w.splits > 1) {
+            const PartRow pr = part_row(a.parts, a.bhs, w.bh, rows, r);
+            float* out = a.part + (pr.at + w.split * pr.step) * DP;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4*>(out + 32 * d + reg_row(i)) =
+                        f32x4{dq[d][b][i], dq[d][b][i + 1], dq[d][b][i + 2], dq[d][b][i + 3]};
+            continue;
+        }
+        const int tok = r / a.group, head = w.h * a.group + r - tok * a.group;
+        T* row = static_cast<T*>(a.dq) + (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = dq[d][b][i];
+            store_block<T>(row, 32 * d, a.dim, x);
+        }
+    }
+}
+
+// The sinks' one-wave workgroups: as many to a CU as their tiles' LDS allows.
+#ifndef V_KVP
+#define V_KVP 2
+#endif
+constexpr int window_dkv_per_cu(int np, int ns, int dp, int nw) {
+    return nw > 1 && np == 1 && dp == 64 && ns == 2 ? V_KVP : nw > 1 ? dkv_per_cu(np, ns, dp) : np > 1 ? (dp > 96 ? 1 : dp > 32 ? 2 : 4) : dp > 64 ? 3 : dp > 32 ? 6 : 8;
+}
+constexpr int dkv_bound(int np, int ns, int dp, int nw) { return nw > 1 ? window_dkv_per_cu(np, ns, dp, nw) : np > 1 && dp > 32 ? 1 : 2; }
+
+// As k_attn_dkv: keys in the lanes, the queries that see any of the workgroup's keys pass by, head after head.
+template <int NP, int NS, int DP, int KS, int NW, int QT, typename T>
+__global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_dkv(WinBwd a) {
+    static_assert(NW == 1 || NW % 2 == 0, "waves in pairs load the statistics, or one does");
+#ifndef V_PP
+#define V_PP 1
+#endif
+    constexpr int NPP = NP > 1 ? NP : V_PP == 2 ? NS : 1;
+    constexpr int NT = NW * 64, QB = QT / 32, DB = DP / 32;
+    typedef WinTile<NP, DP, QT, NT> TileT;
+    constexpr int kBuffers = buffers(NW > 1 && window_dkv_per_cu(NP, NS, DP, NW) > 2 ? 3 : 2, TileT::kBytes), kAhead = kBuffers - 1;
+    constexpr int kStats = NW == 1 ? 2 : 1;    // loads of statistics a wave
+    __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
+    __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and -delta of the tile's rows
+    static_assert(window_dkv_per_cu(NP, NS, DP, NW) * (sizeof(lds) + sizeof(stat)) <= kLdsBytes, "planned by more workgroups than fit");
+    const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
+    const int wave = g2v::uniform(threadIdx.x >> 6), half = (threadIdx.x >> 5) & 1;
+    const int n = a.all_queries ? min(a.win.sinks, a.nk) : a.nk;
+    const int g0 = w.tile * (NW * 32), g1 = min(g0 + NW * 32, n) - 1;    // the workgroup's keys, the wave's and the lane's
+    const int first = g0 + wave * 32, last = min(first + 32, n) - 1, j = first + (threadIdx.x & 31);
+    auto from = [&](int key) { return min(max(key - a.win.right - a.win.shift, 0), a.nq); };    // queries [from, to) see a key
+    auto to = [&](int key) {
+        return a.all_queries ? a.nq : min(max(key + a.win.left - a.win.shift + 1, 0), a.nq);
+    };
+    const int q0 = g2v::uniform(from(g0)), q1 = g2v::uniform(to(g1));
+    const int tile0 = q0 / QT, per = q0 < q1 ? (q1 + QT - 1) / QT - tile0 : 0;     // tiles of a query head
+    int u0, u1;
+    split_range(per * a.group, w.split, w.splits, u0, u1);
+    const int k0 = from(j), k1 = to(j);
+    bool valid = j < n && k0 < k1;    // (rows that no query sees are not read either)
+    if (valid && a.win.bits) valid = a.win.bits[(int64_t)w.b * a.win.words + (j >> 6)] >> (j & 63) & 1;
+    // blocks of 32 queries of which any sees one of the wave's keys, and those that see all of them
+    WaveBlocks::Range any = {0, 0u}, every = {0, 0u};
+    if (__any(valid)) {
+        const int w0 = g2v::uniform(from(first)), w1 = g2v::uniform(to(last)), w2 = g2v::uniform(from(last)), w3 = g2v::uniform(to(first));
+        if (w1 > w0) any = {w0 - 31, (uint32_t)(w1 - w0 + 31)};
+        if (w3 - 31 > w2) every = {w2, (uint32_t)(w3 - 31 - w2)};
+    }
+    if (a.win.bits && !__syncthreads_or(valid)) u1 = u0;    // nothing to add up
+
+    bf16x8 k[KS][NP], v[KS][NP];
+    {
+        const char* krow = a.k.p + w.b * a.k.sb + w.h * a.k.sh + j * a.k.sn;
+        const char* vrow = a.v.p + w.b * a.v.sb + w.h * a.v.sh + j * a.v.sn;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl) {
+                k[ks][pl] = mem_frag<DP>(krow, valid, a.k.chunks, pl, ks);
+                v[ks][pl] = mem_frag<DP>(vrow, valid, a.v.chunks, pl, ks);
+            }
+    }
+
+    TileT qtile, gtile;
+    qtile.init(a.q);
+    gtile.init(a.g);
+    Frags<DP> frags;
+    frags.init(lds_off(lds));
+    // unit u is tile `at` of the head's `per` tiles; the loads' place and the products' step through them without a division
+    struct Place {
+        int head, at;
+    };
+    auto step = [&](Place& p) {
+        if (++p.at == per) {
+            p.at = 0;
+            ++p.head;
+        }
+    };
+    const int skip = per ? g2v::uniform(u0 / per) : 0;
+    Place here = {w.h * a.group + skip, u0 - skip * per}, there = here;
+    auto load = [&](int buf) {
+        const int t = tile0 + there.at, head = there.head;
+        const char* qbase = a.q.p + w.b * a.q.sb + head * a.q.sh;
+        const char* gbase = a.g.p + w.b * a.g.sb + head * a.g.sh;
+        if ((t + 1) * QT <= a.nq) {
+            qtile.load(qbase + (int64_t)t * QT * a.q.sn, lds_off(lds[buf][0]));
+            gtile.load(gbase + (int64_t)t * QT * a.g.sn, lds_off(lds[buf][1]));
+        } else {
+            TileT::load_tail(a.q, qbase, t * QT, a.nq, lds_off(lds[buf][0]));
+            TileT::load_tail(a.g, gbase, t * QT, a.nq, lds_off(lds[buf][1]));
+        }
+        step(there);
+        // rows past the end are there in the padded statistics: lse +inf makes their probabilities 0
+        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + t * QT;
+        const uint32_t lane = threadIdx.x & 63;
+        if constexpr (NW == 1) {
+            if (lane < QT) {
+                dma4(a.lse + at, lane * 4, lds_off(stat[buf][0]));
+                dma4(a.delta + at, lane * 4, lds_off(stat[buf][1]));
+            }
+        } else {    // even waves load lse and odd ones delta, each pair the same values: every wave has as many loads
+            if (lane < QT) dma4(((wave & 1) ? a.delta : a.lse) + at, lane * 4, lds_off(stat[buf][wave & 1]));
+        }
+    };
+
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.0f;
+    if (u0 < u1) load(0);
+    if (kAhead > 1 && u0 + 1 < u1) load(1);
+    for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
+        next_tile<kBuffers, TileT::kLoads ? 2 * TileT::kLoads + kStats : 0>(u + 1 < u1);
+        if (u + kAhead < u1) load(buf == 0 ? kBuffers - 1 : buf - 1);
+        const uint32_t at = buf * 2 * TileT::kBytes;
+        const int i0 = (tile0 + here.at) * QT;
+        step(here);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            const int ib = i0 + 32 * qb;
+            if (!any.has(ib)) continue;
+            const int g4 = 4 * half;
+            f32x16 s, dp;    // dP begins at -delta
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[buf][1][qb * 32 + 2 * i + g4]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[i + e] = 0.0f;
+                    dp[i + e] = de[e];
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 fq[NP], fg[NP];
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) {
+                    fq[pl] = frags.rows(at, pl * QT * DP * 2, qb, ks);
+                    fg[pl] = frags.rows(at, TileT::kBytes + pl * QT * DP * 2, qb, ks);
+                }
+                s = mma(fq, k[ks], s);
+                dp = mma(fg, v[ks], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[buf][0][qb * 32 + 2 * i + g4]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i + e] = exp2_fast(fmaf(s[i + e], a.c, -ls[e]));
+            }
+            if (!every.has(ib)) {
+                const uint32_t x = (bits_below(k1 - ib) & ~bits_below(k0 - ib)) >> g4;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = or_zero(spread_bit(x, 8 * (i >> 2) + (i & 3)), s[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                bf16x8 p[NPP], ds[NS];
+                to_operand(s, st, p);
+                to_operand(dp, st, ds);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    bf16x8 fg[NP], fq[NP];
+#pragma unroll
+                    for (int pl = 0; pl < NP; ++pl) {
+                        fg[pl] = frags.cols(at, TileT::kBytes + pl * QT * DP * 2, qb, st, d);
+                        fq[pl] = frags.cols(at, pl * QT * DP * 2, qb, st, d);
+                    }
+                    dv[d] = mma(fg, p, dv[d]);
+                    dk[d] = mma(fq, ds, dk[d]);
+                }
+            }
+        }
+    }
+    if (j >= n) return;
+    if (!valid) {    // a masked key's gradients are zero
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.0f;
+    }
+    if (w.splits > 1) {
+        const PartRow pr = part_row(a.parts, a.bhs, w.bh, n, j);
+        float* out = a.part + (pr.at + w.split * pr.step) * (2 * DP);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                *reinterpret_cast<f32x4*>(out + 32 * d + reg_row(i)) = f32x4{dk[d][i], dk[d][i + 1], dk[d][i + 2], dk[d][i + 3]};
+                *reinterpret_cast<f32x4*>(out + DP + 32 * d + reg_row(i)) =
+                    f32x4{dv[d][i], dv[d][i + 1], dv[d][i + 2], dv[d][i + 3]};
+            }
+        return;
+    }
+    const int64_t at = (((int64_t)w.b * a.nk + j) * a.hk + w.h) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+        float x[16], y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = dk[d][i] * a.scale;
+            y[i] = dv[d][i];
+        }
+        store_block<T>(static_cast<T*>(a.dk) + at, 32 * d, a.dim, x);
+        store_block<T>(static_cast<T*>(a.dv) + at, 32 * d, a.dim, y);
+    }
+}
+
+// Sums of the splits of the sinks' gradients, in a fixed order (k_attn_dkv_join's way, over the first n keys).
+template <int DP, typename T>
+__global__ void __launch_bounds__(256) k_window_sinks_join(WinBwd a, int n, int parts) {
+    constexpr int kLanes = DP / 2;    // dK, then dV
+    __shared__ float red[4][256];
+    const int per = 256 / (kLanes * parts), e = threadIdx.x / parts, d = e % kLanes * 4, at = blockIdx.x * per + e / kLanes;
+    const bool live = e / kLanes < per && at < a.bhs * n;
+    const int bh = live ? at / n : 0, j = live ? at - bh * n : 0, b = bh / a.hk;
+    const PartRow pr = part_row(a.parts, a.bhs, bh, n, j);
+    const f32x4 o = join_sum(a.part + pr.at * (2 * DP) + d, pr.step * (2 * DP), pr.splits, parts, live, red);
+    if (!live || threadIdx.x % parts) return;
+    const float f = d < DP ? a.scale : 1.0f;
+    T* row = static_cast<T*>(d < DP ? a.dk : a.dv) + (((int64_t)b * a.nk + j) * a.hk + bh % a.hk) * a.dim;
+    store4<T>(row, d < DP ? d : d - DP, a.dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+}
+
+template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+hipError_t dq_launch(const WinBwd& a, hipStream_t s) {
+    G2V_LAUNCH((k_window_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    return launch_attn_dq_join(a, NP > 1, DP, s);
+}
+template <int NP, int DP, int NQB, int KT, typename T>
+hipError_t dq_waves(const WinBwd& a, const AttnShape& g, hipStream_t s) {
+    const bool full = a.dim > DP - 16;
+    if constexpr (NP == 1)
+        if (g.waves == 1)
+            return full ? dq_launch<NP, DP, DP / 16, 1, 1, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, 1, 1, KT, T>(a, s);
+    return full ? dq_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
+}
+
+template <int NP, int NS, int DP, int NW, int QT, typename T>
+hipError_t dkv_launch(const WinBwd& a, hipStream_t s) {
+    const dim3 grid((unsigned)workgroups(a.parts, a.bhs)), block(NW * 64);
+    if (a.dim > DP - 16) G2V_LAUNCH((k_window_dkv<NP, NS, DP, DP / 16, NW, QT, T>), grid, block, 0, s, a);
+    else G2V_LAUNCH((k_window_dkv<NP, NS, DP, DP / 16 - 1, NW, QT, T>), grid, block, 0, s, a);
+    if (!a.all_queries) return launch_attn_dkv_join(a, NP > 1, DP, s);
+    const int n = std::min(a.win.sinks, a.nk);
+    if (a.parts.head_splits > 1) {
+        const int64_t rows = (int64_t)a.bhs * n;
+        const int parts = attn_join_parts(rows, DP / 2, a.parts.head_splits);
+        G2V_LAUNCH((k_window_sinks_join<DP, T>), dim3((unsigned)ceil_div(rows, 256 / (DP / 2 * parts))), dim3(256), 0, s, a, n, parts);
+    }
+    return hipGetLastError();
+}
+// QT: tile of the four-wave workgroups; the sinks' one-wave ones take 32 rows.
+template <int DP, int QT, typename T>
+hipError_t dkv_planes(const WinBwd& a, int planes, hipStream_t s) {
+    if constexpr (sizeof(T) == 4) {
+        return a.all_queries ? dkv_launch<3, 3, DP, 1, 32, T>(a, s) : dkv_launch<3, 3, DP, 4, QT, T>(a, s);
+    } else {
+        if (planes == 2) return a.all_queries ? dkv_launch<1, 2, DP, 1, 32, T>(a, s) : dkv_launch<1, 2, DP, 4, QT, T>(a, s);
+        return a.all_queries ? dkv_launch<1, 1, DP, 1, 32, T>(a, s) : dkv_launch<1, 1, DP, 4, QT, T>(a, s);
+    }
+}
+
+}  // namespace
+
+AttnShape window_dq_shape(bool f32, int dp, int64_t rows) {
+    AttnShape g = attn_dq_shape(f32, dp, rows);
+    g.per_cu = window_dq_per_cu(f32 ? 3 : 1, dp, g.waves);
+    if (!f32 && dp == 64 && g.waves > 1) g.blocks = V_DQB64;
+    return g;
+}
+AttnShape window_dkv_shape(bool f32, int dp, int planes, bool all_queries) {
+    AttnShape g = attn_dkv_shape(f32, dp, planes);
+    g.per_cu = window_dkv_per_cu(f32 ? 3 : 1, planes, dp, g.waves);
+    if (all_queries) {
+        g.waves = 1;
+        g.tile = 32;
+        g.per_cu = window_dkv_per_cu(f32 ? 3 : 1, planes, dp, 1);
+    }
+    return g;
+}
+
+hipError_t launch_window_dq(const WinBwd& a, bool f32, int dp, hipStream_t s) {
+    const AttnShape g = window_dq_shape(f32, dp, (int64_t)a.group * a.nq);
+    if (f32) {
+        switch (dp) {
+            case 32: return dq_waves<3, 32, 1, 64, float>(a, g, s);
+            case 64: return dq_waves<3, 64, 1, 32, float>(a, g, s);
+            case 96: return dq_waves<3, 96, 1, 32, float>(a, g, s);
+            default: return dq_waves<3, 128, 1, 32, float>(a, g, s);
+        }
+    }
+    switch (dp) {
+        case 32: return dq_waves<1, 32, 2, 64, __bf16>(a, g, s);
+        case 64: return dq_waves<1, 64, V_DQB64, 64, __bf16>(a, g, s);
+        case 96: return dq_waves<1, 96, 1, 64, __bf16>(a, g, s);
+        default: return dq_waves<1, 128, 1, 64, __bf16>(a, g, s);
+    }
+}
+
+hipError_t launch_window_dkv(const WinBwd& a, bool f32, int dp, int planes, hipStream_t s) {
+    if (f32) {
+        switch (dp) {
+            case 32: return dkv_planes<32, 64, float>(a, planes, s);
+            case 64: return dkv_planes<64, 32, float>(a, planes, s);
+            case 96: return dkv_planes<96, 32, float>(a, planes, s);
+            default: return dkv_planes<128, 32, float>(a, planes, s);
+        }
+    }
+    switch (dp) {
+        case 32: return dkv_planes<32, 64, __bf16>(a, planes, s);
+        case 64: return dkv_planes<64, 64, __bf16>(a, planes, s);
+        case 96: return dkv_planes<96, 64, __bf16>(a, planes, s);
+        default: return dkv_planes<128, 32, __bf16>(a, planes, s);
+    }
+}
+
+}  // namespace g2v

@@ -16,7 +16,10 @@ namespace g2v {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr int kClipParts = 1024;     // most workgroups of a launch of the norm: partial sums that every scaling workgroup adds
+// Most workgroups of a launch of the norm: partial sums that every scaling workgroup adds.  12 layers of 1024 channels, 302 MB of
+// bfloat16 gradients: the norm takes 112, 100, 89 and 91 us with 512, 1024, 2048 and 4096 (3.4 TB/s), writing 604 MB of float32
+// 221, 198, 184 and 187 (4.9 TB/s).
+constexpr int kClipParts = 2048;
 
 // As many elements of a row of memory as 16 bytes hold.
 template <typename T>
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(kClipThreads) k_clip_scale(ClipArgs a, const d
     const double q = (double)max_norm / (n + 1e-6);
     const double c = q > 1.0 ? 1.0 : q;     // NaN stays
     for (int i = blockIdx.x; i < a.chunks; i += gridDim.x) {
-        const ClipAt at = clip_at(a, i);
+        const ClipAt at = clip_at(a, a.chunks - 1 - i);    // the last ones read are the likeliest in the cache
         const void* g = a.g[at.k];
         void* out = a.out[at.k];
         if (c == 1.0 && g == out) continue;     // in place and of one type
@@ -184,7 +187,7 @@ hipError_t launch_clip(int64_t count, const void* const* g, void* const* out, co
         if (blocks > 0) G2V_LAUNCH(k_clip_norm, dim3(blocks), dim3(kClipThreads), 0, s, a, part + parts);
         parts += blocks;
     }
-    for (int64_t l = 0; l < launches; ++l) {
+    for (int64_t l = launches - 1; l >= 0; --l) {
         fill(l);
         if (l > 0 && a.chunks == 0) continue;
         G2V_LAUNCH(k_clip_scale, dim3(std::max(1, a.chunks)), dim3(kClipThreads), 0, s, a, part, parts, max_norm,

@@ -361,7 +361,7 @@ hipError_t launch_attn_join(const AttnFwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_attn_dq_join(const AttnBwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_attn_dkv_join(const AttnBwd& a, bool f32, int dp, hipStream_t s);
 
-// ---- attention within a window (g2v_attention_window.hip) -----------------------------------
+// ---- attention within a window (g2v_attention_window_fwd.hip, g2v_attention_window_bwd.hip) -----------------------------------
 struct WinFwd;
 struct WinBwd;
 // Bits of the valid keys of each scene, 64 keys a word, by mask (batch, nk + gap); key j of the words is key j + gap of the mask
