@@ -1041,22 +1041,21 @@ def attention_backward(grad_out, q, k, v, out, rest, lse, key_list=None, scale=N
 
 # ---- attention within a window ----------------------------------------------------------------------
 
-def _window_side(side, name):
-    """A side of a window as the library takes it: places, -1 without a bound."""
-    if side is None:
-        return -1
-    if isinstance(side, bool) or not isinstance(side, int) or side < 0:
-        raise RuntimeError(f"window: {name} must be a number of places or None, got {side!r}")
-    return min(side, 1 << 30)
+@functools.lru_cache(maxsize=256, typed=True)
+def _window_bounds(left, right, sinks):
+    """(left, right, sinks) as the library takes them: places, -1 without a bound."""
+    for side, name in ((left, "left"), (right, "right")):
+        if side is not None and (isinstance(side, bool) or not isinstance(side, int) or side < 0):
+            raise RuntimeError(f"window: {name} must be a number of places or None, got {side!r}")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise RuntimeError(f"sinks must be a number of keys, got {sinks!r}")
+    return tuple(-1 if side is None else min(side, 1 << 30) for side in (left, right)) + (min(sinks, 1 << 30),)
 
 
 def _window(window, sinks):
-    """(left, right, sinks) as the library takes them."""
     if not isinstance(window, (tuple, list)) or len(window) != 2:
         raise RuntimeError(f"window must be (left, right), got {window!r}")
-    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
-        raise RuntimeError(f"sinks must be a number of keys, got {sinks!r}")
-    return _window_side(window[0], "left"), _window_side(window[1], "right"), min(sinks, 1 << 30)
+    return _window_bounds(window[0], window[1], sinks)
 
 
 def _window_attention_forward(inputs, call, window, for_backward):

@@ -443,12 +443,11 @@ __device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, f
 }  // namespace attn
 
 // What a query sees of its scene's keys (g2v_attention_window.h).  Query i stands at key place i + shift and sees key j if
-// j <= i + shift + right and (j >= i + shift - left or j < sinks), and bit j of the scene is set.  Rows of k and v in place skip
-// `gap` rows behind the sinks, which no query sees (those of the backward and packed ones skip none).
+// j <= i + shift + right and (j >= i + shift - left or j < sinks), and the mask keeps it.  Behind the sinks the mask's bytes skip `gap` keys
+// that no query sees, and the rows of k and v `skip` (where they are packed without these keys, none).
 struct AttnWindow {
-    int left, right, sinks, shift, gap;
-    const uint64_t* bits;   // (batch, words), null: all keys are valid
-    int words;
+    int left, right, sinks, shift, gap, skip;
+    const unsigned char* mask;    // (batch, nk + gap), null: all keys are valid
 };
 struct WinFwd : AttnFwd {
     AttnWindow win;

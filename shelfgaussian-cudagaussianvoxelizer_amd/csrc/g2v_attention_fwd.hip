@@ -341,8 +341,8 @@ __global__ void __launch_bounds__(256) k_attn_pack(AttnPack a) {
     if (!have) return;
     bool zero = false;
     if (a.keys[k]) {
-        if (a.bits) zero = !(a.bits[b * a.words + (i >> 6)] >> (i & 63) & 1);
         if (a.gap && i >= a.sinks) i += a.gap;
+        if (a.valid) zero = !a.valid[b * (a.n[k] + a.gap) + i];
     }
     const T* src = static_cast<const T*>(a.src[k]) + b * a.sb[k] + i * a.sn[k] + bh % a.heads[k] * a.sh[k];
     const int64_t row = bh * a.n[k] + slot;

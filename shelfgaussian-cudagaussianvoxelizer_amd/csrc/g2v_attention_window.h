@@ -2,7 +2,7 @@
 //
 //   [0, min(sinks, p + right + 1))  and  [p - left, p + right],
 //
-// those among them whose bit is set, and O, dQ, dK and dV are those of g2v_attention_fwd.hip and g2v_attention_bwd.hip over
+// those among them that the mask keeps, and O, dQ, dK and dV are those of g2v_attention_fwd.hip and g2v_attention_bwd.hip over
 // these keys.  A wave's 32 or 64 rows see a range of keys little longer than a window, so a workgroup walks the tiles of the
 // sinks and then those of its rows' ranges, and a wave skips the tiles that none of its rows sees.  Where a tile lies inside
 // every row's range no score is looked at; at the range's ends a lane makes 32 bits of what its row sees of a block of 32 keys, and
@@ -59,7 +59,8 @@ struct KeyTiles {
 };
 
 // Which keys of a tile are valid, bit j for the tile's key j: all of them in the tiles of one range, by which most tiles are told;
-// else a lane holds the word of one of 64 units, so that the loop over the units reads no memory for them.
+// else a lane holds the word of one of 64 units, made from the
+// mask's bytes, so that the loop over the units reads no memory for them and no kernel before it makes them.
 template <int KT>
 struct TileWords {
     static constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
@@ -67,13 +68,32 @@ struct TileWords {
     uint64_t held;
     int from;
     __device__ __forceinline__ void init(const AttnWindow& w, int nk) {
-        // keys between the sinks and the first query's window are seen by no query; with a gap the sinks' rows lie elsewhere
+        // keys between the sinks and the first query's window are seen by no query; and the sinks' rows may lie elsewhere
         const int unseen = w.shift - w.left;
-        whole0 = unseen > w.sinks || w.gap ? (max(unseen, w.sinks) + KT - 1) / KT : 0;
-        whole = w.bits ? 0 : max(0, nk / KT - whole0);
+        whole0 = unseen > w.sinks || w.skip ? (max(unseen, w.sinks) + KT - 1) / KT : 0;
+        whole = w.mask ? 0 : max(0, nk / KT - whole0);
         from = -64;
     }
     __device__ __forceinline__ bool all(int t) const { return (uint32_t)(t - whole0) < (uint32_t)whole; }
+    // Takes the keys that the mask does not keep out of the held words: a byte a lane for each unit, several units' loads at a time.
+    __device__ __forceinline__ void keep(const AttnWindow& w, const KeyTiles<KT>& tiles, int nk, int b, int u, int u1) {
+        constexpr int kUnits = 8;
+        const unsigned char* row = w.mask + (int64_t)b * (nk + w.gap);
+        const int lane = threadIdx.x & 63, n = min(64, u1 - u);
+        for (int i0 = 0; i0 < n; i0 += kUnits) {
+            unsigned char x[kUnits];
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int j = tiles.at(u + i0 + i) * KT + lane;
+                x[i] = i0 + i < n && lane < KT && j < nk ? row[j + (j >= w.sinks ? w.gap : 0)] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const uint64_t kept = __ballot(x[i] != 0);
+                if (lane == i0 + i) held &= kept;
+            }
+        }
+    }
     // The word of unit u, tile t, which is none of the range's.
     __device__ __forceinline__ uint64_t at(const AttnWindow& w, const KeyTiles<KT>& tiles, int nk, int b, int u, int u1) {
         if ((uint32_t)(u - from) >= 64u) {
@@ -85,11 +105,8 @@ struct TileWords {
                 const int sinks = min(max(w.sinks - t * KT, 0), KT);
                 held = left >= KT ? kAll : (1ull << left) - 1;
                 if (unseen > sinks) held &= ~((unseen == 64 ? ~0ull : (1ull << unseen) - 1) & ~((1ull << sinks) - 1));
-                if (w.bits) {
-                    const uint64_t* row = w.bits + (int64_t)b * w.words;
-                    held &= KT == 64 ? row[t] : row[t >> 1] >> (32 * (t & 1));
-                }
             }
+            if (w.mask) keep(w, tiles, nk, b, u, u1);
         }
         const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)held, u - from);
         const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(held >> 32), u - from);
@@ -129,14 +146,14 @@ struct WinTile {
             if (on(it)) dma16(p, off[it], dst(lds, it));
     }
     // Rows j0 .. of base, those of the word's bits; zeros in the others' place, nothing where there are none.  Rows from `sinks` on
-    // are `gap` rows further.
-    __device__ __forceinline__ static void load_some(const RowSrc& s, const char* base, int j0, uint64_t word, int sinks, int gap, char* lds) {
+    // are `skip` rows further.
+    __device__ __forceinline__ static void load_some(const RowSrc& s, const char* base, int j0, uint64_t word, int sinks, int skip, char* lds) {
         if (word == 0) return;
 #pragma unroll
         for (int it = 0; it < kIter; ++it) {
             if (!on(it)) continue;
             const int j = j0 + row(it);
-            if (word >> row(it) & 1) dma16(base + ((int64_t)j + (j >= sinks ? gap : 0)) * s.sn + chunk(it, s.chunks), dst(lds_off(lds), it));
+            if (word >> row(it) & 1) dma16(base + ((int64_t)j + (j >= sinks ? skip : 0)) * s.sn + chunk(it, s.chunks), dst(lds_off(lds), it));
             else *reinterpret_cast<f32x4*>(lds + (it * NT + threadIdx.x) * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }

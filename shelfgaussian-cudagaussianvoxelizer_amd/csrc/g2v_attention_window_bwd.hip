@@ -7,14 +7,9 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-#ifndef V_DQB64
-#define V_DQB64 1
-#endif
-#ifndef V_DQP64
-#define V_DQP64 3
-#endif
+// Workgroups that share a CU, as in g2v_attention.h, and blocks of 32 rows a wave.
 constexpr int window_dq_per_cu(int np, int dp, int waves) {
-    return np == 1 && dp == 64 && waves > 1 ? V_DQP64 : dq_per_cu(np, dp, waves);
+    return np == 1 && waves > 1 && dp <= 64 ? (dp == 32 ? 4 : 3) : dq_per_cu(np, dp, waves);
 }
 
 // As k_attn_dq.
@@ -69,7 +64,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     frags.init(lds_off(lds));
     Words words;
     words.init(a.win, a.nk);
-    auto load = [&](int u, int buf) {
+    auto load = [&](int u, int buf) __attribute__((always_inline)) {
         const int t = tiles.at(u), j0 = t * KT;
         if (words.all(t)) {
             ktile.load(kbase + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
@@ -194,11 +189,8 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
 }
 
 // The sinks' one-wave workgroups: as many to a CU as their tiles' LDS allows.
-#ifndef V_KVP
-#define V_KVP 2
-#endif
 constexpr int window_dkv_per_cu(int np, int ns, int dp, int nw) {
-    return nw > 1 && np == 1 && dp == 64 && ns == 2 ? V_KVP : nw > 1 ? dkv_per_cu(np, ns, dp) : np > 1 ? (dp > 96 ? 1 : dp > 32 ? 2 : 4) : dp > 64 ? 3 : dp > 32 ? 6 : 8;
+    return nw > 1 && np == 1 && dp >= 64 ? 2 : nw > 1 ? dkv_per_cu(np, ns, dp) : np > 1 ? (dp > 96 ? 1 : dp > 32 ? 2 : 4) : dp > 64 ? 3 : dp > 32 ? 6 : 8;
 }
 constexpr int dkv_bound(int np, int ns, int dp, int nw) { return nw > 1 ? window_dkv_per_cu(np, ns, dp, nw) : np > 1 && dp > 32 ? 1 : 2; }
 
@@ -206,13 +198,12 @@ constexpr int dkv_bound(int np, int ns, int dp, int nw) { return nw > 1 ? window
 template <int NP, int NS, int DP, int KS, int NW, int QT, typename T>
 __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_dkv(WinBwd a) {
     static_assert(NW == 1 || NW % 2 == 0, "waves in pairs load the statistics, or one does");
-#ifndef V_PP
-#define V_PP 1
-#endif
-    constexpr int NPP = NP > 1 ? NP : V_PP == 2 ? NS : 1;
+    // planes of P: one of bfloat16, as in the forward's product (dV 2.0e-3 off, its own rounding 1.7e-3); a second one would be a
+    // sixth product (200,000 x 8 heads x 64, 513 keys a window: 741 -> 800 us)
+    constexpr int NPP = NP;
     constexpr int NT = NW * 64, QB = QT / 32, DB = DP / 32;
     typedef WinTile<NP, DP, QT, NT> TileT;
-    constexpr int kBuffers = buffers(NW > 1 && window_dkv_per_cu(NP, NS, DP, NW) > 2 ? 3 : 2, TileT::kBytes), kAhead = kBuffers - 1;
+    constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     constexpr int kStats = NW == 1 ? 2 : 1;    // loads of statistics a wave
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and -delta of the tile's rows
@@ -232,7 +223,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
     split_range(per * a.group, w.split, w.splits, u0, u1);
     const int k0 = from(j), k1 = to(j);
     bool valid = j < n && k0 < k1;    // (rows that no query sees are not read either)
-    if (valid && a.win.bits) valid = a.win.bits[(int64_t)w.b * a.win.words + (j >> 6)] >> (j & 63) & 1;
+    if (valid && a.win.mask) valid = a.win.mask[(int64_t)w.b * a.nk + j];
     // blocks of 32 queries of which any sees one of the wave's keys, and those that see all of them
     WaveBlocks::Range any = {0, 0u}, every = {0, 0u};
     if (__any(valid)) {
@@ -240,7 +231,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
         if (w1 > w0) any = {w0 - 31, (uint32_t)(w1 - w0 + 31)};
         if (w3 - 31 > w2) every = {w2, (uint32_t)(w3 - 31 - w2)};
     }
-    if (a.win.bits && !__syncthreads_or(valid)) u1 = u0;    // nothing to add up
+    if (a.win.mask && !__syncthreads_or(valid)) u1 = u0;    // nothing to add up
 
     bf16x8 k[KS][NP], v[KS][NP];
     {
@@ -264,7 +255,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
     struct Place {
         int head, at;
     };
-    auto step = [&](Place& p) {
+    auto step = [](Place& p, int per) __attribute__((always_inline)) {
         if (++p.at == per) {
             p.at = 0;
             ++p.head;
@@ -272,7 +263,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
     };
     const int skip = per ? g2v::uniform(u0 / per) : 0;
     Place here = {w.h * a.group + skip, u0 - skip * per}, there = here;
-    auto load = [&](int buf) {
+    auto load = [&](int buf) __attribute__((always_inline)) {
         const int t = tile0 + there.at, head = there.head;
         const char* qbase = a.q.p + w.b * a.q.sb + head * a.q.sh;
         const char* gbase = a.g.p + w.b * a.g.sb + head * a.g.sh;
@@ -283,7 +274,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
             TileT::load_tail(a.q, qbase, t * QT, a.nq, lds_off(lds[buf][0]));
             TileT::load_tail(a.g, gbase, t * QT, a.nq, lds_off(lds[buf][1]));
         }
-        step(there);
+        step(there, per);
         // rows past the end are there in the padded statistics: lse +inf makes their probabilities 0
         const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + t * QT;
         const uint32_t lane = threadIdx.x & 63;
@@ -309,7 +300,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
         if (u + kAhead < u1) load(buf == 0 ? kBuffers - 1 : buf - 1);
         const uint32_t at = buf * 2 * TileT::kBytes;
         const int i0 = (tile0 + here.at) * QT;
-        step(here);
+        step(here, per);
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
             const int ib = i0 + 32 * qb;
@@ -462,7 +453,7 @@ hipError_t dkv_planes(const WinBwd& a, int planes, hipStream_t s) {
 AttnShape window_dq_shape(bool f32, int dp, int64_t rows) {
     AttnShape g = attn_dq_shape(f32, dp, rows);
     g.per_cu = window_dq_per_cu(f32 ? 3 : 1, dp, g.waves);
-    if (!f32 && dp == 64 && g.waves > 1) g.blocks = V_DQB64;
+    if (!f32 && g.waves > 1) g.blocks = 1;
     return g;
 }
 AttnShape window_dkv_shape(bool f32, int dp, int planes, bool all_queries) {
@@ -487,8 +478,8 @@ hipError_t launch_window_dq(const WinBwd& a, bool f32, int dp, hipStream_t s) {
         }
     }
     switch (dp) {
-        case 32: return dq_waves<1, 32, 2, 64, __bf16>(a, g, s);
-        case 64: return dq_waves<1, 64, V_DQB64, 64, __bf16>(a, g, s);
+        case 32: return dq_waves<1, 32, 1, 64, __bf16>(a, g, s);
+        case 64: return dq_waves<1, 64, 1, 64, __bf16>(a, g, s);
         case 96: return dq_waves<1, 96, 1, 64, __bf16>(a, g, s);
         default: return dq_waves<1, 128, 1, 64, __bf16>(a, g, s);
     }

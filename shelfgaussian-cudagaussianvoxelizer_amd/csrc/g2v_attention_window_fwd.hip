@@ -5,15 +5,90 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-#ifndef V_NQB64
-#define V_NQB64 1
-#endif
-#ifndef V_PER64
-#define V_PER64 3
-#endif
+// Workgroups that share a CU, as in g2v_attention.h.
 constexpr int window_fwd_per_cu(int np, int dp, int waves) {
-    return np == 1 && dp == 64 && waves > 1 ? V_PER64 : fwd_per_cu(np, dp, waves);
+    return np == 1 && waves > 1 ? (dp == 32 ? 4 : dp > 96 ? 2 : 3) : fwd_per_cu(np, dp, waves);
 }
+
+// Eight float32 values as three bfloat16 planes, exact to 24 bits.  A finite value above the largest bfloat16 starts with that (what
+// is left is small); an infinity is its first plane alone.
+constexpr float kMaxBf16 = 0x1.fep127f;
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void split_planes(const f32x8 x, bf16x8 (&o)[3]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+    const bool large = most > kMaxBf16;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float r = x[j];
+#pragma unroll
+        for (int pl = 0; pl < 3; ++pl) {
+            const __bf16 h = (__bf16)r;
+            o[pl][j] = h;
+            r -= (float)h;
+        }
+    }
+    if (large) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float r = x[j], h = (float)(__bf16)r;
+            if (!__builtin_isfinite(h) && __builtin_isfinite(r)) h = copysignf(kMaxBf16, r);
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl) {
+                o[pl][j] = (__bf16)h;
+                r = __builtin_isfinite(h) ? r - h : 0.0f;
+                h = (float)(__bf16)r;
+            }
+        }
+    }
+}
+// Values 8 c .. 8 c + 7 of a row of dim, zeros past its end or without a row.
+__device__ __forceinline__ f32x8 load_floats(const float* row, bool have, int c, int dim) {
+    typedef f32x4 any_f32x4 __attribute__((aligned(4)));
+    f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (have && 8 * c + 8 <= dim) {
+        const f32x4 lo = *reinterpret_cast<const any_f32x4*>(row + 8 * c), hi = *reinterpret_cast<const any_f32x4*>(row + 8 * c + 4);
+        x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else if (have) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (8 * c + j < dim) x[j] = row[8 * c + j];
+    }
+    return x;
+}
+
+// A tile of float32 rows on its way to LDS (as Tile's three planes): in registers while the tile before it is computed.
+template <int DP, int ROWS, int NT>
+struct FloatTile {
+    static constexpr int C = DP / 8, kChunks = ROWS * C, kIter = (kChunks + NT - 1) / NT;
+    f32x8 x0, x1;    // (an array of them is kept in memory by the compiler)
+    __device__ __forceinline__ static bool on(int it) { return kChunks % NT == 0 || it * NT + (int)threadIdx.x < kChunks; }
+    // Rows j0 .. of base, those of the word's bits, zeros in the others' place.
+    __device__ __forceinline__ void fetch(const RowSrc& s, const char* base, int dim, int j0, uint64_t word, int sinks, int skip) {
+        static_assert(kIter <= 2, "chunks of a thread");
+        auto one = [&](int it) __attribute__((always_inline)) {
+            const int L = it * NT + threadIdx.x, row = L / C, j = j0 + row;
+            return load_floats(reinterpret_cast<const float*>(base + ((int64_t)j + (j >= sinks ? skip : 0)) * s.sn),
+                               on(it) && (word >> row & 1), L % C, dim);
+        };
+        x0 = one(0);
+        if constexpr (kIter > 1) x1 = one(1);
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+        auto one = [&](int it, const f32x8 x) __attribute__((always_inline)) {
+            const int L = it * NT + threadIdx.x, row = L / C, c = L % C;
+            if (!on(it)) return;
+            bf16x8 o[3];
+            split_planes(x, o);
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl)
+                *reinterpret_cast<bf16x8*>(lds + (pl * kChunks + row * C + swz<DP>(row, c)) * 16) = o[pl];
+        };
+        one(0, x0);
+        if constexpr (kIter > 1) one(1, x1);
+    }
+};
 
 // As k_attn_fwd (rows in the lanes, keys in the registers).
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
@@ -21,7 +96,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
     typedef WinTile<NP, DP, KT, NT> TileT;
     typedef TileWords<KT> Words;
-    constexpr int kBuffers = buffers(window_fwd_per_cu(NP, DP, NW) > 3 ? 4 : NP == 1 && NQB == 1 ? 3 : 2, TileT::kBytes), kAhead = kBuffers - 1;
+    constexpr int kBuffers = NP > 1 ? 2 : buffers(window_fwd_per_cu(NP, DP, NW), TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     static_assert(window_fwd_per_cu(NP, DP, NW) * sizeof(lds) <= kLdsBytes, "planned by more workgroups than fit");
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
@@ -49,30 +124,43 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         m[b] = r < rows ? -INFINITY : 0.0f;
         l[b] = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int pl = 0; pl < NP; ++pl) q[b][ks][pl] = mem_frag<DP>(row, r < rows, a.q.chunks, pl, ks);
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (NP > 1) {
+                split_planes(load_floats(reinterpret_cast<const float*>(row), r < rows, 2 * ks + half, a.dim), q[b][ks]);
+            } else {
+                q[b][ks][0] = mem_frag<DP>(row, r < rows, a.q.chunks, 0, ks);
+            }
+        }
     }
 
     TileT ktile, vtile;
-    ktile.init(a.k);
-    vtile.init(a.v);
+    FloatTile<DP, KT, NT> kfloat, vfloat;
+    if constexpr (NP == 1) {
+        ktile.init(a.k);
+        vtile.init(a.v);
+    }
     Frags<DP> frags;
     frags.init(lds_off(lds));
     Words words;
     words.init(a.win, a.nk);
-    const char* kfar = kbase + (int64_t)a.win.gap * a.k.sn;
-    const char* vfar = vbase + (int64_t)a.win.gap * a.v.sn;
-    auto load = [&](int u, int buf) {
+    const char* kfar = kbase + (int64_t)a.win.skip * a.k.sn;
+    const char* vfar = vbase + (int64_t)a.win.skip * a.v.sn;
+    auto load = [&](int u, int buf) __attribute__((always_inline)) {
         const int t = tiles.at(u), j0 = t * KT;
+        if constexpr (NP > 1) {    // into registers
+            const uint64_t word = words.all(t) ? Words::kAll : words.at(a.win, tiles, a.nk, w.b, u, u1);
+            kfloat.fetch(a.k, kbase, a.dim, j0, word, a.win.sinks, a.win.skip);
+            vfloat.fetch(a.v, vbase, a.dim, j0, word, a.win.sinks, a.win.skip);
+            return word;
+        }
         if (words.all(t)) {
             ktile.load(kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
             vtile.load(vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
             return Words::kAll;
         }
         const uint64_t word = words.at(a.win, tiles, a.nk, w.b, u, u1);
-        TileT::load_some(a.k, kbase, j0, word, a.win.sinks, a.win.gap, lds[buf][0]);
-        TileT::load_some(a.v, vbase, j0, word, a.win.sinks, a.win.gap, lds[buf][1]);
+        TileT::load_some(a.k, kbase, j0, word, a.win.sinks, a.win.skip, lds[buf][0]);
+        TileT::load_some(a.v, vbase, j0, word, a.win.sinks, a.win.skip, lds[buf][1]);
         return word;
     };
 
@@ -83,12 +171,21 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][b][i] = 0.0f;
+    auto store = [&](int buf) __attribute__((always_inline)) {    // float32: from registers to LDS
+        if constexpr (NP > 1) {
+            kfloat.store(lds[buf][0]);
+            vfloat.store(lds[buf][1]);
+        }
+    };
     uint64_t word = 0, next = 0, after = 0;    // of units u, u + 1 and u + 2
-    if (u0 < u1) word = load(u0, 0);
+    if (u0 < u1) {
+        word = load(u0, 0);
+        store(0);
+    }
     if (kAhead > 1 && u0 + 1 < u1) next = load(u0 + 1, 1);
     for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
         // (a partly valid tile's loads are not the same number for every wave)
-        next_tile<kBuffers, 2 * TileT::kLoads>(u + 1 < u1 && words.all(tiles.at(u + 1)));
+        next_tile<kBuffers, (NP > 1 ? 0 : 2 * TileT::kLoads)>(u + 1 < u1 && words.all(tiles.at(u + 1)));
         after = 0;
         if (u + kAhead < u1) {
             const uint64_t x = load(u + kAhead, buf == 0 ? kBuffers - 1 : buf - 1);
@@ -202,6 +299,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
                     }
             }
         }
+        if (u + 1 < u1) store(buf ^ 1);
         word = next;
         next = after;
     }
@@ -245,18 +343,6 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     }
 }
 
-// Bits of the valid keys, a wave a word.
-__global__ void __launch_bounds__(256) k_window_bits(int nk, int sinks, int gap, int words, int64_t all, const unsigned char* mask,
-                                                     uint64_t* bits) {
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= all) return;
-    const int64_t b = at / words;
-    const int j = (int)(at - b * words) * 64 + (threadIdx.x & 63);
-    const bool valid = j < nk && mask[b * (nk + gap) + j + (j >= sinks ? gap : 0)];
-    const uint64_t x = __ballot(valid);
-    if ((threadIdx.x & 63) == 0) bits[at] = x;
-}
-
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 hipError_t fwd_launch(const WinFwd& a, hipStream_t s) {
     G2V_LAUNCH((k_window_fwd<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
@@ -276,7 +362,7 @@ hipError_t fwd_waves(const WinFwd& a, const AttnShape& g, hipStream_t s) {
 AttnShape window_fwd_shape(bool f32, int dp, int64_t rows) {
     AttnShape g = attn_fwd_shape(f32, dp, rows);
     g.per_cu = window_fwd_per_cu(f32 ? 3 : 1, dp, g.waves);
-    if (!f32 && dp == 64 && g.waves > 1) g.blocks = V_NQB64;
+    if (!f32 && g.waves > 1) g.blocks = 1;
     return g;
 }
 
@@ -291,18 +377,11 @@ hipError_t launch_window_fwd(const WinFwd& a, bool f32, int dp, hipStream_t s) {
         }
     }
     switch (dp) {
-        case 32: return fwd_waves<1, 32, 2, 64, __bf16>(a, g, s);
-        case 64: return fwd_waves<1, 64, V_NQB64, 64, __bf16>(a, g, s);
+        case 32: return fwd_waves<1, 32, 1, 64, __bf16>(a, g, s);
+        case 64: return fwd_waves<1, 64, 1, 64, __bf16>(a, g, s);
         case 96: return fwd_waves<1, 96, 1, 64, __bf16>(a, g, s);
-        default: return fwd_waves<1, 128, 2, 32, __bf16>(a, g, s);
+        default: return fwd_waves<1, 128, 1, 32, __bf16>(a, g, s);
     }
-}
-
-hipError_t launch_window_bits(int batch, int nk, int sinks, int gap, const unsigned char* mask, int words, uint64_t* bits,
-                              hipStream_t s) {
-    const int64_t all = (int64_t)batch * words;
-    if (all > 0) G2V_LAUNCH(k_window_bits, dim3((unsigned)ceil_div(all, 4)), dim3(256), 0, s, nk, sinks, gap, words, all, mask, bits);
-    return hipGetLastError();
 }
 
 }  // namespace g2v

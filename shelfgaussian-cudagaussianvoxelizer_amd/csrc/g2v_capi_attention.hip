@@ -315,8 +315,7 @@ size_t attn_bwd_bytes(const AttnSizes& z, const AttnRun& dq, const AttnRun& dkv,
 
 // ---- attention within a window -----------------------------------------------------------------
 
-// Sizes and window as the kernels take them: z.nk without the keys between the sinks and the first window (forward only; in
-// steps of 64, the mask's words).
+// Sizes and window as the kernels take them: z.nk without the keys between the sinks and the first window (forward only).
 struct WinSizes {
     AttnSizes z;
     AttnWindow w;
@@ -337,11 +336,10 @@ int win_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_di
     x.span = (int64_t)x.w.left + x.w.right + 1;
     if (forward) {
         const int first = std::max(0, x.w.shift - x.w.left);
-        x.w.gap = first > x.w.sinks ? (first - x.w.sinks) / 64 * 64 : 0;
+        x.w.gap = first > x.w.sinks ? first - x.w.sinks : 0;
         x.z.nk -= x.w.gap;
         x.w.shift -= x.w.gap;
     }
-    x.w.words = (int)ceil_div(x.z.nk, 64);
     return G2V_OK;
 }
 
@@ -382,18 +380,6 @@ AttnRun win_sinks_run(const WinSizes& x, int planes) {
     return {r, part_rows(r, x.z.bhs, x.w.sinks)};
 }
 
-struct WinFwdWs {
-    uint64_t* bits;
-    float *part_o, *part_ml;
-};
-WinFwdWs carve_win_fwd(Carver& c, const WinSizes& x, const AttnRun& r, bool masked) {
-    WinFwdWs w;
-    const AttnFwdWs f = carve_attn_fwd(c, x.z, r);
-    w.part_o = f.part_o;
-    w.part_ml = f.part_ml;
-    w.bits = masked ? c.take<uint64_t>((size_t)x.z.batch * x.w.words) : nullptr;
-    return w;
-}
 struct WinBwdRuns {
     int planes;
     AttnRun dq, dkv, sinks;
@@ -406,38 +392,27 @@ WinBwdRuns win_bwd_runs(const WinSizes& x, bool masked) {
     r.sinks = win_sinks_run(x, r.planes);
     return r;
 }
-struct WinBwdWs {
-    int nqp;
-    float *lse, *delta, *part;
-    uint64_t* bits;
-};
-WinBwdWs carve_win_bwd(Carver& c, const WinSizes& x, const WinBwdRuns& r, bool masked) {
-    WinBwdWs w;
-    AttnRun dkv = r.dkv;    // the sinks' partial results take the area of the others' after them
+// The sinks' partial results take the area of the others' after them.
+AttnBwdWs carve_win_bwd(Carver& c, const WinSizes& x, const WinBwdRuns& r) {
+    AttnRun dkv = r.dkv;
     dkv.part_rows = std::max(dkv.part_rows, r.sinks.part_rows);
-    const AttnBwdWs f = carve_attn_bwd(c, x.z, r.dq, dkv);
-    w.nqp = f.nqp;
-    w.lse = f.lse;
-    w.delta = f.delta;
-    w.part = f.part;
-    w.bits = masked ? c.take<uint64_t>((size_t)x.z.batch * x.w.words) : nullptr;
-    return w;
+    return carve_attn_bwd(c, x.z, r.dq, dkv);
 }
-size_t win_fwd_bytes(const WinSizes& x, const AttnRun& r, bool packed, bool masked) {
+size_t win_fwd_bytes(const WinSizes& x, const AttnRun& r, bool packed) {
     Carver c(nullptr, (size_t)-1);
-    carve_win_fwd(c, x, r, masked);
+    carve_attn_fwd(c, x.z, r);
     carve_packed(c, x.z, packed, false, false);
     return c.off + 256;
 }
-size_t win_bwd_bytes(const WinSizes& x, const WinBwdRuns& r, bool packed, bool masked) {
+size_t win_bwd_bytes(const WinSizes& x, const WinBwdRuns& r, bool packed) {
     Carver c(nullptr, (size_t)-1);
-    carve_win_bwd(c, x, r, masked);
+    carve_win_bwd(c, x, r);
     carve_packed(c, x.z, packed, false, true);
     return c.off + 256;
 }
 
 // The tensors as the kernels read them: all in place, or all packed without the gap and with zeros in masked keys' rows.
-hipError_t win_sources(const WinSizes& x, const Strided* t, int count, bool packed, const uint64_t* bits, Carver& c,
+hipError_t win_sources(const WinSizes& x, const Strided* t, int count, bool packed, const unsigned char* mask, Carver& c,
                        attn::RowSrc* out, hipStream_t s) {
     const AttnSizes& z = x.z;
     AttnPack a = {};
@@ -447,11 +422,11 @@ hipError_t win_sources(const WinSizes& x, const Strided* t, int count, bool pack
     a.list_tensor = -1;
     a.sinks = x.w.sinks;
     a.gap = x.w.gap;
-    a.words = x.w.words;
-    a.bits = bits;
+    a.valid = mask;
     for (int i = 0; i < count; ++i) {
         if (!packed) {
-            out[i] = {static_cast<const char*>(t[i].p), t[i].s[0] * 2, t[i].s[1] * 2, t[i].s[2] * 2, z.dim / 8};
+            const int size = z.f32 ? 4 : 2;
+            out[i] = {static_cast<const char*>(t[i].p), t[i].s[0] * size, t[i].s[1] * size, t[i].s[2] * size, z.dim / 8};
             continue;
         }
         const int64_t row = (int64_t)(z.f32 ? 3 : 1) * z.dp * 2;
@@ -626,7 +601,7 @@ size_t g2v_window_attention_forward_workspace(int batch, int n_q, int n_k, int h
                                               int left, int right, int sinks, int in_place, int masked) {
     WinSizes x;
     if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, true, x) != G2V_OK) return 0;
-    return win_fwd_bytes(x, win_fwd_run(x), x.z.f32 || !in_place, masked != 0);
+    return win_fwd_bytes(x, win_fwd_run(x), !x.z.f32 && !in_place);
 }
 
 int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -650,16 +625,17 @@ int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int h
     const Strided t[3] = {{q, q_strides, n_q, heads_q, false},
                           {k, keys ? k_strides : none, z.nk, heads_k, true},
                           {v, keys ? v_strides : none, z.nk, heads_k, true}};
-    const bool packed = !attn_in_place(z, t, 3), masked = keys && key_mask;
+    // (the forward splits float32 rows into planes on their way)
+    const bool packed = !z.f32 && !attn_in_place(z, t, 3);
+    if (!keys) key_mask = nullptr;
     const AttnRun r = win_fwd_run(x);
-    const size_t need = win_fwd_bytes(x, r, packed, masked);
+    const size_t need = win_fwd_bytes(x, r, packed);
     if (!workspace || workspace_bytes < need)
         return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
     Carver c(workspace, workspace_bytes);
-    const WinFwdWs w = carve_win_fwd(c, x, r, masked);
-    if (masked) G2V_HIP(launch_window_bits(batch, z.nk, x.w.sinks, x.w.gap, key_mask, x.w.words, w.bits, s));
+    const AttnFwdWs w = carve_attn_fwd(c, z, r);
     attn::RowSrc src[3];
-    G2V_HIP(win_sources(x, t, 3, packed, w.bits, c, src, s));
+    G2V_HIP(win_sources(x, t, 3, packed, key_mask, c, src, s));
     WinFwd a = {};
     a.q = src[0];
     a.k = src[1];
@@ -679,8 +655,8 @@ int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int h
     a.part_o = w.part_o;
     a.part_ml = w.part_ml;
     a.win = x.w;
-    a.win.bits = w.bits;
-    if (packed) a.win.gap = 0;
+    a.win.mask = key_mask;
+    a.win.skip = packed ? 0 : x.w.gap;
     G2V_HIP(launch_window_fwd(a, z.f32, z.dp, s));
     return G2V_OK;
 }
@@ -689,7 +665,7 @@ size_t g2v_window_attention_backward_workspace(int batch, int n_q, int n_k, int 
                                                int left, int right, int sinks, int in_place, int masked) {
     WinSizes x;
     if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, false, x) != G2V_OK) return 0;
-    return win_bwd_bytes(x, win_bwd_runs(x, masked != 0), x.z.f32 || !in_place, masked != 0);
+    return win_bwd_bytes(x, win_bwd_runs(x, masked != 0), x.z.f32 || !in_place);
 }
 
 int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -718,16 +694,16 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
                           {v, keys ? v_strides : none, n_k, heads_k, true},
                           {grad_out, sg, n_q, heads_q, false}};
     const AttnSizes& z = x.z;
-    const bool packed = !attn_in_place(z, t, 4), masked = keys && key_mask;
-    const WinBwdRuns r = win_bwd_runs(x, masked);
-    const size_t need = win_bwd_bytes(x, r, packed, masked);
+    const bool packed = !attn_in_place(z, t, 4);
+    if (!keys) key_mask = nullptr;
+    const WinBwdRuns r = win_bwd_runs(x, key_mask != nullptr);
+    const size_t need = win_bwd_bytes(x, r, packed);
     if (!workspace || workspace_bytes < need)
         return api_fail(G2V_ERR_INVALID, "workspace too small: %zu bytes, need %zu", workspace ? workspace_bytes : (size_t)0, need);
     Carver c(workspace, workspace_bytes);
-    const WinBwdWs w = carve_win_bwd(c, x, r, masked);
-    if (masked) G2V_HIP(launch_window_bits(batch, n_k, x.w.sinks, 0, key_mask, x.w.words, w.bits, s));
+    const AttnBwdWs w = carve_win_bwd(c, x, r);
     attn::RowSrc src[4];
-    G2V_HIP(win_sources(x, t, 4, packed, w.bits, c, src, s));
+    G2V_HIP(win_sources(x, t, 4, packed, key_mask, c, src, s));
     G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, out_rest, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
                               w.delta, s));
     WinBwd a = {};
@@ -752,7 +728,7 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
     a.dv = grad_v;
     a.part = w.part;
     a.win = x.w;
-    a.win.bits = w.bits;
+    a.win.mask = key_mask;
     if (grad_k && keys) {
         WinBwd kv = a;
         if (n_k == 1 || (x.span == 1 && x.w.sinks == 0)) kv.scale = 0.0f;    // a query's only key: its probability is 1

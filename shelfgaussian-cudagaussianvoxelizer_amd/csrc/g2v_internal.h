@@ -324,10 +324,10 @@ struct AttnPack {
     const unsigned char* mask;
     int *count_out, *list_out;
     int list_tensor;
-    // rows of the keys from `sinks` on are `gap` rows further in src, and those whose bit is not set are packed as zeros,
-    // unread (64 keys a word; null: all)
-    int sinks, gap, words;
-    const uint64_t* bits;
+    // rows of the keys from `sinks` on are `gap` rows further in src, and those that `valid` (batch, n + gap; null: all are) does
+    // not keep are packed as zeros, unread
+    int sinks, gap;
+    const unsigned char* valid;
     int64_t blocks[4];   // set by the launch
 };
 // A kernel's workgroup: waves, blocks of 32 rows of a wave, rows of a tile of the long axis, workgroups that fit a CU; and
@@ -364,10 +364,6 @@ hipError_t launch_attn_dkv_join(const AttnBwd& a, bool f32, int dp, hipStream_t 
 // ---- attention within a window (g2v_attention_window_fwd.hip, g2v_attention_window_bwd.hip) -----------------------------------
 struct WinFwd;
 struct WinBwd;
-// Bits of the valid keys of each scene, 64 keys a word, by mask (batch, nk + gap); key j of the words is key j + gap of the mask
-// behind the sinks.
-hipError_t launch_window_bits(int batch, int nk, int sinks, int gap, const unsigned char* mask, int words, uint64_t* bits,
-                              hipStream_t s);
 AttnShape window_fwd_shape(bool f32, int dp, int64_t rows);
 AttnShape window_dq_shape(bool f32, int dp, int64_t rows);
 AttnShape window_dkv_shape(bool f32, int dp, int planes, bool all_queries);
