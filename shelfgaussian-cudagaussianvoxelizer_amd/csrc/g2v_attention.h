@@ -421,6 +421,7 @@ struct AttnBwd {
     int nq, nk, hq, hk, group, dim, bhs;
     attn::Parts parts;
     bool by_count;       // set by launch_attn_dkv
+    int gap_at, gap;     // dk and dv have `gap` rows more from row gap_at on, which are none of k and v
     int nqp;             // nq rounded up to 64: rows of lse and delta, padded with +inf and 0
     float c, scale;
     const float *lse, *delta;   // (batch, hq, nqp); -delta
@@ -429,6 +430,11 @@ struct AttnBwd {
 };
 
 namespace attn {
+// Row of dk and dv that key j of scene b has.
+__device__ __forceinline__ int64_t grad_row(const AttnBwd& a, int b, int64_t j) {
+    return (int64_t)b * (a.nk + a.gap) + j + (a.gap && j >= a.gap_at ? a.gap : 0);
+}
+
 // Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
 // to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
 // the same error on all of them, which their sum dS K does not average out (dQ then 3.2e-3 off instead of 2.2e-3).
@@ -453,7 +459,7 @@ struct WinFwd : AttnFwd {
     AttnWindow win;
 };
 struct WinBwd : AttnBwd {
-    AttnWindow win;
+    AttnWindow win;      // dk and dv have the gap, too
     bool all_queries;    // dK and dV: of the sinks, from every query that sees them (else of all keys, from those within the window)
 };
 

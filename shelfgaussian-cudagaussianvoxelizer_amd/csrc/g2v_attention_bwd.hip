@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(AttnBwd a, int parts) {
     if (!live || threadIdx.x % parts) return;
     const int64_t key = a.list ? a.list[(int64_t)b * a.nk + j] : j;
     const float f = d < DP ? a.scale : 1.0f;
-    T* row = static_cast<T*>(d < DP ? a.dk : a.dv) + (((int64_t)b * a.nk + key) * a.hk + bh % a.hk) * a.dim;
+    T* row = static_cast<T*>(d < DP ? a.dk : a.dv) + (grad_row(a, b, key) * a.hk + bh % a.hk) * a.dim;
     store4<T>(row, d < DP ? d : d - DP, a.dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
 }
 

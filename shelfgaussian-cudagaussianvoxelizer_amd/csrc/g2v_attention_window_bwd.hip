@@ -64,16 +64,18 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     frags.init(lds_off(lds));
     Words words;
     words.init(a.win, a.nk);
+    const char* kfar = kbase + (int64_t)a.win.skip * a.k.sn;
+    const char* vfar = vbase + (int64_t)a.win.skip * a.v.sn;
     auto load = [&](int u, int buf) __attribute__((always_inline)) {
         const int t = tiles.at(u), j0 = t * KT;
         if (words.all(t)) {
-            ktile.load(kbase + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
-            vtile.load(vbase + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
+            ktile.load(kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
+            vtile.load(vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
             return Words::kAll;
         }
         const uint64_t word = words.at(a.win, tiles, a.nk, w.b, u, u1);
-        TileT::load_some(a.k, kbase, j0, word, a.win.sinks, 0, lds[buf][0]);
-        TileT::load_some(a.v, vbase, j0, word, a.win.sinks, 0, lds[buf][1]);
+        TileT::load_some(a.k, kbase, j0, word, a.win.sinks, a.win.skip, lds[buf][0]);
+        TileT::load_some(a.v, vbase, j0, word, a.win.sinks, a.win.skip, lds[buf][1]);
         return word;
     };
 
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
     split_range(per * a.group, w.split, w.splits, u0, u1);
     const int k0 = from(j), k1 = to(j);
     bool valid = j < n && k0 < k1;    // (rows that no query sees are not read either)
-    if (valid && a.win.mask) valid = a.win.mask[(int64_t)w.b * a.nk + j];
+    if (valid && a.win.mask) valid = a.win.mask[grad_row(a, w.b, j)];
     // blocks of 32 queries of which any sees one of the wave's keys, and those that see all of them
     WaveBlocks::Range any = {0, 0u}, every = {0, 0u};
     if (__any(valid)) {
@@ -235,8 +237,9 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
 
     bf16x8 k[KS][NP], v[KS][NP];
     {
-        const char* krow = a.k.p + w.b * a.k.sb + w.h * a.k.sh + j * a.k.sn;
-        const char* vrow = a.v.p + w.b * a.v.sb + w.h * a.v.sh + j * a.v.sn;
+        const int64_t row = j + (j >= a.win.sinks ? a.win.skip : 0);
+        const char* krow = a.k.p + w.b * a.k.sb + w.h * a.k.sh + row * a.k.sn;
+        const char* vrow = a.v.p + w.b * a.v.sb + w.h * a.v.sh + row * a.v.sn;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
             }
         return;
     }
-    const int64_t at = (((int64_t)w.b * a.nk + j) * a.hk + w.h) * a.dim;
+    const int64_t at = (grad_row(a, w.b, j) * a.hk + w.h) * a.dim;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
         float x[16], y[16];
@@ -405,8 +408,25 @@ __global__ void __launch_bounds__(256) k_window_sinks_join(WinBwd a, int n, int 
     const f32x4 o = join_sum(a.part + pr.at * (2 * DP) + d, pr.step * (2 * DP), pr.splits, parts, live, red);
     if (!live || threadIdx.x % parts) return;
     const float f = d < DP ? a.scale : 1.0f;
-    T* row = static_cast<T*>(d < DP ? a.dk : a.dv) + (((int64_t)b * a.nk + j) * a.hk + bh % a.hk) * a.dim;
+    T* row = static_cast<T*>(d < DP ? a.dk : a.dv) + (grad_row(a, b, j) * a.hk + bh % a.hk) * a.dim;
     store4<T>(row, d < DP ? d : d - DP, a.dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+}
+
+// Zeros in the rows of dk and dv that are no query's (grid y: which): `each` values of a scene, 16 bytes a thread at any alignment.
+template <typename T>
+__global__ void __launch_bounds__(256) k_window_zeros(WinBwd a, int64_t each, int64_t blocks) {
+    constexpr int N = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    const int64_t b = blockIdx.x / blocks, at = ((blockIdx.x - b * blocks) * 256 + threadIdx.x) * N;
+    T* row = static_cast<T*>(blockIdx.y ? a.dv : a.dk) + ((b * (a.nk + a.gap) + a.gap_at) * a.hk) * a.dim;
+    if (at + N <= each) {
+        vec zero;
+#pragma unroll
+        for (int j = 0; j < N; ++j) zero[j] = (T)0.0f;
+        *reinterpret_cast<vec*>(row + at) = zero;
+    } else {
+        for (int64_t j = at; j < each; ++j) row[j] = (T)0.0f;
+    }
 }
 
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
@@ -483,6 +503,15 @@ hipError_t launch_window_dq(const WinBwd& a, bool f32, int dp, hipStream_t s) {
         case 96: return dq_waves<1, 96, 1, 64, __bf16>(a, g, s);
         default: return dq_waves<1, 128, 1, 64, __bf16>(a, g, s);
     }
+}
+
+hipError_t launch_window_zeros(const WinBwd& a, int batch, bool f32, hipStream_t s) {
+    const int64_t each = (int64_t)a.gap * a.hk * a.dim, blocks = ceil_div(each, 256 * (f32 ? 4 : 8));
+    if (batch * blocks == 0) return hipSuccess;
+    const dim3 grid((unsigned)(batch * blocks), 2), block(256);
+    if (f32) G2V_LAUNCH((k_window_zeros<float>), grid, block, 0, s, a, each, blocks);
+    else G2V_LAUNCH((k_window_zeros<__bf16>), grid, block, 0, s, a, each, blocks);
+    return hipGetLastError();
 }
 
 hipError_t launch_window_dkv(const WinBwd& a, bool f32, int dp, int planes, hipStream_t s) {

@@ -315,14 +315,14 @@ size_t attn_bwd_bytes(const AttnSizes& z, const AttnRun& dq, const AttnRun& dkv,
 
 // ---- attention within a window -----------------------------------------------------------------
 
-// Sizes and window as the kernels take them: z.nk without the keys between the sinks and the first window (forward only).
+// Sizes and window as the kernels take them: z.nk without the keys between the sinks and the first window, which no query sees.
 struct WinSizes {
     AttnSizes z;
     AttnWindow w;
     int64_t span;    // keys of a query's window
 };
 int win_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype, int left, int right, int sinks,
-              bool forward, WinSizes& x) {
+              WinSizes& x) {
     const int rc = attn_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, x.z);
     if (rc != G2V_OK) return rc;
     if (left < -1 || right < -1 || sinks < 0)
@@ -334,12 +334,9 @@ int win_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_di
     x.w.sinks = std::min(sinks, n_k);
     x.w.shift = n_k - n_q;
     x.span = (int64_t)x.w.left + x.w.right + 1;
-    if (forward) {
-        const int first = std::max(0, x.w.shift - x.w.left);
-        x.w.gap = first > x.w.sinks ? first - x.w.sinks : 0;
-        x.z.nk -= x.w.gap;
-        x.w.shift -= x.w.gap;
-    }
+    x.w.gap = std::max(0, std::min(x.w.shift - x.w.left, n_k) - x.w.sinks);
+    x.z.nk -= x.w.gap;
+    x.w.shift -= x.w.gap;
     return G2V_OK;
 }
 
@@ -600,7 +597,7 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
 size_t g2v_window_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
                                               int left, int right, int sinks, int in_place, int masked) {
     WinSizes x;
-    if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, true, x) != G2V_OK) return 0;
+    if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, x) != G2V_OK) return 0;
     return win_fwd_bytes(x, win_fwd_run(x), !x.z.f32 && !in_place);
 }
 
@@ -611,7 +608,7 @@ int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int h
                                  size_t workspace_bytes, void* stream) {
     api_begin();
     WinSizes x;
-    int rc = win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, true, x);
+    int rc = win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, x);
     if (rc != G2V_OK) return rc;
     rc = attn_scale(scale);
     if (rc != G2V_OK) return rc;
@@ -664,7 +661,7 @@ int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int h
 size_t g2v_window_attention_backward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,
                                                int left, int right, int sinks, int in_place, int masked) {
     WinSizes x;
-    if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, false, x) != G2V_OK) return 0;
+    if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, x) != G2V_OK) return 0;
     return win_bwd_bytes(x, win_bwd_runs(x, masked != 0), x.z.f32 || !in_place);
 }
 
@@ -676,7 +673,7 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
                                   void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
     api_begin();
     WinSizes x;
-    int rc = win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, false, x);
+    int rc = win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, x);
     if (rc != G2V_OK) return rc;
     rc = attn_scale(scale);
     if (rc != G2V_OK) return rc;
@@ -690,8 +687,8 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
     static const long long none[3] = {0, 0, 0};
     const long long* sg = queries ? grad_out_strides : none;
     const Strided t[4] = {{q, queries ? q_strides : none, n_q, heads_q, false},
-                          {k, keys ? k_strides : none, n_k, heads_k, true},
-                          {v, keys ? v_strides : none, n_k, heads_k, true},
+                          {k, keys ? k_strides : none, x.z.nk, heads_k, true},
+                          {v, keys ? v_strides : none, x.z.nk, heads_k, true},
                           {grad_out, sg, n_q, heads_q, false}};
     const AttnSizes& z = x.z;
     const bool packed = !attn_in_place(z, t, 4);
@@ -712,7 +709,9 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
     a.v = src[2];
     a.g = src[3];
     a.nq = n_q;
-    a.nk = n_k;
+    a.nk = z.nk;
+    a.gap_at = x.w.sinks;
+    a.gap = x.w.gap;
     a.hq = heads_q;
     a.hk = heads_k;
     a.group = z.group;
@@ -729,11 +728,13 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
     a.part = w.part;
     a.win = x.w;
     a.win.mask = key_mask;
+    a.win.skip = packed ? 0 : x.w.gap;
     if (grad_k && keys) {
+        G2V_HIP(launch_window_zeros(a, batch, z.f32, s));
         WinBwd kv = a;
-        if (n_k == 1 || (x.span == 1 && x.w.sinks == 0)) kv.scale = 0.0f;    // a query's only key: its probability is 1
+        if (z.nk == 1 || (x.span == 1 && x.w.sinks == 0)) kv.scale = 0.0f;    // a query's only key: its probability is 1
         kv.parts = r.dkv.parts;
-        G2V_HIP(launch_window_dkv(kv, z.f32, z.dp, r.planes, s));
+        if (z.nk > 0) G2V_HIP(launch_window_dkv(kv, z.f32, z.dp, r.planes, s));    // (no queries: all keys are the gap's)
         if (queries && win_has_far(x)) {    // written anew behind them
             kv.all_queries = true;
             kv.parts = r.sinks.parts;

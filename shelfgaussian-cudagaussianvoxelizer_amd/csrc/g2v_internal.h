@@ -369,6 +369,8 @@ AttnShape window_dq_shape(bool f32, int dp, int64_t rows);
 AttnShape window_dkv_shape(bool f32, int dp, int planes, bool all_queries);
 hipError_t launch_window_fwd(const WinFwd& a, bool f32, int dp, hipStream_t s);
 hipError_t launch_window_dq(const WinBwd& a, bool f32, int dp, hipStream_t s);
+// Zeros in the gap's rows of dk and dv.
+hipError_t launch_window_zeros(const WinBwd& a, int batch, bool f32, hipStream_t s);
 // planes: of P and dS.  With a.all_queries a.parts splits all tiles of the sinks alike.
 hipError_t launch_window_dkv(const WinBwd& a, bool f32, int dp, int planes, hipStream_t s);
 

@@ -349,13 +349,13 @@ def test_runs_are_equal_and_streams_are_the_callers(nq, nk, dtype):
 @pytest.mark.parametrize("dtype", BOTH, ids=IDS)
 def test_empty(dtype):
     from CudaGaussianVoxelizer import gaussian_attention
-    for B, nq, nk in ((0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 0)):
+    for B, nq, nk in ((0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 0), (2, 0, 300), (1, 0, 1)):
         leaves = [torch.randn(B, n, 2, 32, device="cuda", dtype=dtype, requires_grad=True) for n in (nq, nk, nk)]
-        out = gaussian_attention(*leaves, torch.ones(B, nk, dtype=torch.bool, device="cuda"), window=(3, 3), sinks=1)
-        assert out.shape == (B, nq, 2, 32) and torch.count_nonzero(out) == 0
-        out.sum().backward()
-        for t in leaves:
-            assert t.grad.shape == t.shape and torch.count_nonzero(t.grad) == 0
+        for window, sinks in (((3, 3), 1), ((0, 0), 0), ((None, 0), 0)):
+            out = gaussian_attention(*leaves, torch.ones(B, nk, dtype=torch.bool, device="cuda"), window=window, sinks=sinks)
+            assert out.shape == (B, nq, 2, 32) and torch.count_nonzero(out) == 0
+            for g in torch.autograd.grad(out.sum(), leaves):
+                assert torch.count_nonzero(g) == 0
 
 
 def test_partial_gradients():
