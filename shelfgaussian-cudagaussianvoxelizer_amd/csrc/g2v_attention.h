@@ -460,6 +460,11 @@ struct WinFwd : AttnFwd {
 };
 struct WinBwd : AttnBwd {
     AttnWindow win;      // dk and dv have the gap, too
+    // dQ's kernel makes delta from the output and what rounding took from it (or null), and leaves it and lse, padded, for dK and
+    // dV; without a dq it does that alone
+    const void *out, *rest;
+    const float* lse_in;    // (batch, hq, nq)
+    float *lse_pad, *delta_pad;
     bool all_queries;    // dK and dV: of the sinks, from every query that sees them (else of all keys, from those within the window)
 };
 

@@ -186,5 +186,59 @@ struct WaveBlocks {
     }
 };
 
+// Eight float32 values as three bfloat16 planes, exact to 24 bits.  A finite value above the largest bfloat16 starts with that (what
+// is left is small); an infinity is its first plane alone.
+constexpr float kMaxBf16 = 0x1.fep127f;
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void split_planes(const f32x8 x, bf16x8 (&o)[3]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+    const bool large = most > kMaxBf16;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float r = x[j];
+#pragma unroll
+        for (int pl = 0; pl < 3; ++pl) {
+            const __bf16 h = (__bf16)r;
+            o[pl][j] = h;
+            r -= (float)h;
+        }
+    }
+    if (large) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float r = x[j], h = (float)(__bf16)r;
+            if (!__builtin_isfinite(h) && __builtin_isfinite(r)) h = copysignf(kMaxBf16, r);
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl) {
+                o[pl][j] = (__bf16)h;
+                r = __builtin_isfinite(h) ? r - h : 0.0f;
+                h = (float)(__bf16)r;
+            }
+        }
+    }
+}
+// Values 8 c .. 8 c + 7 of a row of dim, zeros past its end or without a row.
+template <typename T>
+__device__ __forceinline__ f32x8 load_floats(const T* row, bool have, int c, int dim) {
+    constexpr int N = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (have && 8 * c + 8 <= dim) {
+#pragma unroll
+        for (int h = 0; h < 8; h += N) {
+            const vec v = *reinterpret_cast<const vec*>(row + 8 * c + h);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[h + j] = (float)v[j];
+        }
+    } else if (have) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (8 * c + j < dim) x[j] = (float)row[8 * c + j];
+    }
+    return x;
+}
+
 }  // namespace attn
 }  // namespace g2v

@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
 
     bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
     KeyRange see[NQB];
-    float lse[NQB], delta[NQB];    // delta: negative, as it is stored, and times scale
+    float lse[NQB], delta[NQB];    // delta = sum_d dO O, negative and times scale
 #pragma unroll
     for (int b = 0; b < NQB; ++b) {
         const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
@@ -53,9 +53,37 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
                 g[b][ks][pl] = mem_frag<DP>(grow, r < rows, a.g.chunks, pl, ks);
             }
         const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
-        lse[b] = a.lse[at];
-        delta[b] = a.delta[at] * a.scale;
+        lse[b] = a.lse_in[((int64_t)w.b * a.hq + head) * a.nq + tok];
+        const int64_t orow = (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+        float sum = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            f32x8 o = load_floats(static_cast<const T*>(a.out) + orow, r < rows, 2 * ks + half, a.dim);
+            if (sizeof(T) == 2 && a.rest) o += load_floats(static_cast<const T*>(a.rest) + orow, r < rows, 2 * ks + half, a.dim);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float x = (float)g[b][ks][0][j];
+#pragma unroll
+                for (int pl = 1; pl < NP; ++pl) x += (float)g[b][ks][pl][j];
+                sum = fmaf(o[j], x, sum);
+            }
+        }
+        sum = half_sum(sum);
+        delta[b] = -sum * a.scale;
+        if (w.split == 0 && half == 0 && r < rows) {
+            a.lse_pad[at] = lse[b];
+            a.delta_pad[at] = -sum;
+        }
     }
+    if (w.split == 0 && (w.tile + 1) * (NW * NQB * 32) >= rows) {    // the heads' padding
+        const int pad = a.nqp - a.nq;
+        for (int i = threadIdx.x; i < a.group * pad; i += NT) {
+            const int64_t at = ((int64_t)w.b * a.hq + w.h * a.group + i / pad) * a.nqp + a.nq + i % pad;
+            a.lse_pad[at] = INFINITY;
+            a.delta_pad[at] = 0.0f;
+        }
+    }
+    if (!a.dq) return;    // dK and dV alone are wanted
 
     TileT ktile, vtile;
     ktile.init(a.k);
@@ -432,7 +460,7 @@ __global__ void __launch_bounds__(256) k_window_zeros(WinBwd a, int64_t each, in
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 hipError_t dq_launch(const WinBwd& a, hipStream_t s) {
     G2V_LAUNCH((k_window_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
-    return launch_attn_dq_join(a, NP > 1, DP, s);
+    return a.dq ? launch_attn_dq_join(a, NP > 1, DP, s) : hipGetLastError();
 }
 template <int NP, int DP, int NQB, int KT, typename T>
 hipError_t dq_waves(const WinBwd& a, const AttnShape& g, hipStream_t s) {

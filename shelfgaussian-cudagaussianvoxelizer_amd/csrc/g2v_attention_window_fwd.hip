@@ -10,54 +10,6 @@ constexpr int window_fwd_per_cu(int np, int dp, int waves) {
     return np == 1 && waves > 1 ? (dp == 32 ? 4 : dp > 96 ? 2 : 3) : fwd_per_cu(np, dp, waves);
 }
 
-// Eight float32 values as three bfloat16 planes, exact to 24 bits.  A finite value above the largest bfloat16 starts with that (what
-// is left is small); an infinity is its first plane alone.
-constexpr float kMaxBf16 = 0x1.fep127f;
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ void split_planes(const f32x8 x, bf16x8 (&o)[3]) {
-    float most = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-    const bool large = most > kMaxBf16;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float r = x[j];
-#pragma unroll
-        for (int pl = 0; pl < 3; ++pl) {
-            const __bf16 h = (__bf16)r;
-            o[pl][j] = h;
-            r -= (float)h;
-        }
-    }
-    if (large) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float r = x[j], h = (float)(__bf16)r;
-            if (!__builtin_isfinite(h) && __builtin_isfinite(r)) h = copysignf(kMaxBf16, r);
-#pragma unroll
-            for (int pl = 0; pl < 3; ++pl) {
-                o[pl][j] = (__bf16)h;
-                r = __builtin_isfinite(h) ? r - h : 0.0f;
-                h = (float)(__bf16)r;
-            }
-        }
-    }
-}
-// Values 8 c .. 8 c + 7 of a row of dim, zeros past its end or without a row.
-__device__ __forceinline__ f32x8 load_floats(const float* row, bool have, int c, int dim) {
-    typedef f32x4 any_f32x4 __attribute__((aligned(4)));
-    f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (have && 8 * c + 8 <= dim) {
-        const f32x4 lo = *reinterpret_cast<const any_f32x4*>(row + 8 * c), hi = *reinterpret_cast<const any_f32x4*>(row + 8 * c + 4);
-        x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    } else if (have) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (8 * c + j < dim) x[j] = row[8 * c + j];
-    }
-    return x;
-}
-
 // A tile of float32 rows on its way to LDS (as Tile's three planes): in registers while the tile before it is computed.
 template <int DP, int ROWS, int NT>
 struct FloatTile {

@@ -701,8 +701,6 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
     const AttnBwdWs w = carve_win_bwd(c, x, r);
     attn::RowSrc src[4];
     G2V_HIP(win_sources(x, t, 4, packed, key_mask, c, src, s));
-    G2V_HIP(launch_attn_delta(batch, n_q, w.nqp, heads_q, head_dim, out, out_rest, grad_out, sg[0], sg[1], sg[2], z.f32, lse, w.lse,
-                              w.delta, s));
     WinBwd a = {};
     a.q = src[0];
     a.k = src[1];
@@ -729,6 +727,19 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
     a.win = x.w;
     a.win.mask = key_mask;
     a.win.skip = packed ? 0 : x.w.gap;
+    a.out = out;
+    a.rest = out_rest;
+    a.lse_in = lse;
+    a.lse_pad = w.lse;
+    a.delta_pad = w.delta;
+    if (queries) {
+        a.parts = r.dq.parts;
+        if (!grad_q) {
+            a.parts.head = 0;
+            a.parts.splits = 1;
+        }
+        G2V_HIP(launch_window_dq(a, z.f32, z.dp, s));
+    }
     if (grad_k && keys) {
         G2V_HIP(launch_window_zeros(a, batch, z.f32, s));
         WinBwd kv = a;
@@ -740,10 +751,6 @@ int g2v_window_attention_backward(int batch, int n_q, int n_k, int heads_q, int 
             kv.parts = r.sinks.parts;
             G2V_HIP(launch_window_dkv(kv, z.f32, z.dp, r.planes, s));
         }
-    }
-    if (grad_q && queries) {
-        a.parts = r.dq.parts;
-        G2V_HIP(launch_window_dq(a, z.f32, z.dp, s));
     }
     return G2V_OK;
 }
