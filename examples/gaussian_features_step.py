@@ -2,8 +2,10 @@
 voxelizer splats them, and the feature cosine loss against a target grid trains the layer and the Gaussians' means.
 
     python examples/gaussian_features_step.py [--gaussians 2000] [--scenes 2] [--channels 64] [--steps 5] [--bf16]
+                                              [--window 256] [--clip 35]
 
-Synthetic scenes, random weights.  Prints the loss of every step.
+With --window the Gaussians are sorted along a space-filling curve, and each attends to that many before and behind it and to the
+first ones.  The gradients' norm is clipped.  Synthetic scenes, random weights.  Prints the loss of every step.
 """
 import argparse
 import os
@@ -15,19 +17,35 @@ import torch.nn as nn
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "shelfgaussian-cudagaussianvoxelizer_amd"))
 
-from CudaGaussianVoxelizer import PyCudaFeatsCosineLoss, PyCudaGaussianVoxelizer, PyGaussianAttention  # noqa: E402
+from CudaGaussianVoxelizer import (PyCudaFeatsCosineLoss, PyCudaGaussianVoxelizer, PyGaussianAttention,  # noqa: E402
+                                   PyLayerNorm, clip_grad_norm_)
 
 VOXEL = [0.4, 0.4, 0.4]
 RANGE = [-10.0, -10.0, -1.0, 10.0, 10.0, 2.2]
 
 
+SINKS = 4
+
+
+def curve_order(means):
+    """Order of each scene's Gaussians (B, N) along a Z-order curve: 10 bits of each coordinate, interleaved."""
+    lo, hi = torch.tensor(RANGE[:3], device="cuda"), torch.tensor(RANGE[3:], device="cuda")
+    cell = ((means - lo) / (hi - lo) * 1024).long().clamp(0, 1023)
+    code = torch.zeros_like(cell[..., 0])
+    for bit in range(10):
+        for axis in range(3):
+            code |= (cell[..., axis] >> bit & 1) << (3 * bit + axis)
+    return code.argsort(-1)
+
+
 class GaussianFeatures(nn.Module):
     """Residual attention over the Gaussians of each scene, then a projection to the splatted channels."""
 
-    def __init__(self, channels, heads, dtype):
+    def __init__(self, channels, heads, dtype, window=None):
         super().__init__()
-        self.attention = PyGaussianAttention(channels, heads, wavelengths=(0.8, 40.0), dtype=dtype)
-        self.norm = nn.LayerNorm(channels, device="cuda", dtype=dtype)
+        near = {} if window is None else dict(window=(window, window), sinks=SINKS)
+        self.attention = PyGaussianAttention(channels, heads, wavelengths=(0.8, 40.0), dtype=dtype, **near)
+        self.norm = PyLayerNorm(channels, dtype=dtype)
         self.head = nn.Linear(channels, channels, device="cuda", dtype=dtype)
 
     def forward(self, x, means, valid):
@@ -35,7 +53,7 @@ class GaussianFeatures(nn.Module):
         return self.head(x)
 
 
-def train(gaussians=2000, scenes=2, channels=64, steps=5, bf16=False, seed=0):
+def train(gaussians=2000, scenes=2, channels=64, steps=5, bf16=False, seed=0, window=None, clip=35.0):
     """The losses of `steps` steps."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     torch.manual_seed(seed)
@@ -45,7 +63,10 @@ def train(gaussians=2000, scenes=2, channels=64, steps=5, bf16=False, seed=0):
         return torch.rand(*shape, generator=g, device="cuda")
 
     lo, hi = torch.tensor(RANGE[:3], device="cuda"), torch.tensor(RANGE[3:], device="cuda")
-    means = (lo + (hi - lo) * rand(scenes, gaussians, 3)).requires_grad_()
+    means = lo + (hi - lo) * rand(scenes, gaussians, 3)
+    if window is not None:
+        means = means.gather(1, curve_order(means)[..., None].expand_as(means))
+    means.requires_grad_()
     opacity = rand(scenes, gaussians)
     variance = 0.2 + rand(scenes, gaussians, 3)
     covariances = torch.diag_embed(variance).flatten(2)
@@ -55,7 +76,7 @@ def train(gaussians=2000, scenes=2, channels=64, steps=5, bf16=False, seed=0):
     valid = torch.arange(gaussians, device="cuda") < count[:, None]
     opacity = opacity * valid
 
-    model = GaussianFeatures(channels, max(1, channels // 32), dtype)
+    model = GaussianFeatures(channels, max(1, channels // 32), dtype, window)
     voxelizer = PyCudaGaussianVoxelizer(voxel_size=VOXEL, voxel_range=RANGE)
     cosine = PyCudaFeatsCosineLoss(voxel_size=VOXEL, voxel_range=RANGE)
     optimizer = torch.optim.Adam([{"params": model.parameters(), "lr": 1e-2}, {"params": [means], "lr": 1e-2}])
@@ -73,6 +94,7 @@ def train(gaussians=2000, scenes=2, channels=64, steps=5, bf16=False, seed=0):
         optimizer.zero_grad()
         with torch.autograd.set_multithreading_enabled(False):   # one GPU: no waiting for the engine's thread
             loss.backward()
+        clip_grad_norm_([*model.parameters(), means], clip)
         optimizer.step()
         losses.append(float(loss.detach()))
     return losses
@@ -85,6 +107,8 @@ def main():
     p.add_argument("--channels", type=int, default=64)
     p.add_argument("--steps", type=int, default=5)
     p.add_argument("--bf16", action="store_true")
+    p.add_argument("--window", type=int)
+    p.add_argument("--clip", type=float, default=35.0)
     for i, loss in enumerate(train(**vars(p.parse_args()))):
         print(f"step {i}: loss {loss:.5f}", flush=True)
 
