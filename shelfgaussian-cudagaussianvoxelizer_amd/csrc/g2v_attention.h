@@ -457,6 +457,7 @@ struct AttnWindow {
 };
 struct WinFwd : AttnFwd {
     AttnWindow win;
+    bool floats;    // float32 rows in place: the kernel splits them into planes
 };
 struct WinBwd : AttnBwd {
     AttnWindow win;      // dk and dv have the gap, too

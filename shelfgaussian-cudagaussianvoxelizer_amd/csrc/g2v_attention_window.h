@@ -3,16 +3,22 @@
 //   [0, min(sinks, p + right + 1))  and  [p - left, p + right],
 //
 // those among them that the mask keeps, and O, dQ, dK and dV are those of g2v_attention_fwd.hip and g2v_attention_bwd.hip over
-// these keys.  A wave's 32 or 64 rows see a range of keys little longer than a window, so a workgroup walks the tiles of the
-// sinks and then those of its rows' ranges, and a wave skips the tiles that none of its rows sees.  Where a tile lies inside
-// every row's range no score is looked at; at the range's ends a lane makes 32 bits of what its row sees of a block of 32 keys, and
-// an operation spreads one of them over a register (v_bfe) and another lets the score through or not (v_bfi).  Masked keys are
-// not packed away: the word of a tile's 64 valid keys is in a scalar register, their rows alone are loaded, and zeros stand in
-// the other rows' place, as what they hold may be NaN.
+// these keys.  A wave's 32 rows see a range of keys little longer than a window, so a workgroup walks the tiles of the
+// sinks and then those of its rows' ranges, and a wave skips the blocks of 32 keys that none of its rows sees.  Where a block lies
+// inside every row's range no score is looked at; at the range's ends a lane makes 32 bits of what its row sees of the block, one
+// operation spreads one of them over a register and another lets the score through or not.  Masked keys are not packed away: the word
+// of a tile's valid keys is in scalar registers, their rows alone are loaded, and zeros stand in the other rows' place, as what they hold
+// may be NaN.
 //
 // For dK and dV keys are in the lanes and a key's queries are a range, too: p - right .. p + left, and for a sink all from
 // p - right on.  As that would have one workgroup walk all queries, the sinks' gradients are computed again by one-wave
 // workgroups that share out the queries, and joined.
+//
+// Bound by memory at the shortest windows and then, like the attention over all keys, by matrix and vector work taking turns:
+// 200,000 x 8 heads x 64 bfloat16, windows of 1 / 513 / 2049 keys, us: forward that a backward follows 260, 398, 1096 (1.0 GB: 200 at a
+// copy's rate; a key more for every query takes 0.44, 930 TFLOP/s), dQ with delta 375, 626, 1781, dK and dV 261, 735, 1807.  One block of
+// 32 rows a wave and three workgroups a CU where the attention over all keys takes two and two: a row block's range is shorter
+// than two blocks' together, and their prologues and ends hide one another (forward 726 -> 504, dQ 831 -> 561 us).
 #pragma once
 #include "g2v_attention.h"
 
@@ -134,16 +140,28 @@ struct WinTile {
     __device__ __forceinline__ static uint32_t dst(uint32_t lds, int it) {
         return lds + it * NT * 16 + (uint32_t)g2v::uniform(threadIdx.x >> 6) * 1024;
     }
-    uint32_t off[kIter];    // of its chunk from the tile's first row
+    static constexpr bool kKept = kIter <= 5;     // (more of them are spilled: see load)
+    uint32_t off[kKept ? kIter : 1];    // of its chunk from the tile's first row
     __device__ __forceinline__ void init(const RowSrc& s) {
+        if constexpr (kKept)
 #pragma unroll
-        for (int it = 0; it < kIter; ++it) off[it] = (uint32_t)row(it) * (uint32_t)s.sn + chunk(it, s.chunks);
+            for (int it = 0; it < kIter; ++it) off[it] = (uint32_t)row(it) * (uint32_t)s.sn + chunk(it, s.chunks);
     }
-    // The rows from p on, all of them there.
-    __device__ __forceinline__ void load(const char* p, uint32_t lds) const {
+    // The rows from p on, all of them there.  (Many offsets are made anew for each tile: 40,000 x 8 heads in float32, dK and dV at 128
+    // channels 2.01 -> 1.44 ms, what eight sinks take at 96 channels 0.31 -> 0.13.)
+    __device__ __forceinline__ void load(const RowSrc& s, const char* p, uint32_t lds) const {
+        int tid = threadIdx.x;
+        if constexpr (!kKept) asm volatile("" : "+v"(tid));    // so that the compiler keeps no offset over the loop either
 #pragma unroll
-        for (int it = 0; it < kIter; ++it)
-            if (on(it)) dma16(p, off[it], dst(lds, it));
+        for (int it = 0; it < kIter; ++it) {
+            if (!on(it)) continue;
+            if constexpr (kKept) {
+                dma16(p, off[it], dst(lds, it));
+            } else {
+                const int L = it * NT + tid, pl = L / (ROWS * C), r = L % (ROWS * C) / C, c = swz<DP>(r, L % C);
+                dma16(p, (uint32_t)r * (uint32_t)s.sn + (uint32_t)(pl * C + min(c, s.chunks - 1)) * 16, dst(lds, it));
+            }
+        }
     }
     // Rows j0 .. of base, those of the word's bits; zeros in the others' place, nothing where there are none.  Rows from `sinks` on
     // are `skip` rows further.
@@ -232,7 +250,7 @@ __device__ __forceinline__ f32x8 load_floats(const T* row, bool have, int c, int
 #pragma unroll
             for (int j = 0; j < N; ++j) x[h + j] = (float)v[j];
         }
-    } else if (have) {
+    } else if (have && 8 * c < dim) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (8 * c + j < dim) x[j] = (float)row[8 * c + j];

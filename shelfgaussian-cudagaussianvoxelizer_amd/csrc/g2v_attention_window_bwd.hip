@@ -7,7 +7,7 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-// Workgroups that share a CU, as in g2v_attention.h, and blocks of 32 rows a wave.
+// Workgroups that share a CU, as in g2v_attention.h, at one block of rows a wave.
 constexpr int window_dq_per_cu(int np, int dp, int waves) {
     return np == 1 && waves > 1 && dp <= 64 ? (dp == 32 ? 4 : 3) : dq_per_cu(np, dp, waves);
 }
@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     auto load = [&](int u, int buf) __attribute__((always_inline)) {
         const int t = tiles.at(u), j0 = t * KT;
         if (words.all(t)) {
-            ktile.load(kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
-            vtile.load(vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
+            ktile.load(a.k, kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
+            vtile.load(a.v, vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
             return Words::kAll;
         }
         const uint64_t word = words.at(a.win, tiles, a.nk, w.b, u, u1);
@@ -218,9 +218,12 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     }
 }
 
-// The sinks' one-wave workgroups: as many to a CU as their tiles' LDS allows.
+// Two workgroups a CU from 64 channels on (three spill at 64: 18,000 x 16 x 64, 1025 keys a window, 267 -> 191 us).  The sinks' one-wave
+// workgroups: as many as their tiles' LDS allows.
 constexpr int window_dkv_per_cu(int np, int ns, int dp, int nw) {
-    return nw > 1 && np == 1 && dp >= 64 ? 2 : nw > 1 ? dkv_per_cu(np, ns, dp) : np > 1 ? (dp > 96 ? 1 : dp > 32 ? 2 : 4) : dp > 64 ? 3 : dp > 32 ? 6 : 8;
+    if (nw > 1) return np == 1 && dp >= 64 ? 2 : dkv_per_cu(np, ns, dp);
+    if (np > 1) return dp > 96 ? 1 : dp > 64 ? 2 : dp > 32 ? 3 : 6;
+    return dp > 64 ? 3 : dp > 32 ? 6 : 8;
 }
 constexpr int dkv_bound(int np, int ns, int dp, int nw) { return nw > 1 ? window_dkv_per_cu(np, ns, dp, nw) : np > 1 && dp > 32 ? 1 : 2; }
 
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
     constexpr int NPP = NP;
     constexpr int NT = NW * 64, QB = QT / 32, DB = DP / 32;
     typedef WinTile<NP, DP, QT, NT> TileT;
-    constexpr int kBuffers = buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
+    constexpr int kBuffers = NP > 1 && NW == 1 ? 2 : buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
     constexpr int kStats = NW == 1 ? 2 : 1;    // loads of statistics a wave
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     __shared__ __attribute__((aligned(16))) float stat[kBuffers][2][64];   // lse and -delta of the tile's rows
@@ -299,8 +302,8 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
         const char* qbase = a.q.p + w.b * a.q.sb + head * a.q.sh;
         const char* gbase = a.g.p + w.b * a.g.sb + head * a.g.sh;
         if ((t + 1) * QT <= a.nq) {
-            qtile.load(qbase + (int64_t)t * QT * a.q.sn, lds_off(lds[buf][0]));
-            gtile.load(gbase + (int64_t)t * QT * a.g.sn, lds_off(lds[buf][1]));
+            qtile.load(a.q, qbase + (int64_t)t * QT * a.q.sn, lds_off(lds[buf][0]));
+            gtile.load(a.g, gbase + (int64_t)t * QT * a.g.sn, lds_off(lds[buf][1]));
         } else {
             TileT::load_tail(a.q, qbase, t * QT, a.nq, lds_off(lds[buf][0]));
             TileT::load_tail(a.g, gbase, t * QT, a.nq, lds_off(lds[buf][1]));

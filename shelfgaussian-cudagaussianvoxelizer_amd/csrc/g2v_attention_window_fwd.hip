@@ -5,7 +5,9 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-// Workgroups that share a CU, as in g2v_attention.h.
+// Workgroups that share a CU, as in g2v_attention.h, at one block of rows a wave.  (With two blocks at 32 channels and at 128, where
+// they spill, 60,000 x 16 x 32 and 40,000 x 8 x 128 take 315 and 981 us instead of 193 and 190; 96 channels with two workgroups a CU 148
+// instead of 135; 64 channels with four 517 instead of 410, 200,000 x 8.)
 constexpr int window_fwd_per_cu(int np, int dp, int waves) {
     return np == 1 && waves > 1 ? (dp == 32 ? 4 : dp > 96 ? 2 : 3) : fwd_per_cu(np, dp, waves);
 }
@@ -43,12 +45,14 @@ struct FloatTile {
 };
 
 // As k_attn_fwd (rows in the lanes, keys in the registers).
-template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+// FLOATS: q, k and v are float32 rows, split into planes here; else bfloat16 rows, planes packed before.
+template <int NP, bool FLOATS, int DP, int KS, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP, DP, NW))) k_window_fwd(WinFwd a) {
+    static_assert(!FLOATS || NP == 3, "planes of float32");
     constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
     typedef WinTile<NP, DP, KT, NT> TileT;
     typedef TileWords<KT> Words;
-    constexpr int kBuffers = NP > 1 ? 2 : buffers(window_fwd_per_cu(NP, DP, NW), TileT::kBytes), kAhead = kBuffers - 1;
+    constexpr int kBuffers = FLOATS ? 2 : buffers(NP > 1 ? 2 : window_fwd_per_cu(NP, DP, NW), TileT::kBytes), kAhead = kBuffers - 1;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers][2][TileT::kBytes];
     static_assert(window_fwd_per_cu(NP, DP, NW) * sizeof(lds) <= kLdsBytes, "planned by more workgroups than fit");
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
@@ -77,17 +81,18 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         l[b] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (NP > 1) {
+            if constexpr (FLOATS) {
                 split_planes(load_floats(reinterpret_cast<const float*>(row), r < rows, 2 * ks + half, a.dim), q[b][ks]);
             } else {
-                q[b][ks][0] = mem_frag<DP>(row, r < rows, a.q.chunks, 0, ks);
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) q[b][ks][pl] = mem_frag<DP>(row, r < rows, a.q.chunks, pl, ks);
             }
         }
     }
 
     TileT ktile, vtile;
     FloatTile<DP, KT, NT> kfloat, vfloat;
-    if constexpr (NP == 1) {
+    if constexpr (!FLOATS) {
         ktile.init(a.k);
         vtile.init(a.v);
     }
@@ -99,15 +104,15 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     const char* vfar = vbase + (int64_t)a.win.skip * a.v.sn;
     auto load = [&](int u, int buf) __attribute__((always_inline)) {
         const int t = tiles.at(u), j0 = t * KT;
-        if constexpr (NP > 1) {    // into registers
+        if constexpr (FLOATS) {    // into registers
             const uint64_t word = words.all(t) ? Words::kAll : words.at(a.win, tiles, a.nk, w.b, u, u1);
             kfloat.fetch(a.k, kbase, a.dim, j0, word, a.win.sinks, a.win.skip);
             vfloat.fetch(a.v, vbase, a.dim, j0, word, a.win.sinks, a.win.skip);
             return word;
         }
         if (words.all(t)) {
-            ktile.load(kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
-            vtile.load(vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
+            ktile.load(a.k, kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
+            vtile.load(a.v, vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
             return Words::kAll;
         }
         const uint64_t word = words.at(a.win, tiles, a.nk, w.b, u, u1);
@@ -123,8 +128,8 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][b][i] = 0.0f;
-    auto store = [&](int buf) __attribute__((always_inline)) {    // float32: from registers to LDS
-        if constexpr (NP > 1) {
+    auto store = [&](int buf) __attribute__((always_inline)) {    // from registers to LDS
+        if constexpr (FLOATS) {
             kfloat.store(lds[buf][0]);
             vfloat.store(lds[buf][1]);
         }
@@ -137,7 +142,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     if (kAhead > 1 && u0 + 1 < u1) next = load(u0 + 1, 1);
     for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
         // (a partly valid tile's loads are not the same number for every wave)
-        next_tile<kBuffers, (NP > 1 ? 0 : 2 * TileT::kLoads)>(u + 1 < u1 && words.all(tiles.at(u + 1)));
+        next_tile<kBuffers, (FLOATS ? 0 : 2 * TileT::kLoads)>(u + 1 < u1 && words.all(tiles.at(u + 1)));
         after = 0;
         if (u + kAhead < u1) {
             const uint64_t x = load(u + kAhead, buf == 0 ? kBuffers - 1 : buf - 1);
@@ -297,7 +302,13 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
 
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 hipError_t fwd_launch(const WinFwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_window_fwd<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    const dim3 grid((unsigned)workgroups(a.parts, a.bhs)), block(NW * 64);
+    if constexpr (NP > 1) {
+        if (a.floats) G2V_LAUNCH((k_window_fwd<NP, true, DP, KS, NQB, NW, KT, T>), grid, block, 0, s, a);
+        else G2V_LAUNCH((k_window_fwd<NP, false, DP, KS, NQB, NW, KT, T>), grid, block, 0, s, a);
+    } else {
+        G2V_LAUNCH((k_window_fwd<NP, false, DP, KS, NQB, NW, KT, T>), grid, block, 0, s, a);
+    }
     return launch_attn_join(a, NP > 1, DP, s);
 }
 template <int NP, int DP, int NQB, int KT, typename T>

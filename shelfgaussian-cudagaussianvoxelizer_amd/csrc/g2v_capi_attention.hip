@@ -344,6 +344,14 @@ int win_sizes(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_di
 int64_t win_keys(const WinSizes& x, AttnShape g) {
     return std::min<int64_t>(x.z.nk, x.span + g.waves * g.blocks * 32 / x.z.group + (x.w.sinks ? g.tile : 0));
 }
+// Whether the forward splits float32 rows into planes as it loads them, every workgroup that sees a row for itself, instead of
+// reading planes packed before.  Short windows: a launch and a pass over the rows less; long ones: each row is split again and again.
+// (40,000 x 8 heads, windows of 256 / 1024 / 2048 keys, packed and split us: 64 channels 312, 648, 1037 and 217, 567, 1043; 128
+// channels 804, 1629, 2652 and 587, 1516, 2762; 96 channels 598, 1136, 1858 and 523, 1367, 2499; 72 channels 599, 1124, 1835 and 653,
+// 1576, 2769.  Rows that are not whole chunks of 8 load their ends one by one: 75 channels 649, 1166, 1867 and 821, 2014, 3446.)
+bool win_splits_rows(const WinSizes& x) {
+    return x.z.dim % 8 == 0 && win_keys(x, window_fwd_shape(true, x.z.dp, x.z.rows())) <= (x.z.dp == 96 ? 384 : 1024);
+}
 AttnRun win_fwd_run(const WinSizes& x) {
     const AttnShape g = window_fwd_shape(x.z.f32, x.z.dp, x.z.rows());
     return attn_run(x.z, g, x.z.rows(), win_keys(x, g), 1, x.z.dp, false);
@@ -370,10 +378,9 @@ AttnRun win_sinks_run(const WinSizes& x, int planes) {
     r.tiles = r.head = (int)ceil_div(x.w.sinks, 32);
     r.row0 = x.w.sinks;
     r.splits = 1;
-    const int units = (int)std::min<int64_t>(ceil_div(x.z.nq, g.tile) * x.z.group, 1 << 30);
-    const double unit_us = std::max(1.0, 2.0 * g.products * 32 * g.tile * x.z.dp * g.per_cu / ((x.z.f32 ? 0.15e9 : 1.0e9) / kCus));
-    double least;
-    r.head_splits = attn_splits((int64_t)x.z.bhs * r.tiles, units, g.per_cu, unit_us, 8.0 * x.w.sinks * x.z.bhs * 2 * x.z.dp / 3e6, least);
+    // as many workgroups as the card holds, of four tiles at least (200,000 queries x 8 heads x 64, 192 for 128: 116 -> 92 us)
+    const int64_t units = ceil_div(x.z.nq, g.tile) * x.z.group, most = kCus * g.per_cu / std::max<int64_t>((int64_t)x.z.bhs * r.tiles, 1);
+    r.head_splits = (int)std::max<int64_t>(1, std::min(units / 4, most));
     return {r, part_rows(r, x.z.bhs, x.w.sinks)};
 }
 
@@ -598,7 +605,7 @@ size_t g2v_window_attention_forward_workspace(int batch, int n_q, int n_k, int h
                                               int left, int right, int sinks, int in_place, int masked) {
     WinSizes x;
     if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, x) != G2V_OK) return 0;
-    return win_fwd_bytes(x, win_fwd_run(x), !x.z.f32 && !in_place);
+    return win_fwd_bytes(x, win_fwd_run(x), x.z.f32 ? !win_splits_rows(x) : !in_place);
 }
 
 int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -622,8 +629,7 @@ int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int h
     const Strided t[3] = {{q, q_strides, n_q, heads_q, false},
                           {k, keys ? k_strides : none, z.nk, heads_k, true},
                           {v, keys ? v_strides : none, z.nk, heads_k, true}};
-    // (the forward splits float32 rows into planes on their way)
-    const bool packed = !z.f32 && !attn_in_place(z, t, 3);
+    const bool packed = z.f32 ? !win_splits_rows(x) : !attn_in_place(z, t, 3);
     if (!keys) key_mask = nullptr;
     const AttnRun r = win_fwd_run(x);
     const size_t need = win_fwd_bytes(x, r, packed);
@@ -654,6 +660,7 @@ int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int h
     a.win = x.w;
     a.win.mask = key_mask;
     a.win.skip = packed ? 0 : x.w.gap;
+    a.floats = z.f32 && !packed;
     G2V_HIP(launch_window_fwd(a, z.f32, z.dp, s));
     return G2V_OK;
 }

@@ -66,6 +66,9 @@ def test_window_workspaces(query):
             base = q(1, n, n, 8, 4, 64, BF16, left, right, sinks, 1, 0)
             assert 0 < base < 1 << 40 and 0 < q(1, n, n, 8, 4, 64, BF16, left, right, sinks, 1, 1) < 1 << 40
             assert base < q(1, n, n, 8, 4, 64, BF16, left, right, sinks, 0, 0) and 0 < q(1, n, n, 8, 4, 64, F32, left, right, sinks, 1, 0)
+    for B, nq, nk in ((0, 5, 5), (2, 0, 500), (2, 500, 0), (0, 0, 0), (2, 0, 0)):     # nothing to do, with sinks too
+        for sinks in (0, 3):
+            assert q(B, nq, nk, 8, 4, 64, F32, 2, 0, sinks, 0, 1) > 0 and q(B, nq, nk, 8, 4, 64, BF16, 2, 0, sinks, 1, 0) > 0
     # a single query of a long stream needs room for its window, not for the stream
     lib = _lib()
     assert lib.g2v_window_attention_forward_workspace(1, 1, 200000, 8, 8, 64, F32, 512, 0, 4, 0, 1) < 1 << 23
