@@ -408,7 +408,8 @@ int g2v_attention_backward(int batch, int n_q, int n_k, int heads_q, int heads_k
  *     j <= p + right  and  (j >= p - left  or  j < sinks).
  * left, right: -1 for no bound.  right = 0 with a bound to the left is the window of a causal order, whose first `sinks`
  * keys stay visible.  p may be negative (n_q > n_k).  A query that sees no key gives 0 and no gradient.  Arguments, types and
- * limits as above; the mask is given to the backward again (no key_list); what a masked key's rows hold is never read.  A forward
+ * limits as above; the mask is given to the backward again (no key_list); what a masked key's rows hold is never read.  Valid
+ * rows have to be finite in either type: a NaN or an infinity may also reach rows near it that do not see it.  A forward
  * reads none of the keys between the sinks and the first query's window: one query costs what its window holds.
  * The gradients of the first `sinks` keys are sums over all queries that see them, in a fixed order.  Asynchronous. */
 size_t g2v_window_attention_forward_workspace(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, int dtype,

@@ -15,10 +15,11 @@
 // workgroups that share out the queries, and joined.
 //
 // Bound by memory at the shortest windows and then, like the attention over all keys, by matrix and vector work taking turns:
-// 200,000 x 8 heads x 64 bfloat16, windows of 1 / 513 / 2049 keys, us: forward that a backward follows 260, 398, 1096 (1.0 GB: 200 at a
-// copy's rate; a key more for every query takes 0.44, 930 TFLOP/s), dQ with delta 375, 626, 1781, dK and dV 261, 735, 1807.  One block of
-// 32 rows a wave and three workgroups a CU where the attention over all keys takes two and two: a row block's range is shorter
-// than two blocks' together, and their prologues and ends hide one another (forward 726 -> 504, dQ 831 -> 561 us).
+// 200,000 x 8 heads x 64 bfloat16, windows of 1 / 513 / 2049 keys, us: forward that a backward follows 260, 414, 1057 (its 1.0 GB
+// take 200 at a copy's rate; a key more for every query takes 0.42, 980 TFLOP/s), dQ with delta 373, 615, 1735, dK and dV 259, 725,
+// 1757.  A wave has one block of 32 rows and bfloat16 has more workgroups to a CU than the attention over all keys, as a row block's
+// range is shorter than two blocks' together, and prologues and ends hide one another: with that attention's blocks and workgroups
+// the forward takes 278, 478, 1062 and dQ 453, 747, 1795.
 #pragma once
 #include "g2v_attention.h"
 

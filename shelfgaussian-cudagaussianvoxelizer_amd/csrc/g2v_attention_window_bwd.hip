@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     }
 }
 
-// Two workgroups a CU from 64 channels on (three spill at 64: 18,000 x 16 x 64, 1025 keys a window, 267 -> 191 us).  The sinks' one-wave
-// workgroups: as many as their tiles' LDS allows.
+// Two workgroups a CU from 64 channels on: three spill where P and dS are in one plane (18,000 x 16 x 64, 1025 keys a window, 266 us
+// for 176).  The sinks' one-wave workgroups: as many as their tiles' LDS allows.
 constexpr int window_dkv_per_cu(int np, int ns, int dp, int nw) {
     if (nw > 1) return np == 1 && dp >= 64 ? 2 : dkv_per_cu(np, ns, dp);
     if (np > 1) return dp > 96 ? 1 : dp > 64 ? 2 : dp > 32 ? 3 : 6;

@@ -5,9 +5,9 @@ namespace g2v {
 namespace {
 using namespace attn;
 
-// Workgroups that share a CU, as in g2v_attention.h, at one block of rows a wave.  (With two blocks at 32 channels and at 128, where
-// they spill, 60,000 x 16 x 32 and 40,000 x 8 x 128 take 315 and 981 us instead of 193 and 190; 96 channels with two workgroups a CU 148
-// instead of 135; 64 channels with four 517 instead of 410, 200,000 x 8.)
+// Workgroups that share a CU, as in g2v_attention.h, at one block of rows a wave.  Windows of 513 keys and 8 sinks, us: 60,000 x 16
+// heads x 32, four 156 (two blocks, three workgroups, spilling: 330); 40,000 x 8 x 128, two 166 (two blocks, spilling: 937); 40,000 x 8
+// x 96, three 110 and two 121; 200,000 x 8 x 64 without sinks, three 392 and four, spilling, 594.
 constexpr int window_fwd_per_cu(int np, int dp, int waves) {
     return np == 1 && waves > 1 ? (dp == 32 ? 4 : dp > 96 ? 2 : 3) : fwd_per_cu(np, dp, waves);
 }

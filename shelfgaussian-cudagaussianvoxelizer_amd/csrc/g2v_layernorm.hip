@@ -5,11 +5,12 @@
 // Backward, from dy and the gradient ds that reaches s by another way, with xh = (s - m) r and g = w dy:
 //   dx = ds + r (g - mean g - xh mean(g xh))   (of x and of residual),   dw = sum over rows of dy xh,   db = sum of dy.
 //
-// Bound by bytes: 18000 x 1024 bfloat16 with a residual takes 27 us forward and 27 + 7 backward, 5.4 TB/s, a copy's rate (and more than
-// it, where inputs are still in the last cache).  A row is read once, held in registers, and the variance is taken from the differences to the mean (nothing
-// cancels).  A row goes to 2^shift lanes of a wave, up to two 16-byte vectors each, or to a workgroup where it is longer; the
-// next row is asked for before the present one is summed.  Weights stay in registers, as do, in the backward, the sums of dw and db
-// of a workgroup's rows: their parts go to memory once a workgroup, and k_layer_norm_sums adds them in a fixed order.
+// Bound by bytes: 18000 x 1024 bfloat16 with a residual takes 27 us forward and 27 + 7 backward, 5.4 TB/s, a copy's rate (and
+// more than it, where inputs are still in the last cache).  A row is read once, held in registers, and the variance is taken from
+// the differences to the mean (nothing cancels).  A row goes to 2^shift lanes of a wave, up to two 16-byte vectors each, or to a
+// workgroup where it is longer; the next row is asked for before the present one is summed.  Weights stay in registers, as do, in
+// the backward, the sums of dw and db of a workgroup's rows: their parts go to memory once a workgroup, and k_layer_norm_sums adds
+// them in a fixed order.
 #include <algorithm>
 
 #include "../../include/g2v.h"
