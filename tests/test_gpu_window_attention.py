@@ -274,15 +274,16 @@ def test_layouts(D, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", BOTH, ids=IDS)
 @pytest.mark.parametrize("masked", [False, True])
-def test_offsets_beyond_32_bits(masked):
+def test_offsets_beyond_32_bits(masked, dtype):
     """A long cache whose rows lie far apart: keys behind 4 GiB, reached from the sinks over the gap."""
     nk, stride, D = 70000, 40000, 64
-    base = torch.zeros((nk - 1) * stride + 2 * D, dtype=torch.bfloat16, device="cuda")
+    base = torch.zeros((nk - 1) * stride + 2 * D, dtype=dtype, device="cuda")
     assert base.numel() * 2 > 1 << 32
     k = torch.as_strided(base, (1, nk, 1, D), (base.numel(), stride, D, 1))
     v = torch.as_strided(base, (1, nk, 1, D), (base.numel(), stride, D, 1), D)
-    q, kc, vc, _ = (t.cuda() for t in make(1, 3, nk, 1, 1, D, torch.bfloat16, 2))
+    q, kc, vc, _ = (t.cuda() for t in make(1, 3, nk, 1, 1, D, dtype, 2))
     k.copy_(kc)
     v.copy_(vc)
     mask = random_mask(1, nk, 0.7, 5).cuda() if masked else None
@@ -291,7 +292,7 @@ def test_offsets_beyond_32_bits(masked):
     assert torch.equal(got, gaussian_attention(q, kc, vc, mask, window=(200, 0), sinks=5))
     keys = torch.cat([torch.arange(0, 5), torch.arange(nk - 400, nk)])
     small = [t[:, keys].contiguous() for t in (kc, vc)]
-    assert rel(got, plain(q, *small, (200, 0), 5, None if mask is None else mask[:, keys.cuda()])[0]) < TOL[torch.bfloat16][0]
+    assert rel(got, plain(q, *small, (200, 0), 5, None if mask is None else mask[:, keys.cuda()])[0]) < TOL[dtype][0]
 
 
 @pytest.mark.parametrize("dtype", BOTH, ids=IDS)
