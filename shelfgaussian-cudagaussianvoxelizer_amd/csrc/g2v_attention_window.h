@@ -15,11 +15,11 @@
 // workgroups that share out the queries, and joined.
 //
 // Bound by memory at the shortest windows and then, like the attention over all keys, by matrix and vector work taking turns:
-// 200,000 x 8 heads x 64 bfloat16, windows of 1 / 513 / 2049 keys, us: forward that a backward follows 260, 414, 1057 (its 1.0 GB
-// take 200 at a copy's rate; a key more for every query takes 0.42, 980 TFLOP/s), dQ with delta 373, 615, 1735, dK and dV 259, 725,
-// 1757.  A wave has one block of 32 rows and bfloat16 has more workgroups to a CU than the attention over all keys, as a row block's
-// range is shorter than two blocks' together, and prologues and ends hide one another: with that attention's blocks and workgroups
-// the forward takes 278, 478, 1062 and dQ 453, 747, 1795.
+// 200,000 x 8 heads x 64 bfloat16, windows of 1 / 513 / 2049 keys, us: forward that a backward follows 258, 398, 1059 (its 1.0 GB
+// take 200 at a copy's rate; a key more for every query takes 0.43, 950 TFLOP/s), dQ with delta 406, 595, 1713, dK and dV 315, 735,
+// 1750.  A wave has one block of 32 rows and bfloat16 has more workgroups to a CU than the attention over all keys, as a row block's
+// range is shorter than two blocks' together, and prologues and ends hide one another (with that attention's blocks and workgroups,
+// 513 keys: forward 478 for 414, dQ 747 for 615, before rows were loaded as below).
 #pragma once
 #include "g2v_attention.h"
 
@@ -82,17 +82,18 @@ struct TileWords {
         from = -64;
     }
     __device__ __forceinline__ bool all(int t) const { return (uint32_t)(t - whole0) < (uint32_t)whole; }
-    // Takes the keys that the mask does not keep out of the held words: a byte a lane for each unit, several units' loads at a time.
+    // Takes the keys that the mask does not keep out of the held words: a byte a lane for each unit, several units' loads at a time
+    // (repeated past the ends, where no held word has a bit).
     __device__ __forceinline__ void keep(const AttnWindow& w, const KeyTiles<KT>& tiles, int nk, int b, int u, int u1) {
         constexpr int kUnits = 8;
         const unsigned char* row = w.mask + (int64_t)b * (nk + w.gap);
-        const int lane = threadIdx.x & 63, n = min(64, u1 - u);
+        const int lane = threadIdx.x & 63, key = min(lane, KT - 1), n = min(64, u1 - u);
         for (int i0 = 0; i0 < n; i0 += kUnits) {
             unsigned char x[kUnits];
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int j = tiles.at(u + i0 + i) * KT + lane;
-                x[i] = i0 + i < n && lane < KT && j < nk ? row[j + (j >= w.sinks ? w.gap : 0)] : 0;
+                const int j = min(tiles.at(min(u + i0 + i, u1 - 1)) * KT + key, nk - 1);
+                x[i] = row[j + (j >= w.sinks ? w.gap : 0)];
             }
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
@@ -238,25 +239,72 @@ __device__ __forceinline__ void split_planes(const f32x8 x, bf16x8 (&o)[3]) {
         }
     }
 }
-// Values 8 c .. 8 c + 7 of a row of dim, zeros past its end or without a row.
-template <typename T>
-__device__ __forceinline__ f32x8 load_floats(const T* row, bool have, int c, int dim) {
-    constexpr int N = 16 / sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+// Values 8 c .. 8 c + 7 of a float32 row of whole chunks of 8, zeros past its end or without a row.
+__device__ __forceinline__ f32x8 load_floats(const float* row, bool have, int c, int dim) {
+    typedef float vec __attribute__((ext_vector_type(8), aligned(sizeof(float))));
     f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (have && 8 * c + 8 <= dim) {
+    if (have && 8 * c < dim) x = *reinterpret_cast<const vec*>(row + 8 * c);
+    return x;
+}
+// Values of a row of dim at any alignment, as float32: 16 ks + 8 half + 0 .. 7 for every step ks, zeros past its end.
+template <int KS, typename T>
+struct RowValues {
+    typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    vec x[KS];
+    T tail[8];    // what is behind the last whole 8
+    __device__ __forceinline__ void load(const T* row, int dim) {
+        const int half = (threadIdx.x >> 5) & 1, whole = dim / 8;
 #pragma unroll
-        for (int h = 0; h < 8; h += N) {
-            const vec v = *reinterpret_cast<const vec*>(row + 8 * c + h);
+        for (int j = 0; j < 8; ++j) tail[j] = (T)0.0f;
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[h + j] = (float)v[j];
-        }
-    } else if (have && 8 * c < dim) {
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[ks][j] = (T)0.0f;
+        if (whole > 0)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) x[ks] = *reinterpret_cast<const vec*>(row + 8 * min(2 * ks + half, whole - 1));
+        if (dim % 8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) tail[j] = row[min(8 * whole + j, dim - 1)];
+    }
+    __device__ __forceinline__ f32x8 at(int ks, int dim) const {
+        const int c = 2 * ks + ((threadIdx.x >> 5) & 1), whole = dim / 8;
+        f32x8 o;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (8 * c + j < dim) x[j] = (float)row[8 * c + j];
+            o[j] = c < whole ? (float)x[ks][j] : c == whole && j < dim % 8 ? (float)tail[j] : 0.0f;
+        return o;
     }
-    return x;
+};
+
+// A lane's row as B operands (mem_frag's), in two parts: the loads, which all go out before any is waited for, and what ends the wait
+// for them and puts zeros where there is no row or no chunk (the last step alone may lack some).  A wait that is left to a loop's first
+// use is waited for in every turn, and with it the tiles that are on their way.  Against mem_frag, dQ and dK with dV in us, windows of 513
+// keys: 200,000 x 8 heads x 64 618 -> 586 and 734 -> 726, 40,000 x 8 x 96 206 -> 186 and 245 -> 226, x 128 245 -> 224 and 524 -> 487.
+// (Windows of one key, whose tensors pass the last cache: 200,000 x 8 x 64 377 -> 406 and 260 -> 314; 33 keys 401 -> 399 and 348 -> 348.)
+template <int DP, int KS, int NP>
+__device__ __forceinline__ void load_row(const char* row, int chunks, bf16x8 (&x)[KS][NP]) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl)
+            x[ks][pl] = *reinterpret_cast<const bf16x8*>(row + (pl * (DP / 8) + min(2 * ks + half, chunks - 1)) * 16);
+}
+template <int KS, int NP>
+__device__ __forceinline__ void settle_row(bool have, int chunks, bf16x8 (&x)[KS][NP]) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) {
+            f32x4 v = __builtin_bit_cast(f32x4, x[ks][pl]);
+            asm volatile("" : "+v"(v));
+            const bool keep = have && (ks < KS - 1 || 2 * ks + half < chunks);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = keep ? v[e] : 0.0f;
+            x[ks][pl] = __builtin_bit_cast(bf16x8, v);
+        }
 }
 
 }  // namespace attn

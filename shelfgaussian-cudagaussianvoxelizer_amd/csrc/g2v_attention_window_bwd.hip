@@ -32,12 +32,14 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     tiles.init(a.win, a.nk, g2v::uniform(g0 / a.group), g2v::uniform(g1 / a.group));
     int u0, u1;
     split_range(tiles.all, w.split, w.splits, u0, u1);
+    if (!a.dq) u1 = u0;    // delta alone
     WaveBlocks blocks;
     blocks.init(a.win, a.nk, a.group, rows, first, NQB * 32, tiles.sinks * KT);
 
     bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
     KeyRange see[NQB];
     float lse[NQB], delta[NQB];    // delta = sum_d dO O, negative and times scale
+    RowValues<KS, T> out[NQB], rest[NQB];
 #pragma unroll
     for (int b = 0; b < NQB; ++b) {
         const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
@@ -45,21 +47,50 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
         const char* qrow = a.q.p + w.b * a.q.sb + tok * a.q.sn + head * a.q.sh;
         const char* grow = a.g.p + w.b * a.g.sb + tok * a.g.sn + head * a.g.sh;
         see[b] = key_range(a.win, a.nk, tok);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int pl = 0; pl < NP; ++pl) {
-                q[b][ks][pl] = mem_frag<DP>(qrow, r < rows, a.q.chunks, pl, ks);
-                g[b][ks][pl] = mem_frag<DP>(grow, r < rows, a.g.chunks, pl, ks);
-            }
-        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
+        load_row<DP>(qrow, a.q.chunks, q[b]);
+        load_row<DP>(grow, a.g.chunks, g[b]);
         lse[b] = a.lse_in[((int64_t)w.b * a.hq + head) * a.nq + tok];
         const int64_t orow = (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+        out[b].load(static_cast<const T*>(a.out) + orow, a.dim);
+        if (sizeof(T) == 2 && a.rest) rest[b].load(static_cast<const T*>(a.rest) + orow, a.dim);
+    }
+
+    TileT ktile, vtile;
+    ktile.init(a.k);
+    vtile.init(a.v);
+    Frags<DP> frags;
+    frags.init(lds_off(lds));
+    Words words;
+    words.init(a.win, a.nk);
+    const char* kfar = kbase + (int64_t)a.win.skip * a.k.sn;
+    const char* vfar = vbase + (int64_t)a.win.skip * a.v.sn;
+    auto load = [&](int u, int buf) __attribute__((always_inline)) {
+        const int t = tiles.at(u), j0 = t * KT;
+        if (words.all(t)) {
+            ktile.load(a.k, kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
+            vtile.load(a.v, vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
+            return Words::kAll;
+        }
+        const uint64_t word = words.at(a.win, tiles, a.nk, w.b, u, u1);
+        TileT::load_some(a.k, kbase, j0, word, a.win.sinks, a.win.skip, lds[buf][0]);
+        TileT::load_some(a.v, vbase, j0, word, a.win.sinks, a.win.skip, lds[buf][1]);
+        return word;
+    };
+    uint64_t word = 0, next = 0, after = 0;
+    if (u0 < u1) word = load(u0, 0);
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
+        const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
+        settle_row(r < rows, a.q.chunks, q[b]);
+        settle_row(r < rows, a.g.chunks, g[b]);
+        asm volatile("" : "+v"(lse[b]));
+        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
         float sum = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            f32x8 o = load_floats(static_cast<const T*>(a.out) + orow, r < rows, 2 * ks + half, a.dim);
-            if (sizeof(T) == 2 && a.rest) o += load_floats(static_cast<const T*>(a.rest) + orow, r < rows, 2 * ks + half, a.dim);
+            f32x8 o = out[b].at(ks, a.dim);
+            if (sizeof(T) == 2 && a.rest) o += rest[b].at(ks, a.dim);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float x = (float)g[b][ks][0][j];
@@ -85,28 +116,6 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     }
     if (!a.dq) return;    // dK and dV alone are wanted
 
-    TileT ktile, vtile;
-    ktile.init(a.k);
-    vtile.init(a.v);
-    Frags<DP> frags;
-    frags.init(lds_off(lds));
-    Words words;
-    words.init(a.win, a.nk);
-    const char* kfar = kbase + (int64_t)a.win.skip * a.k.sn;
-    const char* vfar = vbase + (int64_t)a.win.skip * a.v.sn;
-    auto load = [&](int u, int buf) __attribute__((always_inline)) {
-        const int t = tiles.at(u), j0 = t * KT;
-        if (words.all(t)) {
-            ktile.load(a.k, kfar + (int64_t)j0 * a.k.sn, lds_off(lds[buf][0]));
-            vtile.load(a.v, vfar + (int64_t)j0 * a.v.sn, lds_off(lds[buf][1]));
-            return Words::kAll;
-        }
-        const uint64_t word = words.at(a.win, tiles, a.nk, w.b, u, u1);
-        TileT::load_some(a.k, kbase, j0, word, a.win.sinks, a.win.skip, lds[buf][0]);
-        TileT::load_some(a.v, vbase, j0, word, a.win.sinks, a.win.skip, lds[buf][1]);
-        return word;
-    };
-
     f32x16 dq[DB][NQB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -114,8 +123,6 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
         for (int b = 0; b < NQB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
-    uint64_t word = 0, next = 0, after = 0;
-    if (u0 < u1) word = load(u0, 0);
     if (kAhead > 1 && u0 + 1 < u1) next = load(u0 + 1, 1);
     for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
         next_tile<kBuffers, 2 * TileT::kLoads>(u + 1 < u1 && words.all(tiles.at(u + 1)));
@@ -274,10 +281,11 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int pl = 0; pl < NP; ++pl) {
-                k[ks][pl] = mem_frag<DP>(krow, valid, a.k.chunks, pl, ks);
-                v[ks][pl] = mem_frag<DP>(vrow, valid, a.v.chunks, pl, ks);
-            }
+            for (int pl = 0; pl < NP; ++pl) k[ks][pl] = v[ks][pl] = __builtin_bit_cast(bf16x8, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        if (valid) {
+            load_row<DP>(krow, a.k.chunks, k);
+            load_row<DP>(vrow, a.v.chunks, v);
+        }
     }
 
     TileT qtile, gtile;
@@ -328,6 +336,8 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
 #pragma unroll
         for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.0f;
     if (u0 < u1) load(0);
+    settle_row(valid, a.k.chunks, k);
+    settle_row(valid, a.v.chunks, v);
     if (kAhead > 1 && u0 + 1 < u1) load(1);
     for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
         next_tile<kBuffers, TileT::kLoads ? 2 * TileT::kLoads + kStats : 0>(u + 1 < u1);

@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     blocks.init(a.win, a.nk, a.group, rows, first, NQB * 32, tiles.sinks * KT);
 
     bf16x8 q[NQB][KS][NP];
+    f32x8 qf[NQB][FLOATS ? KS : 1];
     KeyRange see[NQB];
     float m[NQB], l[NQB];
 #pragma unroll
@@ -79,15 +80,11 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         see[b] = key_range(a.win, a.nk, tok);
         m[b] = r < rows ? -INFINITY : 0.0f;
         l[b] = 0.0f;
+        if constexpr (FLOATS)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (FLOATS) {
-                split_planes(load_floats(reinterpret_cast<const float*>(row), r < rows, 2 * ks + half, a.dim), q[b][ks]);
-            } else {
-#pragma unroll
-                for (int pl = 0; pl < NP; ++pl) q[b][ks][pl] = mem_frag<DP>(row, r < rows, a.q.chunks, pl, ks);
-            }
-        }
+            for (int ks = 0; ks < KS; ++ks)
+                qf[b][ks] = load_floats(reinterpret_cast<const float*>(row), r < rows, 2 * ks + half, a.dim);
+        else load_row<DP>(row, a.q.chunks, q[b]);
     }
 
     TileT ktile, vtile;
@@ -138,6 +135,13 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     if (u0 < u1) {
         word = load(u0, 0);
         store(0);
+    }
+#pragma unroll
+    for (int b = 0; b < NQB; ++b) {
+        if constexpr (FLOATS)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) split_planes(qf[b][ks], q[b][ks]);
+        settle_row(FLOATS || r0 + 32 * b < rows, FLOATS ? DP / 8 : a.q.chunks, q[b]);
     }
     if (kAhead > 1 && u0 + 1 < u1) next = load(u0 + 1, 1);
     for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
