@@ -1282,23 +1282,24 @@ def clip_gradients(grads, max_norm, outs=None):
     # a model's hundreds of tensors are looked over by a few passes, half a microsecond each; whatever is out of line is named by
     # the slower way
     T, src, dst, back = torch.Tensor, grads, into, ()
-    kinds = set(map(_tensor_dtype, grads))
-    plain = set(map(T.get_device, grads)) == {dev.index} and all(map(T.is_contiguous, grads))
+    types = list(map(_tensor_dtype, grads))
+    into_types = types if outs is None else list(map(_tensor_dtype, outs))
+    plain = {*types, *into_types} <= _FEAT_DTYPES.keys() and set(map(T.get_device, grads)) == {dev.index} \
+        and all(map(T.is_contiguous, grads))
     if plain and outs is not None:
-        kinds |= set(map(_tensor_dtype, outs))
         plain = set(map(T.get_device, outs)) == {dev.index} and all(map(T.is_contiguous, outs)) \
             and list(map(_tensor_shape, grads)) == list(map(_tensor_shape, outs))
-    if not (plain and kinds <= _FEAT_DTYPES.keys()):
+    if not plain:
         src, dst, back = _clip_checked(grads, into, dev)
 
-    def arrays(tensors):
-        return (array.array("Q", map(T.data_ptr, tensors)), array.array("i", map(_FEAT_DTYPES.__getitem__, map(_tensor_dtype, tensors))))
+    def arrays(tensors, types):
+        return array.array("Q", map(T.data_ptr, tensors)), array.array("i", map(_FEAT_DTYPES.__getitem__, types))
 
     with _OnDevice(dev):
         n = len(src)
         numels = array.array("q", map(T.numel, src))
-        gp, gd = arrays(src)
-        op, od = (gp, gd) if dst is src else arrays(dst)
+        gp, gd = arrays(src, types)
+        op, od = (gp, gd) if dst is src else arrays(dst, into_types)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         nws = _workspace_bytes("g2v_clip_gradients_workspace", n)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev)

@@ -29,7 +29,7 @@ def clip_grad_norm_(tensors, max_norm, *, out=None):
         raise RuntimeError(f"max_norm must not be negative, got {max_norm}")
     if out is not None:
         out = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(out) != len(tensors) or not all(isinstance(t, torch.Tensor) for t in out):
+        if len(out) != len(tensors) or not (set(map(type, out)) <= _TYPES or all(isinstance(t, torch.Tensor) for t in out)):
             raise RuntimeError(f"out must hold {len(tensors)} tensors")
     grads = [t.grad if t.requires_grad else t for t in tensors]
     if any(g is None for g in grads):
