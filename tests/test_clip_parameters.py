@@ -95,3 +95,29 @@ def test_gradients_themselves(passed):
     clip_grad_norm_(iter(grads), 0.1)
     clip_grad_norm_(grads[0], 0.1)
     assert same(passed[0][0], grads) and same(passed[1][0], grads[:1])
+
+
+def test_gradients_with_a_graph_are_refused(passed):
+    """A gradient made with create_graph requires grad and is no parameter: it was taken for one without a gradient, and the norm was 0."""
+    from CudaGaussianVoxelizer import clip_grad_norm_
+    leaf = torch.ones(3, requires_grad=True)
+    grad, = torch.autograd.grad(leaf.pow(3).sum(), leaf, create_graph=True)
+    before = grad.detach().clone()
+    for tensors in ([grad], [torch.ones(2), grad], grad):
+        with pytest.raises(RuntimeError, match="detached"):
+            clip_grad_norm_(tensors, 1.0)
+    assert not passed and torch.equal(grad, before)
+    clip_grad_norm_([grad.detach()], 1.0)
+    assert torch.equal(passed[0][0][0], grad)
+
+
+def test_parameters_whose_gradients_have_a_graph(passed):
+    """A parameter's .grad is clipped, made with create_graph or not; so is what a graph's inner tensor retains."""
+    from CudaGaussianVoxelizer import clip_grad_norm_
+    leaf = torch.nn.Parameter(torch.ones(3))
+    inner = 2.0 * leaf
+    inner.retain_grad()
+    inner.pow(3).sum().backward(create_graph=True)
+    assert leaf.grad.requires_grad
+    clip_grad_norm_([leaf, inner], 1e9)
+    assert same(passed[0][0], [leaf.grad, inner.grad])
