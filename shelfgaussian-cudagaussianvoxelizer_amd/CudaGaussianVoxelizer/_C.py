@@ -9,6 +9,7 @@ from __future__ import annotations
 import array
 import ctypes
 import functools
+import math
 import operator
 
 import torch
@@ -1245,15 +1246,99 @@ def _dense(t):
     return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
 
 
+def _reaches(target, steps):
+    """Whether target is a sum of step x over the (step, most) of steps, 0 <= x <= most: the largest step first, whose x the others' reach
+    and divisor leave few values (one or two where strides nest).  Also True where 10,000 looks do not tell."""
+    merged = {}
+    for step, most in steps:
+        if step and most > 0:
+            merged[step] = merged.get(step, 0) + most
+    order = sorted(merged.items(), reverse=True)
+    reach, divisor = [0], [0]    # of the steps behind each
+    for step, most in reversed(order):
+        reach.append(reach[-1] + step * most)
+        divisor.append(math.gcd(divisor[-1], step))
+    reach.reverse()
+    divisor.reverse()
+    looks = 0
+    todo = [(0, target)]
+    while todo:
+        k, left = todo.pop()
+        if left == 0:
+            return True
+        if left < 0 or left > reach[k] or left % divisor[k]:
+            continue
+        step, most = order[k]
+        lo, hi = max(0, -((reach[k + 1] - left) // step)), min(most, left // step)
+        looks += hi - lo + 1
+        if looks > 10000:
+            return True
+        todo.extend((k + 1, left - step * x) for x in range(lo, hi + 1))
+    return False
+
+
+def _byte_steps(t):
+    size = t.element_size()
+    return [(step * size, n - 1) for step, n in zip(t.stride(), t.shape)]
+
+
+def _reach_of(t):
+    """Bytes from a tensor's first element to its last one's end."""
+    return sum(step * most for step, most in _byte_steps(t)) + t.element_size()
+
+
+def _share_memory(t, o):
+    """Whether two tensors with elements have bytes in common: t + i = o + j for bytes i and j of theirs, j taken from its end."""
+    return _reaches(o.data_ptr() - t.data_ptr() + _reach_of(o) - 1,
+                    _byte_steps(t) + _byte_steps(o) + [(1, t.element_size() - 1), (1, o.element_size() - 1)])
+
+
+def _overlaps_itself(t):
+    """Whether two elements of a tensor have one place: the first dimension whose indexes differ, by one at least, and those behind it, by
+    anything, make up for each other."""
+    steps = sorted((step, n) for step, n in zip(t.stride(), t.shape) if n > 1)
+    reach = 0
+    for step, n in steps:
+        if step <= reach:
+            break
+        reach += step * (n - 1)
+    else:    # every step is beyond what the smaller ones reach
+        return False
+    return any(_reaches(sum(s * (m - 1) for s, m in steps[k + 1:]) - step, [(step, n - 2)] + [(s, 2 * (m - 1)) for s, m in steps[k + 1:]])
+               for k, (step, n) in enumerate(steps))
+
+
+def _check_sharing(grads, outs):
+    """Refuses what the library refuses among flat tensors, whose memory it sees: an output that shares memory with another one, or with a
+    gradient but for its own at the same places, and with itself."""
+    spans = [(t.data_ptr(), t.data_ptr() + _reach_of(t), i, t, written) for written, tensors in ((True, outs), (False, grads))
+             for i, t in enumerate(tensors) if t.numel() and (written or t is not outs[i])]
+    spans.sort(key=lambda span: span[0])
+    open_ = []
+    for at, end, i, t, written in spans:
+        if written and _overlaps_itself(t):
+            raise RuntimeError(f"clip_gradients: elements of tensor {i}, which is written, share memory")
+        open_ = [span for span in open_ if span[1] > at]
+        for _, _, k, o, other in open_:
+            if (written or other) and not (i == k and (t.data_ptr(), t.dtype, t.stride()) == (o.data_ptr(), o.dtype, o.stride())) \
+                    and _share_memory(t, o):
+                raise RuntimeError(f"clip_gradients: tensors {min(i, k)} and {max(i, k)} share memory that is written")
+        open_.append((at, end, i, t, written))
+
+
 def _clip_checked(grads, outs, dev):
     """(gradients, outputs, results to copy back) as flat memory: tensors of other layouts go through contiguous copies."""
-    src, dst, back = [], [], []
     for i, (g, o) in enumerate(zip(grads, outs)):
         for t, what in ((g, "gradient"), (o, "output")):
             if t.device != dev or t.layout != torch.strided or t.dtype not in _FEAT_DTYPES or t.shape != g.shape:
                 raise RuntimeError(f"{what} {i} must be float32 or bfloat16 {tuple(g.shape)} on {dev}, got {t.dtype} "
                                    f"{tuple(t.shape)} ({t.layout}) on {t.device}")
-        if not (g.stride() == o.stride() and _dense(g)):
+    flat = [g.stride() == o.stride() and _dense(g) for g, o in zip(grads, outs)]
+    if not all(flat):    # the library sees the copies' memory
+        _check_sharing(grads, outs)
+    src, dst, back = [], [], []
+    for g, o, as_is in zip(grads, outs, flat):
+        if not as_is:
             same = o is g
             g = g.contiguous()
             if same or not o.is_contiguous():

@@ -27,11 +27,12 @@ def clip_grad_norm_(tensors, max_norm, *, out=None):
     tensors: parameters (a module's ``parameters()``, frozen ones among them), whose .grad is clipped and which are skipped where they
     have none, or gradients themselves: tensors that are no torch.nn.Parameter, require no gradient and have none (one made with
     create_graph is refused as such and clipped as a parameter's .grad).  float32 and bfloat16 may be mixed, on one GPU; one tensor
-    may come alone.  A tensor must not be there twice, nor two that share memory.  In place; with ``out``, a list of as many float32
-    or bfloat16 tensors of the same shapes, the scaled gradients go there and the gradients stay (the float32 gradients of an
-    optimizer's main weights from a bfloat16 layer's).  Squares are summed in 64 bits: the norm is finite where float32 holds it.
-    NaN or infinite gradients give a norm that is, and outputs as the formula says: nothing is skipped.  Two launches for up to 120
-    tensors, two more for every 120; they may be captured into a graph, which keeps the tensors' addresses."""
+    may come alone.  In place, of any strides; with ``out``, a list of as many float32 or bfloat16 tensors of the same shapes, the
+    scaled gradients go there and the gradients stay (the float32 gradients of an optimizer's main weights from a bfloat16 layer's).
+    What is written must not be there twice, nor share memory with another tensor but its own gradient as it lies (refused).  Squares
+    are summed in 64 bits: the norm is finite where float32 holds it.  NaN or infinite gradients give a norm that is, and outputs as
+    the formula says: nothing is skipped.  Two launches for up to 120 tensors, two more for every 120; they may be captured into a
+    graph, which keeps the tensors' addresses."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not set(map(type, tensors)) <= _TYPES and not all(isinstance(t, torch.Tensor) for t in tensors):
         raise RuntimeError("tensors must be parameters or gradients")

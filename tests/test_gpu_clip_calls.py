@@ -42,3 +42,25 @@ def test_a_partly_frozen_model(dtype, max_norm):
         else:
             torch.testing.assert_close(o, t.grad, rtol=2e-6, atol=0)
             torch.testing.assert_close(p.grad.float(), t.grad, rtol=2e-6 + (2.0 ** -8 if dtype == torch.bfloat16 else 0.0), atol=0)
+
+
+def test_strided_tensors_that_share_memory_are_refused():
+    """Tensors that go through copies: refused before anything is written, as flat ones are."""
+    from CudaGaussianVoxelizer import clip_grad_norm_
+    w, square = torch.ones(6, 140, device="cuda"), torch.ones(8, 8, device="cuda")
+    for tensors, out in (([w[:, ::2], w[:, ::2]], None), ([square], [square.t()]), ([w[:, :50], w[:, 50:100]], [w[:, 50:100], w[:, :50]]),
+                         ([torch.ones(4, device="cuda").expand(3, 4)], None)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip_grad_norm_(tensors, 0.1, out=out)
+    assert bool((w == 1).all()) and bool((square == 1).all())
+
+
+def test_columns_beside_one_another():
+    """Slices of a fused gradient, whose spans of memory cross but share no element, are clipped in place."""
+    from CudaGaussianVoxelizer import clip_grad_norm_
+    fused = torch.randn(300, 96, generator=torch.Generator().manual_seed(2)).cuda()
+    before = fused.double()
+    norm = clip_grad_norm_([fused[:, :32], fused[:, 32:64], fused[:, 64:]], 0.5)
+    want = float(before.square().sum().sqrt())
+    assert abs(float(norm) - want) <= 2.0 ** -23 * want
+    assert bool(((fused.double() - before * 0.5 / (want + 1e-6)).abs() <= 2.0 ** -23 * before.abs()).all())
