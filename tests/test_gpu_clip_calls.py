@@ -29,7 +29,7 @@ def test_a_partly_frozen_model(dtype, max_norm):
     before = [p.detach().clone() for p in params]
     twins = [torch.nn.Parameter(p.detach().float()) for p in params]
     for t, p in zip(twins, params):
-        t.grad = None if p.grad is None else p.grad.float()
+        t.grad = None if p.grad is None else p.grad.float().clone()
     want = torch.nn.utils.clip_grad_norm_(twins, max_norm)
     out = [torch.full(p.shape, 7.0, device="cuda") for p in params]
     for got in (clip_grad_norm_(params, max_norm, out=out), clip_grad_norm_(layers.parameters(), max_norm)):
