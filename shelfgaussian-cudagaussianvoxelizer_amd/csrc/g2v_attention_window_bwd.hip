@@ -226,21 +226,21 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
 }
 
 // Two workgroups a CU from 64 channels on: three spill where P and dS are in one plane (18,000 x 16 x 64, 1025 keys a window, 266 us
-// for 176).  The sinks' one-wave workgroups: as many as their tiles' LDS allows.
+// for 176).  At 32 channels four, or three where they are in two planes, with which four spill (60,000 x 16 x 32, 513 keys, 323 us for
+// 296).  The sinks' one-wave workgroups: as many as their tiles' LDS allows.
 constexpr int window_dkv_per_cu(int np, int ns, int dp, int nw) {
-    if (nw > 1) return np == 1 && dp >= 64 ? 2 : dkv_per_cu(np, ns, dp);
+    if (nw > 1) return np > 1 ? dkv_per_cu(np, ns, dp) : dp >= 64 ? 2 : ns > 1 ? 3 : 4;
     if (np > 1) return dp > 96 ? 1 : dp > 64 ? 2 : dp > 32 ? 3 : 6;
     return dp > 64 ? 3 : dp > 32 ? 6 : 8;
 }
 constexpr int dkv_bound(int np, int ns, int dp, int nw) { return nw > 1 ? window_dkv_per_cu(np, ns, dp, nw) : np > 1 && dp > 32 ? 1 : 2; }
 
-// As k_attn_dkv: keys in the lanes, the queries that see any of the workgroup's keys pass by, head after head.
+// As k_attn_dkv: keys in the lanes, the queries that see any of the workgroup's keys pass by, head after head.  NS: planes of P and dS,
+// as there.  (P in one plane throughout is less work, 200,000 x 8 heads x 64, 513 keys a window 820 -> 706 us, and puts dV 2.3e-3 off
+// where its own rounding is 1.7e-3.)
 template <int NP, int NS, int DP, int KS, int NW, int QT, typename T>
 __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_dkv(WinBwd a) {
     static_assert(NW == 1 || NW % 2 == 0, "waves in pairs load the statistics, or one does");
-    // planes of P: one of bfloat16, as in the forward's product (dV 2.0e-3 off, its own rounding 1.7e-3); a second one would be a
-    // sixth product (200,000 x 8 heads x 64, 513 keys a window: 741 -> 800 us)
-    constexpr int NPP = NP;
     constexpr int NT = NW * 64, QB = QT / 32, DB = DP / 32;
     typedef WinTile<NP, DP, QT, NT> TileT;
     constexpr int kBuffers = NP > 1 && NW == 1 ? 2 : buffers(2, TileT::kBytes), kAhead = kBuffers - 1;
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(NW * 64, dkv_bound(NP, NS, DP, NW)) k_window_d
             for (int i = 0; i < 16; ++i) dp[i] *= s[i];
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                bf16x8 p[NPP], ds[NS];
+                bf16x8 p[NS], ds[NS];
                 to_operand(s, st, p);
                 to_operand(dp, st, ds);
 #pragma unroll
