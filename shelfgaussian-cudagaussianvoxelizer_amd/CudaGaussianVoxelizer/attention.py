@@ -135,19 +135,22 @@ def gaussian_attention(q, k, v, key_mask=None, scale=None, *, window=None, sinks
     multiple of Hkv (consecutive query heads share a key head), D at most 128.  key_mask (B, Nk) bool is False at keys
     that are not attended to (padding of a batch, pruned Gaussians): what their rows hold, NaN included, reaches no result
     and they get zero gradients; a query without any key gives zeros.  float32 values of valid rows have to be finite (an
-    infinity gives NaN, as they are split into three bfloat16 planes), and sums within float32's range (include/g2v.h says which).  scale None: D^-1/2.  Returns (B, Nq, Hq, D) of
-    q's type, contiguous.  Any number of queries and keys, zero and one included: a single query that pools a scene has its
+    infinity gives NaN, as they are split into three bfloat16 planes), and sums within float32's range (include/g2v.h says which).
+    scale None: D^-1/2.  Returns (B, Nq, Hq, D) of q's type, contiguous.  Any number of queries and keys, zero and one included: a single query that pools a scene has its
     keys split over the GPU.
 
     window (left, right): query i stands at place p = i + Nk - Nq of the keys (of its own, where queries and keys are the same
     tokens; of the last one, if it is alone) and sees the places p - left to p + right, None for no bound, and the first
     ``sinks`` places up to p + right, however far.  Time and memory go with the window, not with the square of the scene:
     Gaussians sorted along a space-filling curve see their neighbours and a few global tokens in front, those of a stream
-    (right = 0) what came before them.  A query may see no key.
+    (right = 0) what came before them.  A query may see no key.  With a window, valid rows of either type and upstream gradients have to
+    be finite: a NaN or an infinity may also reach rows near it that do not see it, earlier ones of a causal order among them.
 
     Scores and sums are float32.  With bfloat16 inputs the probabilities are rounded to bfloat16 before their product with v, and
     the backward's factors likewise (as two such planes where keys or queries are few): outputs and gradients are off by 1.7e-3 to
-    2.4e-3 of their norm, where rounding exact ones would put them 1.7e-3 off.  float32 keeps 24 bits throughout.
+    2.4e-3 of their norm, where rounding exact ones would put them 1.7e-3 off.  float32 keeps 24 bits of all products and sums, so that outputs and
+    gradients are off by less than 1e-6 of the terms that they add up.  That is a part of their own norm, too, but where terms cancel:
+    the gradients of q and k are what is left of P (dP - delta), which is little where one key has nearly all of a row's probability.
 
     Gradients flow to q, k and v; the backward recomputes the probabilities and gives the same bits on every run.  Gradients
     of gradients and forward-mode derivatives are refused."""
