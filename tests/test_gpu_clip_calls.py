@@ -64,3 +64,20 @@ def test_columns_beside_one_another():
     want = float(before.square().sum().sqrt())
     assert abs(float(norm) - want) <= 2.0 ** -23 * want
     assert bool(((fused.double() - before * 0.5 / (want + 1e-6)).abs() <= 2.0 ** -23 * before.abs()).all())
+
+
+@pytest.mark.parametrize("size,count", [(3e38, 1), (1.5e38, 5), (1e38, 11)])
+def test_norms_just_below_float32s_largest(size, count):
+    """Values whose squares float32 does not hold and whose norm it does, 2 % to 12 % below its largest: finite, and off by its rounding."""
+    from CudaGaussianVoxelizer import clip_grad_norm_
+    big = torch.zeros(5000, device="cuda")
+    big[::400][:count] = size
+    small = torch.full((300,), 1.0, device="cuda")
+    before = [big.double(), small.double()]
+    want = float(sum(b.square().sum() for b in before).sqrt())
+    assert 0.85 * torch.finfo(torch.float32).max < want < torch.finfo(torch.float32).max
+    norm = float(clip_grad_norm_([big, small], 1e30))
+    assert abs(norm - want) <= 2.0 ** -23 * want
+    for g, b in zip((big, small), before):
+        exact = b * 1e30 / want
+        assert bool(((g.double() - exact).abs() <= 2.0 ** -23 * exact + 2.0 ** -126).all())
