@@ -105,7 +105,6 @@ __device__ __forceinline__ void next_tile(bool counted) {
 template <int NP, int DP, int ROWS, int NT>
 struct Tile {
     static constexpr int C = DP / 8;                    // chunks of a row
-    static constexpr int kThreads = NT;
     static constexpr int kChunks = NP * ROWS * C;
     static constexpr int kBytes = kChunks * 16;
     static constexpr int kIter = (kChunks + NT - 1) / NT;
@@ -308,10 +307,6 @@ __device__ __forceinline__ float lost_by_rounding(float x) { return x - (float)(
 // (a tenth of the vector instructions; matrix and vector work of a SIMD take their time one after the other).
 constexpr float kFar = 1048576.0f;
 
-// The reference (times c) of a row whose scores were all -inf so far: any other one passes kFar from it
-// (or, where c is so small that the reference itself is at float32's lowest values, is in its reach).
-constexpr float kLowest = -1e37f;
-
 // Into which workgroups the tiles of the heads go: the first `head` tiles of each (row0 rows) to head_splits each, the others
 // to `splits` each.  A tile's only workgroup writes its result; more write partial results, which are joined: rows [0, row0)
 // as (head_splits, bhs, row0, ..) where they are split, behind them (splits, bhs, rows - row0, ..).
@@ -433,18 +428,6 @@ namespace attn {
 // Row of dk and dv that key j of scene b has.
 __device__ __forceinline__ int64_t grad_row(const AttnBwd& a, int b, int64_t j) {
     return (int64_t)b * (a.nk + a.gap) + j + (a.gap && j >= a.gap_at ? a.gap : 0);
-}
-
-// Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
-// to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
-// the same error on all of them, which their sum dS K does not average out (dQ then 3.2e-3 off instead of 2.2e-3).
-template <typename T>
-__device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, float x0, float x1, float x2, float x3) {
-    store4<T>(static_cast<T*>(a.out) + at, d, a.dim, x0, x1, x2, x3);
-    if constexpr (sizeof(T) == 2)
-        if (a.rest)
-            store4<T>(static_cast<T*>(a.rest) + at, d, a.dim, lost_by_rounding(x0), lost_by_rounding(x1),
-                      lost_by_rounding(x2), lost_by_rounding(x3));
 }
 }  // namespace attn
 

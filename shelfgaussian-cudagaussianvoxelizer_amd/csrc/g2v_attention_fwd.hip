@@ -18,6 +18,22 @@ namespace g2v {
 namespace {
 using namespace attn;
 
+// The reference (times c) of a row whose scores were all -inf so far: any other one passes kFar from it
+// (or, where c is so small that the reference itself is at float32's lowest values, is in its reach).
+constexpr float kLowest = -1e37f;
+
+// Four values of the output's row at `at`.  For a bfloat16 output that a backward follows, what its rounding leaves goes
+// to `rest`: the backward's delta = sum_d dO O is subtracted from every dP of a row, and an output rounded to 2^-9 puts
+// the same error on all of them, which their sum dS K does not average out (dQ then 3.2e-3 off instead of 2.2e-3).
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnFwd& a, int64_t at, int d, float x0, float x1, float x2, float x3) {
+    store4<T>(static_cast<T*>(a.out) + at, d, a.dim, x0, x1, x2, x3);
+    if constexpr (sizeof(T) == 2)
+        if (a.rest)
+            store4<T>(static_cast<T*>(a.rest) + at, d, a.dim, lost_by_rounding(x0), lost_by_rounding(x1),
+                      lost_by_rounding(x2), lost_by_rounding(x3));
+}
+
 // KS: steps of 16 that the head's width takes in the scores' product (the last of DP / 16 may hold nothing but padding).
 template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, launch_bound(NW, fwd_per_cu(NP, DP, NW))) k_attn_fwd(AttnFwd a) {

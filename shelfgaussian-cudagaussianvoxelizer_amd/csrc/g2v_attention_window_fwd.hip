@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
             }
             store_block<T>(static_cast<T*>(a.out) + at, 32 * d, a.dim, x);
             if constexpr (sizeof(T) == 2)
-                if (a.rest) store_block<T>(static_cast<T*>(a.rest) + at, 32 * d, a.dim, lost);    // see store_out
+                if (a.rest) store_block<T>(static_cast<T*>(a.rest) + at, 32 * d, a.dim, lost);    // see store_out of g2v_attention_fwd.hip
         }
     }
 }
