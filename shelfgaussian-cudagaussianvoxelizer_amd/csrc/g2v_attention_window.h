@@ -194,10 +194,10 @@ struct WaveBlocks {
         __device__ __forceinline__ bool has(int j) const { return (uint32_t)(j - at) < n; }
     };
     Range any, every, any_far, every_far;    // of the window; of the sinks' tiles
-    __device__ __forceinline__ void init(const AttnWindow& w, int nk, int group, int rows, int first, int count, int sinks_end) {
+    __device__ __forceinline__ void init(const AttnWindow& w, int nk, int group, int rows, int first, int sinks_end) {
         any = every = any_far = every_far = {0, 0u};
         if (first >= rows) return;
-        const KeyRange a = key_range(w, nk, first / group), b = key_range(w, nk, (min(first + count, rows) - 1) / group);
+        const KeyRange a = key_range(w, nk, first / group), b = key_range(w, nk, (min(first + 32, rows) - 1) / group);
         const int lo0 = g2v::uniform(a.lo), lo1 = g2v::uniform(b.lo), hi0 = g2v::uniform(a.hi), hi1 = g2v::uniform(b.hi);
         if (hi1 > lo0) any = {lo0 - 31, (uint32_t)(hi1 - lo0 + 31)};
         if (hi0 - 31 > lo1) every = {lo1, (uint32_t)(hi0 - 31 - lo1)};

@@ -13,7 +13,7 @@ constexpr int window_dq_per_cu(int np, int dp, int waves) {
 }
 
 // As k_attn_dq.
-template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+template <int NP, int DP, int KS, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP, DP, NW))) k_window_dq(WinBwd a) {
     constexpr int NS = NP == 1 ? 2 : NP;    // planes of dS, see k_attn_dq
     constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
@@ -24,8 +24,8 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     static_assert(window_dq_per_cu(NP, DP, NW) * sizeof(lds) <= kLdsBytes, "planned by more workgroups than fit");
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int rows = a.group * a.nq, half = (threadIdx.x >> 5) & 1;
-    const int first = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32), r0 = first + (threadIdx.x & 31);
-    const int g0 = w.tile * (NW * NQB * 32), g1 = min(g0 + NW * NQB * 32, rows) - 1;
+    const int first = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * 32, r = first + (threadIdx.x & 31);
+    const int g0 = w.tile * (NW * 32), g1 = min(g0 + NW * 32, rows) - 1;
     const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
     const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
     KeyTiles<KT> tiles;
@@ -34,26 +34,22 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     split_range(tiles.all, w.split, w.splits, u0, u1);
     if (!a.dq) u1 = u0;    // delta alone
     WaveBlocks blocks;
-    blocks.init(a.win, a.nk, a.group, rows, first, NQB * 32, tiles.sinks * KT);
+    blocks.init(a.win, a.nk, a.group, rows, first, tiles.sinks * KT);
 
-    bf16x8 q[NQB][KS][NP], g[NQB][KS][NP];
-    KeyRange see[NQB];
-    float lse[NQB], delta[NQB];    // delta = sum_d dO O, negative and times scale
-    RowValues<KS, T> out[NQB], rest[NQB];
-#pragma unroll
-    for (int b = 0; b < NQB; ++b) {
-        const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
-        const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
-        const char* qrow = a.q.p + w.b * a.q.sb + tok * a.q.sn + head * a.q.sh;
-        const char* grow = a.g.p + w.b * a.g.sb + tok * a.g.sn + head * a.g.sh;
-        see[b] = key_range(a.win, a.nk, tok);
-        load_row<DP>(qrow, a.q.chunks, q[b]);
-        load_row<DP>(grow, a.g.chunks, g[b]);
-        lse[b] = a.lse_in[((int64_t)w.b * a.hq + head) * a.nq + tok];
-        const int64_t orow = (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
-        out[b].load(static_cast<const T*>(a.out) + orow, a.dim);
-        if (sizeof(T) == 2 && a.rest) rest[b].load(static_cast<const T*>(a.rest) + orow, a.dim);
-    }
+    bf16x8 q[KS][NP], g[KS][NP];
+    float lse, delta;    // delta = sum_d dO O, negative and times scale
+    RowValues<KS, T> out, rest;
+    const int rc = r < rows ? r : rows - 1;
+    const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
+    const char* qrow = a.q.p + w.b * a.q.sb + tok * a.q.sn + head * a.q.sh;
+    const char* grow = a.g.p + w.b * a.g.sb + tok * a.g.sn + head * a.g.sh;
+    const KeyRange see = key_range(a.win, a.nk, tok);
+    load_row<DP>(qrow, a.q.chunks, q);
+    load_row<DP>(grow, a.g.chunks, g);
+    lse = a.lse_in[((int64_t)w.b * a.hq + head) * a.nq + tok];
+    const int64_t orow = (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+    out.load(static_cast<const T*>(a.out) + orow, a.dim);
+    if (sizeof(T) == 2 && a.rest) rest.load(static_cast<const T*>(a.rest) + orow, a.dim);
 
     TileT ktile, vtile;
     ktile.init(a.k);
@@ -78,35 +74,30 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     };
     uint64_t word = 0, next = 0, after = 0;
     if (u0 < u1) word = load(u0, 0);
+    settle_row(r < rows, a.q.chunks, q);
+    settle_row(r < rows, a.g.chunks, g);
+    asm volatile("" : "+v"(lse));
+    float sum = 0.0f;
 #pragma unroll
-    for (int b = 0; b < NQB; ++b) {
-        const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
-        const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
-        settle_row(r < rows, a.q.chunks, q[b]);
-        settle_row(r < rows, a.g.chunks, g[b]);
-        asm volatile("" : "+v"(lse[b]));
-        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
-        float sum = 0.0f;
+    for (int ks = 0; ks < KS; ++ks) {
+        f32x8 o = out.at(ks, a.dim);
+        if (sizeof(T) == 2 && a.rest) o += rest.at(ks, a.dim);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            f32x8 o = out[b].at(ks, a.dim);
-            if (sizeof(T) == 2 && a.rest) o += rest[b].at(ks, a.dim);
+        for (int j = 0; j < 8; ++j) {
+            float x = (float)g[ks][0][j];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float x = (float)g[b][ks][0][j];
-#pragma unroll
-                for (int pl = 1; pl < NP; ++pl) x += (float)g[b][ks][pl][j];
-                sum = fmaf(o[j], x, sum);
-            }
-        }
-        sum = half_sum(sum);
-        delta[b] = -sum * a.scale;
-        if (w.split == 0 && half == 0 && r < rows) {
-            a.lse_pad[at] = lse[b];
-            a.delta_pad[at] = -sum;
+            for (int pl = 1; pl < NP; ++pl) x += (float)g[ks][pl][j];
+            sum = fmaf(o[j], x, sum);
         }
     }
-    if (w.split == 0 && (w.tile + 1) * (NW * NQB * 32) >= rows) {    // the heads' padding
+    sum = half_sum(sum);
+    delta = -sum * a.scale;
+    if (w.split == 0 && half == 0 && r < rows) {
+        const int64_t at = ((int64_t)w.b * a.hq + head) * a.nqp + tok;
+        a.lse_pad[at] = lse;
+        a.delta_pad[at] = -sum;
+    }
+    if (w.split == 0 && (w.tile + 1) * (NW * 32) >= rows) {    // the heads' padding
         const int pad = a.nqp - a.nq;
         for (int i = threadIdx.x; i < a.group * pad; i += NT) {
             const int64_t at = ((int64_t)w.b * a.hq + w.h * a.group + i / pad) * a.nqp + a.nq + i % pad;
@@ -116,13 +107,11 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
     }
     if (!a.dq) return;    // dK and dV alone are wanted
 
-    f32x16 dq[DB][NQB];
+    f32x16 dq[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int b = 0; b < NQB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
+        for (int i = 0; i < 16; ++i) dq[d][i] = 0.0f;
     if (kAhead > 1 && u0 + 1 < u1) next = load(u0 + 1, 1);
     for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
         next_tile<kBuffers, 2 * TileT::kLoads>(u + 1 < u1 && words.all(tiles.at(u + 1)));
@@ -141,11 +130,9 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
             const uint32_t part = (uint32_t)(word >> (32 * kb));
             const int jb = j0 + 32 * kb;
             if (!some.has(jb) || !part) continue;
-            f32x16 s[NQB], dp[NQB];
+            f32x16 s, dp;
 #pragma unroll
-            for (int b = 0; b < NQB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = dp[b][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 bf16x8 fk[NP], fv[NP];
@@ -154,74 +141,59 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_dq_per_cu(NP,
                     fk[pl] = frags.rows(at, pl * KT * DP * 2, kb, ks);
                     fv[pl] = frags.rows(at, TileT::kBytes + pl * KT * DP * 2, kb, ks);
                 }
-#pragma unroll
-                for (int b = 0; b < NQB; ++b) {
-                    s[b] = mma(fk, q[b][ks], s[b]);
-                    dp[b] = mma(fv, g[b][ks], dp[b]);
-                }
+                s = mma(fk, q[ks], s);
+                dp = mma(fv, g[ks], dp);
             }
 #pragma unroll
-            for (int b = 0; b < NQB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[b][i] = exp2_fast(fmaf(s[b][i], a.c, -lse[b])) * fmaf(dp[b][i], a.scale, delta[b]);   // scale dS
+            for (int i = 0; i < 16; ++i)
+                s[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * fmaf(dp[i], a.scale, delta);   // scale dS
             if (!every.has(jb) || part != ~0u) {
+                const uint32_t x = (seen_bits(see, a.win.sinks, jb) & part) >> (4 * half);
 #pragma unroll
-                for (int b = 0; b < NQB; ++b) {
-                    const uint32_t x = (seen_bits(see[b], a.win.sinks, jb) & part) >> (4 * half);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[b][i] = or_zero(spread_bit(x, 8 * (i >> 2) + (i & 3)), s[b][i]);
-                }
+                for (int i = 0; i < 16; ++i) s[i] = or_zero(spread_bit(x, 8 * (i >> 2) + (i & 3)), s[i]);
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                bf16x8 p[NQB][NS];
-#pragma unroll
-                for (int b = 0; b < NQB; ++b) to_operand(s[b], st, p[b]);
+                bf16x8 p[NS];
+                to_operand(s, st, p);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     bf16x8 f[NP];
 #pragma unroll
                     for (int pl = 0; pl < NP; ++pl) f[pl] = frags.cols(at, pl * KT * DP * 2, kb, st, d);
-#pragma unroll
-                    for (int b = 0; b < NQB; ++b) dq[d][b] = mma(f, p[b], dq[d][b]);
+                    dq[d] = mma(f, p, dq[d]);
                 }
             }
         }
         word = next;
         next = after;
     }
+    if (r >= rows) return;
+    // one key: its probability is 1 whatever q is
+    const bool one = see.hi - see.lo + min(a.win.sinks, see.lo) < 2;
+    if (one)
 #pragma unroll
-    for (int b = 0; b < NQB; ++b) {
-        const int r = r0 + 32 * b;
-        if (r >= rows) continue;
-        // one key: its probability is 1 whatever q is
-        const bool one = see[b].hi - see[b].lo + min(a.win.sinks, see[b].lo) < 2;
-        if (one)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int i = 0; i < 16; ++i) dq[d][i] = 0.0f;
+    if (w.splits > 1) {
+        const PartRow pr = part_row(a.parts, a.bhs, w.bh, rows, r);
+        float* out = a.part + (pr.at + w.split * pr.step) * DP;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) dq[d][b][i] = 0.0f;
-        if (w.splits > 1) {
-            const PartRow pr = part_row(a.parts, a.bhs, w.bh, rows, r);
-            float* out = a.part + (pr.at + w.split * pr.step) * DP;
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4*>(out + 32 * d + reg_row(i)) =
+                    f32x4{dq[d][i], dq[d][i + 1], dq[d][i + 2], dq[d][i + 3]};
+        return;
+    }
+    T* row = static_cast<T*>(a.dq) + (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<f32x4*>(out + 32 * d + reg_row(i)) =
-                        f32x4{dq[d][b][i], dq[d][b][i + 1], dq[d][b][i + 2], dq[d][b][i + 3]};
-            continue;
-        }
-        const int tok = r / a.group, head = w.h * a.group + r - tok * a.group;
-        T* row = static_cast<T*>(a.dq) + (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+    for (int d = 0; d < DB; ++d) {
+        float x[16];
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = dq[d][b][i];
-            store_block<T>(row, 32 * d, a.dim, x);
-        }
+        for (int i = 0; i < 16; ++i) x[i] = dq[d][i];
+        store_block<T>(row, 32 * d, a.dim, x);
     }
 }
 
@@ -470,18 +442,18 @@ __global__ void __launch_bounds__(256) k_window_zeros(WinBwd a, int64_t each, in
     }
 }
 
-template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+template <int NP, int DP, int KS, int NW, int KT, typename T>
 hipError_t dq_launch(const WinBwd& a, hipStream_t s) {
-    G2V_LAUNCH((k_window_dq<NP, DP, KS, NQB, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
+    G2V_LAUNCH((k_window_dq<NP, DP, KS, NW, KT, T>), dim3((unsigned)workgroups(a.parts, a.bhs)), dim3(NW * 64), 0, s, a);
     return a.dq ? launch_attn_dq_join(a, NP > 1, DP, s) : hipGetLastError();
 }
-template <int NP, int DP, int NQB, int KT, typename T>
+template <int NP, int DP, int KT, typename T>
 hipError_t dq_waves(const WinBwd& a, const AttnShape& g, hipStream_t s) {
     const bool full = a.dim > DP - 16;
     if constexpr (NP == 1)
         if (g.waves == 1)
-            return full ? dq_launch<NP, DP, DP / 16, 1, 1, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, 1, 1, KT, T>(a, s);
-    return full ? dq_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
+            return full ? dq_launch<NP, DP, DP / 16, 1, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, 1, KT, T>(a, s);
+    return full ? dq_launch<NP, DP, DP / 16, 4, KT, T>(a, s) : dq_launch<NP, DP, DP / 16 - 1, 4, KT, T>(a, s);
 }
 
 template <int NP, int NS, int DP, int NW, int QT, typename T>
@@ -514,7 +486,7 @@ hipError_t dkv_planes(const WinBwd& a, int planes, hipStream_t s) {
 AttnShape window_dq_shape(bool f32, int dp, int64_t rows) {
     AttnShape g = attn_dq_shape(f32, dp, rows);
     g.per_cu = window_dq_per_cu(f32 ? 3 : 1, dp, g.waves);
-    if (!f32 && g.waves > 1) g.blocks = 1;
+    g.blocks = 1;
     return g;
 }
 AttnShape window_dkv_shape(bool f32, int dp, int planes, bool all_queries) {
@@ -532,17 +504,17 @@ hipError_t launch_window_dq(const WinBwd& a, bool f32, int dp, hipStream_t s) {
     const AttnShape g = window_dq_shape(f32, dp, (int64_t)a.group * a.nq);
     if (f32) {
         switch (dp) {
-            case 32: return dq_waves<3, 32, 1, 64, float>(a, g, s);
-            case 64: return dq_waves<3, 64, 1, 32, float>(a, g, s);
-            case 96: return dq_waves<3, 96, 1, 32, float>(a, g, s);
-            default: return dq_waves<3, 128, 1, 32, float>(a, g, s);
+            case 32: return dq_waves<3, 32, 64, float>(a, g, s);
+            case 64: return dq_waves<3, 64, 32, float>(a, g, s);
+            case 96: return dq_waves<3, 96, 32, float>(a, g, s);
+            default: return dq_waves<3, 128, 32, float>(a, g, s);
         }
     }
     switch (dp) {
-        case 32: return dq_waves<1, 32, 1, 64, __bf16>(a, g, s);
-        case 64: return dq_waves<1, 64, 1, 64, __bf16>(a, g, s);
-        case 96: return dq_waves<1, 96, 1, 64, __bf16>(a, g, s);
-        default: return dq_waves<1, 128, 1, 64, __bf16>(a, g, s);
+        case 32: return dq_waves<1, 32, 64, __bf16>(a, g, s);
+        case 64: return dq_waves<1, 64, 64, __bf16>(a, g, s);
+        case 96: return dq_waves<1, 96, 64, __bf16>(a, g, s);
+        default: return dq_waves<1, 128, 64, __bf16>(a, g, s);
     }
 }
 

@@ -46,7 +46,7 @@ struct FloatTile {
 
 // As k_attn_fwd (rows in the lanes, keys in the registers).
 // FLOATS: q, k and v are float32 rows, split into planes here; else bfloat16 rows, planes packed before.
-template <int NP, bool FLOATS, int DP, int KS, int NQB, int NW, int KT, typename T>
+template <int NP, bool FLOATS, int DP, int KS, int NW, int KT, typename T>
 __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP, DP, NW))) k_window_fwd(WinFwd a) {
     static_assert(!FLOATS || NP == 3, "planes of float32");
     constexpr int NT = NW * 64, KB = KT / 32, DB = DP / 32;
@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     static_assert(window_fwd_per_cu(NP, DP, NW) * sizeof(lds) <= kLdsBytes, "planned by more workgroups than fit");
     const Item w = item_of(blockIdx.x, a.bhs, a.hk, a.parts);
     const int lane = threadIdx.x & 63, rows = a.group * a.nq, half = lane >> 5;
-    const int first = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * (NQB * 32), r0 = first + (lane & 31);
-    const int g0 = w.tile * (NW * NQB * 32), g1 = min(g0 + NW * NQB * 32, rows) - 1;    // the workgroup's rows
+    const int first = (w.tile * NW + g2v::uniform(threadIdx.x >> 6)) * 32, r = first + (lane & 31);
+    const int g0 = w.tile * (NW * 32), g1 = min(g0 + NW * 32, rows) - 1;    // the workgroup's rows
     const char* kbase = a.k.p + w.b * a.k.sb + w.h * a.k.sh;
     const char* vbase = a.v.p + w.b * a.v.sb + w.h * a.v.sh;
     KeyTiles<KT> tiles;
@@ -66,26 +66,19 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
     int u0, u1;
     split_range(tiles.all, w.split, w.splits, u0, u1);
     WaveBlocks blocks;
-    blocks.init(a.win, a.nk, a.group, rows, first, NQB * 32, tiles.sinks * KT);
+    blocks.init(a.win, a.nk, a.group, rows, first, tiles.sinks * KT);
 
-    bf16x8 q[NQB][KS][NP];
-    f32x8 qf[NQB][FLOATS ? KS : 1];
-    KeyRange see[NQB];
-    float m[NQB], l[NQB];
+    bf16x8 q[KS][NP];
+    f32x8 qf[FLOATS ? KS : 1];
+    float m = r < rows ? -INFINITY : 0.0f, l = 0.0f;
+    const int rc = r < rows ? r : rows - 1, load_tok = rc / a.group, load_head = w.h * a.group + rc - load_tok * a.group;
+    const char* row = a.q.p + w.b * a.q.sb + load_tok * a.q.sn + load_head * a.q.sh;
+    const KeyRange see = key_range(a.win, a.nk, load_tok);
+    if constexpr (FLOATS)
 #pragma unroll
-    for (int b = 0; b < NQB; ++b) {
-        const int r = r0 + 32 * b, rc = r < rows ? r : rows - 1;
-        const int tok = rc / a.group, head = w.h * a.group + rc - tok * a.group;
-        const char* row = a.q.p + w.b * a.q.sb + tok * a.q.sn + head * a.q.sh;
-        see[b] = key_range(a.win, a.nk, tok);
-        m[b] = r < rows ? -INFINITY : 0.0f;
-        l[b] = 0.0f;
-        if constexpr (FLOATS)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                qf[b][ks] = load_floats(reinterpret_cast<const float*>(row), r < rows, 2 * ks + half, a.dim);
-        else load_row<DP>(row, a.q.chunks, q[b]);
-    }
+        for (int ks = 0; ks < KS; ++ks)
+            qf[ks] = load_floats(reinterpret_cast<const float*>(row), r < rows, 2 * ks + half, a.dim);
+    else load_row<DP>(row, a.q.chunks, q);
 
     TileT ktile, vtile;
     FloatTile<DP, KT, NT> kfloat, vfloat;
@@ -118,13 +111,11 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         return word;
     };
 
-    f32x16 o[DB][NQB];
+    f32x16 o[DB];
 #pragma unroll
-    for (int b = 0; b < NQB; ++b)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][b][i] = 0.0f;
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     auto store = [&](int buf) __attribute__((always_inline)) {    // from registers to LDS
         if constexpr (FLOATS) {
             kfloat.store(lds[buf][0]);
@@ -136,13 +127,10 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         word = load(u0, 0);
         store(0);
     }
+    if constexpr (FLOATS)
 #pragma unroll
-    for (int b = 0; b < NQB; ++b) {
-        if constexpr (FLOATS)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) split_planes(qf[b][ks], q[b][ks]);
-        settle_row(FLOATS || r0 + 32 * b < rows, FLOATS ? DP / 8 : a.q.chunks, q[b]);
-    }
+        for (int ks = 0; ks < KS; ++ks) split_planes(qf[ks], q[ks]);
+    settle_row(FLOATS || r < rows, FLOATS ? DP / 8 : a.q.chunks, q);
     if (kAhead > 1 && u0 + 1 < u1) next = load(u0 + 1, 1);
     for (int u = u0, buf = 0; u < u1; ++u, buf = buf == kBuffers - 1 ? 0 : buf + 1) {
         // (a partly valid tile's loads are not the same number for every wave)
@@ -170,81 +158,64 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
             any = any || on[kb];
         }
         if (any) {
-            bf16x8 p[KB][2][NQB][NP];
-            float sum[NQB];
-            bool unseen = false;
-#pragma unroll
-            for (int b = 0; b < NQB; ++b) unseen = unseen || m[b] == -INFINITY;    // a row's first key may be here
-            for (bool fresh = __any(unseen);; fresh = true) {
-                f32x16 s[KB][NQB];
+            bf16x8 p[KB][2][NP];
+            float sum;
+            for (bool fresh = __any(m == -INFINITY);; fresh = true) {    // (a row's first key may be here)
+                f32x16 s[KB];
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     if (!on[kb]) continue;
 #pragma unroll
-                    for (int b = 0; b < NQB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[kb][b][i] = 0.0f;
+                    for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
                         bf16x8 f[NP];
 #pragma unroll
                         for (int pl = 0; pl < NP; ++pl) f[pl] = frags.rows(at, pl * KT * DP * 2, kb, ks);
-#pragma unroll
-                        for (int b = 0; b < NQB; ++b) s[kb][b] = mma(f, q[b][ks], s[kb][b]);
+                        s[kb] = mma(f, q[ks], s[kb]);
                     }
-                    if (part[kb])
+                    if (part[kb]) {
+                        const uint32_t x = (seen_bits(see, a.win.sinks, j0 + 32 * kb) & (uint32_t)(word >> (32 * kb))) >> (4 * half);
 #pragma unroll
-                        for (int b = 0; b < NQB; ++b) {
-                            const uint32_t x = (seen_bits(see[b], a.win.sinks, j0 + 32 * kb) & (uint32_t)(word >> (32 * kb))) >> (4 * half);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                s[kb][b][i] = or_lowest(spread_bit(x, 8 * (i >> 2) + (i & 3)), s[kb][b][i]);
-                        }
+                        for (int i = 0; i < 16; ++i)
+                            s[kb][i] = or_lowest(spread_bit(x, 8 * (i >> 2) + (i & 3)), s[kb][i]);
+                    }
                 }
                 if (fresh) {
+                    float top = m;
 #pragma unroll
-                    for (int b = 0; b < NQB; ++b) {
-                        float top = m[b];
+                    for (int kb = 0; kb < KB; ++kb)
+                        if (on[kb])
 #pragma unroll
-                        for (int kb = 0; kb < KB; ++kb)
-                            if (on[kb])
+                            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+                    top = half_max(top);
+                    const float f = m == -INFINITY ? 0.0f : exp2_fast((m - top) * a.c);
+                    m = top;
+                    l *= f;
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][b][i]);
-                        top = half_max(top);
-                        const float f = m[b] == -INFINITY ? 0.0f : exp2_fast((m[b] - top) * a.c);
-                        m[b] = top;
-                        l[b] *= f;
+                    for (int d = 0; d < DB; ++d)
 #pragma unroll
-                        for (int d = 0; d < DB; ++d)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[d][b][i] *= f;
-                    }
+                        for (int i = 0; i < 16; ++i) o[d][i] *= f;
                 }
-                bool over = false;
+                const float mc = m == -INFINITY ? 0.0f : m * a.c;    // no key yet: all probabilities are 0
+                sum = 0.0f;
 #pragma unroll
-                for (int b = 0; b < NQB; ++b) {
-                    const float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;    // no key yet: all probabilities are 0
-                    sum[b] = 0.0f;
+                for (int kb = 0; kb < KB; ++kb) {
+                    if (!on[kb]) continue;
 #pragma unroll
-                    for (int kb = 0; kb < KB; ++kb) {
-                        if (!on[kb]) continue;
+                    for (int i = 0; i < 16; ++i) s[kb][i] = exp2_fast(fmaf(s[kb][i], a.c, -mc));
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) s[kb][b][i] = exp2_fast(fmaf(s[kb][b][i], a.c, -mc));
-#pragma unroll
-                        for (int st = 0; st < 2; ++st) {
-                            to_operand(s[kb][b], st, p[kb][st][b]);
-                            if constexpr (NP == 1) sum[b] = add_operand(p[kb][st][b][0], sum[b]);
-                        }
-                        if constexpr (NP > 1)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) sum[b] += s[kb][b][i];
+                    for (int st = 0; st < 2; ++st) {
+                        to_operand(s[kb], st, p[kb][st]);
+                        if constexpr (NP == 1) sum = add_operand(p[kb][st][0], sum);
                     }
-                    over = over || sum[b] > kFar;
+                    if constexpr (NP > 1)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum += s[kb][i];
                 }
-                if (fresh || !__any(over)) break;
+                if (fresh || !__any(sum > kFar)) break;
             }
-#pragma unroll
-            for (int b = 0; b < NQB; ++b) l[b] += sum[b];
+            l += sum;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 if (!on[kb]) continue;
@@ -255,8 +226,7 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
                         bf16x8 f[NP];
 #pragma unroll
                         for (int pl = 0; pl < NP; ++pl) f[pl] = frags.cols(at, TileT::kBytes + pl * KT * DP * 2, kb, st, d);
-#pragma unroll
-                        for (int b = 0; b < NQB; ++b) o[d][b] = mma(f, p[kb][st][b], o[d][b]);
+                        o[d] = mma(f, p[kb][st], o[d]);
                     }
             }
         }
@@ -264,64 +234,61 @@ __global__ void __launch_bounds__(NW * 64, launch_bound(NW, window_fwd_per_cu(NP
         word = next;
         next = after;
     }
-#pragma unroll
-    for (int b = 0; b < NQB; ++b) {
-        const int r = r0 + 32 * b;
-        const float total = half_sum(l[b]);
-        if (r >= rows) continue;
-        if (w.splits > 1) {
-            const PartRow pr = part_row(a.parts, a.bhs, w.bh, rows, r);
-            const int64_t at = pr.at + w.split * pr.step;
-            if (lane < 32) {
-                a.part_ml[2 * at] = m[b] * a.c;
-                a.part_ml[2 * at + 1] = total;
-            }
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<f32x4*>(a.part_o + at * DP + 32 * d + reg_row(i)) =
-                        f32x4{o[d][b][i], o[d][b][i + 1], o[d][b][i + 2], o[d][b][i + 3]};
-            continue;
+    const float total = half_sum(l);
+    if (r >= rows) return;
+    if (w.splits > 1) {
+        const PartRow pr = part_row(a.parts, a.bhs, w.bh, rows, r);
+        const int64_t at = pr.at + w.split * pr.step;
+        if (lane < 32) {
+            a.part_ml[2 * at] = m * a.c;
+            a.part_ml[2 * at + 1] = total;
         }
-        const int tok = r / a.group, head = w.h * a.group + r - tok * a.group;
-        const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-        if (a.lse && lane < 32)
-            a.lse[((int64_t)w.b * a.hq + head) * a.nq + tok] = total > 0.0f ? fmaf(m[b], a.c, log2f(total)) : INFINITY;
-        const int64_t at = (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            float x[16], lost[16];
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = o[d][b][i] * inv;
-                lost[i] = lost_by_rounding(x[i]);
-            }
-            store_block<T>(static_cast<T*>(a.out) + at, 32 * d, a.dim, x);
-            if constexpr (sizeof(T) == 2)
-                if (a.rest) store_block<T>(static_cast<T*>(a.rest) + at, 32 * d, a.dim, lost);    // see store_out of g2v_attention_fwd.hip
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4*>(a.part_o + at * DP + 32 * d + reg_row(i)) =
+                    f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        return;
+    }
+    // (made again from r: kept over the loop, they spill at 96 channels, 134 -> 153 us)
+    const int tok = r / a.group, head = w.h * a.group + r - tok * a.group;
+    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+    if (a.lse && lane < 32)
+        a.lse[((int64_t)w.b * a.hq + head) * a.nq + tok] = total > 0.0f ? fmaf(m, a.c, log2f(total)) : INFINITY;
+    const int64_t at = (((int64_t)w.b * a.nq + tok) * a.hq + head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+        float x[16], lost[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = o[d][i] * inv;
+            lost[i] = lost_by_rounding(x[i]);
         }
+        store_block<T>(static_cast<T*>(a.out) + at, 32 * d, a.dim, x);
+        if constexpr (sizeof(T) == 2)
+            if (a.rest) store_block<T>(static_cast<T*>(a.rest) + at, 32 * d, a.dim, lost);    // see store_out of g2v_attention_fwd.hip
     }
 }
 
-template <int NP, int DP, int KS, int NQB, int NW, int KT, typename T>
+template <int NP, int DP, int KS, int NW, int KT, typename T>
 hipError_t fwd_launch(const WinFwd& a, hipStream_t s) {
     const dim3 grid((unsigned)workgroups(a.parts, a.bhs)), block(NW * 64);
     if constexpr (NP > 1) {
-        if (a.floats) G2V_LAUNCH((k_window_fwd<NP, true, DP, KS, NQB, NW, KT, T>), grid, block, 0, s, a);
-        else G2V_LAUNCH((k_window_fwd<NP, false, DP, KS, NQB, NW, KT, T>), grid, block, 0, s, a);
+        if (a.floats) G2V_LAUNCH((k_window_fwd<NP, true, DP, KS, NW, KT, T>), grid, block, 0, s, a);
+        else G2V_LAUNCH((k_window_fwd<NP, false, DP, KS, NW, KT, T>), grid, block, 0, s, a);
     } else {
-        G2V_LAUNCH((k_window_fwd<NP, false, DP, KS, NQB, NW, KT, T>), grid, block, 0, s, a);
+        G2V_LAUNCH((k_window_fwd<NP, false, DP, KS, NW, KT, T>), grid, block, 0, s, a);
     }
     return launch_attn_join(a, NP > 1, DP, s);
 }
-template <int NP, int DP, int NQB, int KT, typename T>
+template <int NP, int DP, int KT, typename T>
 hipError_t fwd_waves(const WinFwd& a, const AttnShape& g, hipStream_t s) {
     const bool full = a.dim > DP - 16;
     if constexpr (NP == 1)
         if (g.waves == 1)
-            return full ? fwd_launch<NP, DP, DP / 16, 1, 1, KT, T>(a, s) : fwd_launch<NP, DP, DP / 16 - 1, 1, 1, KT, T>(a, s);
-    return full ? fwd_launch<NP, DP, DP / 16, NQB, 4, KT, T>(a, s) : fwd_launch<NP, DP, DP / 16 - 1, NQB, 4, KT, T>(a, s);
+            return full ? fwd_launch<NP, DP, DP / 16, 1, KT, T>(a, s) : fwd_launch<NP, DP, DP / 16 - 1, 1, KT, T>(a, s);
+    return full ? fwd_launch<NP, DP, DP / 16, 4, KT, T>(a, s) : fwd_launch<NP, DP, DP / 16 - 1, 4, KT, T>(a, s);
 }
 
 }  // namespace
@@ -329,7 +296,7 @@ hipError_t fwd_waves(const WinFwd& a, const AttnShape& g, hipStream_t s) {
 AttnShape window_fwd_shape(bool f32, int dp, int64_t rows) {
     AttnShape g = attn_fwd_shape(f32, dp, rows);
     g.per_cu = window_fwd_per_cu(f32 ? 3 : 1, dp, g.waves);
-    if (!f32 && g.waves > 1) g.blocks = 1;
+    g.blocks = 1;
     return g;
 }
 
@@ -337,17 +304,17 @@ hipError_t launch_window_fwd(const WinFwd& a, bool f32, int dp, hipStream_t s) {
     const AttnShape g = window_fwd_shape(f32, dp, (int64_t)a.group * a.nq);
     if (f32) {
         switch (dp) {
-            case 32: return fwd_waves<3, 32, 1, 64, float>(a, g, s);
-            case 64: return fwd_waves<3, 64, 1, 32, float>(a, g, s);
-            case 96: return fwd_waves<3, 96, 1, 32, float>(a, g, s);
-            default: return fwd_waves<3, 128, 1, 32, float>(a, g, s);
+            case 32: return fwd_waves<3, 32, 64, float>(a, g, s);
+            case 64: return fwd_waves<3, 64, 32, float>(a, g, s);
+            case 96: return fwd_waves<3, 96, 32, float>(a, g, s);
+            default: return fwd_waves<3, 128, 32, float>(a, g, s);
         }
     }
     switch (dp) {
-        case 32: return fwd_waves<1, 32, 1, 64, __bf16>(a, g, s);
-        case 64: return fwd_waves<1, 64, 1, 64, __bf16>(a, g, s);
-        case 96: return fwd_waves<1, 96, 1, 64, __bf16>(a, g, s);
-        default: return fwd_waves<1, 128, 1, 32, __bf16>(a, g, s);
+        case 32: return fwd_waves<1, 32, 64, __bf16>(a, g, s);
+        case 64: return fwd_waves<1, 64, 64, __bf16>(a, g, s);
+        case 96: return fwd_waves<1, 96, 64, __bf16>(a, g, s);
+        default: return fwd_waves<1, 128, 32, __bf16>(a, g, s);
     }
 }
 
