@@ -345,12 +345,22 @@ int64_t win_keys(const WinSizes& x, AttnShape g) {
     return std::min<int64_t>(x.z.nk, x.span + g.waves * g.blocks * 32 / x.z.group + (x.w.sinks ? g.tile : 0));
 }
 // Whether the forward splits float32 rows into planes as it loads them, every workgroup that sees a row for itself, instead of
-// reading planes packed before.  Short windows: a launch and a pass over the rows less; long ones: each row is split again and again.
-// (40,000 x 8 heads, windows of 256 / 1024 / 2048 keys, packed and split us: 64 channels 312, 648, 1037 and 217, 567, 1043; 128
-// channels 804, 1629, 2652 and 587, 1516, 2762; 96 channels 598, 1136, 1858 and 523, 1367, 2499; 72 channels 599, 1124, 1835 and 653,
-// 1576, 2769.  Rows that are not whole chunks of 8 load their ends one by one: 75 channels 649, 1166, 1867 and 821, 2014, 3446.)
-bool win_splits_rows(const WinSizes& x) {
-    return x.z.dim % 8 == 0 && win_keys(x, window_fwd_shape(true, x.z.dp, x.z.rows())) <= (x.z.dp == 96 ? 384 : 1024);
+// reading planes packed before: a launch and a pass over the rows less, but each row of k and v is split again by all workgroups that see
+// it.  Ten rows are split in the time that packing one takes (3.3 at 96 channels, where its registers are short), and packing takes all
+// rows of q, k and v once; where a mask has tiles of planes loaded row by row, too, 32 (13).  us at 257 / 513 / 1025 / 2049 keys,
+// 40,000 x 8 heads, the rule's side first: 32 channels (split) 109 for 157, 173 for 210, 295 for 320, (packed) 548 for 548; 64 (split)
+// 204 for 284, 332 for 391, 593 for 617, (packed) 1033 for 1055; 96 (split) 448 for 544, 700 for 723, (packed) 1084 for 1203, 1807 for
+// 2209; 72 (split) 429 for 537, 673 for 706, (packed) 1047 for 1165, 1730 for 2147; 128 (split) 532 for 750, 822 for 1011, 1408 for
+// 1553, (packed) 2617 for 2592.  With a mask, at 2049 / 4097 keys: 64 channels (split) 1009 for 1077, 1902 for 1928; 96 (split) 2329
+// for 2357, (packed) 4232 for 4347.  Shared heads have fewer rows of k and v to pack: 10,000 x 2 x 4 heads, 64 channels (split) 55 for
+// 67, 90 for 96, (packed) 151 for 154, 251 for 275.  Few queries split each row once: one query, 4097 keys x 16 x 64 (split) 25 for 39.
+// (Rows that are not whole chunks of 8 load their ends one by one: 40,000 x 8 x 75, 256 / 1024 / 2048 keys, packed 649, 1166, 1867,
+// split 821, 2014, 3446.)
+bool win_splits_rows(const WinSizes& x, bool masked) {
+    const AttnShape g = window_fwd_shape(true, x.z.dp, x.z.rows());
+    const int64_t split = ceil_div(x.z.rows(), g.waves * 32) * 2 * std::min<int64_t>(x.z.nk, x.span + x.w.sinks);
+    const int64_t packed = x.z.rows() + 2 * (int64_t)x.z.nk;
+    return x.z.dim % 8 == 0 && 3 * split <= (x.z.dp == 96 ? (masked ? 40 : 10) : (masked ? 96 : 30)) * packed;
 }
 AttnRun win_fwd_run(const WinSizes& x) {
     const AttnShape g = window_fwd_shape(x.z.f32, x.z.dp, x.z.rows());
@@ -605,7 +615,7 @@ size_t g2v_window_attention_forward_workspace(int batch, int n_q, int n_k, int h
                                               int left, int right, int sinks, int in_place, int masked) {
     WinSizes x;
     if (win_sizes(batch, n_q, n_k, heads_q, heads_k, head_dim, dtype, left, right, sinks, x) != G2V_OK) return 0;
-    return win_fwd_bytes(x, win_fwd_run(x), x.z.f32 ? !win_splits_rows(x) : !in_place);
+    return win_fwd_bytes(x, win_fwd_run(x), x.z.f32 ? !win_splits_rows(x, masked != 0) : !in_place);
 }
 
 int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int heads_k, int head_dim, const void* q,
@@ -629,8 +639,8 @@ int g2v_window_attention_forward(int batch, int n_q, int n_k, int heads_q, int h
     const Strided t[3] = {{q, q_strides, n_q, heads_q, false},
                           {k, keys ? k_strides : none, z.nk, heads_k, true},
                           {v, keys ? v_strides : none, z.nk, heads_k, true}};
-    const bool packed = z.f32 ? !win_splits_rows(x) : !attn_in_place(z, t, 3);
-    if (!keys) key_mask = nullptr;
+    const bool packed = z.f32 ? !win_splits_rows(x, key_mask != nullptr) : !attn_in_place(z, t, 3);
+    if (!keys) key_mask = nullptr;    // (then there are no rows to pack or to split)
     const AttnRun r = win_fwd_run(x);
     const size_t need = win_fwd_bytes(x, r, packed);
     if (!workspace || workspace_bytes < need)
