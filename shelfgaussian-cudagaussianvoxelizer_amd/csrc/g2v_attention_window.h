@@ -15,11 +15,11 @@
 // workgroups that share out the queries, and joined.
 //
 // Bound by memory at the shortest windows and then, like the attention over all keys, by matrix and vector work taking turns:
-// 200,000 x 8 heads x 64 bfloat16, windows of 1 / 513 / 2049 keys, us: forward that a backward follows 258, 398, 1059 (its 1.0 GB
-// take 200 at a copy's rate; a key more for every query takes 0.43, 950 TFLOP/s), dQ with delta 406, 595, 1713, dK and dV 315, 735,
-// 1750.  A wave has one block of 32 rows and bfloat16 has more workgroups to a CU than the attention over all keys, as a row block's
-// range is shorter than two blocks' together, and prologues and ends hide one another (with that attention's blocks and workgroups,
-// 513 keys: forward 478 for 414, dQ 747 for 615, before rows were loaded as below).
+// 200,000 x 8 heads x 64 bfloat16, windows of 1 / 513 / 2049 keys, us: forward that a backward follows 257, 391, 1101 (its 1.0 GB
+// take 200 at a copy's rate; from 513 keys on a key more for every query takes 0.46, 890 TFLOP/s), dQ with delta 413, 578, 1706, dK and
+// dV 318, 827, 1750 (P and dS in two planes up to 1,024 keys).  A wave has one block of 32 rows and bfloat16 has more workgroups to a CU
+// than the attention over all keys, as a row block's range is shorter than two blocks' together, and prologues and ends hide one another
+// (with that attention's blocks and workgroups, 513 keys: forward 478 for 414, dQ 747 for 615, before rows were loaded as below).
 #pragma once
 #include "g2v_attention.h"
 
@@ -280,7 +280,8 @@ struct RowValues {
 // A lane's row as B operands (mem_frag's), in two parts: the loads, which all go out before any is waited for, and what ends the wait
 // for them and puts zeros where there is no row or no chunk (the last step alone may lack some).  A wait that is left to a loop's first
 // use is waited for in every turn, and with it the tiles that are on their way.  Against mem_frag, dQ and dK with dV in us, windows of 513
-// keys: 200,000 x 8 heads x 64 618 -> 586 and 734 -> 726, 40,000 x 8 x 96 206 -> 186 and 245 -> 226, x 128 245 -> 224 and 524 -> 487.
+// keys and P in one plane: 200,000 x 8 heads x 64 618 -> 586 and 734 -> 726, 40,000 x 8 x 96 206 -> 186 and 245 -> 226, x 128 245 -> 224
+// and 524 -> 487.
 // (Windows of one key, whose tensors pass the last cache: 200,000 x 8 x 64 377 -> 406 and 260 -> 314; 33 keys 401 -> 399 and 348 -> 348.)
 template <int DP, int KS, int NP>
 __device__ __forceinline__ void load_row(const char* row, int chunks, bf16x8 (&x)[KS][NP]) {

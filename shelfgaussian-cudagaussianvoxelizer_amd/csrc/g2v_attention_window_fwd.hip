@@ -293,6 +293,8 @@ hipError_t fwd_waves(const WinFwd& a, const AttnShape& g, hipStream_t s) {
 
 }  // namespace
 
+// Waves as there.  float32 rows take four however few they are: those without a row load and split tiles with the others (one query, 4097
+// keys x 16 heads x 64, 18 us and 10 with its join's).
 AttnShape window_fwd_shape(bool f32, int dp, int64_t rows) {
     AttnShape g = attn_fwd_shape(f32, dp, rows);
     g.per_cu = window_fwd_per_cu(f32 ? 3 : 1, dp, g.waves);
