@@ -1308,6 +1308,12 @@ def _overlaps_itself(t):
                for k, (step, n) in enumerate(steps))
 
 
+def _same_places(t, o):
+    """Whether two tensors of one shape have each element at the same place and of the same type."""
+    return t.data_ptr() == o.data_ptr() and t.dtype == o.dtype \
+        and all(a == b or n == 1 for a, b, n in zip(t.stride(), o.stride(), t.shape))
+
+
 def _check_sharing(grads, outs):
     """Refuses what the library refuses among flat tensors, whose memory it sees: an output that shares memory with another one, or with a
     gradient but for its own at the same places, and with itself."""
@@ -1320,8 +1326,7 @@ def _check_sharing(grads, outs):
             raise RuntimeError(f"clip_gradients: elements of tensor {i}, which is written, share memory")
         open_ = [span for span in open_ if span[1] > at]
         for _, _, k, o, other in open_:
-            if (written or other) and not (i == k and (t.data_ptr(), t.dtype, t.stride()) == (o.data_ptr(), o.dtype, o.stride())) \
-                    and _share_memory(t, o):
+            if (written or other) and not (i == k and _same_places(t, o)) and _share_memory(t, o):
                 raise RuntimeError(f"clip_gradients: tensors {min(i, k)} and {max(i, k)} share memory that is written")
         open_.append((at, end, i, t, written))
 

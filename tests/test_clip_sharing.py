@@ -87,6 +87,7 @@ def test_what_shares_nothing_passes():
     checked([w[:, ::2], w[:, ::2]], [torch.empty(6, 70), torch.empty(6, 70)])
     checked([torch.ones(4).expand(3, 4)], [torch.empty(3, 4)])
     checked([square.t(), w[:, 1::2]])
+    checked([w[2:3, 1:9]], [torch.as_strided(w, (1, 8), (7, 1), 2 * 140 + 1)])    # the same places: the step of one row does not count
     src, dst, back = checked([w[:, ::2], torch.empty(0, 3)[:, ::2], torch.tensor(3.0)])
     assert src[0].is_contiguous() and dst[0] is src[0] and back[0][1] is src[0]
 
